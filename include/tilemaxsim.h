@@ -346,6 +346,67 @@ int tms_codes_check(const void* codes, int64_t count, int code_bytes, int64_t K,
 int tms_codes_verdict(const int64_t* verdict, void* stream);
 
 /*
+ * Training: MaxSim of a batch of queries and a batch of documents, with the positions of the
+ * maxima that its gradients need. No reference counterpart (the reference scores only).
+ *   scores[q, b] = sum over q's real tokens i of max over b's real tokens j of <Qs[q, i], D[b, j]>
+ * Qs (nQ, nq, d); D (B, nd, d) of the same fp16, bf16 or fp32 `dtype`, any d (fp32 products
+ * are formed from three bf16 terms a side, to about 2^-23). qmask (nQ, nq) and dmask (B, nd)
+ * are bytes, non-zero for a real token; NULL: every token is real. nway = 0: every query
+ * with every document, scores (nQ, B). nway > 0: B is nQ * nway, query q with documents
+ * [q nway, (q + 1) nway), scores (nQ, nway). A document without a real token scores -inf;
+ * a query without any scores 0 elsewhere. Embeddings are finite at the real tokens; what
+ * stands at the masked ones is not looked at. nd <= 65535.
+ *   workspace  tms_pairs_workspace_size bytes of device memory, 16-byte aligned (0 for 16-bit
+ *              rows whose d is a multiple of 32: NULL, and Qs and D 16-byte aligned)
+ *   positions  NULL, or tms_pairs_positions uint16 of device memory, 16-byte aligned, for
+ *              tms_maxsim_pairs_grad: the first token j of each maximum, 0xffff for none,
+ *              laid out (B, nQ, nq rounded up to 8), with nway > 0 (B, nq rounded up to 8)
+ */
+int64_t tms_pairs_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nd, int dtype);
+int64_t tms_pairs_positions(int64_t nQ, int64_t nq, int64_t B, int64_t nway);
+int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
+                     int64_t nway, const uint8_t* qmask, const uint8_t* dmask, int dtype, void* workspace,
+                     int64_t workspace_bytes, float* scores, uint16_t* positions, void* stream);
+
+/*
+ * The gradients of tms_maxsim_pairs, from its positions and `grad`, what comes back for each
+ * score (fp32, the scores' shape): dQ[q, i] = sum_b grad[q, b] D[b, j] and dD[b, j] the sum of
+ * grad[q, b] Qs[q, i] over the (q, i) whose maximum is j, in `dtype`, summed in fp32 in one
+ * order. dQ or dD may be NULL. `workspace`: tms_pairs_grad_workspace_size bytes of device
+ * memory (needed for dQ only).
+ */
+int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway);
+int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
+                          int64_t nway, const uint16_t* positions, const float* grad, int dtype, void* workspace,
+                          int64_t workspace_bytes, void* dQ, void* dD, void* stream);
+
+/*
+ * Training: the norm of `count` gradients taken as one vector, and clipping to it. `tensors`
+ * is a HOST array, read during the call: device pointers, element counts (0 is allowed) and
+ * dtypes (fp16, bf16 or fp32, any alignment to the element). The norm is the square root of
+ * the sum of squares (TMS_NORM_2, summed in 64 bits) or the largest absolute value
+ * (TMS_NORM_INF), written to `norm` (one float of device memory).
+ * tms_grad_clip also writes dst[i] = src[i] * min(1, *max_norm / (norm + 1e-6)), in dst's
+ * dtype; dst may be src (then of one dtype), and must not overlap another source. A NaN or
+ * infinite norm gives what that factor gives. *max_norm is read during the call, from the host.
+ * `workspace`: tms_grad_workspace_size(count) bytes of device memory, 8-byte aligned.
+ */
+#define TMS_NORM_INF 0
+#define TMS_NORM_2 2
+typedef struct tms_grad_tensor {
+  const void* src;
+  void* dst;
+  int64_t n;
+  int32_t src_dtype;
+  int32_t dst_dtype;
+} tms_grad_tensor;
+int64_t tms_grad_workspace_size(int64_t count);
+int tms_grad_norm(const tms_grad_tensor* tensors, int64_t count, int norm_type, void* workspace,
+                  int64_t workspace_bytes, float* norm, void* stream);
+int tms_grad_clip(const tms_grad_tensor* tensors, int64_t count, int norm_type, const double* max_norm,
+                  void* workspace, int64_t workspace_bytes, float* norm, void* stream);
+
+/*
  * Measurement helper, not part of the scoring path and with no counterpart in the
  * reference: reads `bytes` (a multiple of 8 KiB) of `buf` once with a read-only
  * streaming kernel and writes one XOR word per thread to `sink`

@@ -11,6 +11,8 @@ from .flash_maxsim_kernel import (flash_maxsim_batch, flash_maxsim_multi_doc, fl
                                   flash_maxsim_single, maxsim_score)
 from .flash_maxsim_v2 import flash_maxsim_batched_queries, flash_maxsim_v2, flash_maxsim_v2_multiquery
 from .flash_pqsim_kernel import TileMaxSimPQ
+from .grad_clip import clip_grad_norm_, grad_norm
+from .pairs import maxsim_pairs
 from .plaid import flashmaxsim_score_packed, flashmaxsim_score_packed_batched
 from .residual import decompress_residual, flashmaxsim_score_residual, flashmaxsim_score_residual_batched
 from .topk import maxsim_topk, topk
@@ -20,5 +22,6 @@ __all__ = [
     "flash_maxsim_single", "flash_maxsim_batch", "flash_maxsim_multi_doc", "flash_maxsim_multi_doc_batched",
     "maxsim_score", "TileMaxSimPQ", "flashmaxsim_score_packed", "flashmaxsim_score_packed_batched", "topk",
     "maxsim_topk",
+    "maxsim_pairs", "grad_norm", "clip_grad_norm_",
     "decompress_residual", "flashmaxsim_score_residual", "flashmaxsim_score_residual_batched",
 ]

@@ -32,6 +32,8 @@ TMS_MAXSIM_TOPK_COUNTER_WORDS = 144  # 32-bit words of tms_maxsim_topk's zeroed 
 TMS_MFMA_PROBE_SINK_WORDS = 131072  # words of the sink tms_mfma_probe writes
 TMS_CHECK_PARTS = 64  # words of a *_checked call's parts (device) and verdict (pinned host)
 TMS_PACKED_SCAN_MAX = 16384  # documents tms_maxsim_packed_checked takes
+TMS_NORM_INF = 0
+TMS_NORM_2 = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -78,8 +80,20 @@ SIGNATURES = {
     "tms_maxsim_residual_checked": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _c_void_p, _int, _c_void_p, _c_void_p,
                                     _i64, _c_void_p, _i64, _c_void_p, _i64, _int, _int, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p],
+    "tms_pairs_workspace_size": [_i64, _i64, _i64, _i64, _i64, _int],
+    "tms_pairs_positions": [_i64, _i64, _i64, _i64],
+    "tms_maxsim_pairs": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int, _c_void_p,
+                         _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tms_pairs_grad_workspace_size": [_i64, _i64, _i64, _i64, _i64],
+    "tms_maxsim_pairs_grad": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int,
+                              _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tms_grad_workspace_size": [_i64],
+    "tms_grad_norm": [_c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "tms_grad_clip": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
 }
-RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64}
+RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
+            "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
+            "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

@@ -33,6 +33,11 @@ HIPCC_FLAGS = [
 ]
 
 
+# The training operators (tms_train_*.hip) take what a training run brings: a NaN or infinite
+# gradient or logit goes through to the result.
+NAN_FLAGS = ["-fhonor-nans"]
+
+
 def _hipcc() -> str:
     for cand in (shutil.which("hipcc"), "/opt/rocm/bin/hipcc"):
         if cand and os.path.exists(cand):
@@ -41,7 +46,8 @@ def _hipcc() -> str:
 
 
 def _compile(src: str, obj: str) -> None:
-    cmd = [_hipcc(), *HIPCC_FLAGS, "-c", src, "-o", obj]
+    nans = NAN_FLAGS if os.path.basename(src).startswith("tms_train_") else []
+    cmd = [_hipcc(), *HIPCC_FLAGS, *nans, "-c", src, "-o", obj]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed for {os.path.basename(src)}:\n{res.stdout}\n{res.stderr}")

@@ -1,0 +1,137 @@
+"""The global gradient norm, and clipping to it, over any number of tensors in a few launches.
+
+The norm stays on the GPU: nothing waits for it, and a training step that clips can be
+captured into a HIP graph. No reference counterpart (the reference does not train).
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from array import array
+
+import torch
+
+from . import _check, _lib
+
+_NORMS = {2.0: _lib.TMS_NORM_2, math.inf: _lib.TMS_NORM_INF}
+
+
+def _norm_type(fn: str, p) -> int:
+    code = _NORMS.get(float(p))
+    if code is None:
+        raise NotImplementedError(f"{fn}: norm_type must be 2 or inf (got {p})")
+    return code
+
+
+def _list(fn: str, tensors) -> list:
+    ts = [tensors] if isinstance(tensors, torch.Tensor) else [t for t in tensors if t is not None]
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{fn}: expected tensors, got {type(t).__name__}")
+        if t.dtype not in _lib.DTYPE_CODES:
+            raise TypeError(f"{fn}: gradients must be float16, bfloat16 or float32 (got {t.dtype})")
+    for t in ts:
+        if not t.is_cuda:
+            raise ValueError(f"{fn}: gradients must be on a ROCm GPU device (got {t.device}); tilemaxsim_amd has no CPU path")
+        if t.device != ts[0].device:
+            raise ValueError(f"{fn}: all gradients must be on one device; got {t.device} and {ts[0].device}")
+    return ts
+
+
+def _table(src: list, dst: list) -> array:
+    """tms_grad_tensor entries: two addresses, the size, and both dtypes in one word."""
+    codes = _lib.DTYPE_CODES
+    words = array("q")
+    for s, d in zip(src, dst):
+        words.extend((s.data_ptr(), d.data_ptr(), s.numel(), codes[s.dtype] | codes[d.dtype] << 32))
+    return words
+
+
+def _workspace(lib, count: int, dev: torch.device) -> torch.Tensor:
+    return torch.empty(lib.tms_grad_workspace_size(count) // 8, dtype=torch.float64, device=dev)
+
+
+def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
+    """The norm of all gradients taken as one vector: a float32 scalar on their device.
+
+    Args:
+        tensors: gradients (float16, bfloat16 or float32, any mix, one device); None entries
+            are passed over, as parameters without a gradient leave them.
+        norm_type: 2.0, or ``inf`` for the largest absolute value.
+    """
+    code = _norm_type("grad_norm", norm_type)
+    ts = [t if t.is_contiguous() else t.contiguous() for t in _list("grad_norm", tensors)]
+    if not ts:
+        return torch.zeros(())
+    dev = ts[0].device
+    lib = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _workspace(lib, len(ts), dev)
+    table = _table(ts, ts)
+    status = _lib.launch(dev, lib.tms_grad_norm, table.buffer_info()[0], len(ts), code, ws.data_ptr(), 8 * ws.numel(),
+                         norm.data_ptr())
+    if status:
+        _lib.check(status)
+    return norm
+
+
+@torch.no_grad()
+def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    out=None) -> torch.Tensor:
+    """Scale all gradients by ``min(1, max_norm / (norm + 1e-6))``, their norm taken together.
+
+    Args:
+        tensors: as for :func:`grad_norm`; changed in place, unless ``out`` is given.
+        max_norm: the norm to clip to (at least 0).
+        norm_type: 2.0 or ``inf``.
+        error_if_nonfinite: wait for the norm, and raise RuntimeError on a NaN or infinite
+            one, before anything is scaled. Without it such a norm goes into the factor
+            (an infinite one gives 0, NaN stays NaN), and nothing waits.
+        out: tensors of the same sizes, one for each of ``tensors``, that take the scaled
+            gradients (in their own dtype: bf16 gradients into an optimizer's fp32 ones).
+
+    Returns:
+        The norm before clipping, a float32 scalar on the gradients' device.
+    """
+    fn = "clip_grad_norm_"
+    code = _norm_type(fn, norm_type)
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"{fn}: max_norm must be at least 0 (got {max_norm})")
+    if out is None:
+        ts = to = _list(fn, tensors)
+    else:
+        pairs_in = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+        pairs_out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(pairs_in) != len(pairs_out):
+            raise ValueError(f"{fn}: {len(pairs_in)} gradients and {len(pairs_out)} tensors in out")
+        kept = [(t, o) for t, o in zip(pairs_in, pairs_out) if t is not None]
+        ts, to = _list(fn, [t for t, _ in kept]), _list(fn, [o for _, o in kept])
+        if len(to) != len(ts):
+            raise ValueError(f"{fn}: out has None in the place of a gradient's tensor")
+        for t, o in zip(ts, to):
+            if t.shape != o.shape:
+                raise ValueError(f"{fn}: a gradient is {tuple(t.shape)}, its tensor in out {tuple(o.shape)}")
+        if to and to[0].device != ts[0].device:
+            raise ValueError(f"{fn}: gradients are on {ts[0].device}, out is on {to[0].device}")
+    if not ts:
+        return torch.zeros(())
+    if error_if_nonfinite and not bool(torch.isfinite(norm := grad_norm(ts, norm_type))):
+        raise RuntimeError(f"{fn}: the norm of the gradients is {norm.item()}; they are left as they are")
+    dev = ts[0].device
+    lib = _lib.load()
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    ws = _workspace(lib, len(ts), dev)
+    src = [t if t.is_contiguous() else t.contiguous() for t in ts]
+    dst = src if to is ts else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in to]
+    table = _table(src, dst)
+    limit = ctypes.c_double(max_norm)
+    status = _lib.launch(dev, lib.tms_grad_clip, table.buffer_info()[0], len(src), code, ctypes.addressof(limit),
+                         ws.data_ptr(), 8 * ws.numel(), norm.data_ptr())
+    if status:
+        _lib.check(status)
+    for o, d in zip(to, dst):
+        if o is not d:
+            o.copy_(d)  # a strided tensor's own elements
+    torch.autograd.graph.increment_version([o for o in to if not o.is_inference()])
+    return norm
