@@ -381,6 +381,33 @@ int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, con
                           int64_t workspace_bytes, void* dQ, void* dD, void* stream);
 
 /*
+ * Training: softmax cross entropy of the logits scale * hidden weight^T against `target`,
+ * without the logits in memory. No reference counterpart. hidden (N, d), weight (V, d), of
+ * one fp16, bf16 or fp32 `dtype`, any d; with a d that is a multiple of 8 in 16 bits, both
+ * 16-byte aligned. target (N) int64: rows with ignore_index have loss 0 and no gradient (what
+ * stands in them is not looked at in the gradients); any other value outside [0, V) makes
+ * its row NaN. *scale (positive, read during the call from the host) multiplies the logits.
+ * loss: N floats (TMS_REDUCE_NONE), or one: the rows' sum, or their mean over the rows that
+ * are not ignored (NaN if none is left). stats: N + 1 floats of device memory that
+ * tms_linear_cross_entropy_grad takes: the rows' log-sum-exp (in powers of two) and that count.
+ * `grad` is what comes back for `loss`; dH (N, d) and dW (V, d) in `dtype`, either may be
+ * NULL. With N = 0 nothing is written to dH and dW. Sums are fp32 in one order.
+ * workspace: tms_lce_workspace_size bytes of device memory (backward = 0 or 1), 256-byte
+ * aligned; its contents need not stay between the two calls.
+ */
+#define TMS_REDUCE_NONE 0
+#define TMS_REDUCE_SUM 1
+#define TMS_REDUCE_MEAN 2
+int64_t tms_lce_workspace_size(int64_t N, int64_t d, int64_t V, int dtype, int backward);
+int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d, const void* weight, int64_t V, int dtype,
+                             const int64_t* target, int64_t ignore_index, const double* scale, int reduction,
+                             void* workspace, int64_t workspace_bytes, float* loss, float* stats, void* stream);
+int tms_linear_cross_entropy_grad(const void* hidden, int64_t N, int64_t d, const void* weight, int64_t V, int dtype,
+                                  const int64_t* target, int64_t ignore_index, const double* scale, int reduction,
+                                  const float* stats, const float* grad, void* workspace, int64_t workspace_bytes,
+                                  void* dH, void* dW, void* stream);
+
+/*
  * Training: the norm of `count` gradients taken as one vector, and clipping to it. `tensors`
  * is a HOST array, read during the call: device pointers, element counts (0 is allowed) and
  * dtypes (fp16, bf16 or fp32, any alignment to the element). The norm is the square root of

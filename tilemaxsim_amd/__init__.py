@@ -7,6 +7,7 @@ documents it scores, and the top-k its callers take); every
 call runs hand-written HIP kernels from ``libtilemaxsim.so`` through its C ABI
 (``include/tilemaxsim.h``). There is no CPU or PyTorch fallback.
 """
+from .cross_entropy import linear_cross_entropy
 from .flash_maxsim_kernel import (flash_maxsim_batch, flash_maxsim_multi_doc, flash_maxsim_multi_doc_batched,
                                   flash_maxsim_single, maxsim_score)
 from .flash_maxsim_v2 import flash_maxsim_batched_queries, flash_maxsim_v2, flash_maxsim_v2_multiquery
@@ -22,6 +23,6 @@ __all__ = [
     "flash_maxsim_single", "flash_maxsim_batch", "flash_maxsim_multi_doc", "flash_maxsim_multi_doc_batched",
     "maxsim_score", "TileMaxSimPQ", "flashmaxsim_score_packed", "flashmaxsim_score_packed_batched", "topk",
     "maxsim_topk",
-    "maxsim_pairs", "grad_norm", "clip_grad_norm_",
+    "maxsim_pairs", "linear_cross_entropy", "grad_norm", "clip_grad_norm_",
     "decompress_residual", "flashmaxsim_score_residual", "flashmaxsim_score_residual_batched",
 ]

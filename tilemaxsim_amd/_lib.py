@@ -34,6 +34,9 @@ TMS_CHECK_PARTS = 64  # words of a *_checked call's parts (device) and verdict (
 TMS_PACKED_SCAN_MAX = 16384  # documents tms_maxsim_packed_checked takes
 TMS_NORM_INF = 0
 TMS_NORM_2 = 2
+TMS_REDUCE_NONE = 0
+TMS_REDUCE_SUM = 1
+TMS_REDUCE_MEAN = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -87,13 +90,19 @@ SIGNATURES = {
     "tms_pairs_grad_workspace_size": [_i64, _i64, _i64, _i64, _i64],
     "tms_maxsim_pairs_grad": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int,
                               _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tms_lce_workspace_size": [_i64, _i64, _i64, _int, _int],
+    "tms_linear_cross_entropy": [_c_void_p, _i64, _i64, _c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _int, _c_void_p,
+                                 _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tms_linear_cross_entropy_grad": [_c_void_p, _i64, _i64, _c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _int,
+                                      _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
     "tms_grad_workspace_size": [_i64],
     "tms_grad_norm": [_c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tms_grad_clip": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
 }
 RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
-            "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64}
+            "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64,
+            "tms_lce_workspace_size": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

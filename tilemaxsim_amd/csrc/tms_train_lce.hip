@@ -1,0 +1,637 @@
+// Softmax cross entropy of the logits scale * H W^T, from the hidden states and the
+// vocabulary's weights, without the logits.
+//
+//   x[n, v] = scale <H[n], W[v]>,  lse[n] = log sum_v exp x[n, v],  loss[n] = lse[n] - x[n, t[n]]
+//   P[n, v] = exp(x[n, v] - lse[n]) - [v = t[n]]
+//   dH[n] = g[n] scale sum_v P[n, v] W[v],   dW[v] = scale sum_n g[n] P[n, v] H[n]
+//
+// Forward: one product whose epilogue reduces each tile's logits to a maximum and a sum of
+// exponentials per row and block of the vocabulary, and a kernel that joins the blocks
+// (8 bytes per row and block instead of 4 per logit).
+// Backward: piece by piece of the vocabulary the logits are formed again (2 N V d operations,
+// where writing and reading them in fp32 would take 8 N V bytes: at d = 768 as long, at less
+// shorter), become P in 16 bits in a workspace, and two more products take P to dH and dW.
+//
+// Everything is in powers of two: x log2(e) goes into exp2, and lse is kept in those units.
+//
+// Precision. Logits, maxima, sums, and the sums of both gradients are fp32. P is rounded to
+// the inputs' type (bf16: 2^-9 of each term, below the rounding of the result; fp16: P is
+// held times 2^15, so that 2^-29 is still a normal number). fp32 inputs are three bf16 terms,
+// and so is their P. P is times g[n] / u before it is rounded, for both gradients, and their
+// sums are times u: u is what a reduction gives every row alike (the ratio is 1), or a power
+// of two above the largest |g| of rows with their own.
+#include <math.h>
+
+#include "tms_train_gemm.h"
+
+namespace tms {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kP16 = 15;  // fp16: P times 2^15
+
+struct RowStat {
+  float top, sum;  // of a block: the largest x log2(e), and the sum of exp2 relative to it
+};
+
+// Rows n of a wave's columns: 16 j + c.
+struct LseEpilogue {
+  RowStat* parts;  // [block of the vocabulary][rows]
+  int32_t rows, V;
+  float s2;  // scale log2(e)
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const float NEG = -__builtin_inff();
+    if (m + 16 * MI > V) {  // past the vocabulary
+#pragma unroll
+      for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (m + 16 * i + 4 * g + e >= V)
+#pragma unroll
+            for (int j = 0; j < NI; j++) acc[i][j][e] = NEG;
+    }
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      float top = NEG;
+#pragma unroll
+      for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, acc[i][j][e]);
+      top = cross_row_max(top) * s2;  // scale > 0
+      const float ref = top == NEG ? 0.f : top;
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], s2, -ref));
+      sum = cross_row_sum(sum);
+      const int row = n + 16 * j + c;
+      if (g == 0 && row < rows && m < V) parts[(int64_t)(m / (16 * MI)) * rows + row] = {top, sum};
+    }
+  }
+};
+
+// P of one piece: [plane][row][ldp]; rows and columns that do not exist are zero.
+template <int DT, int PL>
+struct ProbEpilogue {
+  uint16_t* P;
+  const float* lse2;     // per row; +inf for a row without a gradient
+  const float* g_row;    // per row: g / u
+  const int32_t* target;  // per row; -1 for none
+  int64_t plane;
+  int32_t ldp, rows, V, v0;  // V: columns of the piece that exist; v0: its first
+  float s2;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const float one = DT == TMS_DTYPE_F16 && PL == 1 ? (float)(1 << kP16) : 1.f;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int row = n + 16 * j + c;
+      const bool in = row < rows;
+      const float ref = in ? lse2[row] : __builtin_inff(), w = in ? g_row[row] : 0.f;
+      const int hit = in ? target[row] - v0 - (m + 4 * g) : -1;  // its place among this lane's 4 + 16 i
+      const bool any = __ballot(hit >= 0 && hit < 16 * MI) != 0ull;
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+        float p[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], s2, -ref));
+          if (any) p[e] -= hit == 16 * i + e ? one : 0.f;
+          p[e] *= w;
+          if (m + 16 * MI > V) p[e] = m + 16 * i + 4 * g + e < V ? p[e] : 0.f;
+        }
+        uint16_t* to = P + (int64_t)row * ldp + m + 16 * i + 4 * g;
+#pragma unroll
+        for (int t = 0; t < PL; t++) {
+          uint16_t x[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if constexpr (DT == TMS_DTYPE_F16) {
+              x[e] = __builtin_bit_cast(uint16_t, (_Float16)p[e]);
+            } else {
+              const __bf16 b = (__bf16)p[e];
+              x[e] = __builtin_bit_cast(uint16_t, b);
+              if constexpr (PL > 1) p[e] -= (float)b;
+            }
+          }
+          *(u32x2*)(to + t * plane) = u32x2{(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
+        }
+      }
+    }
+  }
+};
+
+// Sums of dH: [split][row][d], added to from the second piece on.
+struct SumEpilogue {
+  float* out;
+  int64_t split;  // elements of one
+  int32_t rows, d;
+  int32_t first;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int s) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int row = n + 16 * j + c;
+      if (row >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+        const int col = m + 16 * i + 4 * g;
+        if (col >= d) continue;
+        f32x4* to = (f32x4*)(out + s * split + (int64_t)row * d + col);
+        f32x4 v = acc[i][j];
+        if (!first) {
+          const f32x4 old = *to;
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] += old[e];
+        }
+        *to = v;
+      }
+    }
+  }
+};
+
+template <int OUT>
+__device__ __forceinline__ uint16_t to16(float x) {
+  if constexpr (OUT == TMS_DTYPE_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
+  return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+
+// dW of one piece, finished: times *factor, in the inputs' type.
+template <int OUT>
+struct WeightEpilogue {
+  void* out;  // the piece's first row
+  const float* factor;
+  int32_t rows, d;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const float f = *factor;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int row = n + 16 * j + c;
+      if (row >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+        const int col = m + 16 * i + 4 * g;
+        if (col >= d) continue;
+        const int64_t at = (int64_t)row * d + col;
+        if constexpr (OUT == TMS_DTYPE_F32) {
+          float* to = (float*)out + at;
+          if ((d & 3) == 0) *(f32x4*)to = f32x4{acc[i][j][0] * f, acc[i][j][1] * f, acc[i][j][2] * f, acc[i][j][3] * f};
+          else
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (col + e < d) to[e] = acc[i][j][e] * f;
+        } else {
+          uint16_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[e] = to16<OUT>(acc[i][j][e] * f);
+          uint16_t* to = (uint16_t*)out + at;
+          if ((d & 3) == 0) *(u32x2*)to = u32x2{(uint32_t)w[0] | (uint32_t)w[1] << 16, (uint32_t)w[2] | (uint32_t)w[3] << 16};
+          else
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (col + e < d) to[e] = w[e];
+        }
+      }
+    }
+  }
+};
+
+// ---------------------------------------------------------------- rows
+
+__device__ __forceinline__ float element(const void* p, int64_t i, int dt) {
+  if (dt == TMS_DTYPE_F32) return ((const float*)p)[i];
+  if (dt == TMS_DTYPE_F16) return (float)((const _Float16*)p)[i];
+  return (float)((const __bf16*)p)[i];
+}
+
+// Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms. With
+// `ref`, rows without a gradient become zeros: what stands in them (NaN included) takes no part.
+__global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, int dt, uint16_t* dst, int64_t rows, int32_t d, int32_t dp,
+                                                        int64_t plane, const float* ref) {
+  const int64_t n = rows * dp;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int64_t row = k / dp;
+    const int c = (int)(k - row * dp);
+    const bool on = c < d && (!ref || ref[row] != __builtin_inff());
+    float x = on ? element(src, row * d + c, dt) : 0.f;
+    if (dt == TMS_DTYPE_F16) {
+      dst[k] = to16<TMS_DTYPE_F16>(x);
+    } else if (dt == TMS_DTYPE_BF16) {
+      dst[k] = to16<TMS_DTYPE_BF16>(x);
+    } else {
+#pragma unroll
+      for (int p = 0; p < 3; p++) {
+        const __bf16 t = (__bf16)x;
+        dst[p * plane + k] = __builtin_bit_cast(uint16_t, t);
+        x -= (float)t;
+      }
+    }
+  }
+}
+
+// Joins a row's blocks; 16 rows a workgroup, 16 lanes a row, which also form the target's
+// logit from the inputs. A target outside the vocabulary (and not ignored) makes the row NaN.
+__global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int32_t blocks, int32_t rows, const void* H, const void* W,
+                                                       int dt, int32_t V, int32_t d, const int64_t* target, int64_t ignore, float s2,
+                                                       float* lse2, float* loss) {
+  const int lane = threadIdx.x & 15, row = blockIdx.x * 16 + (threadIdx.x >> 4);
+  if (row >= rows) return;  // the 16 lanes of a row together
+  float top = -__builtin_inff(), sum = 0.f;
+  for (int b = lane; b < blocks; b += 16) {
+    const RowStat s = parts[(int64_t)b * rows + row];
+    const float t = fmaxf(top, s.top), ref = t == -__builtin_inff() ? 0.f : t;
+    sum = sum * __builtin_amdgcn_exp2f(top - ref) + s.sum * __builtin_amdgcn_exp2f(s.top - ref);
+    top = t;
+  }
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) {
+    const float t2 = __shfl_xor(top, o), u2 = __shfl_xor(sum, o);
+    const float t = fmaxf(top, t2), ref = t == -__builtin_inff() ? 0.f : t;
+    sum = sum * __builtin_amdgcn_exp2f(top - ref) + u2 * __builtin_amdgcn_exp2f(t2 - ref);
+    top = t;
+  }
+  float lse = top + log2f(sum);
+  const int64_t t = target[row];
+  const bool kept = t != ignore, fine = t >= 0 && t < V;
+  float dot = 0.f;
+  if (kept && fine)
+    for (int k = lane; k < d; k += 16) dot += element(H, (int64_t)row * d + k, dt) * element(W, t * d + k, dt);
+#pragma unroll
+  for (int o = 8; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
+  if (kept && !fine) lse = __builtin_nanf("");
+  if (lane == 0) {
+    lse2[row] = lse;
+    loss[row] = kept ? (lse - dot * s2) * kLn2 : 0.f;
+  }
+}
+
+// The sum or mean of the rows' losses, and how many rows count.
+__global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* rows_loss, const int64_t* target, int64_t ignore, int32_t rows,
+                                                          int mean, float* loss, float* count) {
+  __shared__ double sums[16];
+  __shared__ int counts[16];
+  double s = 0;
+  int c = 0;
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    s += (double)rows_loss[i];
+    c += target[i] != ignore;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    s += __shfl_xor(s, o);
+    c += __shfl_xor(c, o);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    sums[threadIdx.x >> 6] = s;
+    counts[threadIdx.x >> 6] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 16; w++) {
+      s += sums[w];
+      c += counts[w];
+    }
+    *count = (float)c;
+    *loss = mean ? (float)(s / (double)c) : (float)s;
+  }
+}
+
+// What the backward kernels take for each row: g / u, its reference for exp2 and its target;
+// and u with the factor of both gradients' sums.
+__global__ __launch_bounds__(1024) void lce_rows_kernel(const float* lse2, const int64_t* target, int64_t ignore, int32_t V, int32_t rows,
+                                                        const float* grad, int per_row, const float* count, float up, float scale,
+                                                        float* g, float* ref, int32_t* hit, float* factor) {
+  __shared__ float tops[16];
+  float unit = 1.f;
+  if (per_row) {
+    float top = 0.f;
+    for (int i = threadIdx.x; i < rows; i += 1024)
+      if (target[i] != ignore) top = fmaxf(top, fabsf(grad[i]));
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    for (int w = 0; w < 16; w++) top = fmaxf(top, tops[w]);
+    int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 0xffu) + 1;  // 2^(e - 127) > top
+    e = top == 0.f || e > 252 ? 127 : e < 2 ? 2 : e;  // an infinite factor stays as it is
+    unit = __builtin_bit_cast(float, (uint32_t)e << 23);
+  } else {
+    const float all = *grad / (count ? *count : 1.f);
+    if (all != 0.f && fabsf(all) < 1e38f) unit = all;
+  }
+  if (threadIdx.x == 0) *factor = unit * scale * exp2f(-up);
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const int64_t t = target[i];
+    const bool kept = t != ignore;
+    g[i] = !kept ? 0.f : (per_row ? grad[i] : *grad / (count ? *count : 1.f)) / unit;
+    ref[i] = kept ? lse2[i] - up : __builtin_inff();
+    hit[i] = kept && t >= 0 && t < V ? (int32_t)t : -1;
+  }
+}
+
+// dH: the splits' sums, times the factor, in the inputs' type.
+template <int OUT>
+__global__ __launch_bounds__(256) void lce_hidden_kernel(const float* sums, int splits, int64_t split, int32_t rows, int32_t d, int32_t dp,
+                                                         const float* factor, void* dH) {
+  const int64_t n = (int64_t)rows * d;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int64_t row = k / d, at = row * dp + (k - row * d);
+    float x = 0.f;
+    for (int s = 0; s < splits; s++) x += sums[s * split + at];
+    x *= *factor;
+    if constexpr (OUT == TMS_DTYPE_F32) ((float*)dH)[k] = x;
+    else ((uint16_t*)dH)[k] = to16<OUT>(x);
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+static int64_t up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
+static int planes(int dtype) { return dtype == TMS_DTYPE_F32 ? 3 : 1; }
+static bool as_is(const void* p, int64_t d, int dtype) { return dtype != TMS_DTYPE_F32 && d % 8 == 0 && (uintptr_t)p % 16 == 0; }
+static unsigned blocks_for(int64_t n) { return (unsigned)(n > 256 * 16384 ? 16384 : n > 0 ? (n + 255) / 256 : 1); }
+
+// Rows up to which the tiles hold 64 of them (the fewest that four waves side by side take).
+constexpr int kFewRows = 64;
+
+// How the backward pass goes over the vocabulary.
+struct LcePlan {
+  int64_t rows_p;  // rows of P: N up to a multiple of 256 (of 64 for few rows)
+  int64_t piece;   // columns of P, a multiple of 256
+  int splits;      // of the vocabulary in dH's product
+  int64_t dp;
+};
+
+// A piece of P takes up to 2^28 elements (512 MB in 16 bits, of 288 GB; 256 MB of it would
+// stay in the last cache, and reading the rest is far below the products' time). Among the
+// sizes within that, the one whose dW tiles (256 x 256, one a CU) leave the fewest CUs idle
+// over all pieces, the larger of equal ones.
+static LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int dtype) {
+  LcePlan p;
+  p.dp = up_to(d > 0 ? d : 8, 8);
+  p.rows_p = N <= kFewRows ? kFewRows : up_to(N, 256);
+  const int64_t all = up_to(V, 256) / 256, dt = (p.dp + 255) / 256;
+  int64_t most = ((int64_t)1 << 28) / planes(dtype) / p.rows_p / 256;
+  most = most < 1 ? 1 : most > all ? all : most;
+  int64_t best = most, fewest = INT64_MAX;
+  for (int64_t t = most; t >= 1 && t * 4 >= most; t--) {
+    const int64_t whole = all / t, rest = all - whole * t;
+    const int64_t rounds = whole * ((t * dt + 255) / 256) + (rest ? (rest * dt + 255) / 256 : 0);
+    if (rounds < fewest) fewest = rounds, best = t;
+  }
+  p.piece = best * 256;
+  // dH's tiles are few: split the piece so that they fill the chip, as long as a split's sums
+  // (read and written once a piece) cost less than the idle CUs would. Times in microseconds
+  // of a 64-step of a 256 x 256 tile (1.8) and of a megabyte of sums (0.25).
+  const int64_t tiles = dt * (N <= kFewRows ? 1 : p.rows_p / 256), steps = p.piece / 64;
+  const double mb = (double)N * (double)p.dp * 8e-6;
+  double least = 1e30;
+  p.splits = 1;
+  for (int64_t s = 1; s <= 64 && s * 4 <= steps; s++) {
+    const double us = (double)((tiles * s + 255) / 256) * (double)((steps + s - 1) / s) * 1.8 + (double)s * mb * 0.25;
+    if (us < least) least = us, p.splits = (int)s;
+  }
+  return p;
+}
+
+// Workspaces, as offsets into one buffer.
+struct Carve {
+  int64_t at = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t a = at;
+    at += up_to(bytes, 256);
+    return a;
+  }
+};
+struct LceSpace {
+  int64_t h, w, parts, loss, g, ref, hit, factor, p, sums, bytes;
+};
+static LceSpace lce_space(int64_t N, int64_t V, int64_t d, int dtype, bool backward, bool terms) {
+  LceSpace s = {};
+  Carve c;
+  const int64_t dp = up_to(d > 0 ? d : 8, 8);
+  if (terms || backward) s.h = c.take(N * dp * 2 * planes(dtype));
+  if (terms) s.w = c.take(V * dp * 2 * planes(dtype));
+  if (!backward) {
+    s.parts = c.take((V + 63) / 64 * N * (int64_t)sizeof(RowStat));
+    s.loss = c.take(N * 4);
+  } else {
+    const LcePlan p = lce_plan(N, V, d, dtype);
+    s.g = c.take(N * 4);
+    s.ref = c.take(N * 4);
+    s.hit = c.take(N * 4);
+    s.factor = c.take(4);
+    s.p = c.take(p.rows_p * p.piece * 2 * planes(dtype));
+    s.sums = c.take(p.splits * N * dp * 4);
+  }
+  s.bytes = c.at;
+  return s;
+}
+
+static int check_lce(const char* fn, int64_t N, int64_t d, int64_t V, int dtype, const double* scale, int reduction) {
+  if (N < 0 || d < 0 || V < 0) return fail(TMS_ERR_INVALID, "%s: negative size", fn);
+  if (dtype != TMS_DTYPE_F16 && dtype != TMS_DTYPE_BF16 && dtype != TMS_DTYPE_F32)
+    return fail(TMS_ERR_UNSUPPORTED, "%s: dtype must be fp16, bf16 or fp32", fn);
+  if (reduction != TMS_REDUCE_NONE && reduction != TMS_REDUCE_SUM && reduction != TMS_REDUCE_MEAN)
+    return fail(TMS_ERR_INVALID, "%s: unknown reduction %d", fn, reduction);
+  if (!scale || !(*scale > 0) || !(*scale < 1e30)) return fail(TMS_ERR_INVALID, "%s: scale must be positive and finite", fn);
+  if (V == 0 && N > 0) return fail(TMS_ERR_INVALID, "%s: an empty vocabulary", fn);
+  if (d > 65536 || N > (1 << 24) || V > (1 << 28)) return fail(TMS_ERR_UNSUPPORTED, "%s: sizes up to d = 65536, N = 2^24, V = 2^28", fn);
+  return TMS_OK;
+}
+
+static int run_terms(const void* src, int dtype, void* dst, int64_t rows, int64_t d, int64_t dp, const float* ref, hipStream_t st) {
+  const int64_t n = rows * dp;
+  hipLaunchKernelGGL(lce_terms_kernel, dim3(blocks_for(n)), dim3(256), 0, st, src, dtype, (uint16_t*)dst, rows, (int32_t)d, (int32_t)dp,
+                     n, ref);
+  return check_launch("lce_terms_kernel");
+}
+
+// The logits' product: m over vocabulary rows, n over hidden rows.
+static GemmArgs logits_args(const void* H, const void* W, int64_t N, int64_t V, int64_t Vall, int64_t dp, int dtype) {
+  GemmArgs a = {};
+  a.A = (const uint16_t*)W;
+  a.B = (const uint16_t*)H;
+  a.aplane = Vall * dp;
+  a.bplane = N * dp;
+  a.lda = a.ldb = (int32_t)dp;
+  a.M = (int32_t)V;
+  a.N = (int32_t)N;
+  a.K = (int32_t)dp;
+  a.pairs = dtype == TMS_DTYPE_F32 ? kTermPairs : 1;
+  a.splits = 1;
+  return a;
+}
+
+template <int DT, class Epi>
+static int run_logits(const GemmArgs& a, const Epi& epi, hipStream_t st, const char* what) {
+  if (a.N <= kFewRows) return run_gemm<DT, 4, 1, false, false>(a, epi, st, what);
+  return run_gemm<DT, 8, 4, false, false>(a, epi, st, what);
+}
+
+template <int DT>  // the type of the terms: fp32 inputs have bf16 ones
+static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
+                       float s2, int reduction, uint8_t* ws, const LceSpace& s, bool terms, float* loss, float* stats, hipStream_t st) {
+  const int64_t dp = up_to(d > 0 ? d : 8, 8);
+  const void *h = H, *w = W;
+  int rc;
+  if (terms) {
+    h = ws + s.h;
+    w = ws + s.w;
+    if ((rc = run_terms(H, dtype, ws + s.h, N, d, dp, nullptr, st))) return rc;
+    if ((rc = run_terms(W, dtype, ws + s.w, V, d, dp, nullptr, st))) return rc;
+  }
+  const GemmArgs a = logits_args(h, w, N, V, V, dp, dtype);
+  LseEpilogue e = {(RowStat*)(ws + s.parts), (int32_t)N, (int32_t)V, s2};
+  if ((rc = run_logits<DT>(a, e, st, "train_gemm_kernel (lse)"))) return rc;
+  const int wide = N <= kFewRows ? 64 : 128;
+  float* rows = reduction == TMS_REDUCE_NONE ? loss : (float*)(ws + s.loss);
+  // blocks past the vocabulary inside the last tile hold no row's sum: (-inf, 0) or nothing written
+  hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, (const RowStat*)(ws + s.parts),
+                     (int32_t)((V + wide - 1) / wide), (int32_t)N, H, W, dtype, (int32_t)V, (int32_t)d, target, ignore, s2, stats, rows);
+  return check_launch("lce_join_kernel");
+}
+
+template <int DT, int PL, int OUT>
+static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
+                        float scale, int reduction, const float* stats, const float* grad, uint8_t* ws, const LceSpace& s, bool terms,
+                        void* dH, void* dW, hipStream_t st) {
+  const LcePlan p = lce_plan(N, V, d, dtype);
+  const float up = DT == TMS_DTYPE_F16 ? (float)kP16 : 0.f;
+  float *g = (float*)(ws + s.g), *ref = (float*)(ws + s.ref), *factor = (float*)(ws + s.factor), *sums = (float*)(ws + s.sums);
+  int32_t* hit = (int32_t*)(ws + s.hit);
+  uint16_t *h = (uint16_t*)(ws + s.h), *P = (uint16_t*)(ws + s.p);
+  const void* w = terms ? ws + s.w : W;
+  int rc;
+  hipLaunchKernelGGL(lce_rows_kernel, dim3(1), dim3(1024), 0, st, stats, target, ignore, (int32_t)V, (int32_t)N, grad,
+                     reduction == TMS_REDUCE_NONE ? 1 : 0, reduction == TMS_REDUCE_MEAN ? stats + N : nullptr, up, scale, g, ref, hit, factor);
+  if ((rc = check_launch("lce_rows_kernel"))) return rc;
+  if ((rc = run_terms(H, dtype, h, N, d, p.dp, ref, st))) return rc;
+  if (terms && (rc = run_terms(W, dtype, ws + s.w, V, d, p.dp, nullptr, st))) return rc;
+  const int64_t pplane = p.rows_p * p.piece;
+  for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+    const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
+    GemmArgs a = logits_args(h, (const uint16_t*)w + v0 * p.dp, N, nv, V, p.dp, dtype);
+    ProbEpilogue<DT, PL> e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e};
+    if ((rc = run_logits<DT>(a, e, st, "train_gemm_kernel (P)"))) return rc;
+    if (dH && d > 0) {  // m over d, n over rows, k over the piece
+      GemmArgs b = {};
+      b.A = (const uint16_t*)w + v0 * p.dp;
+      b.B = P;
+      b.aplane = V * p.dp;
+      b.bplane = pplane;
+      b.lda = (int32_t)p.dp;
+      b.ldb = (int32_t)p.piece;
+      b.M = (int32_t)p.dp;
+      b.N = (int32_t)N;
+      b.K = (int32_t)nv;
+      b.pairs = PL == 3 ? kTermPairs : 1;
+      b.splits = p.splits;
+      SumEpilogue se = {sums, N * p.dp, (int32_t)N, (int32_t)p.dp, v0 == 0};
+      if (N <= kFewRows) rc = run_gemm<DT, 4, 1, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      else if (p.dp <= 128) rc = run_gemm<DT, 4, 4, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      else rc = run_gemm<DT, 8, 4, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      if (rc) return rc;
+    }
+    if (dW && d > 0) {  // m over d, n over the piece, k over rows
+      GemmArgs b = {};
+      b.A = h;
+      b.B = P;
+      b.aplane = N * p.dp;
+      b.bplane = pplane;
+      b.lda = (int32_t)p.dp;
+      b.ldb = (int32_t)p.piece;
+      b.M = (int32_t)p.dp;
+      b.N = (int32_t)up_to(nv, 8);
+      b.K = (int32_t)N;
+      b.pairs = PL == 3 ? kTermPairs : 1;
+      b.splits = 1;
+      WeightEpilogue<OUT> we = {(uint8_t*)dW + v0 * d * (OUT == TMS_DTYPE_F32 ? 4 : 2), factor, (int32_t)nv, (int32_t)d};
+      if (p.dp <= 128) rc = run_gemm<DT, 4, 4, true, true>(b, we, st, "train_gemm_kernel (dW)");
+      else rc = run_gemm<DT, 8, 4, true, true>(b, we, st, "train_gemm_kernel (dW)");
+      if (rc) return rc;
+    }
+  }
+  if (dH && d > 0) {
+    hipLaunchKernelGGL(lce_hidden_kernel<OUT>, dim3(blocks_for(N * d)), dim3(256), 0, st, sums, p.splits, N * p.dp, (int32_t)N, (int32_t)d,
+                       (int32_t)p.dp, factor, dH);
+    return check_launch("lce_hidden_kernel");
+  }
+  return TMS_OK;
+}
+
+}  // namespace tms
+
+using namespace tms;
+
+extern "C" int64_t tms_lce_workspace_size(int64_t N, int64_t d, int64_t V, int dtype, int backward) {
+  if (N <= 0 || d < 0 || V <= 0) return 0;
+  return lce_space(N, V, d, dtype, backward != 0, dtype == TMS_DTYPE_F32 || d % 8 != 0 || d == 0).bytes;
+}
+
+static int lce_workspace(const char* fn, const void* H, const void* W, int64_t N, int64_t d, int64_t V, int dtype, bool backward,
+                         const void* ws, int64_t bytes, bool& terms, LceSpace& s) {
+  terms = dtype == TMS_DTYPE_F32 || d % 8 != 0 || d == 0;
+  if (!terms && !(as_is(H, d, dtype) && as_is(W, d, dtype))) return fail(TMS_ERR_INVALID, "%s: hidden and weight must be 16-byte aligned", fn);
+  s = lce_space(N, V, d, dtype, backward, terms);
+  if (!ws || (uintptr_t)ws % 256 || bytes < s.bytes)
+    return fail(TMS_ERR_INVALID, "%s: a workspace of %lld bytes is needed, 256-byte aligned", fn, (long long)s.bytes);
+  return TMS_OK;
+}
+
+extern "C" int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d, const void* weight, int64_t V, int dtype,
+                                        const int64_t* target, int64_t ignore_index, const double* scale, int reduction, void* workspace,
+                                        int64_t workspace_bytes, float* loss, float* stats, void* stream) {
+  const char* fn = "tms_linear_cross_entropy";
+  int rc = check_lce(fn, N, d, V, dtype, scale, reduction);
+  if (rc) return rc;
+  if ((!loss && (N > 0 || reduction != TMS_REDUCE_NONE)) || !stats || (N > 0 && (!target || (d > 0 && (!hidden || !weight)))))
+    return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  const hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = (uint8_t*)workspace;
+  LceSpace s = {};
+  bool terms = false;
+  if (N > 0) {
+    if ((rc = lce_workspace(fn, hidden, weight, N, d, V, dtype, false, ws, workspace_bytes, terms, s))) return rc;
+    const float s2 = (float)(*scale * 1.4426950408889634);
+    if (dtype == TMS_DTYPE_F16) rc = lce_forward<TMS_DTYPE_F16>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
+    else rc = lce_forward<TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
+    if (rc) return rc;
+  }
+  if (reduction == TMS_REDUCE_NONE) return TMS_OK;
+  hipLaunchKernelGGL(lce_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)(ws + s.loss), target, ignore_index, (int32_t)N,
+                     reduction == TMS_REDUCE_MEAN ? 1 : 0, loss, stats + N);
+  return check_launch("lce_reduce_kernel");
+}
+
+extern "C" int tms_linear_cross_entropy_grad(const void* hidden, int64_t N, int64_t d, const void* weight, int64_t V, int dtype,
+                                             const int64_t* target, int64_t ignore_index, const double* scale, int reduction,
+                                             const float* stats, const float* grad, void* workspace, int64_t workspace_bytes, void* dH,
+                                             void* dW, void* stream) {
+  const char* fn = "tms_linear_cross_entropy_grad";
+  int rc = check_lce(fn, N, d, V, dtype, scale, reduction);
+  if (rc) return rc;
+  if (N == 0 || (!dH && !dW)) return TMS_OK;  // no rows: the caller's zeros
+  if (!target || !stats || !grad || (d > 0 && (!hidden || !weight))) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  LceSpace s = {};
+  bool terms = false;
+  if ((rc = lce_workspace(fn, hidden, weight, N, d, V, dtype, true, workspace, workspace_bytes, terms, s))) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = (uint8_t*)workspace;
+  const float sc = (float)*scale;
+  if (dtype == TMS_DTYPE_F16)
+    return lce_backward<TMS_DTYPE_F16, 1, TMS_DTYPE_F16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
+  if (dtype == TMS_DTYPE_BF16)
+    return lce_backward<TMS_DTYPE_BF16, 1, TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
+  return lce_backward<TMS_DTYPE_BF16, 3, TMS_DTYPE_F32>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
+}
