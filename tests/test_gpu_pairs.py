@@ -114,6 +114,15 @@ def test_shared(cuda, nQ, Nq, B, Nd, d, dtype):
     check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
 
 
+# many queries and documents: the gradients' forms that share documents, whose tokens come in
+# one stage or several, in 16-byte pieces or (odd widths) element by element
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("nQ,Nq,B,Nd,d", [(8, 32, 70, 270, 40), (16, 20, 65, 30, 77), (9, 33, 64, 17, 136), (12, 32, 100, 130, 33),
+                                          (20, 3, 300, 65, 160)])
+def test_many(cuda, nQ, Nq, B, Nd, d, dtype):
+    check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
+
+
 def test_no_masks(cuda):
     check(5, 32, 500, 47, 128, "fp16", masks=False)
     check(2, 20, 6, 100, 128, "bf16", masks=False)

@@ -68,6 +68,11 @@ __device__ __forceinline__ Best across_rows(Best r) {
   return better({__builtin_bit_cast(float, (unsigned)v1[0]), (int)i1[0]}, {__builtin_bit_cast(float, (unsigned)v1[1]), (int)i1[1]});
 }
 
+template <bool V>
+struct Flag {
+  static constexpr bool value = V;
+};
+
 // Values of masked tokens never win: bit t of `live` is token base + t of the tile.
 __device__ __forceinline__ void mask_tile(f32x4& s, uint32_t live, int g) {
 #pragma unroll
@@ -146,7 +151,7 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
       }
 #pragma unroll
       for (int h = 0; h < 2; h++) {
-        if (bits != 0xffffu) mask_tile(acc[h], bits, g);
+        mask_tile(acc[h], bits, g);  // not behind a branch, for one would follow an MFMA
         take(best[h], acc[h], t * 16 + 4 * g);
       }
     }
@@ -281,18 +286,23 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
       for (int p = 0; p < PL; p++)
 #pragma unroll
         for (int s = 0; s < KS; s++) df[p][s] = ring[buf][(tile * PL + p) * KS + s][lane];
+      // one body for whole tiles and one for masked ones: no branch behind an MFMA
+      auto score = [&](auto masked) {
 #pragma unroll
-      for (int j = 0; j < NB; j++)
+        for (int j = 0; j < NB; j++)
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
-          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+          for (int h = 0; h < 2; h++) {
+            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int p = PL == 1 ? 5 : 0; p < 6; p++)
+            for (int p = PL == 1 ? 5 : 0; p < 6; p++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) acc = mfma16x16x32<DT>(df[kPairD[p]][s], qf[j][kPairQ[p]][s][h], acc);
-          if (bits != 0xffffu) mask_tile(acc, bits, g);
-          take(best[j][h], acc, t0 + tile * 16 + 4 * g);
-        }
+              for (int s = 0; s < KS; s++) acc = mfma16x16x32<DT>(df[kPairD[p]][s], qf[j][kPairQ[p]][s][h], acc);
+            if constexpr (decltype(masked)::value) mask_tile(acc, bits, g);
+            take(best[j][h], acc, t0 + tile * 16 + 4 * g);
+          }
+      };
+      if (bits == 0xffffu) score(Flag<false>());
+      else score(Flag<true>());
     }
     const int after = nxt < total ? seek(nxt + 1) : total;
     if (nxt >= total || nxt / stages != doc) {  // the document's end
@@ -384,104 +394,372 @@ struct El<TMS_DTYPE_F32> {
 struct PairsGradArgs {
   const void* Q;
   const void* D;
+  const uint8_t* qmask;
   const uint16_t* arg;
   const float* G;  // (nQ, B) or (nQ, nway)
   void* dQ;
   void* dD;
+  u32x4* frags;  // [plane][block of 32 query tokens][16 columns][lane]
   float* parts;  // [split][nQ * nq][d]
   int64_t B;
   int32_t nQ, nq, nqp, nd, d, nway;
-  int32_t rows;            // dD: document tokens whose sums a workgroup keeps
-  int32_t splits, chunk;   // dQ: splits of the documents, documents each
+  int32_t nbq, blocks, cts;       // blocks a query, blocks in all, column tiles
+  int32_t splits, chunk, tokens;  // dQ: splits of the documents, documents each; document tokens per LDS stage
 };
 
-// dD: one wave keeps 64 columns of a document's gradient in LDS, a column a lane, and adds
-// every maximum's query token to the row that won it. Only the column's own lane touches a
-// sum, in the order of the queries, so that the result does not depend on timing. Positions
-// and G come through the scalar unit, eight maxima at a time; the query rows are read ahead.
+__device__ __forceinline__ float grad_of(const PairsGradArgs& a, int q, int64_t b) {
+  return a.G[a.nway ? b : (int64_t)q * a.B + b];
+}
+
+// Queries as MFMA operands with the block's 32 tokens inside: lane (c, g) holds column
+// 16 ct + c of tokens 8 g .. 8 g + 7. Masked tokens and what lies past the ends are zero.
 template <int DT>
-__global__ __launch_bounds__(64) void pairs_grad_d_kernel(PairsGradArgs a) {
-  extern __shared__ float sums[];  // [rows + 1][64]: the last row takes what is not ours
+__global__ __launch_bounds__(256) void pairs_frags_kernel(PairsGradArgs a) {
   typedef typename El<DT>::T T;
-  const int lane = threadIdx.x;
-  const int64_t b = blockIdx.x;
-  const int col = (int)blockIdx.y * 64 + lane, t0 = (int)blockIdx.z * a.rows;
-  const int rows = t0 + a.rows < a.nd ? a.rows : a.nd - t0;
-  for (int i = 0; i <= rows; i++) sums[i * 64 + lane] = 0.f;
-  const bool in = col < a.d;
-  const int qa = a.nway ? (int)(b / a.nway) : 0, qn = a.nqp == 0 ? 0 : a.nway ? 1 : a.nQ;
-  const uint16_t* arg = a.arg + (a.nway ? b : b * a.nQ) * a.nqp;
-  const T* Q = (const T*)a.Q + (int64_t)qa * a.nq * a.d + (in ? col : 0);
-  for (int q = 0; q < qn; q++) {
-    const float w = a.G[a.nway ? b : (int64_t)(qa + q) * a.B + b];
-    for (int i = 0; i < a.nqp; i += 8) {
-      const u32x4 at = *(const u32x4*)(arg + (int64_t)q * a.nqp + i);  // nqp is a multiple of 8
-      float x[8];
+  constexpr int PL = DT == TMS_DTYPE_F32 ? 3 : 1;
+  const int64_t n = (int64_t)a.blocks * a.cts * 64;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int lane = (int)(k & 63), c = lane & 15, g = lane >> 4;
+    const int64_t f = k >> 6;
+    const int kb = (int)(f / a.cts), col = (int)(f - (int64_t)kb * a.cts) * 16 + c;
+    const int q = kb / a.nbq, i0 = (kb - q * a.nbq) * 32 + 8 * g;
+    uint16_t v[PL][8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        const int tok = i + k < a.nq ? i + k : a.nq - 1;
-        x[k] = (float)Q[((int64_t)q * a.nq + tok) * a.d];
-      }
+    for (int e = 0; e < 8; e++) {
+      const int64_t row = (int64_t)q * a.nq + i0 + e;
+      const bool on = i0 + e < a.nq && col < a.d && (!a.qmask || a.qmask[row] != 0);
+      if constexpr (PL == 1) {
+        v[0][e] = on ? ((const uint16_t*)a.Q)[row * a.d + col] : (uint16_t)0;
+      } else {
+        float x = on ? ((const float*)a.Q)[row * a.d + col] : 0.f;
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        uint32_t j = (at[k / 2] >> (16 * (k & 1))) & 0xffffu;
-        j = __builtin_amdgcn_readfirstlane(j) - (uint32_t)t0;
-        j = j < (uint32_t)rows ? j : (uint32_t)rows;  // kNone is beyond every document
-        __hip_atomic_fetch_add(&sums[j * 64 + lane], w * x[k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WAVEFRONT);
+        for (int p = 0; p < 3; p++) {
+          const __bf16 t = (__bf16)x;
+          v[p][e] = __builtin_bit_cast(uint16_t, t);
+          x -= (float)t;
+        }
       }
     }
-  }
-  if (in) {
-    T* out = (T*)a.dD + ((int64_t)b * a.nd + t0) * a.d + col;
-    for (int i = 0; i < rows; i++) out[(int64_t)i * a.d] = (T)sums[i * 64 + lane];
+#pragma unroll
+    for (int p = 0; p < PL; p++) {
+      u32x4 w;
+#pragma unroll
+      for (int e = 0; e < 4; e++) w[e] = (uint32_t)v[p][2 * e] | (uint32_t)v[p][2 * e + 1] << 16;
+      a.frags[p * n + k] = w;
+    }
   }
 }
 
-// dQ: a wave takes eight query tokens and 128 columns (two a lane) over a run of documents,
-// and adds the token that each document answered with. Runs are a power of two to the XCDs,
-// so that the waves of an XCD walk the same documents and find their rows in its L2.
+// Elements that are 1 where the position equals this lane's token (both halves of t2), else 0.
 template <int DT>
-__global__ __launch_bounds__(64) void pairs_grad_q_kernel(PairsGradArgs a) {
+__device__ __forceinline__ u32x4 one_hot(u32x4 at, uint32_t t2) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  constexpr uint16_t ONE = DT == TMS_DTYPE_F16 ? 0x3c00 : 0x3f80;
+  u32x4 r;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    const uint32_t x = at[i] ^ t2;
+    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), u16x2{1, 1});
+    r[i] = __builtin_bit_cast(uint32_t, (u16x2)(u16x2{ONE, ONE} - m * u16x2{ONE, ONE}));
+  }
+  return r;
+}
+
+// dD as products: for a block of 32 query tokens, the matrix that is 1 where token i's
+// maximum is document token j, times the block, is the sum of the query tokens that j won,
+// exactly (each product is by 0 or 1); times the pair's G it is added to the document's sums
+// in fp32, block after block, so in one order. The ones are made in registers from the
+// positions. A workgroup has one document's up to 4 TT tiles of 16 tokens (a wave every
+// fourth) and 128 columns; the blocks' fragments pass through LDS, one barrier a block.
+// Adding a query's rows one by one in LDS instead was bound by the latency of their loads
+// at the three waves a CU whose sums fit it, 20 times as long at 64 queries x 4096
+// documents x 180 tokens. Bound by the VALU: a tile and block take 8 MFMAs of 16 cycles,
+// and 32 multiply-adds and 12 integer instructions of 4.
+//
+// All CT column tiles of 16 are computed, those past the width on zeros: with a branch between
+// an MFMA and the instruction that takes its result, this compiler leaves out the wait states
+// between the two, and the first of its four values is read before it is there.
+template <int DT, int TT, int CT, int PL>
+__global__ __launch_bounds__(256, TT * CT > 16 ? 2 : 3) void pairs_grad_d_kernel(PairsGradArgs a) {
+  constexpr int MT = PL == 3 ? TMS_DTYPE_BF16 : DT;
+  constexpr int LD = (CT + 3) / 4;  // column tiles a wave loads
+  __shared__ u32x4 ring[2][PL][4 * LD][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int c = lane & 15, g = lane >> 4;
+  const int64_t b = blockIdx.x;
+  const int ct0 = (int)blockIdx.y * CT, cts = a.cts - ct0;
+  const int tile0 = (int)blockIdx.z * 4 * TT + wave;  // and every fourth
+  const int first = a.nway ? (int)(b / a.nway) * a.nbq : 0, count = a.nway ? a.nbq : a.blocks;
+  const uint16_t* arg = a.arg + (a.nway ? b : b * a.nQ) * a.nqp + 8 * g;
+  const int64_t plane = (int64_t)a.blocks * a.cts * 64;
+
+  f32x4 acc[TT][CT];
+#pragma unroll
+  for (int t = 0; t < TT; t++)
+#pragma unroll
+    for (int k = 0; k < CT; k++) acc[t][k] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  u32x4 fr[PL][LD], at_next = {0u, 0u, 0u, 0u};
+  float w_next = 0.f;
+  auto load = [&](int k) {
+    const int kb = first + k;
+#pragma unroll
+    for (int p = 0; p < PL; p++)
+#pragma unroll
+      for (int i = 0; i < LD; i++) {
+        const int ct = wave * LD + i;
+        fr[p][i] = u32x4{0u, 0u, 0u, 0u};
+        if (ct < cts) fr[p][i] = a.frags[p * plane + ((int64_t)kb * a.cts + ct0 + ct) * 64 + lane];
+      }
+  };
+  auto load_at = [&](int k) {
+    at_next = *(const u32x4*)(arg + k * 32);
+    w_next = grad_of(a, (first + k) / a.nbq, b);
+  };
+  auto put = [&](int buf) {
+#pragma unroll
+    for (int p = 0; p < PL; p++)
+#pragma unroll
+      for (int i = 0; i < LD; i++) ring[buf][p][wave * LD + i][lane] = fr[p][i];
+  };
+  if (count > 0) {
+    load(0);
+    load_at(0);
+    put(0);
+    if (count > 1) load(1);
+  }
+  __syncthreads();
+  for (int k = 0; k < count; k++) {
+    const u32x4 at = at_next;
+    const float w = w_next;
+    if (k + 1 < count) load_at(k + 1);
+    const int buf = k & 1;
+#pragma unroll
+    for (int t = 0; t < TT; t++) {
+      const uint32_t tok = (uint32_t)(tile0 + 4 * t) * 16 + c;
+      const u32x4 hot = one_hot<MT>(at, tok | tok << 16);
+      if (__ballot((hot[0] | hot[1] | hot[2] | hot[3]) != 0u) == 0ull) continue;  // nothing won here
+#pragma unroll
+      for (int ct = 0; ct < CT; ct++) {
+        f32x4 r = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int p = PL - 1; p >= 0; p--) r = mfma16x16x32<MT>(ring[buf][p][ct][lane], hot, r);
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[t][ct][e] = __builtin_fmaf(w, r[e], acc[t][ct][e]);
+      }
+    }
+    if (k + 1 < count) put(buf ^ 1);
+    if (k + 2 < count) load(k + 2);
+    __syncthreads();
+  }
   typedef typename El<DT>::T T;
-  const int lane = threadIdx.x;
-  const int split = (int)(blockIdx.x % a.splits);
-  const int unit = (int)(blockIdx.x / a.splits);
-  const int groups = a.nqp / 8;
+  const bool four = a.d % 4 == 0;  // and then rows begin at multiples of four elements
+#pragma unroll
+  for (int t = 0; t < TT; t++) {
+    const int tok = (tile0 + 4 * t) * 16 + c;
+    if (tok >= a.nd) continue;
+    T* row = (T*)a.dD + ((int64_t)b * a.nd + tok) * a.d;
+#pragma unroll
+    for (int ct = 0; ct < CT; ct++) {
+      const int col = (ct0 + ct) * 16 + 4 * g;
+      if (col >= a.d) continue;
+      struct alignas(4 * sizeof(T)) Four {
+        T v[4];
+      } x;
+#pragma unroll
+      for (int e = 0; e < 4; e++) x.v[e] = (T)acc[t][ct][e];
+      if (four) *(Four*)(row + col) = x;
+      else
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (col + e < a.d) row[col + e] = x.v[e];
+    }
+  }
+}
+
+// Two neighbouring columns of a row, as floats.
+template <int DT>
+__device__ __forceinline__ f32x2 two(const uint8_t* p) {
+  if constexpr (DT == TMS_DTYPE_F32) {
+    return *(const f32x2*)p;
+  } else {
+    const uint32_t x = *(const uint32_t*)p;
+    if constexpr (DT == TMS_DTYPE_BF16) {
+      return f32x2{__builtin_bit_cast(float, x << 16), __builtin_bit_cast(float, x & 0xffff0000u)};
+    } else {
+      typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+      const f16x2 h = __builtin_bit_cast(f16x2, x);
+      return f32x2{(float)h[0], (float)h[1]};
+    }
+  }
+}
+
+// Where dQ's sums go: the gradient itself, or a split's part.
+template <int DT>
+__device__ __forceinline__ void put_q(const PairsGradArgs& a, int split, int64_t row, int col, float x0, float x1) {
+  typedef typename El<DT>::T T;
+  if (col >= a.d) return;
+  const int64_t at = row * a.d + col;
+  if (a.splits == 1) {
+    T* out = (T*)a.dQ + at;
+    out[0] = (T)x0;
+    if (col + 1 < a.d) out[1] = (T)x1;
+  } else {
+    float* out = a.parts + (int64_t)split * a.nQ * a.nq * a.d + at;
+    out[0] = x0;
+    if (col + 1 < a.d) out[1] = x1;
+  }
+}
+
+// dQ, many queries: sixteen waves, each with a block of 32 query tokens and 128 columns (two
+// a lane) in registers, walk the same run of documents. A document's tokens come to LDS
+// once for the 512 query tokens, while the one before is added up: each query token reads the
+// row that answered it, 256 bytes in one wave's access. Positions come through the scalar
+// unit; where there is none, a row of zeros and a factor of 0 stand in. The runs' sums are
+// joined by the kernel below, in order.
+template <int DT>
+__global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
+  constexpr int ES = DT == TMS_DTYPE_F32 ? 4 : 2, ROW = 128 * ES;
+  constexpr int LD = 4;  // 16-byte loads a thread and stage: 64 KB
+  extern __shared__ __attribute__((aligned(16))) uint8_t docs[];  // [2][tokens + 1][ROW]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int split = (int)(blockIdx.x % a.splits), group = (int)(blockIdx.x / a.splits);
+  const int kb = group * 16 + wave;
+  const bool mine = kb < a.blocks;
+  const int q = mine ? kb / a.nbq : 0;
+  const int col0 = (int)blockIdx.y * 128, cols = a.d - col0 < 128 ? a.d - col0 : 128;
+  const int64_t e0 = (int64_t)split * a.chunk, e1 = e0 + a.chunk < a.B ? e0 + a.chunk : a.B;
+  const int stages = (a.nd + a.tokens - 1) / a.tokens;
+  const int64_t items = e1 > e0 ? (e1 - e0) * stages : 0;
+  const int size = (a.tokens + 1) * ROW;
+  const bool whole = a.d % (16 / ES) == 0 && (uintptr_t)a.D % 16 == 0;  // rows in 16-byte pieces
+
+  for (int k = threadIdx.x; k < 2 * ROW / 4; k += 1024)  // the rows of zeros
+    *(uint32_t*)(docs + (k / (ROW / 4)) * size + a.tokens * ROW + (k % (ROW / 4)) * 4) = 0u;
+
+  u32x4 reg[LD];
+  auto load = [&](int64_t it) {
+    const int64_t b = e0 + it / stages;
+    const int t0 = (int)(it % stages) * a.tokens, n = a.nd - t0 < a.tokens ? a.nd - t0 : a.tokens;
+    const uint8_t* base = (const uint8_t*)a.D + (((int64_t)b * a.nd + t0) * a.d + col0) * ES;
+#pragma unroll
+    for (int i = 0; i < LD; i++) {
+      const int k = i * 1024 + (int)threadIdx.x, row = k / (ROW / 16), at = k % (ROW / 16);
+      if (row < n) {
+        if (whole) {
+          if (at * (16 / ES) < cols) reg[i] = *(const u32x4*)(base + (int64_t)row * a.d * ES + at * 16);
+        } else {
+          uint16_t h[8];
+#pragma unroll
+          for (int e = 0; e < 8; e++) {
+            const int col = at * (16 / ES) + e * 2 / ES;
+            h[e] = col < cols ? *(const uint16_t*)(base + (int64_t)row * a.d * ES + at * 16 + e * 2) : (uint16_t)0;
+          }
+          reg[i] = u32x4{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16};
+        }
+      }
+    }
+  };
+  auto put = [&](int64_t it, int buf) {
+    const int t0 = (int)(it % stages) * a.tokens, n = a.nd - t0 < a.tokens ? a.nd - t0 : a.tokens;
+#pragma unroll
+    for (int i = 0; i < LD; i++) {
+      const int k = i * 1024 + (int)threadIdx.x;
+      if (k / (ROW / 16) < n) *(u32x4*)(docs + buf * size + k * 16) = reg[i];
+    }
+  };
+
+  float acc[32][2] = {};
+  if (items > 0) {
+    load(0);
+    put(0, 0);
+    if (items > 1) load(1);
+  }
+  __syncthreads();
+  for (int64_t it = 0; it < items; it++) {
+    const int64_t b = e0 + it / stages;
+    const int t0 = (int)(it % stages) * a.tokens;
+    const int buf = (int)(it & 1);
+    if (mine) {
+      const float w = grad_of(a, q, b);
+      const uint32_t* at = (const uint32_t*)(a.arg + (b * a.nQ) * a.nqp + (int64_t)kb * 32);
+      const uint8_t* base = docs + buf * size + lane * 2 * ES;
+#pragma unroll
+      for (int i = 0; i < 32; i++) {
+        uint32_t j = ((at[i / 2] >> (16 * (i & 1))) & 0xffffu) - (uint32_t)t0;
+        const bool here = j < (uint32_t)a.tokens;  // kNone is beyond every stage
+        j = here ? j : (uint32_t)a.tokens;
+        const f32x2 x = two<DT>(base + j * ROW);
+        const float f = here ? w : 0.f;
+        acc[i][0] = __builtin_fmaf(f, x[0], acc[i][0]);
+        acc[i][1] = __builtin_fmaf(f, x[1], acc[i][1]);
+      }
+    }
+    if (it + 1 < items) put(it + 1, buf ^ 1);
+    if (it + 2 < items) load(it + 2);
+    __syncthreads();
+  }
+  if (!mine) return;
+  const int i0 = (kb - q * a.nbq) * 32;
+#pragma unroll
+  for (int i = 0; i < 32; i++)
+    if (i0 + i < a.nq) put_q<DT>(a, split, (int64_t)q * a.nq + i0 + i, col0 + 2 * lane, acc[i][0], acc[i][1]);
+}
+
+// dQ, few queries or documents of their own: eight waves share eight query tokens and 128
+// columns, take the documents in turn straight from memory, and join through LDS in order.
+template <int DT>
+__global__ __launch_bounds__(512) void pairs_grad_q_few_kernel(PairsGradArgs a) {
+  constexpr int ES = DT == TMS_DTYPE_F32 ? 4 : 2;
+  typedef typename El<DT>::T T;
+  __shared__ float sums[8][8][128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int split = (int)(blockIdx.x % a.splits), unit = (int)(blockIdx.x / a.splits);
+  const int groups = (a.nq + 7) / 8;
   const int q = unit / groups, i0 = (unit - q * groups) * 8;
   const int col = (int)blockIdx.y * 128 + 2 * lane;
-  const bool in0 = col < a.d, in1 = col + 1 < a.d;
   const int64_t first = a.nway ? (int64_t)q * a.nway : 0, n = a.nway ? a.nway : a.B;
   const int64_t e0 = (int64_t)split * a.chunk, e1 = e0 + a.chunk < n ? e0 + a.chunk : n;
+  const bool pair = a.d % 2 == 0 && (uintptr_t)a.D % (2 * ES) == 0;
   float acc[8][2] = {};
-  const T* D = (const T*)a.D;
-  for (int64_t k = e0; k < e1; k++) {
+  for (int64_t k = e0 + wave; k < e1; k += 8) {
     const int64_t b = first + k;
-    const float w = a.G[a.nway ? b : (int64_t)q * a.B + b];
-    const u32x4 at = *(const u32x4*)(a.arg + (a.nway ? b : b * a.nQ + q) * a.nqp + i0);
+    const float w = grad_of(a, q, b);
+    const uint32_t* at = (const uint32_t*)(a.arg + (a.nway ? b : b * a.nQ + q) * a.nqp + i0);
+    f32x2 x[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const uint32_t j = __builtin_amdgcn_readfirstlane((at[i / 2] >> (16 * (i & 1))) & 0xffffu);
-      if (j >= (uint32_t)a.nd) continue;  // kNone
-      const T* row = D + ((int64_t)b * a.nd + j) * a.d;
-      const float x0 = in0 ? (float)row[col] : 0.f, x1 = in1 ? (float)row[col + 1] : 0.f;
-      acc[i][0] += w * x0;
-      acc[i][1] += w * x1;
+      const uint32_t j = (at[i / 2] >> (16 * (i & 1))) & 0xffffu;
+      x[i] = f32x2{0.f, 0.f};
+      if (j < (uint32_t)a.nd && col < a.d) {  // kNone is beyond every document
+        const T* row = (const T*)a.D + ((int64_t)b * a.nd + j) * a.d + col;
+        if (pair) {
+          x[i] = two<DT>((const uint8_t*)row);
+        } else {
+          x[i][0] = (float)row[0];
+          x[i][1] = col + 1 < a.d ? (float)row[1] : 0.f;
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      const uint32_t j = (at[i / 2] >> (16 * (i & 1))) & 0xffffu;
+      const float f = j < (uint32_t)a.nd ? w : 0.f;
+      acc[i][0] = __builtin_fmaf(f, x[i][0], acc[i][0]);
+      acc[i][1] = __builtin_fmaf(f, x[i][1], acc[i][1]);
     }
   }
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    if (i0 + i >= a.nq) break;
-    const int64_t row = (int64_t)q * a.nq + i0 + i;
-    if (a.splits == 1) {
-      T* out = (T*)a.dQ + row * a.d + col;
-      if (in0) out[0] = (T)acc[i][0];
-      if (in1) out[1] = (T)acc[i][1];
-    } else {
-      float* out = a.parts + ((int64_t)split * a.nQ * a.nq + row) * a.d + col;
-      if (in0) out[0] = acc[i][0];
-      if (in1) out[1] = acc[i][1];
-    }
+  for (int i = 0; i < 8; i++) *(f32x2*)&sums[wave][i][2 * lane] = f32x2{acc[i][0], acc[i][1]};
+  __syncthreads();
+  if (i0 + wave >= a.nq) return;
+  f32x2 x = {0.f, 0.f};
+#pragma unroll
+  for (int v = 0; v < 8; v++) {
+    x[0] += sums[v][wave][2 * lane];
+    x[1] += sums[v][wave][2 * lane + 1];
   }
+  put_q<DT>(a, split, (int64_t)q * a.nq + i0 + wave, col, x[0], x[1]);
 }
 
 template <int DT>
@@ -496,8 +774,6 @@ __global__ __launch_bounds__(256) void pairs_grad_q_join_kernel(const float* par
 
 // ---------------------------------------------------------------- host
 
-constexpr int64_t kLdsBytes = 160 * 1024;
-
 static int64_t round_up(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 
 // Whether the forward kernels take these rows as they are.
@@ -506,14 +782,26 @@ static bool as_is(const void* p, int64_t d, int dtype) {
 }
 static int planes(int dtype) { return dtype == TMS_DTYPE_F32 ? 3 : 1; }
 
-// The splits of dQ's documents: enough waves for four on each SIMD's worth of the chip
-// (1,024 SIMDs), at least 16 documents each, a multiple of 8 where there are several.
-static int grad_q_splits(int64_t nQ, int64_t nqp, int64_t cols, int64_t n) {
-  const int64_t units = nQ * (nqp / 8) * cols;
-  int64_t s = units > 0 ? 4096 / units : 1;
-  if (s > n / 16) s = n / 16;
+// dQ's form and its splits of the documents. From 256 query tokens on (half of a workgroup's)
+// the form that shares documents; one workgroup a CU then. The other fills the chip twice
+// over, with at least eight documents (one a wave) a split. The sums of a split are written
+// and read once, so no more splits than fill the chip. A multiple of 8 where there are
+// several: workgroups go to the XCDs in turn, so an XCD then keeps to its own documents.
+struct GradQ {
+  bool shared;
+  int splits;
+};
+static GradQ grad_q_form(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway) {
+  const int64_t cols = (d + 127) / 128, blocks = nQ * ((nq + 31) / 32);
+  GradQ f;
+  f.shared = nway == 0 && blocks >= 8 && B >= 64;
+  const int64_t units = (f.shared ? (blocks + 15) / 16 : nQ * ((nq + 7) / 8)) * cols;
+  const int64_t most = f.shared ? B / 4 : (nway ? nway : B) / 8;
+  int64_t s = (f.shared ? 256 : 512) / (units > 0 ? units : 1);
+  if (s > most) s = most;
   if (s >= 8) s = s / 8 * 8;
-  return (int)(s < 1 ? 1 : s > 512 ? 512 : s);
+  f.splits = (int)(s < 1 ? 1 : s);
+  return f;
 }
 
 static int check_pairs(const char* fn, int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nd, int64_t nway, int dtype) {
@@ -606,23 +894,51 @@ __global__ void pairs_fill_kernel(float* scores, int64_t n, float v, uint16_t* a
   }
 }
 
+template <int DT, int TT, int CT>
+static int run_grad_d(const PairsGradArgs& a, hipStream_t st) {
+  const int tiles = (a.nd + 15) / 16;
+  const dim3 grid((unsigned)a.B, (unsigned)((a.cts + CT - 1) / CT), (unsigned)((tiles + 4 * TT - 1) / (4 * TT)));
+  hipLaunchKernelGGL((pairs_grad_d_kernel<DT, TT, CT, DT == TMS_DTYPE_F32 ? 3 : 1>), grid, dim3(256), 0, st, a);
+  return check_launch("pairs_grad_d_kernel");
+}
+// Tiles a wave: as many as the document has for each of four waves, up to four.
+template <int DT, int CT>
+static int run_grad_d_tiles(const PairsGradArgs& a, hipStream_t st) {
+  if (a.nd <= 64) return run_grad_d<DT, 1, CT>(a, st);
+  if (a.nd <= 128) return run_grad_d<DT, 2, CT>(a, st);
+  if (a.nd <= 192) return run_grad_d<DT, 3, CT>(a, st);
+  return run_grad_d<DT, 4, CT>(a, st);
+}
+
 template <int DT>
-static int run_grads(PairsGradArgs a, hipStream_t st) {
+static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
   int rc;
   if (a.dD && a.B > 0 && a.nd > 0 && a.d > 0) {
-    const unsigned cols = (unsigned)((a.d + 63) / 64);
-    const int tiles = (a.nd + 510) / 511;  // at most 512 rows of 256 bytes: 128 KB of LDS
-    a.rows = (a.nd + tiles - 1) / tiles;
-    const size_t lds = (size_t)(a.rows + 1) * 256;
-    hipLaunchKernelGGL(pairs_grad_d_kernel<DT>, dim3((unsigned)a.B, cols, (unsigned)tiles), dim3(64), lds, st, a);
-    if ((rc = check_launch("pairs_grad_d_kernel"))) return rc;
+    const int64_t n = (int64_t)a.blocks * a.cts * 64;
+    if (n > 0) {
+      hipLaunchKernelGGL(pairs_frags_kernel<DT>, dim3((unsigned)(n > 256 * 4096 ? 4096 : (n + 255) / 256)), dim3(256), 0, st, a);
+      if ((rc = check_launch("pairs_frags_kernel"))) return rc;
+    }
+    rc = a.cts <= 2 ? run_grad_d_tiles<DT, 2>(a, st) : a.cts <= 4 ? run_grad_d_tiles<DT, 4>(a, st) : run_grad_d_tiles<DT, 8>(a, st);
+    if (rc) return rc;
   }
   if (a.dQ && a.nQ > 0 && a.nq > 0 && a.d > 0) {
     const unsigned cols = (unsigned)((a.d + 127) / 128);
     const int64_t n = a.nway ? a.nway : a.B;
+    a.splits = form.splits;
     a.chunk = (int32_t)((n + a.splits - 1) / a.splits);
-    hipLaunchKernelGGL(pairs_grad_q_kernel<DT>, dim3((unsigned)((int64_t)a.nQ * (a.nqp / 8) * a.splits), cols), dim3(64), 0, st, a);
-    if ((rc = check_launch("pairs_grad_q_kernel"))) return rc;
+    if (form.shared && a.nd > 0) {
+      constexpr int es = DT == TMS_DTYPE_F32 ? 4 : 2;
+      const int most = 65536 / (128 * es);  // a stage is at most 64 KB
+      const int stages = (a.nd + most - 1) / most;
+      a.tokens = stages > 0 ? (a.nd + stages - 1) / stages : 0;
+      const size_t lds = 2 * (size_t)(a.tokens + 1) * 128 * es;
+      hipLaunchKernelGGL(pairs_grad_q_kernel<DT>, dim3((unsigned)((a.blocks + 15) / 16 * a.splits), cols), dim3(1024), lds, st, a);
+      if ((rc = check_launch("pairs_grad_q_kernel"))) return rc;
+    } else {
+      hipLaunchKernelGGL(pairs_grad_q_few_kernel<DT>, dim3((unsigned)((int64_t)a.nQ * ((a.nq + 7) / 8) * a.splits), cols), dim3(512), 0, st, a);
+      if ((rc = check_launch("pairs_grad_q_few_kernel"))) return rc;
+    }
     if (a.splits > 1) {
       const int64_t m = (int64_t)a.nQ * a.nq * a.d;
       hipLaunchKernelGGL(pairs_grad_q_join_kernel<DT>, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, a.parts, a.dQ, m, a.splits);
@@ -645,7 +961,7 @@ extern "C" int64_t tms_pairs_workspace_size(int64_t nQ, int64_t nq, int64_t d, i
 
 extern "C" int64_t tms_pairs_positions(int64_t nQ, int64_t nq, int64_t B, int64_t nway) {
   if (nQ < 0 || nq < 0 || B < 0) return 0;
-  return (nway > 0 ? B : nQ * B) * round_up(nq, 8);
+  return (nway > 0 ? B : nQ * B) * round_up(nq, 32);
 }
 
 extern "C" int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
@@ -665,7 +981,7 @@ extern "C" int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t 
   a.B = B;
   a.nQ = (int32_t)nQ;
   a.nq = (int32_t)nq;
-  a.nqp = (int32_t)round_up(nq, 8);
+  a.nqp = (int32_t)round_up(nq, 32);
   a.nd = (int32_t)nd;
   a.nway = (int32_t)nway;
   a.nbq = (int32_t)((nq + 31) / 32);
@@ -699,44 +1015,52 @@ extern "C" int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t 
   return run_pairs<TMS_DTYPE_BF16, 3>(a, st);
 }
 
-extern "C" int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway) {
+static int64_t frags_bytes(int64_t nQ, int64_t nq, int64_t d, int dtype) {
+  return nQ * ((nq + 31) / 32) * ((d + 15) / 16) * 1024 * planes(dtype);
+}
+static int64_t parts_bytes(int64_t nQ, int64_t nq, int64_t d, const GradQ& f) { return f.splits > 1 ? f.splits * nQ * nq * d * 4 : 0; }
+
+extern "C" int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway, int dtype) {
   if (nQ <= 0 || nq <= 0 || d <= 0 || B <= 0) return 0;
-  const int s = grad_q_splits(nQ, round_up(nq, 8), (d + 127) / 128, nway > 0 ? nway : B);
-  return s > 1 ? s * nQ * nq * d * 4 : 0;
+  return frags_bytes(nQ, nq, d, dtype) + parts_bytes(nQ, nq, d, grad_q_form(nQ, nq, d, B, nway));
 }
 
 extern "C" int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
-                                     int64_t nway, const uint16_t* positions, const float* grad, int dtype, void* workspace,
-                                     int64_t workspace_bytes, void* dQ, void* dD, void* stream) {
+                                     int64_t nway, const uint8_t* qmask, const uint16_t* positions, const float* grad, int dtype,
+                                     void* workspace, int64_t workspace_bytes, void* dQ, void* dD, void* stream) {
   const char* fn = "tms_maxsim_pairs_grad";
   const int rc = check_pairs(fn, nQ, nq, d, B, nd, nway, dtype);
   if (rc) return rc;
-  const int64_t nqp = round_up(nq, 8);
   if ((dQ && nQ * nq * d > 0 && B > 0 && nd > 0 && !D) || (dD && B * nd * d > 0 && nQ * nq > 0 && !Qs) ||
       (nQ * nq > 0 && B > 0 && (!positions || !grad)))
     return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
   if ((uintptr_t)positions % 16) return fail(TMS_ERR_INVALID, "%s: positions must be 16-byte aligned", fn);
-  const int64_t need = dQ ? tms_pairs_grad_workspace_size(nQ, nq, d, B, nway) : 0;
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(TMS_ERR_INVALID, "%s: a workspace of %lld bytes is needed", fn, (long long)need);
+  const int64_t need = tms_pairs_grad_workspace_size(nQ, nq, d, B, nway, dtype);
+  if (need > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
+    return fail(TMS_ERR_INVALID, "%s: a workspace of %lld bytes is needed, 16-byte aligned", fn, (long long)need);
   PairsGradArgs a = {};
   a.Q = Qs;
   a.D = D;
+  a.qmask = qmask;
   a.arg = positions;
   a.G = grad;
   a.dQ = dQ;
   a.dD = dD;
-  a.parts = (float*)workspace;
+  a.frags = (u32x4*)workspace;
+  a.parts = (float*)((uint8_t*)workspace + frags_bytes(nQ, nq, d, dtype));
   a.B = B;
   a.nQ = (int32_t)nQ;
   a.nq = (int32_t)nq;
-  a.nqp = (int32_t)nqp;
+  a.nqp = (int32_t)round_up(nq, 32);
   a.nd = (int32_t)nd;
   a.d = (int32_t)d;
   a.nway = (int32_t)nway;
-  a.splits = B > 0 ? grad_q_splits(nQ, nqp, (d + 127) / 128, nway > 0 ? nway : B) : 1;
+  a.nbq = (int32_t)((nq + 31) / 32);
+  a.blocks = a.nQ * a.nbq;
+  a.cts = (int32_t)((d + 15) / 16);
+  const GradQ form = grad_q_form(nQ, nq, d, B, nway);
   const hipStream_t st = (hipStream_t)stream;
-  if (dtype == TMS_DTYPE_F16) return run_grads<TMS_DTYPE_F16>(a, st);
-  if (dtype == TMS_DTYPE_BF16) return run_grads<TMS_DTYPE_BF16>(a, st);
-  return run_grads<TMS_DTYPE_F32>(a, st);
+  if (dtype == TMS_DTYPE_F16) return run_grads<TMS_DTYPE_F16>(a, form, st);
+  if (dtype == TMS_DTYPE_BF16) return run_grads<TMS_DTYPE_BF16>(a, form, st);
+  return run_grads<TMS_DTYPE_F32>(a, form, st);
 }
