@@ -3,11 +3,19 @@
 // outside (rows of m or n), and an epilogue that takes the sums from registers.
 //
 // Eight waves, 2 along m and 4 along n, share tiles of BM x BN with k in steps of 64; a wave
-// keeps MI x NI sums of 16 x 16 (256 x 256: 128 VGPRs). A step's operands go from memory
-// through registers into one of two LDS buffers, in MFMA fragment order, one barrier a step:
-// the loads have a whole step's products to arrive in. Operands with k outside are read back
-// with ds_read_b64_tr_b16 (in each 16 lanes, lane l receives element l % 4 of lanes
-// l / 4, 4 + l / 4, 8 + l / 4, 12 + l / 4), so no transposed copy of anything is made.
+// keeps MI x NI sums of 16 x 16 (256 x 256: 128 VGPRs). The next step's operands go from
+// memory straight to one of two LDS buffers while this step's are multiplied: a wave first
+// reads all its fragments of the step, then issues the loads (an LDS read behind them would
+// wait for them), then multiplies, waits for its loads and meets the others: one barrier a
+// step. Both kinds of operand come in units of 1 KB, eight rows of 128 bytes (whole lines),
+// whose 16-byte pieces are stored permuted so that the fragment reads fall evenly on the
+// LDS banks:
+//  * k inside: rows are m (n); piece p of row r is stored at p ^ (r % 8). A fragment is one
+//    ds_read_b128 a lane.
+//  * k outside: rows are k, 64 of m (n); piece p of row r of the unit of k / 8 = u is stored
+//    at p ^ (4 (r / 2 % 2) + u % 4). A fragment is two ds_read_b64_tr_b16: in each 16 lanes,
+//    lane l receives element l % 4 of lanes l / 4, 4 + l / 4, 8 + l / 4 and 12 + l / 4, so no
+//    transposed copy of anything is made.
 //
 // A 16 x 16 block of sums has lane (c, g) hold column n = c and rows m = 4 g + i: what is
 // reduced over m stays in a lane, and four neighbouring m are one store.
@@ -19,10 +27,11 @@ namespace tms {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // fp32 operands are three bf16 terms ("planes"); of the nine products of two such operands
-// the six above 2^-24 of the whole are formed, small ones first.
+// the six above 2^-24 of the whole are formed, small ones first: planes (2, 0), (0, 2),
+// (1, 1), (1, 0), (0, 1), (0, 0), a hexadecimal digit each from the last on.
 constexpr int kTermPairs = 6;
-__device__ constexpr int kTermA[kTermPairs] = {2, 0, 1, 1, 0, 0};
-__device__ constexpr int kTermB[kTermPairs] = {0, 2, 1, 0, 1, 0};
+__device__ __forceinline__ int term_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
+__device__ __forceinline__ int term_b(int pair) { return (0x010120 >> (4 * pair)) & 3; }
 
 struct GemmArgs {
   const uint16_t* A;
@@ -36,65 +45,73 @@ struct GemmArgs {
 };
 
 constexpr int kGemmThreads = 512;
-constexpr int kOuterBlock = 2080;  // bytes of 16 columns x 64 k: 32 more than they need, so that blocks fall on other banks
 
-constexpr int gemm_lds(int rows, bool outer) { return outer ? rows / 16 * kOuterBlock : rows * 128; }
+// Epilogues are called with the wave's sums, its first m and n, its split, and LDS of its
+// own: kRowBytes for each of its columns n (0: none).
 
-// One operand's share of a step: R rows (or columns) x 64 k.
+// What stands for the elements past the end of k.
+__device__ const u32x4 kGemmZeros = {0u, 0u, 0u, 0u};
+
+// One operand's share of a step: R rows (or columns) x 64 k, R / 8 units.
 template <int R, bool OUTER>
 struct GemmTile {
-  static constexpr int L = R / 64;  // 16-byte loads a thread
-  u32x4 reg[L];
-  int32_t off[L];  // elements from the tile's first, at k = 0 of the step
-  int16_t kk[L];   // k within the step
-  int32_t place[L];
+  static constexpr int L = R / 64;  // units a wave loads
+  uint32_t off[L];                  // bytes from the tile's first element, at k = 0 of the step
+  int32_t kk;                       // k within the step, of unit 0 (k outside: + 8 a unit, see load)
 
-  __device__ __forceinline__ void init(int ld, int limit) {  // limit: rows (columns) of the tile that exist
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  // Units go to the waves in turn: wave w loads units w, w + 8, ...: k inside, rows 8 unit ..;
+  // outside, k 8 (unit % 8) .. of columns 64 (unit / 8) ..
+  __device__ __forceinline__ void init(int ld, int limit, int lane, int wave) {  // limit: rows (columns) that exist
+    const int r = lane >> 3, slot = lane & 7;
+    if constexpr (OUTER) {
+      const int p = slot ^ (4 * ((r >> 1) & 1) + (wave & 3));  // unit % 8 is the wave
+      kk = 8 * wave + r;
 #pragma unroll
-    for (int i = 0; i < L; i++) {
-      if constexpr (OUTER) {
-        const int idx = i * kGemmThreads + (int)threadIdx.x, k = idx / (R / 8), c = idx % (R / 8);
-        kk[i] = (int16_t)k;
-        off[i] = k * ld + (c * 8 < limit ? c * 8 : 0);
-        place[i] = (c >> 1) * kOuterBlock + (k >> 5) * 1024 + ((k >> 2) & 1) * 512 + (((k >> 3) & 3) * 16 + (k & 3) * 4 + 2 * (c & 1)) * 8;
-      } else {
-        const int f = i * 8 + wave, row = (f >> 1) * 16 + (lane & 15);
-        kk[i] = (int16_t)((f & 1) * 32 + (lane >> 4) * 8);
-        off[i] = (row < limit ? row : limit - 1) * ld + kk[i];
-        place[i] = f * 1024 + lane * 16;
+      for (int i = 0; i < L; i++) {
+        const int col = 64 * i + 8 * p;
+        off[i] = 2u * (uint32_t)(kk * ld + (col < limit ? col : 0));
+      }
+    } else {
+      kk = 8 * (slot ^ r);
+#pragma unroll
+      for (int i = 0; i < L; i++) {
+        const int row = (i * 8 + wave) * 8 + r;
+        off[i] = 2u * (uint32_t)((row < limit ? row : limit - 1) * ld + kk);
       }
     }
   }
   // base: the tile's first element at this step's first k; left: how many k there are from it on
-  __device__ __forceinline__ void load(const uint16_t* base, int ld, int left) {
+  __device__ __forceinline__ void load(const uint16_t* base, int left, uint8_t* lds, int wave) const {
+    typedef __attribute__((address_space(1))) const void* GP;
+    typedef __attribute__((address_space(3))) void* LP;
+    const uint8_t* from = (const uint8_t*)base;
     if (left >= 64) {
 #pragma unroll
-      for (int i = 0; i < L; i++) reg[i] = *(const u32x4*)(base + off[i]);
+      for (int i = 0; i < L; i++) __builtin_amdgcn_global_load_lds((GP)(from + off[i]), (LP)(lds + (i * 8 + wave) * 1024), 16, 0, 0);
     } else {
 #pragma unroll
       for (int i = 0; i < L; i++) {
-        const bool in = kk[i] < left;
-        const u32x4 v = *(const u32x4*)(base + (in ? off[i] : off[i] - (OUTER ? kk[i] * ld : kk[i])));
-        reg[i] = in ? v : u32x4{0u, 0u, 0u, 0u};
+        const uint8_t* p = kk < left ? from + off[i] : (const uint8_t*)&kGemmZeros;
+        __builtin_amdgcn_global_load_lds((GP)p, (LP)(lds + (i * 8 + wave) * 1024), 16, 0, 0);
       }
     }
   }
-  __device__ __forceinline__ void put(uint8_t* lds) const {
-#pragma unroll
-    for (int i = 0; i < L; i++) *(u32x4*)(lds + place[i]) = reg[i];
-  }
-  // the fragment of 16 rows and 32 k
+  // The fragment of 16 rows and 32 k. at: this lane's part of the address (frag_at), which
+  // the unrolled block and ks only add constants to.
   __device__ static __forceinline__ u32x4 frag(const uint8_t* lds, int block, int ks, int lane) {
     if constexpr (OUTER) {
       typedef __attribute__((address_space(3))) s16x4* LP;
-      const uint8_t* p = lds + block * kOuterBlock + ks * 1024 + lane * 8;
+      const int g = lane >> 4, j = (lane >> 2) & 3, q = lane & 3;
+      // rows 4 h + j of unit (block / 4, 4 ks + g)
+      const int x = 4 * ((j >> 1) & 1) + g, piece = ((block & 3) * 2 + (q >> 1)) ^ x;
+      const uint8_t* p = lds + ((block >> 2) * 8 + ks * 4 + g) * 1024 + j * 128 + piece * 16 + (q & 1) * 8;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(p + 512));
       const u32x2 a = __builtin_bit_cast(u32x2, lo), b = __builtin_bit_cast(u32x2, hi);
       return u32x4{a[0], a[1], b[0], b[1]};
     } else {
-      return *(const u32x4*)(lds + (block * 2 + ks) * 1024 + lane * 16);
+      const int r = lane & 15, g = lane >> 4;
+      return *(const u32x4*)(lds + (block * 2 + (r >> 3)) * 1024 + (r & 7) * 128 + (((ks * 4 + g) ^ (r & 7)) * 16));
     }
   }
 };
@@ -114,11 +131,16 @@ __device__ __forceinline__ bool gemm_tile_of(const GemmArgs& a, int& m, int& n) 
 }
 static inline unsigned gemm_grid(int tm, int tn) { return (unsigned)(((int64_t)tm * tn + 7) / 8 * 8); }
 
+template <bool V>
+struct More {
+  static constexpr bool value = V;
+};
+
 template <int DT, int MI, int NI, bool AO, bool BO, class Epi>
 __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a, Epi epi) {
   constexpr int BM = 32 * MI, BN = 64 * NI;
-  constexpr int ASZ = gemm_lds(BM, AO), BSZ = gemm_lds(BN, BO);
-  extern __shared__ uint8_t gemm_mem[];
+  constexpr int ASZ = BM * 128, BSZ = BN * 128;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t gemm_mem[];
   int tm, tn;
   if (!gemm_tile_of(a, tm, tn)) return;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -127,8 +149,8 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
 
   GemmTile<BM, AO> ta;
   GemmTile<BN, BO> tb;
-  ta.init(a.lda, a.M - m0);
-  tb.init(a.ldb, a.N - n0);
+  ta.init(a.lda, a.M - m0, lane, wave);
+  tb.init(a.ldb, a.N - n0, lane, wave);
   const int k0 = (int)blockIdx.y * a.per;
   const int steps_all = (a.K + 63) / 64;
   const int nk = k0 + a.per < steps_all ? a.per : steps_all - k0;
@@ -136,15 +158,20 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
   const uint16_t* A = a.A + (AO ? (int64_t)m0 : (int64_t)m0 * a.lda);
   const uint16_t* B = a.B + (BO ? (int64_t)n0 : (int64_t)n0 * a.ldb);
   int pair = kTermPairs - a.pairs, kt = 0;  // the step that is loaded next
-  auto load = [&]() {
+  auto load = [&](int buf) {
     const int64_t k = (int64_t)(k0 + kt) * 64;
     const int left = a.K - (int)k;
-    ta.load(A + kTermA[pair] * a.aplane + (AO ? k * a.lda : k), a.lda, left);
-    tb.load(B + kTermB[pair] * a.bplane + (BO ? k * a.ldb : k), a.ldb, left);
+    uint8_t* to = gemm_mem + buf * (ASZ + BSZ);
+    ta.load(A + term_a(pair) * a.aplane + (AO ? k * a.lda : k), left, to, wave);
+    tb.load(B + term_b(pair) * a.bplane + (BO ? k * a.ldb : k), left, to + ASZ, wave);
     if (++kt == nk) {
       kt = 0;
       pair++;
     }
+  };
+  auto meet = [&]() {  // this wave's loads are in LDS, then everyone's
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    __syncthreads();
   };
 
   f32x4 acc[MI][NI];
@@ -153,39 +180,50 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
 #pragma unroll
     for (int j = 0; j < NI; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  if (steps > 0) {
-    load();
-    ta.put(gemm_mem);
-    tb.put(gemm_mem + ASZ);
-    if (steps > 1) load();
-  }
-  __syncthreads();
-  int buf = 0;
-  for (int t = 0; t < steps; t++) {
+  // One step from buffer `buf`; `more`: the next one's loads go out once a quarter of the
+  // products is issued (behind the loads, a product would wait for all of the wave's LDS
+  // reads together). The scheduler would otherwise move products behind the wait for the loads.
+  auto step = [&](int buf, auto more) {
     const uint8_t* la = gemm_mem + buf * (ASZ + BSZ);
     const uint8_t* lb = la + ASZ;
+    u32x4 fa[2][MI], fb[2][NI];
 #pragma unroll
     for (int ks = 0; ks < 2; ks++) {
-      u32x4 fa[MI], fb[NI];
 #pragma unroll
-      for (int j = 0; j < NI; j++) fb[j] = GemmTile<BN, BO>::frag(lb, wn * NI + j, ks, lane);
+      for (int j = 0; j < NI; j++) fb[ks][j] = GemmTile<BN, BO>::frag(lb, wn * NI + j, ks, lane);
 #pragma unroll
-      for (int i = 0; i < MI; i++) fa[i] = GemmTile<BM, AO>::frag(la, wm * MI + i, ks, lane);
+      for (int i = 0; i < MI; i++) fa[ks][i] = GemmTile<BM, AO>::frag(la, wm * MI + i, ks, lane);
+    }
+    auto products = [&](int ks, int i0, int i1) {
 #pragma unroll
       for (int i = 0; i < MI; i++)
 #pragma unroll
-        for (int j = 0; j < NI; j++) acc[i][j] = mfma16x16x32<DT>(fa[i], fb[j], acc[i][j]);
+        for (int j = 0; j < NI; j++)
+          if (i >= i0 && i < i1) acc[i][j] = mfma16x16x32<DT>(fa[ks][i], fb[ks][j], acc[i][j]);
+    };
+    products(0, 0, MI / 2);
+    if constexpr (decltype(more)::value) {
+      __builtin_amdgcn_sched_barrier(0);
+      load(buf ^ 1);
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (t + 1 < steps) {
-      uint8_t* to = gemm_mem + (buf ^ 1) * (ASZ + BSZ);
-      ta.put(to);
-      tb.put(to + ASZ);
+    products(0, MI / 2, MI);
+    products(1, 0, MI);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (steps > 0) {
+    load(0);
+    meet();
+    int buf = 0;
+    for (int t = 0; t + 1 < steps; t++) {
+      step(buf, More<true>());
+      meet();
+      buf ^= 1;
     }
-    if (t + 2 < steps) load();
-    __syncthreads();
-    buf ^= 1;
+    step(buf, More<false>());
   }
-  epi(acc, m0 + wm * MI * 16, n0 + wn * NI * 16, (int)blockIdx.y);
+  if constexpr (Epi::kRowBytes > 0) __syncthreads();  // the operands' LDS is the epilogue's
+  epi(acc, m0 + wm * MI * 16, n0 + wn * NI * 16, (int)blockIdx.y, gemm_mem + wave * (NI * 16 * Epi::kRowBytes));
 }
 
 template <int DT, int MI, int NI, bool AO, bool BO, class Epi>
@@ -194,7 +232,8 @@ static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what
   a.tn = (a.N + 64 * NI - 1) / (64 * NI);
   const int steps = (a.K + 63) / 64;
   a.per = (steps + a.splits - 1) / a.splits;
-  const size_t lds = 2 * (size_t)(gemm_lds(32 * MI, AO) + gemm_lds(64 * NI, BO));
+  size_t lds = 2 * (size_t)(32 * MI + 64 * NI) * 128;
+  if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
   hipLaunchKernelGGL((train_gemm_kernel<DT, MI, NI, AO, BO, Epi>), dim3(gemm_grid(a.tm, a.tn), (unsigned)a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);
   return check_launch(what);

@@ -35,12 +35,13 @@ struct RowStat {
 
 // Rows n of a wave's columns: 16 j + c.
 struct LseEpilogue {
+  static constexpr int kRowBytes = 0;
   RowStat* parts;  // [block of the vocabulary][rows]
   int32_t rows, V;
   float s2;  // scale log2(e)
 
   template <int MI, int NI>
-  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t*) const {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const float NEG = -__builtin_inff();
     if (m + 16 * MI > V) {  // past the vocabulary
@@ -73,9 +74,12 @@ struct LseEpilogue {
   }
 };
 
-// P of one piece: [plane][row][ldp]; rows and columns that do not exist are zero.
-template <int DT, int PL>
+// P of one piece: [plane][row][ldp]; rows and columns that do not exist are zero. A lane holds
+// four neighbouring columns of a row, so a wave's rows pass through its LDS and leave as whole
+// lines (eight-byte stores left half-written lines: 333 us a piece of 8192 x 21,760 at d = 768).
+template <int DT, int PL, int MIV>
 struct ProbEpilogue {
+  static constexpr int kRowBytes = MIV * 32 + 16;  // 16 more: the rows of four lanes fall on other banks
   uint16_t* P;
   const float* lse2;     // per row; +inf for a row without a gradient
   const float* g_row;    // per row: g / u
@@ -84,42 +88,72 @@ struct ProbEpilogue {
   int32_t ldp, rows, V, v0;  // V: columns of the piece that exist; v0: its first
   float s2;
 
-  template <int MI, int NI>
-  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  // p = (exp2(x - lse) - [v = target]) g of a lane's elements of one row, and its terms
+  template <bool HIT, int MI>
+  __device__ __forceinline__ void row(const f32x4 (&x)[MI], float ref, float w, int hit, u32x2 (&out)[PL][MI]) const {
     const float one = DT == TMS_DTYPE_F16 && PL == 1 ? (float)(1 << kP16) : 1.f;
 #pragma unroll
-    for (int j = 0; j < NI; j++) {
-      const int row = n + 16 * j + c;
-      const bool in = row < rows;
-      const float ref = in ? lse2[row] : __builtin_inff(), w = in ? g_row[row] : 0.f;
-      const int hit = in ? target[row] - v0 - (m + 4 * g) : -1;  // its place among this lane's 4 + 16 i
-      const bool any = __ballot(hit >= 0 && hit < 16 * MI) != 0ull;
+    for (int i = 0; i < MI; i++) {
+      float p[4];
 #pragma unroll
-      for (int i = 0; i < MI; i++) {
-        float p[4];
+      for (int e = 0; e < 4; e++) {
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s2, -ref));
+        if constexpr (HIT) p[e] -= hit == 16 * i + e ? one : 0.f;
+        p[e] *= w;
+      }
+#pragma unroll
+      for (int t = 0; t < PL; t++) {
+        uint16_t b[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], s2, -ref));
-          if (any) p[e] -= hit == 16 * i + e ? one : 0.f;
-          p[e] *= w;
-          if (m + 16 * MI > V) p[e] = m + 16 * i + 4 * g + e < V ? p[e] : 0.f;
-        }
-        uint16_t* to = P + (int64_t)row * ldp + m + 16 * i + 4 * g;
-#pragma unroll
-        for (int t = 0; t < PL; t++) {
-          uint16_t x[4];
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            if constexpr (DT == TMS_DTYPE_F16) {
-              x[e] = __builtin_bit_cast(uint16_t, (_Float16)p[e]);
-            } else {
-              const __bf16 b = (__bf16)p[e];
-              x[e] = __builtin_bit_cast(uint16_t, b);
-              if constexpr (PL > 1) p[e] -= (float)b;
-            }
+          if constexpr (DT == TMS_DTYPE_F16) {
+            b[e] = __builtin_bit_cast(uint16_t, (_Float16)p[e]);
+          } else {
+            const __bf16 h = (__bf16)p[e];
+            b[e] = __builtin_bit_cast(uint16_t, h);
+            if constexpr (PL > 1) p[e] -= (float)h;
           }
-          *(u32x2*)(to + t * plane) = u32x2{(uint32_t)x[0] | (uint32_t)x[1] << 16, (uint32_t)x[2] | (uint32_t)x[3] << 16};
+        }
+        out[t][i] = u32x2{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
+      }
+    }
+  }
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t* lds) const {
+    static_assert(MI == MIV, "rows of the wave's LDS");
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    if (m + 16 * MI > V) {  // past the vocabulary: exp2 gives 0
+#pragma unroll
+      for (int i = 0; i < MI; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (m + 16 * i + 4 * g + e >= V)
+#pragma unroll
+            for (int j = 0; j < NI; j++) acc[i][j][e] = -__builtin_inff();
+    }
+    constexpr int PIECES = MI * 2, ROWS = 64 / PIECES;  // 16-byte pieces of a row; rows a wave stores at once
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int r = n + 16 * j + c;
+      const bool in = r < rows;
+      const float ref = in ? lse2[r] : __builtin_inff(), w = in ? g_row[r] : 0.f;
+      const int hit = in ? target[r] - v0 - (m + 4 * g) : -1;  // its place among this lane's 16 i + e
+      f32x4 x[MI];
+#pragma unroll
+      for (int i = 0; i < MI; i++) x[i] = acc[i][j];
+      u32x2 out[PL][MI];
+      if (__ballot(hit >= 0 && hit < 16 * MI) != 0ull) row<true>(x, ref, w, hit, out);
+      else row<false>(x, ref, w, hit, out);
+#pragma unroll
+      for (int t = 0; t < PL; t++) {
+#pragma unroll
+        for (int i = 0; i < MI; i++) *(u32x2*)(lds + c * kRowBytes + i * 32 + g * 8) = out[t][i];
+#pragma unroll
+        for (int k = 0; k < 16 / ROWS; k++) {
+          const int rr = k * ROWS + lane / PIECES, piece = lane % PIECES;
+          const u32x4 v = *(const u32x4*)(lds + rr * kRowBytes + piece * 16);
+          *(u32x4*)(P + t * plane + (int64_t)(n + 16 * j + rr) * ldp + m + piece * 8) = v;
         }
       }
     }
@@ -128,13 +162,14 @@ struct ProbEpilogue {
 
 // Sums of dH: [split][row][d], added to from the second piece on.
 struct SumEpilogue {
+  static constexpr int kRowBytes = 0;
   float* out;
   int64_t split;  // elements of one
   int32_t rows, d;
   int32_t first;
 
   template <int MI, int NI>
-  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int s) const {
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int s, uint8_t*) const {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
 #pragma unroll
     for (int j = 0; j < NI; j++) {
@@ -166,12 +201,13 @@ __device__ __forceinline__ uint16_t to16(float x) {
 // dW of one piece, finished: times *factor, in the inputs' type.
 template <int OUT>
 struct WeightEpilogue {
+  static constexpr int kRowBytes = 0;
   void* out;  // the piece's first row
   const float* factor;
   int32_t rows, d;
 
   template <int MI, int NI>
-  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int) const {
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t*) const {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const float f = *factor;
 #pragma unroll
@@ -522,8 +558,10 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
     GemmArgs a = logits_args(h, (const uint16_t*)w + v0 * p.dp, N, nv, V, p.dp, dtype);
-    ProbEpilogue<DT, PL> e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e};
-    if ((rc = run_logits<DT>(a, e, st, "train_gemm_kernel (P)"))) return rc;
+    const auto prob = [&](auto e) { e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e}; return e; };
+    if (N <= kFewRows) rc = run_gemm<DT, 4, 1, false, false>(a, prob(ProbEpilogue<DT, PL, 4>()), st, "train_gemm_kernel (P)");
+    else rc = run_gemm<DT, 8, 4, false, false>(a, prob(ProbEpilogue<DT, PL, 8>()), st, "train_gemm_kernel (P)");
+    if (rc) return rc;
     if (dH && d > 0) {  // m over d, n over rows, k over the piece
       GemmArgs b = {};
       b.A = (const uint16_t*)w + v0 * p.dp;
