@@ -13,7 +13,9 @@
 //  * k inside: rows are m (n); piece p of row r is stored at p ^ (r % 8). A fragment is one
 //    ds_read_b128 a lane.
 //  * k outside: rows are k, 64 of m (n); piece p of row r of the unit of k / 8 = u is stored
-//    at p ^ (4 (r / 2 % 2) + u % 4). A fragment is two ds_read_b64_tr_b16: in each 16 lanes,
+//    at p ^ (4 (r / 2 % 2) + 2 (u % 2) + u / 2 % 2), which spreads each half of a wave over all
+//    banks (4 (r / 2 % 2) + u % 4 spreads the wave but not its halves: twice the LDS cycles, and
+//    7 % of the product's time). A fragment is two ds_read_b64_tr_b16: in each 16 lanes,
 //    lane l receives element l % 4 of lanes l / 4, 4 + l / 4, 8 + l / 4 and 12 + l / 4, so no
 //    transposed copy of anything is made.
 //
@@ -64,7 +66,7 @@ struct GemmTile {
   __device__ __forceinline__ void init(int ld, int limit, int lane, int wave) {  // limit: rows (columns) that exist
     const int r = lane >> 3, slot = lane & 7;
     if constexpr (OUTER) {
-      const int p = slot ^ (4 * ((r >> 1) & 1) + (wave & 3));  // unit % 8 is the wave
+      const int p = slot ^ (4 * ((r >> 1) & 1) + 2 * (wave & 1) + ((wave >> 1) & 1));  // unit % 8 is the wave
       kk = 8 * wave + r;
 #pragma unroll
       for (int i = 0; i < L; i++) {
@@ -103,7 +105,7 @@ struct GemmTile {
       typedef __attribute__((address_space(3))) s16x4* LP;
       const int g = lane >> 4, j = (lane >> 2) & 3, q = lane & 3;
       // rows 4 h + j of unit (block / 4, 4 ks + g)
-      const int x = 4 * ((j >> 1) & 1) + g, piece = ((block & 3) * 2 + (q >> 1)) ^ x;
+      const int x = 4 * ((j >> 1) & 1) + 2 * (g & 1) + (g >> 1), piece = ((block & 3) * 2 + (q >> 1)) ^ x;
       const uint8_t* p = lds + ((block >> 2) * 8 + ks * 4 + g) * 1024 + j * 128 + piece * 16 + (q & 1) * 8;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)p);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LP)(p + 512));
@@ -180,9 +182,12 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
 #pragma unroll
     for (int j = 0; j < NI; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // One step from buffer `buf`; `more`: the next one's loads go out once a quarter of the
-  // products is issued (behind the loads, a product would wait for all of the wave's LDS
-  // reads together). The scheduler would otherwise move products behind the wait for the loads.
+  // One step from buffer `buf`; `more`: the next one's loads go out once some of the products
+  // are issued (behind the loads, a product would wait for all of the wave's LDS reads
+  // together): a quarter of them, or an eighth with k outside in both operands (8192^3 in bf16,
+  // an eighth / a quarter: 1.13 / 1.15 PFLOP/s with k inside, 1.23 / 1.29 outside in one, 1.29 /
+  // 1.21 in both). The scheduler would otherwise move products behind the wait for the loads.
+  constexpr int kBefore = AO && BO ? MI / 4 : MI / 2;
   auto step = [&](int buf, auto more) {
     const uint8_t* la = gemm_mem + buf * (ASZ + BSZ);
     const uint8_t* lb = la + ASZ;
@@ -201,13 +206,13 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
         for (int j = 0; j < NI; j++)
           if (i >= i0 && i < i1) acc[i][j] = mfma16x16x32<DT>(fa[ks][i], fb[ks][j], acc[i][j]);
     };
-    products(0, 0, MI / 2);
+    products(0, 0, kBefore);
     if constexpr (decltype(more)::value) {
       __builtin_amdgcn_sched_barrier(0);
       load(buf ^ 1);
       __builtin_amdgcn_sched_barrier(0);
     }
-    products(0, MI / 2, MI);
+    products(0, kBefore, MI);
     products(1, 0, MI);
     __builtin_amdgcn_sched_barrier(0);
   };
