@@ -57,7 +57,7 @@ __device__ const u32x4 kGemmZeros = {0u, 0u, 0u, 0u};
 // One operand's share of a step: R rows (or columns) x 64 k, R / 8 units.
 template <int R, bool OUTER>
 struct GemmTile {
-  static constexpr int L = R / 64;  // units a wave loads
+  static constexpr int L = R / 64;  // units a wave loads (R is a multiple of 64)
   uint32_t off[L];                  // bytes from the tile's first element, at k = 0 of the step
   int32_t kk;                       // k within the step, of unit 0 (k outside: + 8 a unit, see load)
 

@@ -23,6 +23,7 @@
 #include <math.h>
 
 #include "tms_train_gemm.h"
+#include "tms_train_rules.h"
 
 namespace tms {
 
@@ -275,39 +276,89 @@ __global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, int dt,
   }
 }
 
-// Joins a row's blocks; 16 rows a workgroup, 16 lanes a row, which also form the target's
-// logit from the inputs. A target outside the vocabulary (and not ignored) makes the row NaN.
+// (top, sum) of two parts of a row
+__device__ __forceinline__ RowStat join_stats(RowStat a, RowStat b) {
+  const float t = fmaxf(a.top, b.top), ref = t == -__builtin_inff() ? 0.f : t;
+  return {t, a.sum * __builtin_amdgcn_exp2f(a.top - ref) + b.sum * __builtin_amdgcn_exp2f(b.top - ref)};
+}
+
+// Joins a row's blocks, and forms its target's logit from the inputs; LANES lanes a row. A
+// target outside the vocabulary (and not ignored) makes the row NaN. With `loss` and one
+// workgroup, that goes over all rows and then reduces them as the kernel below does: a call
+// of a few rows is bound by its launches.
+template <int LANES>
 __global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int32_t blocks, int32_t rows, const void* H, const void* W,
                                                        int dt, int32_t V, int32_t d, const int64_t* target, int64_t ignore, float s2,
-                                                       float* lse2, float* loss) {
-  const int lane = threadIdx.x & 15, row = blockIdx.x * 16 + (threadIdx.x >> 4);
-  if (row >= rows) return;  // the 16 lanes of a row together
-  float top = -__builtin_inff(), sum = 0.f;
-  for (int b = lane; b < blocks; b += 16) {
-    const RowStat s = parts[(int64_t)b * rows + row];
-    const float t = fmaxf(top, s.top), ref = t == -__builtin_inff() ? 0.f : t;
-    sum = sum * __builtin_amdgcn_exp2f(top - ref) + s.sum * __builtin_amdgcn_exp2f(s.top - ref);
-    top = t;
-  }
+                                                       float* lse2, float* rows_loss, float* loss, float* count, int mean) {
+  constexpr int ROWS = 256 / LANES;
+  __shared__ RowStat stats[4];
+  __shared__ float dots[4];
+  const int lane = threadIdx.x % LANES;
+  double all = 0;
+  int kept_rows = 0;
+  for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
+    const int row = row0 + threadIdx.x / LANES;
+    const bool in = row < rows;
+    RowStat r = {-__builtin_inff(), 0.f};
+    for (int b = lane; in && b < blocks; b += 8 * LANES) {  // eight loads at a time
+      RowStat x[8];
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) {
-    const float t2 = __shfl_xor(top, o), u2 = __shfl_xor(sum, o);
-    const float t = fmaxf(top, t2), ref = t == -__builtin_inff() ? 0.f : t;
-    sum = sum * __builtin_amdgcn_exp2f(top - ref) + u2 * __builtin_amdgcn_exp2f(t2 - ref);
-    top = t;
-  }
-  float lse = top + log2f(sum);
-  const int64_t t = target[row];
-  const bool kept = t != ignore, fine = t >= 0 && t < V;
-  float dot = 0.f;
-  if (kept && fine)
-    for (int k = lane; k < d; k += 16) dot += element(H, (int64_t)row * d + k, dt) * element(W, t * d + k, dt);
+      for (int i = 0; i < 8; i++) {
+        const int at = b + i * LANES;
+        x[i] = at < blocks ? parts[(int64_t)at * rows + row] : RowStat{-__builtin_inff(), 0.f};
+      }
 #pragma unroll
-  for (int o = 8; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
-  if (kept && !fine) lse = __builtin_nanf("");
-  if (lane == 0) {
-    lse2[row] = lse;
-    loss[row] = kept ? (lse - dot * s2) * kLn2 : 0.f;
+      for (int i = 0; i < 8; i++) r = join_stats(r, x[i]);
+    }
+    const int64_t t = in ? target[row] : ignore;
+    const bool kept = t != ignore, fine = t >= 0 && t < V;
+    float dot = 0.f;
+    if (kept && fine) {
+      if (dt != TMS_DTYPE_F32 && d % 8 == 0) {  // then rows begin at 16 bytes
+        for (int k = lane * 8; k < d; k += LANES * 8) {
+          const u32x4 h = *(const u32x4*)((const uint16_t*)H + (int64_t)row * d + k), w = *(const u32x4*)((const uint16_t*)W + t * d + k);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const uint32_t a = h[e], c = w[e];
+            if (dt == TMS_DTYPE_F16) {
+              dot += (float)__builtin_bit_cast(_Float16, (uint16_t)a) * (float)__builtin_bit_cast(_Float16, (uint16_t)c);
+              dot += (float)__builtin_bit_cast(_Float16, (uint16_t)(a >> 16)) * (float)__builtin_bit_cast(_Float16, (uint16_t)(c >> 16));
+            } else {
+              dot += __builtin_bit_cast(float, a << 16) * __builtin_bit_cast(float, c << 16);
+              dot += __builtin_bit_cast(float, a & 0xffff0000u) * __builtin_bit_cast(float, c & 0xffff0000u);
+            }
+          }
+        }
+      } else {
+        for (int k = lane; k < d; k += LANES) dot += element(H, (int64_t)row * d + k, dt) * element(W, t * d + k, dt);
+      }
+    }
+#pragma unroll
+    for (int o = (LANES < 64 ? LANES : 64) / 2; o >= 1; o >>= 1) {
+      r = join_stats(r, RowStat{__shfl_xor(r.top, o), __shfl_xor(r.sum, o)});
+      dot += __shfl_xor(dot, o);
+    }
+    if constexpr (LANES > 64) {
+      __syncthreads();  // the last row's are read
+      if ((threadIdx.x & 63) == 0) stats[threadIdx.x >> 6] = r, dots[threadIdx.x >> 6] = dot;
+      __syncthreads();
+      r = stats[0], dot = dots[0];
+#pragma unroll
+      for (int w = 1; w < 4; w++) r = join_stats(r, stats[w]), dot += dots[w];
+    }
+    float lse = r.top + log2f(r.sum);
+    if (kept && !fine) lse = __builtin_nanf("");
+    const float x = kept ? (lse - dot * s2) * kLn2 : 0.f;
+    if (in && lane == 0) {
+      lse2[row] = lse;
+      if (rows_loss) rows_loss[row] = x;
+    }
+    all += (double)x;
+    kept_rows += kept;
+  }
+  if (LANES == 256 && loss && threadIdx.x == 0) {
+    *count = (float)kept_rows;
+    *loss = mean ? (float)(all / (double)kept_rows) : (float)all;
   }
 }
 
@@ -375,70 +426,62 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float* lse2, const
   }
 }
 
-// dH: the splits' sums, times the factor, in the inputs' type.
+// dH: the splits' sums, in order, times the factor, in the inputs' type. Four elements of a row
+// a thread (rows of sums are whole multiples of four), eight splits' loads at a time.
 template <int OUT>
 __global__ __launch_bounds__(256) void lce_hidden_kernel(const float* sums, int splits, int64_t split, int32_t rows, int32_t d, int32_t dp,
                                                          const float* factor, void* dH) {
-  const int64_t n = (int64_t)rows * d;
+  const int quads = (d + 3) / 4;
+  const int64_t n = (int64_t)rows * quads;
+  const float f = *factor;
   for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
-    const int64_t row = k / d, at = row * dp + (k - row * d);
-    float x = 0.f;
-    for (int s = 0; s < splits; s++) x += sums[s * split + at];
-    x *= *factor;
-    if constexpr (OUT == TMS_DTYPE_F32) ((float*)dH)[k] = x;
-    else ((uint16_t*)dH)[k] = to16<OUT>(x);
+    const int64_t row = k / quads;
+    const int col = (int)(k - row * quads) * 4;
+    const float* from = sums + row * dp + col;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s += 8) {
+      f32x4 y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[i] = s + i < splits ? *(const f32x4*)(from + (s + i) * split) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; i++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += y[i][e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (col + e >= d) break;
+      const float v = x[e] * f;
+      if constexpr (OUT == TMS_DTYPE_F32) ((float*)dH)[row * d + col + e] = v;
+      else ((uint16_t*)dH)[row * d + col + e] = to16<OUT>(v);
+    }
   }
 }
 
 // ---------------------------------------------------------------- host
 
-static int64_t up_to(int64_t x, int64_t m) { return (x + m - 1) / m * m; }
 static int planes(int dtype) { return dtype == TMS_DTYPE_F32 ? 3 : 1; }
 static bool as_is(const void* p, int64_t d, int dtype) { return dtype != TMS_DTYPE_F32 && d % 8 == 0 && (uintptr_t)p % 16 == 0; }
 static unsigned blocks_for(int64_t n) { return (unsigned)(n > 256 * 16384 ? 16384 : n > 0 ? (n + 255) / 256 : 1); }
 
-// Rows up to which the tiles hold 64 of them (the fewest that four waves side by side take).
-constexpr int kFewRows = 64;
-
-// How the backward pass goes over the vocabulary.
-struct LcePlan {
-  int64_t rows_p;  // rows of P: N up to a multiple of 256 (of 64 for few rows)
-  int64_t piece;   // columns of P, a multiple of 256
-  int splits;      // of the vocabulary in dH's product
-  int64_t dp;
+// The tiles' forms: MI and NI of the kernel (two waves along m, four along n).
+template <int S>
+struct SizeOf {
+  static constexpr int MI = S == kGemm256 ? 8 : S == kGemm128 ? 4 : 2, NI = S == kGemm256 ? 4 : S == kGemm128 ? 2 : 1;
 };
-
-// A piece of P takes up to 2^28 elements (512 MB in 16 bits, of 288 GB; 256 MB of it would
-// stay in the last cache, and reading the rest is far below the products' time). Among the
-// sizes within that, the one whose dW tiles (256 x 256, one a CU) leave the fewest CUs idle
-// over all pieces, the larger of equal ones.
-static LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int dtype) {
-  LcePlan p;
-  p.dp = up_to(d > 0 ? d : 8, 8);
-  p.rows_p = N <= kFewRows ? kFewRows : up_to(N, 256);
-  const int64_t all = up_to(V, 256) / 256, dt = (p.dp + 255) / 256;
-  int64_t most = ((int64_t)1 << 28) / planes(dtype) / p.rows_p / 256;
-  most = most < 1 ? 1 : most > all ? all : most;
-  int64_t best = most, fewest = INT64_MAX;
-  for (int64_t t = most; t >= 1 && t * 4 >= most; t--) {
-    const int64_t whole = all / t, rest = all - whole * t;
-    const int64_t rounds = whole * ((t * dt + 255) / 256) + (rest ? (rest * dt + 255) / 256 : 0);
-    if (rounds < fewest) fewest = rounds, best = t;
-  }
-  p.piece = best * 256;
-  // dH's tiles are few: split the piece so that they fill the chip, as long as a split's sums
-  // (read and written once a piece) cost less than the idle CUs would. Times in microseconds
-  // of a 64-step of a 256 x 256 tile (1.8) and of a megabyte of sums (0.25).
-  const int64_t tiles = dt * (N <= kFewRows ? 1 : p.rows_p / 256), steps = p.piece / 64;
-  const double mb = (double)N * (double)p.dp * 8e-6;
-  double least = 1e30;
-  p.splits = 1;
-  for (int64_t s = 1; s <= 64 && s * 4 <= steps; s++) {
-    const double us = (double)((tiles * s + 255) / 256) * (double)((steps + s - 1) / s) * 1.8 + (double)s * mb * 0.25;
-    if (us < least) least = us, p.splits = (int)s;
-  }
-  return p;
+template <class F>
+static int with_size(int size, F&& f) {
+  if (size == kGemm256) return f(SizeOf<kGemm256>());
+  if (size == kGemm128) return f(SizeOf<kGemm128>());
+  return f(SizeOf<kGemm64>());
 }
+static int logits_size(int64_t N, int64_t V, int64_t dp, int dtype) {
+  return gemm_size(V, N, up_to(dp, 64) / 64 * (dtype == TMS_DTYPE_F32 ? kTermPairs : 1));
+}
+// Vocabulary rows that one RowStat of the forward pass covers: a wave's share of a tile.
+static int64_t stat_rows(int size) { return gemm_side(size) / 2; }
+// Rows up to which one workgroup joins them all: below that its launch would take longer.
+constexpr int64_t kJoinAlone = 4;
 
 // Workspaces, as offsets into one buffer.
 struct Carve {
@@ -459,10 +502,11 @@ static LceSpace lce_space(int64_t N, int64_t V, int64_t d, int dtype, bool backw
   if (terms || backward) s.h = c.take(N * dp * 2 * planes(dtype));
   if (terms) s.w = c.take(V * dp * 2 * planes(dtype));
   if (!backward) {
-    s.parts = c.take((V + 63) / 64 * N * (int64_t)sizeof(RowStat));
+    const int64_t per = stat_rows(logits_size(N, V, dp, dtype));
+    s.parts = c.take((V + per - 1) / per * N * (int64_t)sizeof(RowStat));
     s.loss = c.take(N * 4);
   } else {
-    const LcePlan p = lce_plan(N, V, d, dtype);
+    const LcePlan p = lce_plan(N, V, d, planes(dtype));
     s.g = c.take(N * 4);
     s.ref = c.take(N * 4);
     s.hit = c.take(N * 4);
@@ -509,12 +553,6 @@ static GemmArgs logits_args(const void* H, const void* W, int64_t N, int64_t V, 
   return a;
 }
 
-template <int DT, class Epi>
-static int run_logits(const GemmArgs& a, const Epi& epi, hipStream_t st, const char* what) {
-  if (a.N <= kFewRows) return run_gemm<DT, 4, 1, false, false>(a, epi, st, what);
-  return run_gemm<DT, 8, 4, false, false>(a, epi, st, what);
-}
-
 template <int DT>  // the type of the terms: fp32 inputs have bf16 ones
 static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
                        float s2, int reduction, uint8_t* ws, const LceSpace& s, bool terms, float* loss, float* stats, hipStream_t st) {
@@ -529,20 +567,32 @@ static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64
   }
   const GemmArgs a = logits_args(h, w, N, V, V, dp, dtype);
   LseEpilogue e = {(RowStat*)(ws + s.parts), (int32_t)N, (int32_t)V, s2};
-  if ((rc = run_logits<DT>(a, e, st, "train_gemm_kernel (lse)"))) return rc;
-  const int wide = N <= kFewRows ? 64 : 128;
-  float* rows = reduction == TMS_REDUCE_NONE ? loss : (float*)(ws + s.loss);
-  // blocks past the vocabulary inside the last tile hold no row's sum: (-inf, 0) or nothing written
-  hipLaunchKernelGGL(lce_join_kernel, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, (const RowStat*)(ws + s.parts),
-                     (int32_t)((V + wide - 1) / wide), (int32_t)N, H, W, dtype, (int32_t)V, (int32_t)d, target, ignore, s2, stats, rows);
-  return check_launch("lce_join_kernel");
+  const int size = logits_size(N, V, dp, dtype);
+  rc = with_size(size, [&](auto z) { return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, false, false>(a, e, st, "train_gemm_kernel (lse)"); });
+  if (rc) return rc;
+  const bool rows = reduction == TMS_REDUCE_NONE, alone = !rows && N <= kJoinAlone;
+  float* rows_loss = rows ? loss : (float*)(ws + s.loss);
+  const int32_t blocks = (int32_t)((V + stat_rows(size) - 1) / stat_rows(size));
+  const RowStat* parts = (const RowStat*)(ws + s.parts);
+  // Few rows of many blocks take a workgroup each, many rows sixteen lanes each, which read
+  // sixteen rows' neighbouring statistics together.
+  if (N <= 1024)
+    hipLaunchKernelGGL(lce_join_kernel<256>, dim3(alone ? 1u : (unsigned)N), dim3(256), 0, st, parts, blocks, (int32_t)N, H, W, dtype, (int32_t)V,
+                       (int32_t)d, target, ignore, s2, stats, rows_loss, alone ? loss : nullptr, stats + N, reduction == TMS_REDUCE_MEAN ? 1 : 0);
+  else
+    hipLaunchKernelGGL(lce_join_kernel<16>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, parts, blocks, (int32_t)N, H, W, dtype, (int32_t)V,
+                       (int32_t)d, target, ignore, s2, stats, rows_loss, nullptr, nullptr, 0);
+  if ((rc = check_launch("lce_join_kernel")) || rows || alone) return rc;
+  hipLaunchKernelGGL(lce_reduce_kernel, dim3(1), dim3(1024), 0, st, rows_loss, target, ignore, (int32_t)N, reduction == TMS_REDUCE_MEAN ? 1 : 0,
+                     loss, stats + N);
+  return check_launch("lce_reduce_kernel");
 }
 
 template <int DT, int PL, int OUT>
 static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
                         float scale, int reduction, const float* stats, const float* grad, uint8_t* ws, const LceSpace& s, bool terms,
                         void* dH, void* dW, hipStream_t st) {
-  const LcePlan p = lce_plan(N, V, d, dtype);
+  const LcePlan p = lce_plan(N, V, d, planes(dtype));
   const float up = DT == TMS_DTYPE_F16 ? (float)kP16 : 0.f;
   float *g = (float*)(ws + s.g), *ref = (float*)(ws + s.ref), *factor = (float*)(ws + s.factor), *sums = (float*)(ws + s.sums);
   int32_t* hit = (int32_t*)(ws + s.hit);
@@ -558,9 +608,11 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
     GemmArgs a = logits_args(h, (const uint16_t*)w + v0 * p.dp, N, nv, V, p.dp, dtype);
-    const auto prob = [&](auto e) { e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e}; return e; };
-    if (N <= kFewRows) rc = run_gemm<DT, 4, 1, false, false>(a, prob(ProbEpilogue<DT, PL, 4>()), st, "train_gemm_kernel (P)");
-    else rc = run_gemm<DT, 8, 4, false, false>(a, prob(ProbEpilogue<DT, PL, 8>()), st, "train_gemm_kernel (P)");
+    rc = with_size(p.size_p, [&](auto z) {
+      using Z = decltype(z);
+      const ProbEpilogue<DT, PL, Z::MI> e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e};
+      return run_gemm<DT, Z::MI, Z::NI, false, false>(a, e, st, "train_gemm_kernel (P)");
+    });
     if (rc) return rc;
     if (dH && d > 0) {  // m over d, n over rows, k over the piece
       GemmArgs b = {};
@@ -576,9 +628,9 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
       b.pairs = PL == 3 ? kTermPairs : 1;
       b.splits = p.splits;
       SumEpilogue se = {sums, N * p.dp, (int32_t)N, (int32_t)p.dp, v0 == 0};
-      if (N <= kFewRows) rc = run_gemm<DT, 4, 1, true, false>(b, se, st, "train_gemm_kernel (dH)");
-      else if (p.dp <= 128) rc = run_gemm<DT, 4, 4, true, false>(b, se, st, "train_gemm_kernel (dH)");
-      else rc = run_gemm<DT, 8, 4, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      rc = with_size(p.size_h, [&](auto z) {
+        return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      });
       if (rc) return rc;
     }
     if (dW && d > 0) {  // m over d, n over the piece, k over rows
@@ -595,13 +647,14 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
       b.pairs = PL == 3 ? kTermPairs : 1;
       b.splits = 1;
       WeightEpilogue<OUT> we = {(uint8_t*)dW + v0 * d * (OUT == TMS_DTYPE_F32 ? 4 : 2), factor, (int32_t)nv, (int32_t)d};
-      if (p.dp <= 128) rc = run_gemm<DT, 4, 4, true, true>(b, we, st, "train_gemm_kernel (dW)");
-      else rc = run_gemm<DT, 8, 4, true, true>(b, we, st, "train_gemm_kernel (dW)");
+      rc = with_size(p.size_w, [&](auto z) {
+        return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, true, true>(b, we, st, "train_gemm_kernel (dW)");
+      });
       if (rc) return rc;
     }
   }
   if (dH && d > 0) {
-    hipLaunchKernelGGL(lce_hidden_kernel<OUT>, dim3(blocks_for(N * d)), dim3(256), 0, st, sums, p.splits, N * p.dp, (int32_t)N, (int32_t)d,
+    hipLaunchKernelGGL(lce_hidden_kernel<OUT>, dim3(blocks_for(N * ((d + 3) / 4))), dim3(256), 0, st, sums, p.splits, N * p.dp, (int32_t)N, (int32_t)d,
                        (int32_t)p.dp, factor, dH);
     return check_launch("lce_hidden_kernel");
   }
@@ -646,9 +699,8 @@ extern "C" int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d
     else rc = lce_forward<TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
     if (rc) return rc;
   }
-  if (reduction == TMS_REDUCE_NONE) return TMS_OK;
-  hipLaunchKernelGGL(lce_reduce_kernel, dim3(1), dim3(1024), 0, st, (const float*)(ws + s.loss), target, ignore_index, (int32_t)N,
-                     reduction == TMS_REDUCE_MEAN ? 1 : 0, loss, stats + N);
+  if (N > 0 || reduction == TMS_REDUCE_NONE) return TMS_OK;
+  hipLaunchKernelGGL(lce_reduce_kernel, dim3(1), dim3(1024), 0, st, nullptr, target, ignore_index, 0, reduction == TMS_REDUCE_MEAN ? 1 : 0, loss, stats);
   return check_launch("lce_reduce_kernel");
 }
 
