@@ -370,15 +370,15 @@ int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const vo
 
 /*
  * The gradients of tms_maxsim_pairs, from its positions and `grad`, what comes back for each
- * score (fp32, the scores' shape), with the forward call's qmask: dQ[q, i] = sum_b grad[q, b] D[b, j] and dD[b, j] the sum of
+ * score (fp32, the scores' shape): dQ[q, i] = sum_b grad[q, b] D[b, j] and dD[b, j] the sum of
  * grad[q, b] Qs[q, i] over the (q, i) whose maximum is j, in `dtype`, summed in fp32 in one
  * order. dQ or dD may be NULL. `workspace`: tms_pairs_grad_workspace_size bytes of device
  * memory, 16-byte aligned.
  */
-int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway, int dtype);
+int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nd, int64_t nway);
 int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
-                          int64_t nway, const uint8_t* qmask, const uint16_t* positions, const float* grad, int dtype,
-                          void* workspace, int64_t workspace_bytes, void* dQ, void* dD, void* stream);
+                          int64_t nway, const uint16_t* positions, const float* grad, int dtype, void* workspace,
+                          int64_t workspace_bytes, void* dQ, void* dD, void* stream);
 
 /*
  * Training: softmax cross entropy of the logits scale * hidden weight^T against `target`,

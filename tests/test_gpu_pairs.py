@@ -123,6 +123,26 @@ def test_many(cuda, nQ, Nq, B, Nd, d, dtype):
     check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
 
 
+# more than 128 blocks of 32 query tokens: a document's maxima are sorted in two and three runs
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("nQ,Nq,B,Nd,d", [(150, 5, 30, 20, 64), (130, 3, 70, 300, 33), (95, 40, 8, 17, 136)])
+def test_runs(cuda, nQ, Nq, B, Nd, d, dtype):
+    check(nQ, Nq, B, Nd, d, dtype, seed=nQ)
+
+
+def test_one_token_wins_all(cuda):
+    """Every maximum at one token, the first, a middle or the last one."""
+    def at(j):
+        def edit(Q, D, dmask, qmask):
+            D.zero_()
+            Q.abs_()
+            D[:, j] = 0.125
+            dmask[:] = True
+        return edit
+    for j in (0, 77, 149):
+        check(70, 32, 9, 150, 64, "fp16", edit=at(j))
+
+
 def test_no_masks(cuda):
     check(5, 32, 500, 47, 128, "fp16", masks=False)
     check(2, 20, 6, 100, 128, "bf16", masks=False)

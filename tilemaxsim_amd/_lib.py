@@ -87,9 +87,9 @@ SIGNATURES = {
     "tms_pairs_positions": [_i64, _i64, _i64, _i64],
     "tms_maxsim_pairs": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int, _c_void_p,
                          _i64, _c_void_p, _c_void_p, _c_void_p],
-    "tms_pairs_grad_workspace_size": [_i64, _i64, _i64, _i64, _i64, _int],
-    "tms_maxsim_pairs_grad": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
-                              _int, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
+    "tms_pairs_grad_workspace_size": [_i64, _i64, _i64, _i64, _i64, _i64],
+    "tms_maxsim_pairs_grad": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int,
+                              _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
     "tms_lce_workspace_size": [_i64, _i64, _i64, _int, _int],
     "tms_linear_cross_entropy": [_c_void_p, _i64, _i64, _c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _int, _c_void_p,
                                  _i64, _c_void_p, _c_void_p, _c_void_p],

@@ -394,187 +394,21 @@ struct El<TMS_DTYPE_F32> {
 struct PairsGradArgs {
   const void* Q;
   const void* D;
-  const uint8_t* qmask;
   const uint16_t* arg;
   const float* G;  // (nQ, B) or (nQ, nway)
   void* dQ;
   void* dD;
-  u32x4* frags;  // [plane][block of 32 query tokens][16 columns][lane]
   float* parts;  // [split][nQ * nq][d]
+  float* sums;   // (B * nd, d): dD's sums between two runs of queries
   int64_t B;
   int32_t nQ, nq, nqp, nd, d, nway;
-  int32_t nbq, blocks, cts;       // blocks a query, blocks in all, column tiles
+  int32_t nbq, blocks;            // blocks of 32 tokens a query, blocks in all
+  int32_t run;                    // dD: blocks sorted at a time
   int32_t splits, chunk, tokens;  // dQ: splits of the documents, documents each; document tokens per LDS stage
 };
 
 __device__ __forceinline__ float grad_of(const PairsGradArgs& a, int q, int64_t b) {
   return a.G[a.nway ? b : (int64_t)q * a.B + b];
-}
-
-// Queries as MFMA operands with the block's 32 tokens inside: lane (c, g) holds column
-// 16 ct + c of tokens 8 g .. 8 g + 7. Masked tokens and what lies past the ends are zero.
-template <int DT>
-__global__ __launch_bounds__(256) void pairs_frags_kernel(PairsGradArgs a) {
-  typedef typename El<DT>::T T;
-  constexpr int PL = DT == TMS_DTYPE_F32 ? 3 : 1;
-  const int64_t n = (int64_t)a.blocks * a.cts * 64;
-  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
-    const int lane = (int)(k & 63), c = lane & 15, g = lane >> 4;
-    const int64_t f = k >> 6;
-    const int kb = (int)(f / a.cts), col = (int)(f - (int64_t)kb * a.cts) * 16 + c;
-    const int q = kb / a.nbq, i0 = (kb - q * a.nbq) * 32 + 8 * g;
-    uint16_t v[PL][8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int64_t row = (int64_t)q * a.nq + i0 + e;
-      const bool on = i0 + e < a.nq && col < a.d && (!a.qmask || a.qmask[row] != 0);
-      if constexpr (PL == 1) {
-        v[0][e] = on ? ((const uint16_t*)a.Q)[row * a.d + col] : (uint16_t)0;
-      } else {
-        float x = on ? ((const float*)a.Q)[row * a.d + col] : 0.f;
-#pragma unroll
-        for (int p = 0; p < 3; p++) {
-          const __bf16 t = (__bf16)x;
-          v[p][e] = __builtin_bit_cast(uint16_t, t);
-          x -= (float)t;
-        }
-      }
-    }
-#pragma unroll
-    for (int p = 0; p < PL; p++) {
-      u32x4 w;
-#pragma unroll
-      for (int e = 0; e < 4; e++) w[e] = (uint32_t)v[p][2 * e] | (uint32_t)v[p][2 * e + 1] << 16;
-      a.frags[p * n + k] = w;
-    }
-  }
-}
-
-// Elements that are 1 where the position equals this lane's token (both halves of t2), else 0.
-template <int DT>
-__device__ __forceinline__ u32x4 one_hot(u32x4 at, uint32_t t2) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
-  constexpr uint16_t ONE = DT == TMS_DTYPE_F16 ? 0x3c00 : 0x3f80;
-  u32x4 r;
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const uint32_t x = at[i] ^ t2;
-    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, x), u16x2{1, 1});
-    r[i] = __builtin_bit_cast(uint32_t, (u16x2)(u16x2{ONE, ONE} - m * u16x2{ONE, ONE}));
-  }
-  return r;
-}
-
-// dD as products: for a block of 32 query tokens, the matrix that is 1 where token i's
-// maximum is document token j, times the block, is the sum of the query tokens that j won,
-// exactly (each product is by 0 or 1); times the pair's G it is added to the document's sums
-// in fp32, block after block, so in one order. The ones are made in registers from the
-// positions. A workgroup has one document's up to 4 TT tiles of 16 tokens (a wave every
-// fourth) and 128 columns; the blocks' fragments pass through LDS, one barrier a block.
-// Adding a query's rows one by one in LDS instead was bound by the latency of their loads
-// at the three waves a CU whose sums fit it, 20 times as long at 64 queries x 4096
-// documents x 180 tokens. Bound by the VALU: a tile and block take 8 MFMAs of 16 cycles,
-// and 32 multiply-adds and 12 integer instructions of 4.
-//
-// All CT column tiles of 16 are computed, those past the width on zeros: with a branch between
-// an MFMA and the instruction that takes its result, this compiler leaves out the wait states
-// between the two, and the first of its four values is read before it is there.
-template <int DT, int TT, int CT, int PL>
-__global__ __launch_bounds__(256, TT * CT > 16 ? 2 : 3) void pairs_grad_d_kernel(PairsGradArgs a) {
-  constexpr int MT = PL == 3 ? TMS_DTYPE_BF16 : DT;
-  constexpr int LD = (CT + 3) / 4;  // column tiles a wave loads
-  __shared__ u32x4 ring[2][PL][4 * LD][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int c = lane & 15, g = lane >> 4;
-  const int64_t b = blockIdx.x;
-  const int ct0 = (int)blockIdx.y * CT, cts = a.cts - ct0;
-  const int tile0 = (int)blockIdx.z * 4 * TT + wave;  // and every fourth
-  const int first = a.nway ? (int)(b / a.nway) * a.nbq : 0, count = a.nway ? a.nbq : a.blocks;
-  const uint16_t* arg = a.arg + (a.nway ? b : b * a.nQ) * a.nqp + 8 * g;
-  const int64_t plane = (int64_t)a.blocks * a.cts * 64;
-
-  f32x4 acc[TT][CT];
-#pragma unroll
-  for (int t = 0; t < TT; t++)
-#pragma unroll
-    for (int k = 0; k < CT; k++) acc[t][k] = f32x4{0.f, 0.f, 0.f, 0.f};
-
-  u32x4 fr[PL][LD], at_next = {0u, 0u, 0u, 0u};
-  float w_next = 0.f;
-  auto load = [&](int k) {
-    const int kb = first + k;
-#pragma unroll
-    for (int p = 0; p < PL; p++)
-#pragma unroll
-      for (int i = 0; i < LD; i++) {
-        const int ct = wave * LD + i;
-        fr[p][i] = u32x4{0u, 0u, 0u, 0u};
-        if (ct < cts) fr[p][i] = a.frags[p * plane + ((int64_t)kb * a.cts + ct0 + ct) * 64 + lane];
-      }
-  };
-  auto load_at = [&](int k) {
-    at_next = *(const u32x4*)(arg + k * 32);
-    w_next = grad_of(a, (first + k) / a.nbq, b);
-  };
-  auto put = [&](int buf) {
-#pragma unroll
-    for (int p = 0; p < PL; p++)
-#pragma unroll
-      for (int i = 0; i < LD; i++) ring[buf][p][wave * LD + i][lane] = fr[p][i];
-  };
-  if (count > 0) {
-    load(0);
-    load_at(0);
-    put(0);
-    if (count > 1) load(1);
-  }
-  __syncthreads();
-  for (int k = 0; k < count; k++) {
-    const u32x4 at = at_next;
-    const float w = w_next;
-    if (k + 1 < count) load_at(k + 1);
-    const int buf = k & 1;
-#pragma unroll
-    for (int t = 0; t < TT; t++) {
-      const uint32_t tok = (uint32_t)(tile0 + 4 * t) * 16 + c;
-      const u32x4 hot = one_hot<MT>(at, tok | tok << 16);
-      if (__ballot((hot[0] | hot[1] | hot[2] | hot[3]) != 0u) == 0ull) continue;  // nothing won here
-#pragma unroll
-      for (int ct = 0; ct < CT; ct++) {
-        f32x4 r = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int p = PL - 1; p >= 0; p--) r = mfma16x16x32<MT>(ring[buf][p][ct][lane], hot, r);
-#pragma unroll
-        for (int e = 0; e < 4; e++) acc[t][ct][e] = __builtin_fmaf(w, r[e], acc[t][ct][e]);
-      }
-    }
-    if (k + 1 < count) put(buf ^ 1);
-    if (k + 2 < count) load(k + 2);
-    __syncthreads();
-  }
-  typedef typename El<DT>::T T;
-  const bool four = a.d % 4 == 0;  // and then rows begin at multiples of four elements
-#pragma unroll
-  for (int t = 0; t < TT; t++) {
-    const int tok = (tile0 + 4 * t) * 16 + c;
-    if (tok >= a.nd) continue;
-    T* row = (T*)a.dD + ((int64_t)b * a.nd + tok) * a.d;
-#pragma unroll
-    for (int ct = 0; ct < CT; ct++) {
-      const int col = (ct0 + ct) * 16 + 4 * g;
-      if (col >= a.d) continue;
-      struct alignas(4 * sizeof(T)) Four {
-        T v[4];
-      } x;
-#pragma unroll
-      for (int e = 0; e < 4; e++) x.v[e] = (T)acc[t][ct][e];
-      if (four) *(Four*)(row + col) = x;
-      else
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (col + e < a.d) row[col + e] = x.v[e];
-    }
-  }
 }
 
 // Two neighbouring columns of a row, as floats.
@@ -591,6 +425,204 @@ __device__ __forceinline__ f32x2 two(const uint8_t* p) {
       const f16x2 h = __builtin_bit_cast(f16x2, x);
       return f32x2{(float)h[0], (float)h[1]};
     }
+  }
+}
+
+// dD: a document's maxima are sorted by the token that won them, and each token adds the query
+// tokens that it won, read one 256-byte row a wave's access, in the order of the queries: no
+// sum depends on timing, and only rows that won or were won are touched. A workgroup has a
+// document and 128 columns (two a lane). The sort is a counting sort in LDS, four bits of the
+// token at a time: a thread counts and places its own run of maxima, so equal tokens keep their
+// order. Then each wave takes a quarter of the sorted maxima, cut between tokens, with the
+// rows of the next eight in flight while eight are added: 20 cycles of VALU work a maximum.
+// (Products with a matrix of ones made from the positions cost a multiply-add for each column,
+// token and query block as well: 560 us at 64 queries x 4096 documents x 180 tokens.)
+// More than kRun blocks are sorted in runs; the sums stand in memory between them, in fp32.
+constexpr int kRun = 128;  // blocks of 32 maxima: 32 KB of LDS
+
+// Two columns of a row of Q.
+template <int DT, bool PAIR>
+__device__ __forceinline__ f32x2 columns(const typename El<DT>::T* row, int col, int d) {
+  if constexpr (PAIR) return two<DT>((const uint8_t*)(row + col));
+  return f32x2{(float)row[col], col + 1 < d ? (float)row[col + 1] : 0.f};
+}
+
+template <int DT, bool PAIR>
+__global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
+  typedef typename El<DT>::T T;
+  constexpr int AHEAD = 8;
+  extern __shared__ __attribute__((aligned(16))) uint8_t sort_mem[];
+  const int most = a.run * 32;
+  uint16_t* tok = (uint16_t*)sort_mem;                // the maxima's tokens; nd for none
+  uint16_t* order[2] = {tok + most, tok + 2 * most};  // maxima in sorted order
+  uint16_t* count = tok + 3 * most;                   // [digit][thread]
+  float* weight = (float*)(count + 16 * 256);         // G of the run's blocks
+  __shared__ int totals[4], cuts[5];
+  const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+  const int64_t b = blockIdx.x;
+  const int col = (int)blockIdx.y * 128 + 2 * lane;
+  const bool in = col < a.d;
+  const int first = a.nway ? (int)(b / a.nway) * a.nbq : 0, blocks = a.nway ? a.nbq : a.blocks;
+  const uint16_t* arg = a.arg + (a.nway ? b : b * a.nQ) * a.nqp;
+  const T* Q = (const T*)a.Q;
+  int bits = 0;
+  while ((a.nd >> bits) != 0) bits++;
+
+  for (int k0 = 0; k0 < blocks || k0 == 0; k0 += a.run) {
+    const int nb = blocks - k0 < a.run ? blocks - k0 : a.run, n = nb * 32;
+    const int per = (n + 255) / 256;  // maxima a thread, in a row
+    const bool begun = k0 > 0, last = k0 + a.run >= blocks;
+    __syncthreads();  // the run before has read what is written here, and its sums are in memory
+    for (int i = t * 8; i < n; i += 256 * 8) {
+      const u32x4 v = *(const u32x4*)(arg + (int64_t)k0 * 32 + i);
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const uint32_t j = (v[e / 2] >> (16 * (e & 1))) & 0xffffu;
+        tok[i + e] = (uint16_t)(j < (uint32_t)a.nd ? j : (uint32_t)a.nd);
+      }
+    }
+    for (int k = t; k < nb; k += 256) weight[k] = grad_of(a, (first + k0 + k) / a.nbq, b);
+    int from = 0;
+    for (int shift = 0; shift < bits || shift == 0; shift += 4) {
+#pragma unroll
+      for (int g = 0; g < 16; g++) count[g * 256 + t] = 0;
+      __syncthreads();
+      const int i0 = t * per, i1 = i0 + per < n ? i0 + per : n;
+      for (int i = i0; i < i1; i++) {
+        const int e = shift == 0 ? i : order[from][i];
+        count[((tok[e] >> shift) & 15) * 256 + t]++;
+      }
+      __syncthreads();
+      // exclusive sums over (digit, thread): sixteen in a row a thread, then over the threads
+      u32x4* mine = (u32x4*)(count + 16 * t);
+      u32x4 c[2] = {mine[0], mine[1]};
+      int sum = 0;
+#pragma unroll
+      for (int g = 0; g < 16; g++) {
+        const int x = (int)((c[g / 8][(g / 2) & 3] >> (16 * (g & 1))) & 0xffffu);
+        sum += x;
+      }
+      int before = sum;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_up(before, o);
+        before += lane >= o ? x : 0;
+      }
+      if (lane == 63) totals[wave] = before;
+      __syncthreads();
+      before -= sum;
+      for (int w = 0; w < wave; w++) before += totals[w];
+#pragma unroll
+      for (int h = 0; h < 8; h++) {
+        const uint32_t x = c[h / 4][h & 3], lo = x & 0xffffu, hi = x >> 16;
+        c[h / 4][h & 3] = (uint32_t)before | (uint32_t)(before + (int)lo) << 16;
+        before += (int)(lo + hi);
+      }
+      mine[0] = c[0];
+      mine[1] = c[1];
+      __syncthreads();
+      const int to = shift == 0 ? 0 : from ^ 1;
+      for (int i = i0; i < i1; i++) {
+        const int e = shift == 0 ? i : order[from][i];
+        order[to][count[((tok[e] >> shift) & 15) * 256 + t]++] = (uint16_t)e;
+      }
+      from = to;
+      __syncthreads();
+    }
+    // The waves' shares, cut at the first maximum of a token; those of no token come last.
+    const uint16_t* sorted = order[from];
+    if (t < 5) {
+      int lo = 0, hi = n;
+      while (lo < hi) {  // how many have a token
+        const int mid = (lo + hi) / 2;
+        if (tok[sorted[mid]] < a.nd) lo = mid + 1;
+        else hi = mid;
+      }
+      const int real = lo;
+      int k = (int)((int64_t)real * t / 4);
+      if (k > 0 && k < real) {  // the first one of the next token, if this one's is cut
+        const int j = tok[sorted[k - 1]];
+        hi = real;
+        while (k < hi) {
+          const int mid = (k + hi) / 2;
+          if (tok[sorted[mid]] <= j) k = mid + 1;
+          else hi = mid;
+        }
+      }
+      cuts[t] = k;
+    }
+    __syncthreads();
+    const int m0 = __builtin_amdgcn_readfirstlane(cuts[wave]), m1 = __builtin_amdgcn_readfirstlane(cuts[wave + 1]);
+    // this wave's tokens: from the first of its share up to the next wave's first
+    const int real = __builtin_amdgcn_readfirstlane(cuts[4]);
+    const int j0 = wave == 0 ? 0 : m0 < real ? tok[sorted[m0]] : a.nd;
+    const int j1 = wave == 3 || m1 >= real ? a.nd : tok[sorted[m1]];
+    int cur = __builtin_amdgcn_readfirstlane(j0);
+    const int end = __builtin_amdgcn_readfirstlane(j1);
+    float x0 = 0.f, x1 = 0.f;
+    auto flush = [&](int j) {
+      if (in) {
+        const int64_t at = ((int64_t)b * a.nd + j) * a.d + col;
+        if (begun) {
+          x0 += a.sums[at];
+          if (col + 1 < a.d) x1 += a.sums[at + 1];
+        }
+        if (!last) {
+          a.sums[at] = x0;
+          if (col + 1 < a.d) a.sums[at + 1] = x1;
+        } else {
+          T* out = (T*)a.dD + at;
+          if constexpr (PAIR) {
+            struct alignas(2 * sizeof(T)) Two {
+              T v[2];
+            };
+            *(Two*)out = Two{{(T)x0, (T)x1}};
+          } else {
+            out[0] = (T)x0;
+            if (col + 1 < a.d) out[1] = (T)x1;
+          }
+        }
+      }
+      x0 = x1 = 0.f;
+    };
+    // Sixty-four maxima at a time: each lane finds one's row and factor, and the wave takes
+    // them from the lanes one after another.
+    for (int m = m0; m < m1; m += 64) {
+      const int here = m1 - m < 64 ? m1 - m : 64;
+      const int e = sorted[m + (lane < here ? lane : here - 1)];
+      const int k = first + k0 + (e >> 5), q = k / a.nbq;
+      const int row = q * a.nq + (k - q * a.nbq) * 32 + (e & 31);
+      const int j = tok[e];
+      const float w = weight[e >> 5];
+      f32x2 x[2][AHEAD];
+      auto load = [&](int buf, int s) {
+        if (s >= here) return;
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+          const int r = __builtin_amdgcn_readlane(row, s + i < here ? s + i : here - 1);
+          x[buf][i] = in ? columns<DT, PAIR>(Q + (int64_t)r * a.d, col, a.d) : f32x2{0.f, 0.f};
+        }
+      };
+      auto add = [&](int buf, int s) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; i++) {
+          if (s + i >= here) break;
+          const int js = __builtin_amdgcn_readlane(j, s + i);
+          while (cur != js) flush(cur++);
+          const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + i));
+          x0 = __builtin_fmaf(ws, x[buf][i][0], x0);
+          x1 = __builtin_fmaf(ws, x[buf][i][1], x1);
+        }
+      };
+      load(0, 0);
+      for (int s = 0; s < here; s += 2 * AHEAD) {
+        load(1, s + AHEAD);
+        add(0, s);
+        load(0, s + 2 * AHEAD);
+        add(1, s + AHEAD);
+      }
+    }
+    while (cur < end) flush(cur++);
   }
 }
 
@@ -894,33 +926,19 @@ __global__ void pairs_fill_kernel(float* scores, int64_t n, float v, uint16_t* a
   }
 }
 
-template <int DT, int TT, int CT>
-static int run_grad_d(const PairsGradArgs& a, hipStream_t st) {
-  const int tiles = (a.nd + 15) / 16;
-  const dim3 grid((unsigned)a.B, (unsigned)((a.cts + CT - 1) / CT), (unsigned)((tiles + 4 * TT - 1) / (4 * TT)));
-  hipLaunchKernelGGL((pairs_grad_d_kernel<DT, TT, CT, DT == TMS_DTYPE_F32 ? 3 : 1>), grid, dim3(256), 0, st, a);
-  return check_launch("pairs_grad_d_kernel");
-}
-// Tiles a wave: as many as the document has for each of four waves, up to four.
-template <int DT, int CT>
-static int run_grad_d_tiles(const PairsGradArgs& a, hipStream_t st) {
-  if (a.nd <= 64) return run_grad_d<DT, 1, CT>(a, st);
-  if (a.nd <= 128) return run_grad_d<DT, 2, CT>(a, st);
-  if (a.nd <= 192) return run_grad_d<DT, 3, CT>(a, st);
-  return run_grad_d<DT, 4, CT>(a, st);
-}
-
 template <int DT>
 static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
   int rc;
   if (a.dD && a.B > 0 && a.nd > 0 && a.d > 0) {
-    const int64_t n = (int64_t)a.blocks * a.cts * 64;
-    if (n > 0) {
-      hipLaunchKernelGGL(pairs_frags_kernel<DT>, dim3((unsigned)(n > 256 * 4096 ? 4096 : (n + 255) / 256)), dim3(256), 0, st, a);
-      if ((rc = check_launch("pairs_frags_kernel"))) return rc;
-    }
-    rc = a.cts <= 2 ? run_grad_d_tiles<DT, 2>(a, st) : a.cts <= 4 ? run_grad_d_tiles<DT, 4>(a, st) : run_grad_d_tiles<DT, 8>(a, st);
-    if (rc) return rc;
+    const int n = a.nway ? a.nbq : a.blocks;
+    a.run = n < 1 ? 1 : n < kRun ? n : kRun;
+    const size_t lds = (size_t)a.run * 32 * 6 + 16 * 256 * 2 + (size_t)a.run * 4;
+    const dim3 grid((unsigned)a.B, (unsigned)((a.d + 127) / 128));
+    // rows whose pairs of columns are whole words
+    const bool pair = a.d % 2 == 0 && (uintptr_t)a.Q % 8 == 0 && (uintptr_t)a.dD % 8 == 0;
+    if (pair) hipLaunchKernelGGL((pairs_grad_d_kernel<DT, true>), grid, dim3(256), lds, st, a);
+    else hipLaunchKernelGGL((pairs_grad_d_kernel<DT, false>), grid, dim3(256), lds, st, a);
+    if ((rc = check_launch("pairs_grad_d_kernel"))) return rc;
   }
   if (a.dQ && a.nQ > 0 && a.nq > 0 && a.d > 0) {
     const unsigned cols = (unsigned)((a.d + 127) / 128);
@@ -1015,19 +1033,17 @@ extern "C" int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t 
   return run_pairs<TMS_DTYPE_BF16, 3>(a, st);
 }
 
-static int64_t frags_bytes(int64_t nQ, int64_t nq, int64_t d, int dtype) {
-  return nQ * ((nq + 31) / 32) * ((d + 15) / 16) * 1024 * planes(dtype);
-}
-static int64_t parts_bytes(int64_t nQ, int64_t nq, int64_t d, const GradQ& f) { return f.splits > 1 ? f.splits * nQ * nq * d * 4 : 0; }
+static int64_t parts_bytes(int64_t nQ, int64_t nq, int64_t d, const GradQ& f) { return f.splits > 1 ? round_up(f.splits * nQ * nq * d * 4, 256) : 0; }
 
-extern "C" int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway, int dtype) {
-  if (nQ <= 0 || nq <= 0 || d <= 0 || B <= 0) return 0;
-  return frags_bytes(nQ, nq, d, dtype) + parts_bytes(nQ, nq, d, grad_q_form(nQ, nq, d, B, nway));
+extern "C" int64_t tms_pairs_grad_workspace_size(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nd, int64_t nway) {
+  if (nQ <= 0 || nq <= 0 || d <= 0 || B <= 0 || nd < 0) return 0;
+  const int64_t runs = nway > 0 ? (nq + 31) / 32 : nQ * ((nq + 31) / 32);
+  return parts_bytes(nQ, nq, d, grad_q_form(nQ, nq, d, B, nway)) + (runs > kRun ? B * nd * d * 4 : 0);
 }
 
 extern "C" int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, const void* D, int64_t B, int64_t nd,
-                                     int64_t nway, const uint8_t* qmask, const uint16_t* positions, const float* grad, int dtype,
-                                     void* workspace, int64_t workspace_bytes, void* dQ, void* dD, void* stream) {
+                                     int64_t nway, const uint16_t* positions, const float* grad, int dtype, void* workspace,
+                                     int64_t workspace_bytes, void* dQ, void* dD, void* stream) {
   const char* fn = "tms_maxsim_pairs_grad";
   const int rc = check_pairs(fn, nQ, nq, d, B, nd, nway, dtype);
   if (rc) return rc;
@@ -1035,19 +1051,19 @@ extern "C" int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int
       (nQ * nq > 0 && B > 0 && (!positions || !grad)))
     return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
   if ((uintptr_t)positions % 16) return fail(TMS_ERR_INVALID, "%s: positions must be 16-byte aligned", fn);
-  const int64_t need = tms_pairs_grad_workspace_size(nQ, nq, d, B, nway, dtype);
+  const int64_t need = tms_pairs_grad_workspace_size(nQ, nq, d, B, nd, nway);
   if (need > 0 && (!workspace || (uintptr_t)workspace % 16 || workspace_bytes < need))
     return fail(TMS_ERR_INVALID, "%s: a workspace of %lld bytes is needed, 16-byte aligned", fn, (long long)need);
   PairsGradArgs a = {};
   a.Q = Qs;
   a.D = D;
-  a.qmask = qmask;
   a.arg = positions;
   a.G = grad;
   a.dQ = dQ;
   a.dD = dD;
-  a.frags = (u32x4*)workspace;
-  a.parts = (float*)((uint8_t*)workspace + frags_bytes(nQ, nq, d, dtype));
+  const GradQ form = grad_q_form(nQ, nq, d, B, nway);
+  a.parts = (float*)workspace;
+  a.sums = (float*)((uint8_t*)workspace + parts_bytes(nQ, nq, d, form));
   a.B = B;
   a.nQ = (int32_t)nQ;
   a.nq = (int32_t)nq;
@@ -1057,8 +1073,6 @@ extern "C" int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int
   a.nway = (int32_t)nway;
   a.nbq = (int32_t)((nq + 31) / 32);
   a.blocks = a.nQ * a.nbq;
-  a.cts = (int32_t)((d + 15) / 16);
-  const GradQ form = grad_q_form(nQ, nq, d, B, nway);
   const hipStream_t st = (hipStream_t)stream;
   if (dtype == TMS_DTYPE_F16) return run_grads<TMS_DTYPE_F16>(a, form, st);
   if (dtype == TMS_DTYPE_BF16) return run_grads<TMS_DTYPE_BF16>(a, form, st);

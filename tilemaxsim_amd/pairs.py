@@ -49,14 +49,14 @@ class _Pairs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, Q, D, qmask, dmask, nway):
         scores, positions = _forward(Q, D, qmask, dmask, nway, True)
-        ctx.save_for_backward(Q, D, qmask, positions)
+        ctx.save_for_backward(Q, D, positions)
         ctx.nway = nway
         return scores
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        Q, D, qmask, positions = ctx.saved_tensors
+        Q, D, positions = ctx.saved_tensors
         nQ, Nq, d = Q.shape
         nway = ctx.nway
         Nd = D.shape[-2]
@@ -65,11 +65,10 @@ class _Pairs(torch.autograd.Function):
         grad = grad.contiguous()
         dQ = torch.empty_like(Q) if ctx.needs_input_grad[0] else None
         dD = torch.empty_like(D) if ctx.needs_input_grad[1] else None
-        code = _lib.dtype_code(D.dtype)
-        nbytes = lib.tms_pairs_grad_workspace_size(nQ, Nq, d, B, nway, code)
+        nbytes = lib.tms_pairs_grad_workspace_size(nQ, Nq, d, B, Nd, nway)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=D.device) if nbytes else None
         status = _lib.launch(D.device, lib.tms_maxsim_pairs_grad, Q.data_ptr(), nQ, Nq, d, D.data_ptr(), B, Nd, nway,
-                             _lib.ptr(qmask), positions.data_ptr(), grad.data_ptr(), code, _lib.ptr(ws), nbytes,
+                             positions.data_ptr(), grad.data_ptr(), _lib.dtype_code(D.dtype), _lib.ptr(ws), nbytes,
                              _lib.ptr(dQ), _lib.ptr(dD))
         if status:
             _lib.check(status)
