@@ -44,13 +44,10 @@ struct Best {
   float v;
   int at;
 };
-__device__ __forceinline__ void take(Best& r, const f32x4& s, int first) {
-#pragma unroll
-  for (int i = 0; i < 4; i++) {
-    const bool up = s[i] > r.v;
-    r.v = up ? s[i] : r.v;
-    r.at = up ? first + i : r.at;
-  }
+__device__ __forceinline__ void take(Best& r, float s, int at) {
+  const bool up = s > r.v;  // with fmaxf each value would be made canonical first
+  r.at = up ? at : r.at;
+  r.v = up ? s : r.v;
 }
 __device__ __forceinline__ Best better(Best x, Best y) {
   const bool up = y.v > x.v || (y.v == x.v && y.at < x.at);
@@ -66,6 +63,22 @@ __device__ __forceinline__ Best across_rows(Best r) {
   const auto v1 = __builtin_amdgcn_permlane16_swap(w, w, false, false);
   const auto i1 = __builtin_amdgcn_permlane16_swap(j, j, false, false);
   return better({__builtin_bit_cast(float, (unsigned)v1[0]), (int)i1[0]}, {__builtin_bit_cast(float, (unsigned)v1[1]), (int)i1[1]});
+}
+
+// Two registers' rows in one, compared: with 32, lanes 0-31 get x over both halves of the wave
+// and lanes 32-63 y; with 16, even rows get x over their pair of rows and odd rows y.
+template <int N>
+__device__ __forceinline__ Best swap_rows(Best x, Best y) {
+  const unsigned xv = __builtin_bit_cast(unsigned, x.v), yv = __builtin_bit_cast(unsigned, y.v);
+  if constexpr (N == 32) {
+    const auto v = __builtin_amdgcn_permlane32_swap(xv, yv, false, false);
+    const auto i = __builtin_amdgcn_permlane32_swap((unsigned)x.at, (unsigned)y.at, false, false);
+    return better({__builtin_bit_cast(float, (unsigned)v[0]), (int)i[0]}, {__builtin_bit_cast(float, (unsigned)v[1]), (int)i[1]});
+  } else {
+    const auto v = __builtin_amdgcn_permlane16_swap(xv, yv, false, false);
+    const auto i = __builtin_amdgcn_permlane16_swap((unsigned)x.at, (unsigned)y.at, false, false);
+    return better({__builtin_bit_cast(float, (unsigned)v[0]), (int)i[0]}, {__builtin_bit_cast(float, (unsigned)v[1]), (int)i[1]});
+  }
 }
 
 template <bool V>
@@ -152,7 +165,8 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         mask_tile(acc[h], bits, g);  // not behind a branch, for one would follow an MFMA
-        take(best[h], acc[h], t * 16 + 4 * g);
+#pragma unroll
+        for (int i = 0; i < 4; i++) take(best[h], acc[h][i], t * 16 + 4 * g + i);
       }
     }
 #pragma unroll
@@ -187,16 +201,23 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 // Eight waves hold up to 8 NB blocks of 32 query tokens in registers and walk the same
 // documents: each 64-token stage comes from memory once, through registers into one of two
 // LDS buffers in MFMA fragment order (the reads are whole and conflict-free), so a token
-// costs 1 / (8 NB) of a load per block. Bound by the matrix cores and the maxima's VALU work.
-// One barrier a stage: a stage is written to the buffer that every wave left before the
-// last one. Masks become 64-bit words in LDS first; stages of padding are never loaded.
+// costs 1 / (8 NB) of a load per block. One barrier a stage: a stage is written to the buffer
+// that every wave left before the last one. Masks become 64-bit words in LDS first, and the
+// words with a real token a list, so that stages of padding are neither loaded nor looked at.
 // Whole queries belong to a wave, so a score is summed in one place and in one order.
+//
+// A block's 16 x 16 similarities are a chain of MFMAs (4 of 16 cycles at d = 128), and
+// their maxima twelve VALU instructions of 4 cycles; a wave issues in order, so the maxima of
+// one block are put between the MFMAs of the next. (One block after the other, 395 us for
+// 64 queries x 4096 documents x 60 to 180 tokens.)
 template <int DT, int KS, int NB, int PL>
 __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
   constexpr int FS = 4 * PL * KS;  // fragments of a stage
   constexpr int LD = (FS + 7) / 8;  // fragments a wave loads
+  constexpr int NP = (NB + 1) / 2;  // pairs of blocks, at a document's end
   __shared__ u32x4 ring[2][FS][64];
   __shared__ uint64_t words[kMaskWords];
+  __shared__ uint32_t list[kMaskWords + 2];  // document << 16 | stage of the words that are not 0
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int r = lane & 15, g = lane >> 4;
   const int64_t b0 = (int64_t)blockIdx.x * a.docs_per_wg;
@@ -205,13 +226,22 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
   const int64_t width = (int64_t)a.d * 2;
   const int q0 = ((int)blockIdx.y * 8 + wave) * a.qpw;  // this wave's first query
 
-  for (int w = wave; w < ndocs * stages; w += 8) {
-    const int doc = w / stages, tok = (w - doc * stages) * kStage + lane;
-    const bool live = tok < a.nd && (!a.dmask || a.dmask[(b0 + doc) * a.nd + tok] != 0);
-    const uint64_t bits = __ballot(live);
-    if (lane == 0) words[w] = bits;
-  }
-
+  // Everything below reads memory once or twice and then waits: loads first, in batches.
+  const int nwords = ndocs * stages;
+  auto mask_words = [&](int w0) {
+    bool live[8];
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const int w = w0 + 8 * k, doc = w / stages, tok = (w - doc * stages) * kStage + lane;
+      live[k] = w < nwords && tok < a.nd;
+      if (live[k] && a.dmask) live[k] = a.dmask[(b0 + doc) * a.nd + tok] != 0;
+    }
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+      const uint64_t bits = __ballot(live[k]);
+      if (lane == 0 && w0 + 8 * k < nwords) words[w0 + 8 * k] = bits;
+    }
+  };
   u32x4 qf[NB][PL][KS][2];
   uint32_t real = 0;  // bit 2 j + h: this lane's token of half h of block j
 #pragma unroll
@@ -221,28 +251,48 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
       const int q = q0 + j / a.nbq, tok = (j % a.nbq) * 32 + 16 * h + r;
       const bool in = j < a.qpw * a.nbq && q < a.nQ && tok < a.nq;
       const int64_t row = in ? (int64_t)q * a.nq + tok : 0;
-      const bool on = in && (!a.qmask || a.qmask[row] != 0);
+      uint8_t on = in ? 1 : 0;
+      if (a.qmask) on = in ? a.qmask[row] : 0;
       real |= (on ? 1u : 0u) << (2 * j + h);
 #pragma unroll
       for (int p = 0; p < PL; p++)
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-          const u32x4 v = *(const u32x4*)(a.Q + p * a.qplane + row * width + 64 * s + 16 * g);
-          qf[j][p][s][h] = on ? v : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int s = 0; s < KS; s++) qf[j][p][s][h] = *(const u32x4*)(a.Q + p * a.qplane + row * width + 64 * s + 16 * g);
     }
+  for (int w = wave; w < nwords; w += 64) mask_words(w);
+#pragma unroll
+  for (int j = 0; j < NB; j++)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+      for (int p = 0; p < PL; p++)
+#pragma unroll
+        for (int s = 0; s < KS; s++) qf[j][p][s][h] = (real >> (2 * j + h)) & 1u ? qf[j][p][s][h] : u32x4{0u, 0u, 0u, 0u};
   __syncthreads();
+  if (wave == 0) {
+    int n = 0;
+    for (int w = lane; w - lane < nwords; w += 64) {
+      const bool some = w < nwords && words[w] != 0;
+      const uint64_t all = __ballot(some);
+      const int doc = w / stages;
+      if (some) list[n + __popcll(all & ((1ull << lane) - 1))] = (uint32_t)doc << 16 | (uint32_t)(w - doc * stages);
+      n += __popcll(all);
+    }
+    if (lane == 0) list[kMaskWords + 1] = (uint32_t)n;
+  }
+  __syncthreads();
+  const int total = __builtin_amdgcn_readfirstlane((int)list[kMaskWords + 1]);
 
-  const int total = ndocs * stages;
-  // the first stage from w on with a real token; `total` past the end
-  auto seek = [&](int w) -> int {
-    while (w < total && words[w] == 0) w++;
-    return __builtin_amdgcn_readfirstlane(w);
-  };
   u32x4 stg[LD];
-  auto load = [&](int w) {
-    if (w >= total) return;
-    const int doc = w / stages, t0 = (w - doc * stages) * kStage;
+  // the n-th stage of the list, and which of its tokens are real: looked up two stages ahead
+  auto entry = [&](int n) -> uint32_t { return __builtin_amdgcn_readfirstlane(list[n < total ? n : 0]); };
+  auto bits_of = [&](uint32_t e) -> uint64_t {
+    const uint64_t w = words[(int)(e >> 16) * stages + (int)(e & 0xffffu)];
+    return (uint64_t)wave_uniform((int64_t)w);
+  };
+  auto load = [&](uint32_t e) {
+    const int t0 = (int)(e & 0xffffu) * kStage;
+    const int64_t row0 = (b0 + (e >> 16)) * a.nd;
 #pragma unroll
     for (int k = 0; k < LD; k++) {
       const int f = wave + 8 * k;  // fragment: tile, plane, k-step
@@ -250,7 +300,7 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
         const int tile = f / (PL * KS), p = (f / KS) % PL, s = f % KS;
         int tok = t0 + tile * 16 + r;
         tok = tok < a.nd ? tok : a.nd - 1;
-        stg[k] = *(const u32x4*)(a.D + p * a.dplane + ((b0 + doc) * a.nd + tok) * width + 64 * s + 16 * g);
+        stg[k] = *(const u32x4*)(a.D + p * a.dplane + (row0 + tok) * width + 64 * s + 16 * g);
       }
     }
   };
@@ -266,84 +316,131 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
 #pragma unroll
   for (int j = 0; j < NB; j++) best[j][0] = best[j][1] = {-__builtin_inff(), kNone};
 
-  int cur = seek(0), nxt = cur < total ? seek(cur + 1) : total;
-  load(cur);
-  if (cur < total) put(0);
-  load(nxt);
+  uint32_t cur = 0, nxt = 0;
+  uint64_t cur_bits = 0, nxt_bits = 0;
+  if (total > 0) {
+    cur = entry(0);
+    load(cur);
+    nxt = entry(1);
+    cur_bits = bits_of(cur);
+    nxt_bits = bits_of(nxt);
+    put(0);
+    if (total > 1) load(nxt);
+  }
   __syncthreads();
-  int buf = 0;
-  while (cur < total) {
-    const int doc = cur / stages, t0 = (cur - doc * stages) * kStage;
-    const uint64_t bits64 = words[cur];
-    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)bits64);
-    const uint32_t hi = __builtin_amdgcn_readfirstlane((uint32_t)(bits64 >> 32));
-#pragma unroll
-    for (int tile = 0; tile < 4; tile++) {
-      const uint32_t bits = ((tile & 2 ? hi : lo) >> (16 * (tile & 1))) & 0xffffu;
-      if (bits == 0) continue;
-      u32x4 df[PL][KS];
+  for (int n = 0; n < total; n++) {
+    const int buf = n & 1;
+    const int doc = (int)(cur >> 16), t0 = (int)(cur & 0xffffu) * kStage;
+    const uint32_t after_at = list[n + 2 < total ? n + 2 : 0];  // read ahead of the products
+    // a tile's fragments are read while the tile before is scored (three planes have no room)
+    constexpr int AHEAD = PL == 1 ? 2 : 1;
+    u32x4 frags[AHEAD][PL][KS];
+    auto read = [&](int tile) {
 #pragma unroll
       for (int p = 0; p < PL; p++)
 #pragma unroll
-        for (int s = 0; s < KS; s++) df[p][s] = ring[buf][(tile * PL + p) * KS + s][lane];
+        for (int s = 0; s < KS; s++) frags[tile % AHEAD][p][s] = ring[buf][(tile * PL + p) * KS + s][lane];
+    };
+    if constexpr (AHEAD == 2) read(0);
+#pragma unroll
+    for (int tile = 0; tile < 4; tile++) {
+      if constexpr (AHEAD == 1) read(tile);
+      else if (tile < 3) read(tile + 1);
+      const uint32_t bits = (uint32_t)(cur_bits >> (16 * tile)) & 0xffffu;
+      if (bits == 0) continue;
+      const auto& df = frags[tile % AHEAD];
+      const int first = t0 + tile * 16 + 4 * g;
       // one body for whole tiles and one for masked ones: no branch behind an MFMA
       auto score = [&](auto masked) {
+        f32x4 acc[2][2];  // a block's two halves, and the block's before
 #pragma unroll
-        for (int j = 0; j < NB; j++)
-#pragma unroll
-          for (int h = 0; h < 2; h++) {
-            f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j <= NB; j++) {
+          if (j < NB) {
+            f32x4 v[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
 #pragma unroll
             for (int p = PL == 1 ? 5 : 0; p < 6; p++)
 #pragma unroll
-              for (int s = 0; s < KS; s++) acc = mfma16x16x32<DT>(df[kPairD[p]][s], qf[j][kPairQ[p]][s][h], acc);
-            if constexpr (decltype(masked)::value) mask_tile(acc, bits, g);
-            take(best[j][h], acc, t0 + tile * 16 + 4 * g);
+              for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) v[h] = mfma16x16x32<DT>(df[kPairD[p]][s], qf[j < NB ? j : 0][kPairQ[p]][s][h], v[h]);
+            acc[j & 1][0] = v[0];
+            acc[j & 1][1] = v[1];
           }
+          if (j > 0) {
+            f32x4(&v)[2] = acc[(j - 1) & 1];
+            if constexpr (decltype(masked)::value) mask_tile(v[0], bits, g), mask_tile(v[1], bits, g);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+#pragma unroll
+              for (int h = 0; h < 2; h++) take(best[j - 1][h], v[h][i], first + i);
+          }
+          constexpr int MF = (PL == 1 ? KS : 6 * KS) * 2, VA = (24 + MF - 1) / MF;
+          if (j == 0) __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
+          if (j > 0 && j < NB) {
+#pragma unroll
+            for (int s = 0; s < MF; s++) {  // an MFMA, then a share of the maxima
+              __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+              __builtin_amdgcn_sched_group_barrier(0x002, VA, 0);
+            }
+          }
+        }
       };
       if (bits == 0xffffu) score(Flag<false>());
       else score(Flag<true>());
     }
-    const int after = nxt < total ? seek(nxt + 1) : total;
-    if (nxt >= total || nxt / stages != doc) {  // the document's end
+    const uint32_t after = __builtin_amdgcn_readfirstlane(after_at);
+    const uint64_t after_bits = bits_of(after);
+    if (n + 1 >= total || (nxt >> 16) != (uint32_t)doc) {  // the document's end
       const int64_t b = b0 + doc;
-      float sum = 0.f;
+      float sums[NB];
+#pragma unroll
+      for (int P = 0; P < NP; P++) {
+        // Row g of the wave ends with half g / 2 of block 2 P + g % 2: each swap brings two
+        // registers' rows together in one, so two blocks take three comparisons.
+        constexpr int last = NB - 1;
+        const int j1 = 2 * P + 1 < NB ? 2 * P + 1 : last;
+        const Best x = swap_rows<32>(best[2 * P][0], best[2 * P][1]);
+        const Best y = 2 * P + 1 < NB ? swap_rows<32>(best[j1][0], best[j1][1]) : x;
+        const Best z = swap_rows<16>(x, y);
+        const int j = 2 * P + (2 * P + 1 < NB ? (g & 1) : 0), h = g >> 1;
+        const bool on = (real >> (2 * j + h)) & 1u;
+        const int q = q0 + j / a.nbq, tok = (j % a.nbq) * 32 + 16 * h + r;
+        if (a.arg && j < a.qpw * a.nbq && q < a.nQ && tok < a.nqp && (2 * P + 1 < NB || (g & 1) == 0))
+          a.arg[arg_at(a, q, b) + tok] = (uint16_t)(on ? z.at : kNone);
+        float s = row_sum16(on ? z.v : 0.f);
+        const auto hs = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, s), __builtin_bit_cast(unsigned, s), false, false);
+        s = __builtin_bit_cast(float, (unsigned)hs[0]) + __builtin_bit_cast(float, (unsigned)hs[1]);  // the halves of a block
+        sums[2 * P] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), 0));
+        if (2 * P + 1 < NB) sums[j1] = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, s), 16));
+      }
+      float score = 0.f;  // lane k: query q0 + k
 #pragma unroll
       for (int j = 0; j < NB; j++) {
-        const int q = q0 + j / a.nbq, blk = j % a.nbq;
-        const Best x0 = across_rows(best[j][0]), x1 = across_rows(best[j][1]);
+        score += lane == j / a.nbq ? sums[j] : 0.f;
         best[j][0] = best[j][1] = {-__builtin_inff(), kNone};
-        if (j < a.qpw * a.nbq && q < a.nQ) {
-          const bool on0 = (real >> (2 * j)) & 1u, on1 = (real >> (2 * j + 1)) & 1u;
-          if (a.arg && g < 2) {
-            const int tok = blk * 32 + lane;
-            const int at = g == 0 ? (on0 ? x0.at : kNone) : (on1 ? x1.at : kNone);
-            if (tok < a.nqp) a.arg[arg_at(a, q, b) + tok] = (uint16_t)at;
-          }
-          const float s = row_sum16((on0 ? x0.v : 0.f) + (on1 ? x1.v : 0.f));
-          sum = blk == 0 ? s : sum + s;
-          if (blk == a.nbq - 1 && lane == 0) a.scores[score_at(a, q, b)] = sum;
-        }
       }
+      if (lane < a.qpw && q0 + lane < a.nQ) a.scores[score_at(a, q0 + lane, b)] = score;
     }
-    if (nxt < total) put(buf ^ 1);
-    load(after);
+    if (n + 1 < total) put(buf ^ 1);
+    if (n + 2 < total) load(after);
     __syncthreads();
-    buf ^= 1;
     cur = nxt;
     nxt = after;
+    cur_bits = nxt_bits;
+    nxt_bits = after_bits;
   }
 
   // documents without a real token
-  for (int doc = 0; doc < ndocs; doc++) {
-    bool any = false;
-    for (int s = 0; s < stages && !any; s++) any = words[doc * stages + s] != 0;
-    if (any) continue;
-    for (int j = 0; j < a.qpw && q0 + j < a.nQ; j++) {
-      const int q = q0 + j;
-      if (lane == 0) a.scores[score_at(a, q, b0 + doc)] = -__builtin_inff();
-      if (a.arg)
-        for (int i = lane; i < a.nqp; i += 64) a.arg[arg_at(a, q, b0 + doc) + i] = (uint16_t)kNone;
+  for (int d0 = 0; d0 < ndocs; d0 += 64) {
+    bool none = d0 + lane < ndocs;
+    for (int s = 0; s < stages && none; s++) none = words[(d0 + lane) * stages + s] == 0;
+    for (uint64_t left = __ballot(none); left != 0; left &= left - 1) {
+      const int64_t b = b0 + d0 + __builtin_ctzll(left);
+      for (int j = 0; j < a.qpw && q0 + j < a.nQ; j++) {
+        if (lane == 0) a.scores[score_at(a, q0 + j, b)] = -__builtin_inff();
+        if (a.arg)
+          for (int i = lane; i < a.nqp; i += 64) a.arg[arg_at(a, q0 + j, b) + i] = (uint16_t)kNone;
+      }
     }
   }
 }
@@ -861,10 +958,10 @@ static int run_shared(PairsArgs a, hipStream_t st) {
   a.qpw = NB / a.nbq;
   const int64_t groups = (a.nQ + 8 * a.qpw - 1) / (8 * a.qpw);
   const int64_t stages = (a.nd + kStage - 1) / kStage;
-  // Documents a workgroup: its mask words, and at least four workgroups a CU over the launch
-  // (1,024) where there are that many documents, so that the last round is a small part.
+  // Documents a workgroup: its mask words, and two workgroups a CU over the launch (512) where
+  // there are that many documents (four: 5 % longer, for each reads its queries first).
   int64_t docs = kMaskWords / (stages > 0 ? stages : 1);
-  const int64_t even = (a.B * groups + 1023) / 1024;
+  const int64_t even = (a.B * groups + 511) / 512;
   if (docs > even) docs = even;
   if (docs < 1) docs = 1;
   a.docs_per_wg = (int32_t)docs;
