@@ -208,8 +208,9 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 //
 // A block's 16 x 16 similarities are a chain of MFMAs (4 of 16 cycles at d = 128), and
 // their maxima twelve VALU instructions of 4 cycles; a wave issues in order, so the maxima of
-// one block are put between the MFMAs of the next. (One block after the other, 395 us for
-// 64 queries x 4096 documents x 60 to 180 tokens.)
+// one block are put between the MFMAs of the next. 64 queries x 4096 documents of 60 to 180
+// tokens, d = 128, bf16 with positions: 340 us (395 with one block after the other), bound by
+// the SIMDs' issue of the two: neither overlaps the other there.
 template <int DT, int KS, int NB, int PL>
 __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
   constexpr int FS = 4 * PL * KS;  // fragments of a stage
@@ -532,18 +533,19 @@ __device__ __forceinline__ f32x2 two(const uint8_t* p) {
 // token at a time: a thread counts and places its own run of maxima, so equal tokens keep their
 // order. Then each wave takes a quarter of the sorted maxima, cut between tokens, with the
 // rows of the next eight in flight while eight are added: 20 cycles of VALU work a maximum.
-// (Products with a matrix of ones made from the positions cost a multiply-add for each column,
-// token and query block as well: 560 us at 64 queries x 4096 documents x 180 tokens.)
+// 64 queries of 32 tokens x 4096 documents of 60 to 180 tokens, d = 128, bf16: 181 us, bound by
+// issue. (Products with a matrix of ones made from the positions cost a multiply-add for each
+// column, token and query block as well: 560 us.)
 // More than kRun blocks are sorted in runs; the sums stand in memory between them, in fp32.
 constexpr int kRun = 128;  // blocks of 32 maxima: 32 KB of LDS
 
-// Two columns of a row of Q.
-template <int DT, bool PAIR>
+// Two columns of a row of Q, of any width.
+template <int DT>
 __device__ __forceinline__ f32x2 columns(const typename El<DT>::T* row, int col, int d) {
-  if constexpr (PAIR) return two<DT>((const uint8_t*)(row + col));
   return f32x2{(float)row[col], col + 1 < d ? (float)row[col + 1] : 0.f};
 }
 
+// PAIR: an even width, and Q below 4 GB: two columns are one load, at a 32-bit offset.
 template <int DT, bool PAIR>
 __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
   typedef typename El<DT>::T T;
@@ -559,6 +561,7 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
   const int64_t b = blockIdx.x;
   const int col = (int)blockIdx.y * 128 + 2 * lane;
   const bool in = col < a.d;
+  const uint32_t at_col = (uint32_t)((in ? col : 0) * (int)sizeof(T));
   const int first = a.nway ? (int)(b / a.nway) * a.nbq : 0, blocks = a.nway ? a.nbq : a.blocks;
   const uint16_t* arg = a.arg + (a.nway ? b : b * a.nQ) * a.nqp;
   const T* Q = (const T*)a.Q;
@@ -657,16 +660,16 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
     int cur = __builtin_amdgcn_readfirstlane(j0);
     const int end = __builtin_amdgcn_readfirstlane(j1);
     float x0 = 0.f, x1 = 0.f;
-    auto flush = [&](int j) {
+    int64_t at = ((int64_t)b * a.nd + cur) * a.d + col;
+    auto flush = [&]() {  // token `cur` is done
       if (in) {
-        const int64_t at = ((int64_t)b * a.nd + j) * a.d + col;
         if (begun) {
           x0 += a.sums[at];
-          if (col + 1 < a.d) x1 += a.sums[at + 1];
+          if (PAIR || col + 1 < a.d) x1 += a.sums[at + 1];
         }
         if (!last) {
           a.sums[at] = x0;
-          if (col + 1 < a.d) a.sums[at + 1] = x1;
+          if (PAIR || col + 1 < a.d) a.sums[at + 1] = x1;
         } else {
           T* out = (T*)a.dD + at;
           if constexpr (PAIR) {
@@ -681,31 +684,40 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
         }
       }
       x0 = x1 = 0.f;
+      cur++;
+      at += a.d;
     };
-    // Sixty-four maxima at a time: each lane finds one's row and factor, and the wave takes
-    // them from the lanes one after another.
+    // Sixty-four maxima at a time: each lane finds one's row, factor and whether it is the first
+    // of its token, and the wave takes them from the lanes one after another. Past the end the
+    // last one stands in with a factor of 0.
     for (int m = m0; m < m1; m += 64) {
       const int here = m1 - m < 64 ? m1 - m : 64;
       const int e = sorted[m + (lane < here ? lane : here - 1)];
       const int k = first + k0 + (e >> 5), q = k / a.nbq;
-      const int row = q * a.nq + (k - q * a.nbq) * 32 + (e & 31);
+      const uint32_t row = (uint32_t)(q * a.nq + (k - q * a.nbq) * 32 + (e & 31));
+      const uint32_t from = PAIR ? row * (uint32_t)(a.d * (int)sizeof(T)) : row;  // bytes, below 2^32
       const int j = tok[e];
-      const float w = weight[e >> 5];
+      const int before = __shfl_up(j, 1);
+      const uint64_t firsts = __ballot(lane == 0 ? j != cur : j != before);
+      const float w = lane < here ? weight[e >> 5] : 0.f;
       f32x2 x[2][AHEAD];
       auto load = [&](int buf, int s) {
         if (s >= here) return;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-          const int r = __builtin_amdgcn_readlane(row, s + i < here ? s + i : here - 1);
-          x[buf][i] = in ? columns<DT, PAIR>(Q + (int64_t)r * a.d, col, a.d) : f32x2{0.f, 0.f};
+          const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)from, s + i);
+          if constexpr (PAIR) x[buf][i] = two<DT>((const uint8_t*)a.Q + (r + at_col));
+          else x[buf][i] = in ? columns<DT>(Q + (int64_t)r * a.d, col, a.d) : f32x2{0.f, 0.f};
         }
       };
       auto add = [&](int buf, int s) {
+        if (s >= here) return;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
-          if (s + i >= here) break;
-          const int js = __builtin_amdgcn_readlane(j, s + i);
-          while (cur != js) flush(cur++);
+          if ((firsts >> (s + i)) & 1) {
+            const int js = __builtin_amdgcn_readlane(j, s + i);
+            while (cur != js) flush();
+          }
           const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + i));
           x0 = __builtin_fmaf(ws, x[buf][i][0], x0);
           x1 = __builtin_fmaf(ws, x[buf][i][1], x1);
@@ -719,7 +731,7 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
         add(1, s + AHEAD);
       }
     }
-    while (cur < end) flush(cur++);
+    while (cur < end) flush();
   }
 }
 
@@ -743,11 +755,15 @@ __device__ __forceinline__ void put_q(const PairsGradArgs& a, int split, int64_t
 // dQ, many queries: sixteen waves, each with a block of 32 query tokens and 128 columns (two
 // a lane) in registers, walk the same run of documents. A document's tokens come to LDS
 // once for the 512 query tokens, while the one before is added up: each query token reads the
-// row that answered it, 256 bytes in one wave's access. Positions come through the scalar
-// unit; where there is none, a row of zeros and a factor of 0 stand in. The runs' sums are
-// joined by the kernel below, in order.
-template <int DT>
+// row that answered it, 256 bytes in one wave's access. A lane finds its token's row, and the
+// wave takes the rows from the lanes one after another: four VALU instructions a token.
+// Where there is none, a row of zeros stands in. The runs' sums are joined by the kernel
+// below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, bf16: 155 us (with the
+// positions through the scalar unit 278), bound by issue; the join takes 19 us.
+// WHOLE: rows in pieces of 16 bytes, on their way in registers meanwhile; others element by element.
+template <int DT, bool WHOLE>
 __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
+  using T = typename El<DT>::T;
   constexpr int ES = DT == TMS_DTYPE_F32 ? 4 : 2, ROW = 128 * ES;
   constexpr int LD = 4;  // 16-byte loads a thread and stage: 64 KB
   extern __shared__ __attribute__((aligned(16))) uint8_t docs[];  // [2][tokens + 1][ROW]
@@ -758,74 +774,95 @@ __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
   const int q = mine ? kb / a.nbq : 0;
   const int col0 = (int)blockIdx.y * 128, cols = a.d - col0 < 128 ? a.d - col0 : 128;
   const int64_t e0 = (int64_t)split * a.chunk, e1 = e0 + a.chunk < a.B ? e0 + a.chunk : a.B;
-  const int stages = (a.nd + a.tokens - 1) / a.tokens;
-  const int64_t items = e1 > e0 ? (e1 - e0) * stages : 0;
   const int size = (a.tokens + 1) * ROW;
-  const bool whole = a.d % (16 / ES) == 0 && (uintptr_t)a.D % 16 == 0;  // rows in 16-byte pieces
 
   for (int k = threadIdx.x; k < 2 * ROW / 4; k += 1024)  // the rows of zeros
     *(uint32_t*)(docs + (k / (ROW / 4)) * size + a.tokens * ROW + (k % (ROW / 4)) * 4) = 0u;
 
-  u32x4 reg[LD];
-  auto load = [&](int64_t it) {
-    const int64_t b = e0 + it / stages;
-    const int t0 = (int)(it % stages) * a.tokens, n = a.nd - t0 < a.tokens ? a.nd - t0 : a.tokens;
-    const uint8_t* base = (const uint8_t*)a.D + (((int64_t)b * a.nd + t0) * a.d + col0) * ES;
+  struct Stage {  // a document and its tokens from t0 on
+    int64_t b;
+    int t0;
+  };
+  auto next = [&](Stage& s) {
+    s.t0 += a.tokens;
+    if (s.t0 >= a.nd) {
+      s.t0 = 0;
+      s.b++;
+    }
+  };
+  auto tokens = [&](const Stage& s) { return a.nd - s.t0 < a.tokens ? a.nd - s.t0 : a.tokens; };
+  auto from = [&](const Stage& s) { return (const uint8_t*)a.D + ((s.b * a.nd + s.t0) * a.d + col0) * ES; };
+  u32x4 reg[WHOLE ? LD : 1];
+  auto load = [&](const Stage& s) {
+    if constexpr (WHOLE) {
+      if (s.b >= e1) return;
+      const uint8_t* base = from(s);
+      const int n = tokens(s);
 #pragma unroll
-    for (int i = 0; i < LD; i++) {
-      const int k = i * 1024 + (int)threadIdx.x, row = k / (ROW / 16), at = k % (ROW / 16);
-      if (row < n) {
-        if (whole) {
-          if (at * (16 / ES) < cols) reg[i] = *(const u32x4*)(base + (int64_t)row * a.d * ES + at * 16);
-        } else {
-          uint16_t h[8];
-#pragma unroll
-          for (int e = 0; e < 8; e++) {
-            const int col = at * (16 / ES) + e * 2 / ES;
-            h[e] = col < cols ? *(const uint16_t*)(base + (int64_t)row * a.d * ES + at * 16 + e * 2) : (uint16_t)0;
-          }
-          reg[i] = u32x4{h[0] | (uint32_t)h[1] << 16, h[2] | (uint32_t)h[3] << 16, h[4] | (uint32_t)h[5] << 16, h[6] | (uint32_t)h[7] << 16};
-        }
+      for (int i = 0; i < LD; i++) {
+        const int k = i * 1024 + (int)threadIdx.x, row = k / (ROW / 16), at = k % (ROW / 16);
+        if (row < n && at * (16 / ES) < cols) reg[i] = *(const u32x4*)(base + (row * a.d * ES + at * 16));
       }
     }
   };
-  auto put = [&](int64_t it, int buf) {
-    const int t0 = (int)(it % stages) * a.tokens, n = a.nd - t0 < a.tokens ? a.nd - t0 : a.tokens;
+  auto put = [&](const Stage& s, int buf) {
+    if (s.b >= e1) return;
+    const int n = tokens(s);
+    if constexpr (WHOLE) {
 #pragma unroll
-    for (int i = 0; i < LD; i++) {
-      const int k = i * 1024 + (int)threadIdx.x;
-      if (k / (ROW / 16) < n) *(u32x4*)(docs + buf * size + k * 16) = reg[i];
+      for (int i = 0; i < LD; i++) {
+        const int k = i * 1024 + (int)threadIdx.x;
+        if (k / (ROW / 16) < n) *(u32x4*)(docs + buf * size + k * 16) = reg[i];
+      }
+    } else {
+      const T* base = (const T*)from(s);
+      for (int k = threadIdx.x; k < n * (ROW / ES); k += 1024) {
+        const int row = k / (ROW / ES), col = k % (ROW / ES);
+        if (col < cols) ((T*)(docs + buf * size))[k] = base[(int64_t)row * a.d + col];
+      }
     }
   };
 
+  // Lane i's position of the block's token i, and G, read a stage ahead.
+  uint32_t at_next = kNone;
+  float w_next = 0.f;
+  auto look = [&](const Stage& s) {
+    if (!mine || s.b >= e1) return;
+    if (lane < 32) at_next = a.arg[s.b * a.nQ * a.nqp + (int64_t)kb * 32 + lane];
+    w_next = grad_of(a, q, s.b);
+  };
+
   float acc[32][2] = {};
-  if (items > 0) {
-    load(0);
-    put(0, 0);
-    if (items > 1) load(1);
-  }
+  Stage now = {e0, 0}, soon = now;  // the one added up, and the last one asked for
+  load(now);
+  look(now);
+  put(now, 0);
+  next(soon);
+  load(soon);
   __syncthreads();
-  for (int64_t it = 0; it < items; it++) {
-    const int64_t b = e0 + it / stages;
-    const int t0 = (int)(it % stages) * a.tokens;
-    const int buf = (int)(it & 1);
+  for (int buf = 0; now.b < e1; buf ^= 1) {
+    const uint32_t j = at_next - (uint32_t)now.t0;
+    const bool here = j < (uint32_t)a.tokens;  // kNone is beyond every stage
+    const uint32_t row = (here ? j : (uint32_t)a.tokens) * ROW + buf * size;
+    const float w = w_next;
+    look(soon);
     if (mine) {
-      const float w = grad_of(a, q, b);
-      const uint32_t* at = (const uint32_t*)(a.arg + (b * a.nQ) * a.nqp + (int64_t)kb * 32);
-      const uint8_t* base = docs + buf * size + lane * 2 * ES;
+      const uint8_t* base = docs + lane * 2 * ES;
+      // A row of zeros takes any factor but infinities and NaN away: the factor is 0 there too.
+      const uint32_t answered = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)__ballot(here));
+      const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, w)));
 #pragma unroll
       for (int i = 0; i < 32; i++) {
-        uint32_t j = ((at[i / 2] >> (16 * (i & 1))) & 0xffffu) - (uint32_t)t0;
-        const bool here = j < (uint32_t)a.tokens;  // kNone is beyond every stage
-        j = here ? j : (uint32_t)a.tokens;
-        const f32x2 x = two<DT>(base + j * ROW);
-        const float f = here ? w : 0.f;
+        const f32x2 x = two<DT>(base + (uint32_t)__builtin_amdgcn_readlane((int)row, i));
+        const float f = (answered >> i) & 1 ? ws : 0.f;
         acc[i][0] = __builtin_fmaf(f, x[0], acc[i][0]);
         acc[i][1] = __builtin_fmaf(f, x[1], acc[i][1]);
       }
     }
-    if (it + 1 < items) put(it + 1, buf ^ 1);
-    if (it + 2 < items) load(it + 2);
+    put(soon, buf ^ 1);
+    now = soon;
+    next(soon);
+    load(soon);
     __syncthreads();
   }
   if (!mine) return;
@@ -1031,8 +1068,7 @@ static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
     a.run = n < 1 ? 1 : n < kRun ? n : kRun;
     const size_t lds = (size_t)a.run * 32 * 6 + 16 * 256 * 2 + (size_t)a.run * 4;
     const dim3 grid((unsigned)a.B, (unsigned)((a.d + 127) / 128));
-    // rows whose pairs of columns are whole words
-    const bool pair = a.d % 2 == 0 && (uintptr_t)a.Q % 8 == 0 && (uintptr_t)a.dD % 8 == 0;
+    const bool pair = a.d % 2 == 0 && (int64_t)a.nQ * a.nq * a.d * (int64_t)sizeof(typename El<DT>::T) < ((int64_t)1 << 32) && (uintptr_t)a.Q % 8 == 0 && (uintptr_t)a.dD % 8 == 0;
     if (pair) hipLaunchKernelGGL((pairs_grad_d_kernel<DT, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((pairs_grad_d_kernel<DT, false>), grid, dim3(256), lds, st, a);
     if ((rc = check_launch("pairs_grad_d_kernel"))) return rc;
@@ -1048,7 +1084,10 @@ static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
       const int stages = (a.nd + most - 1) / most;
       a.tokens = stages > 0 ? (a.nd + stages - 1) / stages : 0;
       const size_t lds = 2 * (size_t)(a.tokens + 1) * 128 * es;
-      hipLaunchKernelGGL(pairs_grad_q_kernel<DT>, dim3((unsigned)((a.blocks + 15) / 16 * a.splits), cols), dim3(1024), lds, st, a);
+      const bool whole = a.d * es % 16 == 0 && (uintptr_t)a.D % 16 == 0;
+      const dim3 grid((unsigned)((a.blocks + 15) / 16 * a.splits), cols);
+      if (whole) hipLaunchKernelGGL((pairs_grad_q_kernel<DT, true>), grid, dim3(1024), lds, st, a);
+      else hipLaunchKernelGGL((pairs_grad_q_kernel<DT, false>), grid, dim3(1024), lds, st, a);
       if ((rc = check_launch("pairs_grad_q_kernel"))) return rc;
     } else {
       hipLaunchKernelGGL(pairs_grad_q_few_kernel<DT>, dim3((unsigned)((int64_t)a.nQ * ((a.nq + 7) / 8) * a.splits), cols), dim3(512), 0, st, a);
