@@ -251,27 +251,52 @@ __device__ __forceinline__ float element(const void* p, int64_t i, int dt) {
   return (float)((const __bf16*)p)[i];
 }
 
-// Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms. With
-// `ref`, rows without a gradient become zeros: what stands in them (NaN included) takes no part.
-__global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, int dt, uint16_t* dst, int64_t rows, int32_t d, int32_t dp,
-                                                        int64_t plane, const float* ref) {
-  const int64_t n = rows * dp;
+// Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms: three of
+// a float, 16-bit elements as they are; eight a thread. With `ref`, rows without a gradient
+// become zeros: what stands in them (NaN included) takes no part.
+template <bool F32>
+__global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, uint16_t* dst, int64_t rows, int32_t d, int32_t dp, int64_t plane,
+                                                        const float* ref) {
+  const uint32_t eights = (uint32_t)dp / 8;
+  const int64_t n = rows * eights;
+  const bool whole = d == dp && (uintptr_t)src % 16 == 0;  // pieces of eight in 16-byte loads (d = 0: dp = 8, nothing to load)
   for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
-    const int64_t row = k / dp;
-    const int c = (int)(k - row * dp);
-    const bool on = c < d && (!ref || ref[row] != __builtin_inff());
-    float x = on ? element(src, row * d + c, dt) : 0.f;
-    if (dt == TMS_DTYPE_F16) {
-      dst[k] = to16<TMS_DTYPE_F16>(x);
-    } else if (dt == TMS_DTYPE_BF16) {
-      dst[k] = to16<TMS_DTYPE_BF16>(x);
-    } else {
+    const int64_t row = n >> 32 ? k / eights : (int64_t)((uint32_t)k / eights);
+    const int c = (int)(k - row * eights) * 8;
+    const bool on = !ref || ref[row] != __builtin_inff();
+    const int64_t at = row * d + c;
+    if constexpr (F32) {
+      float x[8];
+      if (whole) {
+        const f32x4 lo = ((const f32x4*)((const float*)src + at))[0], hi = ((const f32x4*)((const float*)src + at))[1];
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = on ? lo[e] : 0.f, x[4 + e] = on ? hi[e] : 0.f;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = on && c + e < d ? ((const float*)src)[at + e] : 0.f;
+      }
 #pragma unroll
       for (int p = 0; p < 3; p++) {
-        const __bf16 t = (__bf16)x;
-        dst[p * plane + k] = __builtin_bit_cast(uint16_t, t);
-        x -= (float)t;
+        u32x4 out;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+          const __bf16 t = (__bf16)x[e];
+          const uint32_t bits = __builtin_bit_cast(uint16_t, t);
+          out[e / 2] = e % 2 ? out[e / 2] | bits << 16 : bits;
+          x[e] -= (float)t;
+        }
+        *(u32x4*)(dst + p * plane + k * 8) = out;
       }
+    } else {
+      u32x4 out = {0u, 0u, 0u, 0u};
+      if (on && whole) {
+        out = *(const u32x4*)((const uint16_t*)src + at);
+      } else if (on) {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (c + e < d) out[e / 2] |= (uint32_t)((const uint16_t*)src)[at + e] << (16 * (e % 2));
+      }
+      *(u32x4*)(dst + k * 8) = out;
     }
   }
 }
@@ -532,8 +557,11 @@ static int check_lce(const char* fn, int64_t N, int64_t d, int64_t V, int dtype,
 
 static int run_terms(const void* src, int dtype, void* dst, int64_t rows, int64_t d, int64_t dp, const float* ref, hipStream_t st) {
   const int64_t n = rows * dp;
-  hipLaunchKernelGGL(lce_terms_kernel, dim3(blocks_for(n)), dim3(256), 0, st, src, dtype, (uint16_t*)dst, rows, (int32_t)d, (int32_t)dp,
-                     n, ref);
+  const dim3 grid(blocks_for(n / 8));
+  if (dtype == TMS_DTYPE_F32)
+    hipLaunchKernelGGL(lce_terms_kernel<true>, grid, dim3(256), 0, st, src, (uint16_t*)dst, rows, (int32_t)d, (int32_t)dp, n, ref);
+  else
+    hipLaunchKernelGGL(lce_terms_kernel<false>, grid, dim3(256), 0, st, src, (uint16_t*)dst, rows, (int32_t)d, (int32_t)dp, n, ref);
   return check_launch("lce_terms_kernel");
 }
 
