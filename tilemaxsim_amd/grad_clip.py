@@ -25,25 +25,39 @@ def _norm_type(fn: str, p) -> int:
 
 def _list(fn: str, tensors) -> list:
     ts = [tensors] if isinstance(tensors, torch.Tensor) else [t for t in tensors if t is not None]
-    for t in ts:
-        if not isinstance(t, torch.Tensor):
-            raise TypeError(f"{fn}: expected tensors, got {type(t).__name__}")
-        if t.dtype not in _lib.DTYPE_CODES:
-            raise TypeError(f"{fn}: gradients must be float16, bfloat16 or float32 (got {t.dtype})")
-    for t in ts:
-        if not t.is_cuda:
-            raise ValueError(f"{fn}: gradients must be on a ROCm GPU device (got {t.device}); tilemaxsim_amd has no CPU path")
-        if t.device != ts[0].device:
-            raise ValueError(f"{fn}: all gradients must be on one device; got {t.device} and {ts[0].device}")
+    # a model's hundreds of tensors are few types, dtypes and devices: only a mixture is looked at singly
+    if not all(issubclass(k, torch.Tensor) for k in set(map(type, ts))):
+        bad = next(t for t in ts if not isinstance(t, torch.Tensor))
+        raise TypeError(f"{fn}: expected tensors, got {type(bad).__name__}")
+    for kind in {t.dtype for t in ts}:
+        if kind not in _lib.DTYPE_CODES:
+            raise TypeError(f"{fn}: gradients must be float16, bfloat16 or float32 (got {kind})")
+    on = {t.get_device() for t in ts}  # -1: not on a GPU
+    if len(on) > 1 or -1 in on:
+        for t in ts:
+            if not t.is_cuda:
+                raise ValueError(f"{fn}: gradients must be on a ROCm GPU device (got {t.device}); tilemaxsim_amd has no CPU path")
+            if t.device != ts[0].device:
+                raise ValueError(f"{fn}: all gradients must be on one device; got {t.device} and {ts[0].device}")
     return ts
+
+
+def _codes(ts: list) -> list:
+    kinds = [t.dtype for t in ts]
+    if kinds.count(kinds[0]) == len(kinds):
+        return [_lib.DTYPE_CODES[kinds[0]]] * len(kinds)
+    return [_lib.DTYPE_CODES[k] for k in kinds]
 
 
 def _table(src: list, dst: list) -> array:
     """tms_grad_tensor entries: two addresses, the size, and both dtypes in one word."""
-    codes = _lib.DTYPE_CODES
-    words = array("q")
-    for s, d in zip(src, dst):
-        words.extend((s.data_ptr(), d.data_ptr(), s.numel(), codes[s.dtype] | codes[d.dtype] << 32))
+    words = array("q", bytes(32 * len(src)))
+    from_ = array("q", [t.data_ptr() for t in src])
+    codes = _codes(src)
+    words[0::4] = from_
+    words[1::4] = from_ if dst is src else array("q", [t.data_ptr() for t in dst])
+    words[2::4] = array("q", [t.numel() for t in src])
+    words[3::4] = array("q", [s | d << 32 for s, d in zip(codes, codes if dst is src else _codes(dst))])
     return words
 
 
