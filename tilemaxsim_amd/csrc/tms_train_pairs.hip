@@ -1126,6 +1126,7 @@ extern "C" int tms_maxsim_pairs(const void* Qs, int64_t nQ, int64_t nq, int64_t 
   if (rc) return rc;
   if (nQ == 0 || B == 0) return TMS_OK;
   if (!scores || (nq * d > 0 && !Qs) || (nd * d > 0 && !D)) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  if ((uintptr_t)positions % 16) return fail(TMS_ERR_INVALID, "%s: positions must be 16-byte aligned", fn);
   const hipStream_t st = (hipStream_t)stream;
   PairsArgs a = {};
   a.qmask = qmask;
