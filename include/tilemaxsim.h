@@ -354,8 +354,9 @@ int tms_codes_verdict(const int64_t* verdict, void* stream);
  * are bytes, non-zero for a real token; NULL: every token is real. nway = 0: every query
  * with every document, scores (nQ, B). nway > 0: B is nQ * nway, query q with documents
  * [q nway, (q + 1) nway), scores (nQ, nway). A document without a real token scores -inf;
- * a query without any scores 0 elsewhere. Embeddings are finite at the real tokens; what
- * stands at the masked ones is not looked at. nd <= 65535.
+ * a query without any scores 0 elsewhere. NaN at a real token makes its scores NaN (as an
+ * infinity does where it meets a 0 or its opposite); what stands at the masked ones is not
+ * looked at. nd <= 65535.
  *   workspace  tms_pairs_workspace_size bytes of device memory, 16-byte aligned (0 for 16-bit
  *              rows whose d is a multiple of 32: NULL, and Qs and D 16-byte aligned)
  *   positions  NULL, or tms_pairs_positions uint16 of device memory, 16-byte aligned, for

@@ -262,3 +262,31 @@ def test_nothing(cuda, nQ, Nq, B, Nd):
     dQ, dD = torch.autograd.grad(s, (Q, own), torch.ones_like(s))
     if Nd == 0 or Nq == 0:
         assert bool((dQ == 0).all()) and bool((dD == 0).all())
+
+
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("nQ,B,d", [(2, 5, 64), (3, 6, 77), (9, 300, 64), (9, 300, 77), (5, 700, 128), (3, 6, 200)])
+def test_nan_at_a_real_token_reaches_the_scores(cuda, dt, nQ, B, d):
+    """A NaN or infinity at a real token (of a text of its own) makes that text's scores NaN, at
+    a masked one nothing, with and without positions; and the two forms' scores are the same bits."""
+    import tilemaxsim_amd as tms
+    rng = np.random.default_rng(d)
+    Q, D = _grid(rng, nQ, 7, d).to(DT[dt]).cuda(), _grid(rng, B, 37, d).to(DT[dt]).cuda()
+    qmask, dmask = torch.ones(nQ, 7, dtype=torch.bool, device="cuda"), torch.ones(B, 37, dtype=torch.bool, device="cuda")
+    qmask[0, 6] = dmask[4, 20] = dmask[0, 36] = False
+    dmask[2] = False
+    clean = tms.maxsim_pairs(Q, D, dmask, qmask)
+    Q[0, 6, d - 1] = D[4, 20, 3] = D[2, 5, 0] = math.nan
+    D[0, 36] = math.inf
+    assert torch.equal(tms.maxsim_pairs(Q, D, dmask, qmask), clean)
+    Q[1, 2, d - 1] = math.nan
+    D[3, 36, 0] = math.nan
+    D[B - 1, 0] = math.inf  # inf - inf over a row of both signs
+    want = torch.zeros(nQ, B, dtype=torch.bool, device="cuda")
+    want[1] = want[:, 3] = want[:, B - 1] = True
+    want[:, 2] = False
+    scores = tms.maxsim_pairs(Q, D, dmask, qmask)
+    assert torch.equal(torch.isnan(scores), want)
+    assert torch.equal(scores[~want], clean[~want])
+    kept = tms.maxsim_pairs(Q.requires_grad_(True), D, dmask, qmask).detach()
+    assert torch.equal(torch.isnan(kept), want) and torch.equal(kept[~want], clean[~want])

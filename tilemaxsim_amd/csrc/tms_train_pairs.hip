@@ -38,20 +38,29 @@ __device__ __forceinline__ int64_t arg_at(const PairsArgs& a, int q, int64_t b) 
 
 // Running maximum and its token over one 16-token tile: lane (c, g) sees query token c
 // against tokens base + 4 g + i. A strict comparison keeps the first of equal ones, as
-// tokens rise. Three VALU instructions a value; at d = 128 the four MFMAs behind a value's
-// 16 x 16 block take longer than that, and the two waves of a SIMD overlap them.
+// tokens rise; the maximum keeps a NaN, which has to reach the loss. Three VALU instructions
+// a value, half of one without positions.
 struct Best {
   float v;
   int at;
 };
-__device__ __forceinline__ void take(Best& r, float s, int at) {
-  const bool up = s > r.v;  // with fmaxf each value would be made canonical first
-  r.at = up ? at : r.at;
-  r.v = up ? s : r.v;
+__device__ __forceinline__ float top(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+template <bool POS>
+__device__ __forceinline__ void take(Best& r, const f32x4& s, int first) {
+  if constexpr (POS) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      r.at = s[i] > r.v ? first + i : r.at;
+      r.v = top(r.v, s[i]);
+    }
+  } else {
+    r.v = top(top(r.v, s[0]), s[1]);
+    r.v = top(top(r.v, s[2]), s[3]);
+  }
 }
 __device__ __forceinline__ Best better(Best x, Best y) {
   const bool up = y.v > x.v || (y.v == x.v && y.at < x.at);
-  return {up ? y.v : x.v, up ? y.at : x.at};
+  return {top(x.v, y.v), up ? y.at : x.at};
 }
 // Over the four 16-lane rows; every lane receives the result.
 __device__ __forceinline__ Best across_rows(Best r) {
@@ -165,8 +174,7 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         mask_tile(acc[h], bits, g);  // not behind a branch, for one would follow an MFMA
-#pragma unroll
-        for (int i = 0; i < 4; i++) take(best[h], acc[h][i], t * 16 + 4 * g + i);
+        take<true>(best[h], acc[h], t * 16 + 4 * g);
       }
     }
 #pragma unroll
@@ -207,11 +215,12 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 // Whole queries belong to a wave, so a score is summed in one place and in one order.
 //
 // A block's 16 x 16 similarities are a chain of MFMAs (4 of 16 cycles at d = 128), and
-// their maxima twelve VALU instructions of 4 cycles; a wave issues in order, so the maxima of
-// one block are put between the MFMAs of the next. 64 queries x 4096 documents of 60 to 180
-// tokens, d = 128, bf16 with positions: 340 us (395 with one block after the other), bound by
-// the SIMDs' issue of the two: neither overlaps the other there.
-template <int DT, int KS, int NB, int PL>
+// their maxima twelve VALU instructions of 4 cycles (POS: with positions), or two without; a
+// wave issues in order, so the maxima of one block are put between the MFMAs of the next.
+// 64 queries x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 320 us with positions (395
+// with one block after the other), 277 without, bound by the SIMDs' issue of the two:
+// neither overlaps the other there.
+template <int DT, int KS, int NB, int PL, bool POS>
 __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
   constexpr int FS = 4 * PL * KS;  // fragments of a stage
   constexpr int LD = (FS + 7) / 8;  // fragments a wave loads
@@ -370,12 +379,10 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
           if (j > 0) {
             f32x4(&v)[2] = acc[(j - 1) & 1];
             if constexpr (decltype(masked)::value) mask_tile(v[0], bits, g), mask_tile(v[1], bits, g);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-#pragma unroll
-              for (int h = 0; h < 2; h++) take(best[j - 1][h], v[h][i], first + i);
+            take<POS>(best[j - 1][0], v[0], first);
+            take<POS>(best[j - 1][1], v[1], first);
           }
-          constexpr int MF = (PL == 1 ? KS : 6 * KS) * 2, VA = (24 + MF - 1) / MF;
+          constexpr int MF = (PL == 1 ? KS : 6 * KS) * 2, VA = ((POS ? 24 : 4) + MF - 1) / MF;
           if (j == 0) __builtin_amdgcn_sched_group_barrier(0x008, MF, 0);
           if (j > 0 && j < NB) {
 #pragma unroll
@@ -406,7 +413,7 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
         const int j = 2 * P + (2 * P + 1 < NB ? (g & 1) : 0), h = g >> 1;
         const bool on = (real >> (2 * j + h)) & 1u;
         const int q = q0 + j / a.nbq, tok = (j % a.nbq) * 32 + 16 * h + r;
-        if (a.arg && j < a.qpw * a.nbq && q < a.nQ && tok < a.nqp && (2 * P + 1 < NB || (g & 1) == 0))
+        if (POS && j < a.qpw * a.nbq && q < a.nQ && tok < a.nqp && (2 * P + 1 < NB || (g & 1) == 0))
           a.arg[arg_at(a, q, b) + tok] = (uint16_t)(on ? z.at : kNone);
         float s = row_sum16(on ? z.v : 0.f);
         const auto hs = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, s), __builtin_bit_cast(unsigned, s), false, false);
@@ -439,7 +446,7 @@ __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
       const int64_t b = b0 + d0 + __builtin_ctzll(left);
       for (int j = 0; j < a.qpw && q0 + j < a.nQ; j++) {
         if (lane == 0) a.scores[score_at(a, q0 + j, b)] = -__builtin_inff();
-        if (a.arg)
+        if (POS)
           for (int i = lane; i < a.nqp; i += 64) a.arg[arg_at(a, q0 + j, b) + i] = (uint16_t)kNone;
       }
     }
@@ -1002,8 +1009,9 @@ static int run_shared(PairsArgs a, hipStream_t st) {
   if (docs > even) docs = even;
   if (docs < 1) docs = 1;
   a.docs_per_wg = (int32_t)docs;
-  hipLaunchKernelGGL((pairs_shared_kernel<DT, KS, NB, PL>), dim3((unsigned)((a.B + docs - 1) / docs), (unsigned)groups), dim3(512), 0,
-                     st, a);
+  const dim3 grid((unsigned)((a.B + docs - 1) / docs), (unsigned)groups);
+  if (a.arg) hipLaunchKernelGGL((pairs_shared_kernel<DT, KS, NB, PL, true>), grid, dim3(512), 0, st, a);
+  else hipLaunchKernelGGL((pairs_shared_kernel<DT, KS, NB, PL, false>), grid, dim3(512), 0, st, a);
   return check_launch("pairs_shared_kernel");
 }
 

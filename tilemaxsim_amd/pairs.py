@@ -104,7 +104,7 @@ def maxsim_pairs(Qs: torch.Tensor, D: torch.Tensor, D_mask: torch.Tensor | None 
 
     Returns:
         (nQ, B) or (nQ, nway) float32 scores. A document without a real token scores -inf
-        and takes and gives no gradient.
+        and takes and gives no gradient. NaN at a real token makes its scores NaN.
 
     A maximum's gradient goes to one token, the first of equal ones. Gradients are summed in
     fp32, in one order whatever the timing, and rounded once to the inputs' dtype.
