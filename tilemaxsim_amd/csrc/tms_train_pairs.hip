@@ -217,9 +217,10 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 // A block's 16 x 16 similarities are a chain of MFMAs (4 of 16 cycles at d = 128), and
 // their maxima twelve VALU instructions of 4 cycles (POS: with positions), or two without; a
 // wave issues in order, so the maxima of one block are put between the MFMAs of the next.
-// 64 queries x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 320 us with positions (395
-// with one block after the other), 277 without, bound by the SIMDs' issue of the two:
-// neither overlaps the other there.
+// 64 queries x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 315 us with positions (with
+// one block after the other 80 more), 250 without, bound by the SIMDs' issue of the two:
+// neither overlaps the other there. (32 x 32 products, which overlap half of it, take 365 and
+// 274: documents then end on 32 tokens, and the registers do not hold the next fragments.)
 template <int DT, int KS, int NB, int PL, bool POS>
 __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
   constexpr int FS = 4 * PL * KS;  // fragments of a stage
@@ -1002,10 +1003,12 @@ static int run_shared(PairsArgs a, hipStream_t st) {
   a.qpw = NB / a.nbq;
   const int64_t groups = (a.nQ + 8 * a.qpw - 1) / (8 * a.qpw);
   const int64_t stages = (a.nd + kStage - 1) / kStage;
-  // Documents a workgroup: its mask words, and two workgroups a CU over the launch (512) where
-  // there are that many documents (four: 5 % longer, for each reads its queries first).
+  // Documents a workgroup: its mask words, and as many workgroups as run at once, for each reads
+  // its queries first: one a CU of the forms with the most registers (64 queries x 4096
+  // documents, d = 128: 315 us in 256 workgroups, 324 in 512, 342 in 768), else two.
+  constexpr int kWhole = NB * KS * PL >= 6 ? 256 : 512;
   int64_t docs = kMaskWords / (stages > 0 ? stages : 1);
-  const int64_t even = (a.B * groups + 511) / 512;
+  const int64_t even = (a.B * groups + kWhole - 1) / kWhole;
   if (docs > even) docs = even;
   if (docs < 1) docs = 1;
   a.docs_per_wg = (int32_t)docs;
