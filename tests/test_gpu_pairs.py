@@ -290,3 +290,38 @@ def test_nan_at_a_real_token_reaches_the_scores(cuda, dt, nQ, B, d):
     assert torch.equal(scores[~want], clean[~want])
     kept = tms.maxsim_pairs(Q.requires_grad_(True), D, dmask, qmask).detach()
     assert torch.equal(torch.isnan(kept), want) and torch.equal(kept[~want], clean[~want])
+
+
+@pytest.mark.parametrize("nQ,B,Nd", [(3, 6, 20), (9, 300, 70)])
+def test_graph(cuda, nQ, B, Nd):
+    """Captured scores with both gradients follow their inputs from replay to replay."""
+    import tilemaxsim_amd as tms
+    rng = np.random.default_rng(B)
+    Q, D = (_grid(rng, *s).half().cuda().requires_grad_(True) for s in ((nQ, 10, 64), (B, Nd, 64)))
+    dmask = torch.ones(B, Nd, dtype=torch.bool, device="cuda")
+    G = torch.ones(nQ, B, device="cuda")
+
+    def step():
+        s = tms.maxsim_pairs(Q, D, dmask)
+        return (s.detach(), *torch.autograd.grad(s, (Q, D), G))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step()
+    for replay in range(4):
+        with torch.no_grad():
+            Q.copy_(_grid(rng, *Q.shape).half())
+            D.copy_(_grid(rng, *D.shape).half())
+            dmask.copy_(torch.from_numpy(rng.random((B, Nd)) < 0.7))
+            G.copy_(torch.from_numpy(rng.standard_normal((nQ, B)).astype(np.float32)))
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [x.clone() for x in kept]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b), replay
+        torch.cuda.synchronize()
