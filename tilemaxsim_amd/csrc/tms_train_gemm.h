@@ -29,19 +29,15 @@ namespace tms {
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 // fp32 operands are three bf16 terms ("planes"); of the nine products of two such operands
-// the six above 2^-24 of the whole are formed, small ones first: planes (2, 0), (0, 2),
-// (1, 1), (1, 0), (0, 1), (0, 0), a hexadecimal digit each from the last on.
-constexpr int kTermPairs = 6;
-__device__ __forceinline__ int term_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
-__device__ __forceinline__ int term_b(int pair) { return (0x010120 >> (4 * pair)) & 3; }
-
+// the six above 2^-24 of the whole are formed. A 64-step of k takes them in the order (2, 0),
+// (1, 0), (1, 1), (0, 1), (0, 2), (0, 0): each differs from the one before in one operand, whose tile
+// alone is loaded and read from LDS, so that the six cost seven tiles and not twelve.
 struct GemmArgs {
   const uint16_t* A;
   const uint16_t* B;
   int64_t aplane, bplane;  // elements between planes
   int32_t lda, ldb;        // elements between rows (multiples of 8)
   int32_t M, N, K;         // k inside: K is a multiple of 8, or zeros follow it up to one; outside: M (N) is
-  int32_t pairs;           // 1, or kTermPairs
   int32_t splits, per;     // splits of k, 64-steps each
   int32_t tm, tn;          // tiles
 };
@@ -138,8 +134,9 @@ struct More {
   static constexpr bool value = V;
 };
 
-template <int DT, int MI, int NI, bool AO, bool BO, class Epi>
-__global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a, Epi epi) {
+// PL: planes of both operands, 1 or 3.
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi>
+__global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
   constexpr int BM = 32 * MI, BN = 64 * NI;
   constexpr int ASZ = BM * 128, BSZ = BN * 128;
   extern __shared__ __attribute__((aligned(1024))) uint8_t gemm_mem[];
@@ -156,20 +153,17 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
   const int k0 = (int)blockIdx.y * a.per;
   const int steps_all = (a.K + 63) / 64;
   const int nk = k0 + a.per < steps_all ? a.per : steps_all - k0;
-  const int steps = nk > 0 ? nk * a.pairs : 0;
   const uint16_t* A = a.A + (AO ? (int64_t)m0 : (int64_t)m0 * a.lda);
   const uint16_t* B = a.B + (BO ? (int64_t)n0 : (int64_t)n0 * a.ldb);
-  int pair = kTermPairs - a.pairs, kt = 0;  // the step that is loaded next
-  auto load = [&](int buf) {
-    const int64_t k = (int64_t)(k0 + kt) * 64;
-    const int left = a.K - (int)k;
-    uint8_t* to = gemm_mem + buf * (ASZ + BSZ);
-    ta.load(A + term_a(pair) * a.aplane + (AO ? k * a.lda : k), left, to, wave);
-    tb.load(B + term_b(pair) * a.bplane + (BO ? k * a.ldb : k), left, to + ASZ, wave);
-    if (++kt == nk) {
-      kt = 0;
-      pair++;
-    }
+  uint8_t* const lds_a = gemm_mem;
+  uint8_t* const lds_b = gemm_mem + 2 * ASZ;
+  auto load_a = [&](int buf, int step, int plane) {
+    const int64_t k = (int64_t)(k0 + step) * 64;
+    ta.load(A + plane * a.aplane + (AO ? k * a.lda : k), a.K - (int)k, lds_a + buf * ASZ, wave);
+  };
+  auto load_b = [&](int buf, int step, int plane) {
+    const int64_t k = (int64_t)(k0 + step) * 64;
+    tb.load(B + plane * a.bplane + (BO ? k * a.ldb : k), a.K - (int)k, lds_b + buf * BSZ, wave);
   };
   auto meet = [&]() {  // this wave's loads are in LDS, then everyone's
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
@@ -182,23 +176,26 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
 #pragma unroll
     for (int j = 0; j < NI; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  // One step from buffer `buf`; `more`: the next one's loads go out once some of the products
-  // are issued (behind the loads, a product would wait for all of the wave's LDS reads
-  // together): a quarter of them, or an eighth with k outside in both operands (8192^3 in bf16,
-  // an eighth / a quarter: 1.13 / 1.15 PFLOP/s with k inside, 1.23 / 1.29 outside in one, 1.29 /
+  u32x4 fa[2][MI], fb[2][NI];
+  auto read_a = [&](int buf) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int i = 0; i < MI; i++) fa[ks][i] = GemmTile<BM, AO>::frag(lds_a + buf * ASZ, wm * MI + i, ks, lane);
+  };
+  auto read_b = [&](int buf) {
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int j = 0; j < NI; j++) fb[ks][j] = GemmTile<BN, BO>::frag(lds_b + buf * BSZ, wn * NI + j, ks, lane);
+  };
+  // The products of the fragments; `next`: the next step's loads, which go out once some of the
+  // products are issued (behind the loads, a product would wait for all of the wave's LDS
+  // reads together): a quarter of them, or an eighth with k outside in both operands (8192^3 in
+  // bf16, an eighth / a quarter: 1.13 / 1.15 PFLOP/s with k inside, 1.23 / 1.29 outside in one, 1.29 /
   // 1.21 in both). The scheduler would otherwise move products behind the wait for the loads.
   constexpr int kBefore = AO && BO ? MI / 4 : MI / 2;
-  auto step = [&](int buf, auto more) {
-    const uint8_t* la = gemm_mem + buf * (ASZ + BSZ);
-    const uint8_t* lb = la + ASZ;
-    u32x4 fa[2][MI], fb[2][NI];
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-#pragma unroll
-      for (int j = 0; j < NI; j++) fb[ks][j] = GemmTile<BN, BO>::frag(lb, wn * NI + j, ks, lane);
-#pragma unroll
-      for (int i = 0; i < MI; i++) fa[ks][i] = GemmTile<BM, AO>::frag(la, wm * MI + i, ks, lane);
-    }
+  auto multiply = [&](auto&& next) {
     auto products = [&](int ks, int i0, int i1) {
 #pragma unroll
       for (int i = 0; i < MI; i++)
@@ -207,31 +204,55 @@ __global__ __launch_bounds__(kGemmThreads, 2) void train_gemm_kernel(GemmArgs a,
           if (i >= i0 && i < i1) acc[i][j] = mfma16x16x32<DT>(fa[ks][i], fb[ks][j], acc[i][j]);
     };
     products(0, 0, kBefore);
-    if constexpr (decltype(more)::value) {
-      __builtin_amdgcn_sched_barrier(0);
-      load(buf ^ 1);
-      __builtin_amdgcn_sched_barrier(0);
-    }
+    __builtin_amdgcn_sched_barrier(0);
+    next();
+    __builtin_amdgcn_sched_barrier(0);
     products(0, kBefore, MI);
     products(1, 0, MI);
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (steps > 0) {
-    load(0);
+  if (nk > 0) {
+    load_a(0, 0, PL - 1);
+    load_b(0, 0, 0);
     meet();
-    int buf = 0;
-    for (int t = 0; t + 1 < steps; t++) {
-      step(buf, More<true>());
-      meet();
-      buf ^= 1;
-    }
-    step(buf, More<false>());
   }
+  int buf = 0;
+  auto step = [&](int t, auto more) {
+    read_b(PL == 3 ? 0 : buf);
+    read_a(buf);
+    if constexpr (PL == 3) {  // the fragments of the tile that stays, stay
+      multiply([&]() { load_a(buf ^ 1, t, 1); });
+      meet();
+      read_a(buf ^ 1);
+      multiply([&]() { load_b(1, t, 1); });
+      meet();
+      read_b(1);
+      multiply([&]() { load_a(buf, t, 0); });
+      meet();
+      read_a(buf);
+      multiply([&]() { load_b(0, t, 2); });
+      meet();
+      read_b(0);
+      multiply([&]() { load_b(1, t, 0); });
+      meet();
+      read_b(1);
+    }
+    multiply([&]() {
+      if constexpr (decltype(more)::value) {
+        load_a(buf ^ 1, t + 1, PL - 1);
+        load_b(PL == 3 ? 0 : buf ^ 1, t + 1, 0);
+      }
+    });
+    if constexpr (decltype(more)::value) meet();
+    buf ^= 1;
+  };
+  for (int t = 0; t + 1 < nk; t++) step(t, More<true>());
+  if (nk > 0) step(nk - 1, More<false>());
   if constexpr (Epi::kRowBytes > 0) __syncthreads();  // the operands' LDS is the epilogue's
   epi(acc, m0 + wm * MI * 16, n0 + wn * NI * 16, (int)blockIdx.y, gemm_mem + wave * (NI * 16 * Epi::kRowBytes));
 }
 
-template <int DT, int MI, int NI, bool AO, bool BO, class Epi>
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi>
 static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what) {
   a.tm = (a.M + 32 * MI - 1) / (32 * MI);
   a.tn = (a.N + 64 * NI - 1) / (64 * NI);
@@ -239,7 +260,7 @@ static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what
   a.per = (steps + a.splits - 1) / a.splits;
   size_t lds = 2 * (size_t)(32 * MI + 64 * NI) * 128;
   if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
-  hipLaunchKernelGGL((train_gemm_kernel<DT, MI, NI, AO, BO, Epi>), dim3(gemm_grid(a.tm, a.tn), (unsigned)a.splits), dim3(kGemmThreads),
+  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi>), dim3(gemm_grid(a.tm, a.tn), (unsigned)a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);
   return check_launch(what);
 }

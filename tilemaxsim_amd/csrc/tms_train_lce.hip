@@ -494,14 +494,16 @@ template <int S>
 struct SizeOf {
   static constexpr int MI = S == kGemm256 ? 8 : S == kGemm128 ? 4 : 2, NI = S == kGemm256 ? 4 : S == kGemm128 ? 2 : 1;
 };
-template <class F>
+template <int PL, class F>
 static int with_size(int size, F&& f) {
-  if (size == kGemm256) return f(SizeOf<kGemm256>());
+  if constexpr (PL == 1) {
+    if (size == kGemm256) return f(SizeOf<kGemm256>());
+  }
   if (size == kGemm128) return f(SizeOf<kGemm128>());
   return f(SizeOf<kGemm64>());
 }
 static int logits_size(int64_t N, int64_t V, int64_t dp, int dtype) {
-  return gemm_size(V, N, up_to(dp, 64) / 64 * (dtype == TMS_DTYPE_F32 ? kTermPairs : 1));
+  return gemm_size(V, N, gemm_steps(dp, planes(dtype)), gemm_largest(planes(dtype)));
 }
 // Vocabulary rows that one RowStat of the forward pass covers: a wave's share of a tile.
 static int64_t stat_rows(int size) { return gemm_side(size) / 2; }
@@ -576,12 +578,11 @@ static GemmArgs logits_args(const void* H, const void* W, int64_t N, int64_t V, 
   a.M = (int32_t)V;
   a.N = (int32_t)N;
   a.K = (int32_t)dp;
-  a.pairs = dtype == TMS_DTYPE_F32 ? kTermPairs : 1;
   a.splits = 1;
   return a;
 }
 
-template <int DT>  // the type of the terms: fp32 inputs have bf16 ones
+template <int DT, int PL>  // the terms' type and number: fp32 inputs have three bf16 ones
 static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
                        float s2, int reduction, uint8_t* ws, const LceSpace& s, bool terms, float* loss, float* stats, hipStream_t st) {
   const int64_t dp = up_to(d > 0 ? d : 8, 8);
@@ -596,7 +597,7 @@ static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64
   const GemmArgs a = logits_args(h, w, N, V, V, dp, dtype);
   LseEpilogue e = {(RowStat*)(ws + s.parts), (int32_t)N, (int32_t)V, s2};
   const int size = logits_size(N, V, dp, dtype);
-  rc = with_size(size, [&](auto z) { return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, false, false>(a, e, st, "train_gemm_kernel (lse)"); });
+  rc = with_size<PL>(size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, false, false>(a, e, st, "train_gemm_kernel (lse)"); });
   if (rc) return rc;
   const bool rows = reduction == TMS_REDUCE_NONE, alone = !rows && N <= kJoinAlone;
   float* rows_loss = rows ? loss : (float*)(ws + s.loss);
@@ -636,10 +637,10 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
   for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
     const int64_t nv = V - v0 < p.piece ? V - v0 : p.piece;
     GemmArgs a = logits_args(h, (const uint16_t*)w + v0 * p.dp, N, nv, V, p.dp, dtype);
-    rc = with_size(p.size_p, [&](auto z) {
+    rc = with_size<PL>(p.size_p, [&](auto z) {
       using Z = decltype(z);
       const ProbEpilogue<DT, PL, Z::MI> e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e};
-      return run_gemm<DT, Z::MI, Z::NI, false, false>(a, e, st, "train_gemm_kernel (P)");
+      return run_gemm<DT, PL, Z::MI, Z::NI, false, false>(a, e, st, "train_gemm_kernel (P)");
     });
     if (rc) return rc;
     if (dH && d > 0) {  // m over d, n over rows, k over the piece
@@ -653,11 +654,10 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
       b.M = (int32_t)p.dp;
       b.N = (int32_t)N;
       b.K = (int32_t)nv;
-      b.pairs = PL == 3 ? kTermPairs : 1;
       b.splits = p.splits;
       SumEpilogue se = {sums, N * p.dp, (int32_t)N, (int32_t)p.dp, v0 == 0};
-      rc = with_size(p.size_h, [&](auto z) {
-        return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, true, false>(b, se, st, "train_gemm_kernel (dH)");
+      rc = with_size<PL>(p.size_h, [&](auto z) {
+        return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, false>(b, se, st, "train_gemm_kernel (dH)");
       });
       if (rc) return rc;
     }
@@ -672,11 +672,10 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
       b.M = (int32_t)p.dp;
       b.N = (int32_t)up_to(nv, 8);
       b.K = (int32_t)N;
-      b.pairs = PL == 3 ? kTermPairs : 1;
       b.splits = 1;
       WeightEpilogue<OUT> we = {(uint8_t*)dW + v0 * d * (OUT == TMS_DTYPE_F32 ? 4 : 2), factor, (int32_t)nv, (int32_t)d};
-      rc = with_size(p.size_w, [&](auto z) {
-        return run_gemm<DT, decltype(z)::MI, decltype(z)::NI, true, true>(b, we, st, "train_gemm_kernel (dW)");
+      rc = with_size<PL>(p.size_w, [&](auto z) {
+        return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, true>(b, we, st, "train_gemm_kernel (dW)");
       });
       if (rc) return rc;
     }
@@ -723,8 +722,9 @@ extern "C" int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d
   if (N > 0) {
     if ((rc = lce_workspace(fn, hidden, weight, N, d, V, dtype, false, ws, workspace_bytes, terms, s))) return rc;
     const float s2 = (float)(*scale * 1.4426950408889634);
-    if (dtype == TMS_DTYPE_F16) rc = lce_forward<TMS_DTYPE_F16>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
-    else rc = lce_forward<TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
+    if (dtype == TMS_DTYPE_F16) rc = lce_forward<TMS_DTYPE_F16, 1>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
+    else if (dtype == TMS_DTYPE_BF16) rc = lce_forward<TMS_DTYPE_BF16, 1>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
+    else rc = lce_forward<TMS_DTYPE_BF16, 3>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
     if (rc) return rc;
   }
   if (N > 0 || reduction == TMS_REDUCE_NONE) return TMS_OK;

@@ -26,9 +26,15 @@ inline double gemm_us(int size, int64_t m, int64_t n, int64_t steps, int64_t spl
   return (double)((groups + 1023) / 1024) * ((double)each * 0.95 + 3.0);
 }
 
-inline int gemm_size(int64_t m, int64_t n, int64_t steps) {
-  int best = kGemm256;
-  for (int s = 1; s < kGemmSizes; s++)
+// Products of rows of three bf16 terms take six products a 64-step with seven tiles' loads:
+// as long as four steps. Their largest tile is 128 x 128: 256 x 256 has no registers for the
+// fragments that the next product shares (4096 x 32000 x 1024: 1.23 PFLOP/s against 1.31).
+inline int64_t gemm_steps(int64_t k, int planes) { return up_to(k, 64) / 64 * (planes == 3 ? 4 : 1); }
+inline int gemm_largest(int planes) { return planes == 3 ? kGemm128 : kGemm256; }
+
+inline int gemm_size(int64_t m, int64_t n, int64_t steps, int largest = kGemm256) {
+  int best = largest;
+  for (int s = best + 1; s < kGemmSizes; s++)
     if (gemm_us(s, m, n, steps, 1) < gemm_us(best, m, n, steps, 1)) best = s;
   return best;
 }
@@ -47,13 +53,13 @@ constexpr int64_t kFewRows = 64;
 // The splits and tiles of dH's product (d x N, over a piece of the vocabulary): its tiles are
 // few, so the piece is split until they fill the chip, as long as a split's sums (written,
 // and read but for the first piece, at about 4 TB/s) cost less than idle CUs.
-inline double lce_split(LcePlan& p, int64_t N, int64_t piece, int64_t pairs) {
+inline double lce_split(LcePlan& p, int64_t N, int64_t piece, int planes) {
   static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
-  const int64_t steps = up_to(piece, 64) / 64 * pairs;
+  const int64_t steps = gemm_steps(piece, planes);
   double least = 1e30;
   for (int s : kSplits) {
-    if (s > 1 && s * 2 > steps) break;
-    for (int size = 0; size < kGemmSizes; size++) {
+    if (s > 1 && s * 2 > piece / 64) break;
+    for (int size = gemm_largest(planes); size < kGemmSizes; size++) {
       const double us = gemm_us(size, p.dp, N, steps, s) + (double)s * (double)N * (double)p.dp * 8 / 4e6;
       if (us < least) least = us, p.splits = s, p.size_h = size;
     }
@@ -65,7 +71,8 @@ inline double lce_split(LcePlan& p, int64_t N, int64_t piece, int64_t pairs) {
 // or up to three more, whichever the three products take least over.
 inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   LcePlan best = {};
-  const int64_t pairs = planes == 3 ? 6 : 1, dp = up_to(d > 0 ? d : 8, 8);
+  const int64_t dp = up_to(d > 0 ? d : 8, 8), steps_d = gemm_steps(dp, planes), steps_n = gemm_steps(N, planes);
+  const int largest = gemm_largest(planes);
   const int64_t rows_p = N <= kFewRows ? kFewRows : up_to(N, 256);
   const int64_t tiles = up_to(V, 256) / 256;
   int64_t most = ((int64_t)1 << 28) / planes / rows_p / 256;
@@ -77,10 +84,9 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
     p.dp = dp;
     p.rows_p = rows_p;
     p.piece = (tiles + n - 1) / n * 256;
-    p.size_p = gemm_size(p.piece, N, up_to(dp, 64) / 64 * pairs);
-    p.size_w = gemm_size(dp, p.piece, up_to(N, 64) / 64 * pairs);
-    const double us = gemm_us(p.size_p, p.piece, N, up_to(dp, 64) / 64 * pairs, 1) + gemm_us(p.size_w, dp, p.piece, up_to(N, 64) / 64 * pairs, 1) +
-                      lce_split(p, N, p.piece, pairs);
+    p.size_p = gemm_size(p.piece, N, steps_d, largest);
+    p.size_w = gemm_size(dp, p.piece, steps_n, largest);
+    const double us = gemm_us(p.size_p, p.piece, N, steps_d, 1) + gemm_us(p.size_w, dp, p.piece, steps_n, 1) + lce_split(p, N, p.piece, planes);
     const double all = us * (double)((tiles * 256 + p.piece - 1) / p.piece);
     if (all < least) least = all, best = p;
   }
