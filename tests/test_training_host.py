@@ -255,7 +255,7 @@ def plan(tmp_path_factory):
 
 
 def test_plan_bounds(plan):
-    """Pieces cover the vocabulary, P fits its 2^28 terms (or is one block of 256 columns),
+    """Pieces cover the vocabulary, P fits its 2^29 terms (or is one block of 256 columns),
     and the sums of the splits are bounded."""
     out = (ctypes.c_int64 * 7)()
     sizes = (1, 2, 63, 64, 65, 255, 256, 257, 500, 1024, 1229, 8192, 100_000, 1 << 24)
@@ -265,7 +265,7 @@ def test_plan_bounds(plan):
         assert dp % 8 == 0 and d <= dp < d + 9
         assert rows == 64 if N <= 64 else rows % 256 == 0 and N <= rows < N + 256
         assert piece % 256 == 0 and 256 <= piece <= -(-V // 256) * 256
-        assert rows * piece * planes <= 1 << 28 or piece == 256
+        assert rows * piece * planes <= 1 << 29 or piece == 256
         assert 1 <= splits <= 64 and all(0 <= s <= 2 for s in (size_p, size_h, size_w))
         steps = piece // 64 * (6 if planes == 3 else 1)
         assert splits == 1 or splits * 2 <= steps
@@ -276,7 +276,7 @@ def test_plan_of_large_and_small_products(plan):
     assert plan.gemm_size_of(64, 64, 12) == 2
     out = (ctypes.c_int64 * 7)()
     plan.lce_plan_of(8192, 131_072, 768, 1, out)
-    assert out[2] <= 32768 and out[4] == 0  # 512 MB of P at most, in large tiles
+    assert out[2] <= 65536 and out[4] == 0  # 1 GB of P at most, in large tiles
     plan.lce_plan_of(1024, 16384, 128, 1, out)
     assert out[2] == 16384 and out[3] > 1  # one piece, and dH's few tiles split over the vocabulary
     for size in (0, 1, 2):
