@@ -541,7 +541,7 @@ __device__ __forceinline__ f32x2 two(const uint8_t* p) {
 // token at a time: a thread counts and places its own run of maxima, so equal tokens keep their
 // order. Then each wave takes a quarter of the sorted maxima, cut between tokens, with the
 // rows of the next eight in flight while eight are added: 20 cycles of VALU work a maximum.
-// 64 queries of 32 tokens x 4096 documents of 60 to 180 tokens, d = 128, bf16: 181 us, bound by
+// 64 queries of 32 tokens x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 164 us, bound by
 // issue. (Products with a matrix of ones made from the positions cost a multiply-add for each
 // column, token and query block as well: 560 us.)
 // More than kRun blocks are sorted in runs; the sums stand in memory between them, in fp32.
@@ -701,7 +701,7 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
     for (int m = m0; m < m1; m += 64) {
       const int here = m1 - m < 64 ? m1 - m : 64;
       const int e = sorted[m + (lane < here ? lane : here - 1)];
-      const int k = first + k0 + (e >> 5), q = k / a.nbq;
+      const int k = first + k0 + (e >> 5), q = a.nbq == 1 ? k : k / a.nbq;
       const uint32_t row = (uint32_t)(q * a.nq + (k - q * a.nbq) * 32 + (e & 31));
       const uint32_t from = PAIR ? row * (uint32_t)(a.d * (int)sizeof(T)) : row;  // bytes, below 2^32
       const int j = tok[e];
@@ -710,7 +710,7 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
       const float w = lane < here ? weight[e >> 5] : 0.f;
       f32x2 x[2][AHEAD];
       auto load = [&](int buf, int s) {
-        if (s >= here) return;
+        if (s >= here || s >= 64) return;
 #pragma unroll
         for (int i = 0; i < AHEAD; i++) {
           const uint32_t r = (uint32_t)__builtin_amdgcn_readlane((int)from, s + i);
@@ -724,7 +724,7 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
         for (int i = 0; i < AHEAD; i++) {
           if ((firsts >> (s + i)) & 1) {
             const int js = __builtin_amdgcn_readlane(j, s + i);
-            while (cur != js) flush();
+            while (cur < js) flush();
           }
           const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), s + i));
           x0 = __builtin_fmaf(ws, x[buf][i][0], x0);
@@ -732,7 +732,8 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
         }
       };
       load(0, 0);
-      for (int s = 0; s < here; s += 2 * AHEAD) {
+#pragma unroll
+      for (int s = 0; s < 64; s += 2 * AHEAD) {  // lanes and bits are constants: half of the scalar work
         load(1, s + AHEAD);
         add(0, s);
         load(0, s + 2 * AHEAD);
@@ -766,7 +767,7 @@ __device__ __forceinline__ void put_q(const PairsGradArgs& a, int split, int64_t
 // row that answered it, 256 bytes in one wave's access. A lane finds its token's row, and the
 // wave takes the rows from the lanes one after another: four VALU instructions a token.
 // Where there is none, a row of zeros stands in. The runs' sums are joined by the kernel
-// below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, bf16: 155 us (with the
+// below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, 16 bits: 155 us (with the
 // positions through the scalar unit 278), bound by issue; the join takes 19 us.
 // WHOLE: rows in pieces of 16 bytes, on their way in registers meanwhile; others element by element.
 template <int DT, bool WHOLE>
