@@ -325,3 +325,11 @@ def test_graph(cuda, nQ, B, Nd):
         for a, b in zip(got, step()):
             assert torch.equal(a, b), replay
         torch.cuda.synchronize()
+
+
+# four blocks a wave: queries of one and of two blocks, the last group of waves full and not
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("nQ,Nq,B,Nd,d", [(27, 32, 90, 70, 128), (30, 7, 80, 33, 64), (14, 40, 160, 66, 96), (64, 32, 40, 37, 128),
+                                          (32, 20, 70, 130, 32)])
+def test_four_blocks_a_wave(cuda, nQ, Nq, B, Nd, d, dtype):
+    check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
