@@ -333,3 +333,38 @@ def test_graph(cuda, nQ, B, Nd):
                                           (32, 20, 70, 130, 32)])
 def test_four_blocks_a_wave(cuda, nQ, Nq, B, Nd, d, dtype):
     check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
+
+
+# enough query tokens and documents for the query gradient that shares documents: tokens in one
+# stage or several, rows in 16-byte pieces or element by element, last groups of waves partly empty
+@pytest.mark.parametrize("dtype", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("nQ,Nq,B,Nd,d", [(60, 5, 140, 270, 40), (65, 3, 130, 30, 77), (30, 33, 140, 17, 136), (70, 4, 120, 130, 33),
+                                          (5, 30, 1700, 9, 128), (17, 32, 500, 20, 64)])
+def test_shared_documents_in_the_query_gradient(cuda, nQ, Nq, B, Nd, d, dtype):
+    assert nQ * -(-Nq // 32) * B > 8192
+    check(nQ, Nq, B, Nd, d, dtype, seed=nQ * 3 + Nq + B)
+
+
+@pytest.mark.parametrize("nQ,B", [(6, 40), (60, 140)])
+def test_infinite_gradient_stays_where_it_belongs(cuda, nQ, B):
+    """An infinite gradient of one score: query tokens and documents without a maximum in that
+    pair keep the gradients that they have without it."""
+    import tilemaxsim_amd as tms
+    rng = np.random.default_rng(B)
+    Q, D = (_grid(rng, *s).half().cuda().requires_grad_(True) for s in ((nQ, 9, 64), (B, 30, 64)))
+    qmask, dmask = torch.ones(nQ, 9, dtype=torch.bool, device="cuda"), torch.ones(B, 30, dtype=torch.bool, device="cuda")
+    qmask[2, 4:] = False
+    dmask[5, 20:] = False
+    scores = tms.maxsim_pairs(Q, D, dmask, qmask)
+    G = torch.randn(nQ, B, device="cuda")
+    G[2, 5] = 0
+    dQ, dD = torch.autograd.grad(scores, (Q, D), G, retain_graph=True)
+    G[2, 5] = math.inf
+    eQ, eD = torch.autograd.grad(scores, (Q, D), G)
+    hit = torch.zeros(nQ, 9, dtype=torch.bool, device="cuda")
+    hit[2, :4] = True
+    assert torch.equal(dQ[~hit], eQ[~hit]) and not bool(torch.isfinite(eQ[hit]).any())
+    others = torch.arange(B, device="cuda") != 5
+    assert torch.equal(dD[others], eD[others]) and bool((eD[5, 20:] == 0).all())
+    won = ~torch.isfinite(eD[5]).all(-1)
+    assert 1 <= int(won.sum()) <= 4 and torch.equal(dD[5][~won], eD[5][~won])

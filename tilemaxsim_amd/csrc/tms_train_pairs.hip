@@ -111,7 +111,8 @@ __device__ constexpr int kPairD[6] = {0, 2, 1, 0, 1, 0};
 // Four waves take a document's 16-token tiles in turn, and join through LDS: the form of
 // small calls and of documents that one query alone sees, whose tokens are read once and
 // straight into MFMA fragments. KS > 0: d = 32 KS, the query block's fragments in registers.
-// KS = 0: any d and any number of planes, fragments read as they are used.
+// KS = 0: any d, fragments read as they are used. Bound by the latency of a tile's loads: 32 queries
+// x 8 documents of their own of 171 tokens, d = 128, fp16: 7 us.
 template <int DT, int KS, int PL>
 __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
   __shared__ Best joined[4][32];
@@ -126,7 +127,7 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
   bool some = false;  // a real document token, in any lane of the workgroup
   for (int blk = 0; blk < a.nbq; blk++) {
     bool real[2];
-    u32x4 qf[KS ? KS : 1][2];
+    u32x4 qf[PL][KS ? KS : 1][2];
     const uint8_t* qp[2];
 #pragma unroll
     for (int h = 0; h < 2; h++) {
@@ -135,10 +136,12 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
       qp[h] = a.Q + (qrow + (tok < a.nq ? tok : 0)) * width + 16 * g;
       if constexpr (KS > 0) {
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-          const u32x4 v = *(const u32x4*)(qp[h] + 64 * s);
-          qf[s][h] = real[h] ? v : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int p = 0; p < PL; p++)
+#pragma unroll
+          for (int s = 0; s < KS; s++) {
+            const u32x4 v = *(const u32x4*)(qp[h] + p * a.qplane + 64 * s);
+            qf[p][s][h] = real[h] ? v : u32x4{0u, 0u, 0u, 0u};
+          }
       }
     }
     Best best[2] = {{-__builtin_inff(), kNone}, {-__builtin_inff(), kNone}};
@@ -153,13 +156,17 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
       const uint8_t* dp = a.D + (drow + tok) * width + 16 * g;
       f32x4 acc[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
       if constexpr (KS > 0) {
-        u32x4 df[KS];
+        u32x4 df[PL][KS];
 #pragma unroll
-        for (int s = 0; s < KS; s++) df[s] = *(const u32x4*)(dp + 64 * s);
+        for (int p = 0; p < PL; p++)
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+          for (int s = 0; s < KS; s++) df[p][s] = *(const u32x4*)(dp + p * a.dplane + 64 * s);
 #pragma unroll
-          for (int h = 0; h < 2; h++) acc[h] = mfma16x16x32<DT>(df[s], qf[s][h], acc[h]);
+        for (int p = PL == 1 ? 5 : 0; p < 6; p++)
+#pragma unroll
+          for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int h = 0; h < 2; h++) acc[h] = mfma16x16x32<DT>(df[kPairD[p]][s], qf[kPairQ[p]][s][h], acc[h]);
       } else {
         for (int p = PL == 1 ? 5 : 0; p < 6; p++)
           for (int s = 0; s * 64 < width; s++) {
@@ -768,7 +775,7 @@ __device__ __forceinline__ void put_q(const PairsGradArgs& a, int split, int64_t
 // wave takes the rows from the lanes one after another: four VALU instructions a token.
 // Where there is none, a row of zeros stands in. The runs' sums are joined by the kernel
 // below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, 16 bits: 155 us (with the
-// positions through the scalar unit 278), bound by issue; the join takes 19 us.
+// positions through the scalar unit 278), bound by issue; the join takes 10 us.
 // WHOLE: rows in pieces of 16 bytes, on their way in registers meanwhile; others element by element.
 template <int DT, bool WHOLE>
 __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
@@ -883,6 +890,8 @@ __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
 
 // dQ, few queries or documents of their own: eight waves share eight query tokens and 128
 // columns, take the documents in turn straight from memory, and join through LDS in order.
+// Bound by the latency of a position and then its row, eight of each in flight: 32 queries x 8
+// documents of their own, d = 128: 5 us.
 template <int DT>
 __global__ __launch_bounds__(512) void pairs_grad_q_few_kernel(PairsGradArgs a) {
   constexpr int ES = DT == TMS_DTYPE_F32 ? 4 : 2;
@@ -937,14 +946,28 @@ __global__ __launch_bounds__(512) void pairs_grad_q_few_kernel(PairsGradArgs a) 
   put_q<DT>(a, split, (int64_t)q * a.nq + i0 + wave, col, x[0], x[1]);
 }
 
+// The splits' sums: four waves take a quarter of the splits each for 64 elements, eight loads at
+// a time, and join in order. Bound by latency where there are few elements, else by the read.
 template <int DT>
 __global__ __launch_bounds__(256) void pairs_grad_q_join_kernel(const float* parts, void* dQ, int64_t n, int splits) {
   typedef typename El<DT>::T T;
-  const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (k >= n) return;
+  __shared__ float sums[4][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t k = (int64_t)blockIdx.x * 64 + lane;
+  const int each = (splits + 3) / 4, s0 = wave * each, s1 = s0 + each < splits ? s0 + each : splits;
   float x = 0.f;
-  for (int s = 0; s < splits; s++) x += parts[s * n + k];
-  ((T*)dQ)[k] = (T)x;
+  if (k < n) {
+    for (int s = s0; s < s1; s += 8) {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; i++) y[i] = s + i < s1 ? parts[(s + i) * n + k] : 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; i++) x += y[i];
+    }
+  }
+  sums[wave][lane] = x;
+  __syncthreads();
+  if (wave == 0 && k < n) ((T*)dQ)[k] = (T)(sums[0][lane] + sums[1][lane] + sums[2][lane] + sums[3][lane]);
 }
 
 // ---------------------------------------------------------------- host
@@ -957,11 +980,13 @@ static bool as_is(const void* p, int64_t d, int dtype) {
 }
 static int planes(int dtype) { return dtype == TMS_DTYPE_F32 ? 3 : 1; }
 
-// dQ's form and its splits of the documents. From 256 query tokens on (half of a workgroup's)
-// the form that shares documents; one workgroup a CU then. The other fills the chip twice
-// over, with at least eight documents (one a wave) a split. The sums of a split are written
-// and read once, so no more splits than fill the chip. A multiple of 8 where there are
-// several: workgroups go to the XCDs in turn, so an XCD then keeps to its own documents.
+// dQ's form and its splits of the documents. The form that shares documents takes one workgroup
+// a CU, and pays from about 8,192 blocks of 32 maxima on (32-token queries x documents of 180
+// tokens, d = 128, 16 bits, few / shared: 64 x 100 19 / 28 us, 16 x 1000 53 / 38, 4 x 4000 55 / 40, 64 x 4096 761 / 158).
+// The other fills the chip twice over, with at least eight documents (one a wave) a split. The
+// sums of a split are written and read once, so no more splits than fill the chip. A multiple
+// of 8 where there are several: workgroups go to the XCDs in turn, so an XCD then keeps to its
+// own documents.
 struct GradQ {
   bool shared;
   int splits;
@@ -969,7 +994,7 @@ struct GradQ {
 static GradQ grad_q_form(int64_t nQ, int64_t nq, int64_t d, int64_t B, int64_t nway) {
   const int64_t cols = (d + 127) / 128, blocks = nQ * ((nq + 31) / 32);
   GradQ f;
-  f.shared = nway == 0 && blocks >= 8 && B >= 64;
+  f.shared = nway == 0 && blocks >= 4 && blocks * B > 8192;
   const int64_t units = (f.shared ? (blocks + 15) / 16 : nQ * ((nq + 7) / 8)) * cols;
   const int64_t most = f.shared ? B / 4 : (nway ? nway : B) / 8;
   int64_t s = (f.shared ? 256 : 512) / (units > 0 ? units : 1);
@@ -1042,9 +1067,11 @@ template <int DT, int PL>
 static int run_pairs(PairsArgs& a, hipStream_t st) {
   const int64_t blocks = (int64_t)a.nQ * a.nbq;
   const int ks = a.d / 32;
-  // Sharing pays once the waves are mostly filled; a call of few pairs needs a workgroup for
-  // each instead. A document takes at most kMaskWords stages (65,535 tokens).
-  const bool shared = !a.nway && ks <= 4 && a.nbq <= (PL == 3 ? 1 : 4) && blocks >= 4 && a.B * a.nQ > 2048;
+  // Sharing pays once there are workgroups enough; a call of few pairs needs one for each
+  // instead. (16 bits, d = 128, 180 tokens, direct / shared: 32 x 32 pairs 11 / 17 us, 8 x 128 11 / 11, 8 x 256
+  // 20 / 11, 2 x 2000 41 / 27, 1 x 4000 42 / 46; fp32: 8 x 32 19 / 26, 4 x 125 32 / 31, 32 x 32 42 / 27, 2 x 2000
+  // 234 / 201.) A document takes at most kMaskWords stages (65,535 tokens).
+  const bool shared = !a.nway && ks <= 4 && a.nbq <= (PL == 3 ? 1 : 4) && blocks >= 2 && a.B * a.nQ > (PL == 3 ? 512 : 1024);
   if (shared) {
     switch (ks) {
       case 1: return run_width<DT, 1, PL>(a, st);
@@ -1053,12 +1080,12 @@ static int run_pairs(PairsArgs& a, hipStream_t st) {
       default: return run_width<DT, 4, PL>(a, st);
     }
   }
-  if (PL == 1) switch (ks) {
-      case 1: return run_direct<DT, 1, 1>(a, st);
-      case 2: return run_direct<DT, 2, 1>(a, st);
-      case 3: return run_direct<DT, 3, 1>(a, st);
-      case 4: return run_direct<DT, 4, 1>(a, st);
-    }
+  switch (ks) {
+    case 1: return run_direct<DT, 1, PL>(a, st);
+    case 2: return run_direct<DT, 2, PL>(a, st);
+    case 3: return run_direct<DT, 3, PL>(a, st);
+    case 4: return run_direct<DT, 4, PL>(a, st);
+  }
   return run_direct<DT, 0, PL>(a, st);
 }
 
@@ -1116,7 +1143,7 @@ static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
     }
     if (a.splits > 1) {
       const int64_t m = (int64_t)a.nQ * a.nq * a.d;
-      hipLaunchKernelGGL(pairs_grad_q_join_kernel<DT>, dim3((unsigned)((m + 255) / 256)), dim3(256), 0, st, a.parts, a.dQ, m, a.splits);
+      hipLaunchKernelGGL(pairs_grad_q_join_kernel<DT>, dim3((unsigned)((m + 63) / 64)), dim3(256), 0, st, a.parts, a.dQ, m, a.splits);
       if ((rc = check_launch("pairs_grad_q_join_kernel"))) return rc;
     }
   }
