@@ -14,6 +14,10 @@
 // tensors' first chunks, which the scalar unit reads. A workgroup takes whole chunks of
 // kChunkElems elements, so that tensors of any size share the chip evenly.
 //
+// 390 fp32 gradients (336 M elements): the norm 225 us (6.0 TB/s), both 785 us: 4.03 GB at 5.1
+// TB/s, where a device copy moves 4.94. 198 bf16 ones into fp32 (109 M): 190 us of kernels, 220
+// with the host's work on the list, which bounds that call. Three small ones: 4 + 5 us.
+//
 // Squares are added in 64 bits: an fp32 gradient's square can neither overflow nor vanish,
 // and 10^9 terms lose nothing that 32 bits of the result would show. The vector units have
 // an order of magnitude more fp64 FMAs than memory brings elements.

@@ -34,7 +34,10 @@ struct RowStat {
   float top, sum;  // of a block: the largest x log2(e), and the sum of exp2 relative to it
 };
 
-// Rows n of a wave's columns: 16 j + c.
+// The forward pass's statistics, from the sums in registers: a lane has four rows of the
+// vocabulary for each of its hidden rows, and a wave one RowStat a hidden row and tile. 8192 x
+// 131072 x 768 in bf16: 1.44 ms, 1.15 PFLOP/s, bound by the matrix cores and, with twelve steps
+// a tile, by the 6 us in 25 that a tile's first loads and its exponentials take.
 struct LseEpilogue {
   static constexpr int kRowBytes = 0;
   RowStat* parts;  // [block of the vocabulary][rows]
@@ -77,7 +80,8 @@ struct LseEpilogue {
 
 // P of one piece: [plane][row][ldp]; rows and columns that do not exist are zero. A lane holds
 // four neighbouring columns of a row, so a wave's rows pass through its LDS and leave as whole
-// lines (eight-byte stores left half-written lines: 333 us a piece of 8192 x 21,760 at d = 768).
+// lines (eight-byte stores left half-written lines: a quarter more time). 8192 x 65,536 of them
+// at d = 768 in bf16: 0.85 ms, 0.98 PFLOP/s, bound like the statistics' product; 1 GB leaves with it.
 template <int DT, int PL, int MIV>
 struct ProbEpilogue {
   static constexpr int kRowBytes = MIV * 32 + 16;  // 16 more: the rows of four lanes fall on other banks
@@ -161,7 +165,9 @@ struct ProbEpilogue {
   }
 };
 
-// Sums of dH: [split][row][d], added to from the second piece on.
+// Sums of dH: [split][row][d], added to from the second piece on. A piece of 65,536 at 8192 rows
+// of 768 in bf16, five splits: 0.93 ms, 0.89 PFLOP/s, bound by the product (two rounds of 480 workgroups)
+// and 250 MB of sums read and written.
 struct SumEpilogue {
   static constexpr int kRowBytes = 0;
   float* out;
@@ -199,7 +205,8 @@ __device__ __forceinline__ uint16_t to16(float x) {
   return __builtin_bit_cast(uint16_t, (__bf16)x);
 }
 
-// dW of one piece, finished: times *factor, in the inputs' type.
+// dW of one piece, finished: times *factor, in the inputs' type. 65,536 rows of 768 over 8192 in
+// bf16: 0.75 ms, 1.1 PFLOP/s (three whole rounds of workgroups; pieces half as large take one and a half).
 template <int OUT>
 struct WeightEpilogue {
   static constexpr int kRowBytes = 0;
@@ -253,7 +260,8 @@ __device__ __forceinline__ float element(const void* p, int64_t i, int dt) {
 
 // Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms: three of
 // a float, 16-bit elements as they are; eight a thread. With `ref`, rows without a gradient
-// become zeros: what stands in them (NaN included) takes no part.
+// become zeros: what stands in them (NaN included) takes no part. 8000 rows of 256 floats: 5 us,
+// bound by the launch.
 template <bool F32>
 __global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, uint16_t* dst, int64_t rows, int32_t d, int32_t dp, int64_t plane,
                                                         const float* ref) {
@@ -310,7 +318,8 @@ __device__ __forceinline__ RowStat join_stats(RowStat a, RowStat b) {
 // Joins a row's blocks, and forms its target's logit from the inputs; LANES lanes a row. A
 // target outside the vocabulary (and not ignored) makes the row NaN. With `loss` and one
 // workgroup, that goes over all rows and then reduces them as the kernel below does: a call
-// of a few rows is bound by its launches.
+// of a few rows is bound by its launches. Bound by the latency of a row's statistics and, in
+// turn, its dot product: 1024 rows of 128 blocks 6 us, 8192 of 1024 24 us (67 MB read).
 template <int LANES>
 __global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int32_t blocks, int32_t rows, const void* H, const void* W,
                                                        int dt, int32_t V, int32_t d, const int64_t* target, int64_t ignore, float s2,
@@ -387,7 +396,8 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int
   }
 }
 
-// The sum or mean of the rows' losses, and how many rows count.
+// The sum or mean of the rows' losses, and how many rows count: in 64 bits and one workgroup,
+// bound by its loads' latency, 5 us for 8192 rows.
 __global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* rows_loss, const int64_t* target, int64_t ignore, int32_t rows,
                                                           int mean, float* loss, float* count) {
   __shared__ double sums[16];
@@ -419,7 +429,7 @@ __global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* rows_loss
 }
 
 // What the backward kernels take for each row: g / u, its reference for exp2 and its target;
-// and u with the factor of both gradients' sums.
+// and u with the factor of both gradients' sums. One workgroup, 9 us for 8192 rows.
 __global__ __launch_bounds__(1024) void lce_rows_kernel(const float* lse2, const int64_t* target, int64_t ignore, int32_t V, int32_t rows,
                                                         const float* grad, int per_row, const float* count, float up, float scale,
                                                         float* g, float* ref, int32_t* hit, float* factor) {
@@ -452,7 +462,8 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float* lse2, const
 }
 
 // dH: the splits' sums, in order, times the factor, in the inputs' type. Four elements of a row
-// a thread (rows of sums are whole multiples of four), eight splits' loads at a time.
+// a thread (rows of sums are whole multiples of four), eight splits' loads at a time. 8192 x 768,
+// five splits: 26 us, 5.3 TB/s.
 template <int OUT>
 __global__ __launch_bounds__(256) void lce_hidden_kernel(const float* sums, int splits, int64_t split, int32_t rows, int32_t d, int32_t dp,
                                                          const float* factor, void* dH) {
