@@ -858,7 +858,7 @@ __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
   __syncthreads();
   for (int buf = 0; now.b < e1; buf ^= 1) {
     const uint32_t j = at_next - (uint32_t)now.t0;
-    const bool here = j < (uint32_t)a.tokens;  // kNone is beyond every stage
+    const bool here = j < (uint32_t)tokens(now);  // of the tokens that there are: kNone is none of them
     const uint32_t row = (here ? j : (uint32_t)a.tokens) * ROW + buf * size;
     const float w = w_next;
     look(soon);
