@@ -389,8 +389,10 @@ int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, con
  * stands in them is not looked at in the gradients); any other value outside [0, V) makes
  * its row NaN. *scale (positive, read during the call from the host) multiplies the logits.
  * loss: N floats (TMS_REDUCE_NONE), or one: the rows' sum, or their mean over the rows that
- * are not ignored (NaN if none is left). stats: N + 1 floats of device memory that
- * tms_linear_cross_entropy_grad takes: the rows' log-sum-exp (in powers of two) and that count.
+ * are not ignored (NaN if none is left). stats: tms_lce_stats(N) floats of device memory that
+ * tms_linear_cross_entropy_grad takes: the rows' largest logits (in powers of two), 1 over their
+ * sums of exponentials relative to those, the share of each sum that is not the target's, and
+ * that count.
  * `grad` is what comes back for `loss`; dH (N, d) and dW (V, d) in `dtype`, either may be
  * NULL. With N = 0 nothing is written to dH and dW. Sums are fp32 in one order.
  * workspace: tms_lce_workspace_size bytes of device memory (backward = 0 or 1), 256-byte
@@ -400,6 +402,7 @@ int tms_maxsim_pairs_grad(const void* Qs, int64_t nQ, int64_t nq, int64_t d, con
 #define TMS_REDUCE_SUM 1
 #define TMS_REDUCE_MEAN 2
 int64_t tms_lce_workspace_size(int64_t N, int64_t d, int64_t V, int dtype, int backward);
+int64_t tms_lce_stats(int64_t N); /* 3 N + 1 */
 int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d, const void* weight, int64_t V, int dtype,
                              const int64_t* target, int64_t ignore_index, const double* scale, int reduction,
                              void* workspace, int64_t workspace_bytes, float* loss, float* stats, void* stream);

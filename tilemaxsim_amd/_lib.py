@@ -91,6 +91,7 @@ SIGNATURES = {
     "tms_maxsim_pairs_grad": [_c_void_p, _i64, _i64, _i64, _c_void_p, _i64, _i64, _i64, _c_void_p, _c_void_p, _int,
                               _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
     "tms_lce_workspace_size": [_i64, _i64, _i64, _int, _int],
+    "tms_lce_stats": [_i64],
     "tms_linear_cross_entropy": [_c_void_p, _i64, _i64, _c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _int, _c_void_p,
                                  _i64, _c_void_p, _c_void_p, _c_void_p],
     "tms_linear_cross_entropy_grad": [_c_void_p, _i64, _i64, _c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _int,
@@ -102,7 +103,7 @@ SIGNATURES = {
 RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
             "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64,
-            "tms_lce_workspace_size": ctypes.c_int64}
+            "tms_lce_workspace_size": ctypes.c_int64, "tms_lce_stats": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

@@ -34,7 +34,7 @@ def _forward(H, W, target, scale, ignore_index, reduction):
     code = _lib.dtype_code(H.dtype)
     lib = _lib.load()
     loss = torch.empty(N if reduction == _lib.TMS_REDUCE_NONE else (), dtype=torch.float32, device=H.device)
-    stats = torch.empty(N + 1, dtype=torch.float32, device=H.device)
+    stats = torch.empty(lib.tms_lce_stats(N), dtype=torch.float32, device=H.device)
     ws, nbytes = _workspace(lib, N, d, V, code, 0, H.device)
     factor = ctypes.c_double(scale)
     status = _lib.launch(H.device, lib.tms_linear_cross_entropy, H.data_ptr(), N, d, W.data_ptr(), V, code, target.data_ptr(),

@@ -1,8 +1,8 @@
 // Softmax cross entropy of the logits scale * H W^T, from the hidden states and the
 // vocabulary's weights, without the logits.
 //
-//   x[n, v] = scale <H[n], W[v]>,  lse[n] = log sum_v exp x[n, v],  loss[n] = lse[n] - x[n, t[n]]
-//   P[n, v] = exp(x[n, v] - lse[n]) - [v = t[n]]
+//   x[n, v] = scale <H[n], W[v]>,  loss[n] = log sum_v exp x[n, v] - x[n, t[n]]
+//   P[n, v] = exp x[n, v] / sum_u exp x[n, u] - [v = t[n]]
 //   dH[n] = g[n] scale sum_v P[n, v] W[v],   dW[v] = scale sum_n g[n] P[n, v] H[n]
 //
 // Forward: one product whose epilogue reduces each tile's logits to a maximum and a sum of
@@ -12,7 +12,12 @@
 // where writing and reading them in fp32 would take 8 N V bytes: at d = 768 as long, at less
 // shorter), become P in 16 bits in a workspace, and two more products take P to dH and dW.
 //
-// Everything is in powers of two: x log2(e) goes into exp2, and lse is kept in those units.
+// Everything is in powers of two: x log2(e) goes into exp2. A row keeps its largest logit, the
+// sum of exp2 relative to it, and the others' share of that sum (all but the target's): with
+// rest = sum over v != t of exp(x[v] - x[t]), the loss is log(1 + rest) and P at the target
+// -rest / (1 + rest). Neither is a difference of two numbers of the logits' size, or of a
+// softmax near 1 and 1, so a row that is nearly right keeps its digits. (From one log-sum-exp
+// a row, a loss of 2e-3 at logits near 300 was 1e-2 of itself off, and P at the target as much.)
 //
 // Precision. Logits, maxima, sums, and the sums of both gradients are fp32. P is rounded to
 // the inputs' type (bf16: 2^-9 of each term, below the rounding of the result; fp16: P is
@@ -27,11 +32,12 @@
 
 namespace tms {
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr double kLog2e = 1.4426950408889634;
+constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kP16 = 15;  // fp16: P times 2^15
 
 struct RowStat {
-  float top, sum;  // of a block: the largest x log2(e), and the sum of exp2 relative to it
+  float top, sum;  // of a block: the largest x log2(e), and the sum of exp2 relative to it but the target's
 };
 
 // The forward pass's statistics, from the sums in registers: a lane has four rows of the
@@ -41,13 +47,38 @@ struct RowStat {
 struct LseEpilogue {
   static constexpr int kRowBytes = 0;
   RowStat* parts;  // [block of the vocabulary][rows]
+  const int64_t* target;  // per row; outside the vocabulary: in no block
+  float* hit_sum;         // per row: the product's sum at its target
   int32_t rows, V;
   float s2;  // scale log2(e)
+
+  // The sum of a lane's elements of one row, and its target's element, which takes no part.
+  template <bool HIT, int MI, int NI>
+  __device__ __forceinline__ float sum_of(const f32x4 (&acc)[MI][NI], int j, float ref, int hit, float& at_hit) const {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < MI; i++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], s2, -ref));
+        if constexpr (HIT) {
+          const bool at = hit == 16 * i + e;
+          at_hit = at ? acc[i][j][e] : at_hit;
+          sum += at ? 0.f : p;
+        } else {
+          sum += p;
+        }
+      }
+    return sum;
+  }
 
   template <int MI, int NI>
   __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t*) const {
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
     const float NEG = -__builtin_inff();
+    int64_t t[NI];  // on their way while the maxima are formed
+#pragma unroll
+    for (int j = 0; j < NI; j++) t[j] = n + 16 * j + c < rows ? target[n + 16 * j + c] : -1;
     if (m + 16 * MI > V) {  // past the vocabulary
 #pragma unroll
       for (int i = 0; i < MI; i++)
@@ -57,6 +88,7 @@ struct LseEpilogue {
 #pragma unroll
             for (int j = 0; j < NI; j++) acc[i][j][e] = NEG;
     }
+    float tops[NI];
 #pragma unroll
     for (int j = 0; j < NI; j++) {
       float top = NEG;
@@ -64,15 +96,22 @@ struct LseEpilogue {
       for (int i = 0; i < MI; i++)
 #pragma unroll
         for (int e = 0; e < 4; e++) top = fmaxf(top, acc[i][j][e]);
-      top = cross_row_max(top) * s2;  // scale > 0
-      const float ref = top == NEG ? 0.f : top;
-      float sum = 0.f;
+      tops[j] = cross_row_max(top) * s2;  // scale > 0
+    }
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int i = 0; i < MI; i++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][e], s2, -ref));
-      sum = cross_row_sum(sum);
+    for (int j = 0; j < NI; j++) {
+      const float top = tops[j], ref = top == NEG ? 0.f : top;
       const int row = n + 16 * j + c;
+      const int hit = t[j] >= 0 && t[j] < V ? (int)t[j] - (m + 4 * g) : -1;  // the target's place among this lane's 16 i + e
+      float sum, at_hit = 0.f;
+      if (__ballot(hit >= 0 && hit < 16 * MI) != 0ull) {
+        sum = sum_of<true>(acc, j, ref, hit, at_hit);
+        if (hit >= 0 && hit < 16 * MI && (hit & 15) < 4) hit_sum[row] = at_hit;
+      } else {
+        sum = sum_of<false>(acc, j, ref, hit, at_hit);
+      }
+      sum = cross_row_sum(sum);
       if (g == 0 && row < rows && m < V) parts[(int64_t)(m / (16 * MI)) * rows + row] = {top, sum};
     }
   }
@@ -86,25 +125,24 @@ template <int DT, int PL, int MIV>
 struct ProbEpilogue {
   static constexpr int kRowBytes = MIV * 32 + 16;  // 16 more: the rows of four lanes fall on other banks
   uint16_t* P;
-  const float* lse2;     // per row; +inf for a row without a gradient
-  const float* g_row;    // per row: g / u
+  const float* top;       // per row: its largest logit; +inf for a row without a gradient
+  const float* g_row;     // per row: g / u over the sum of exp2
+  const float* hit_row;   // per row: what P is at its target
   const int32_t* target;  // per row; -1 for none
   int64_t plane;
   int32_t ldp, rows, V, v0;  // V: columns of the piece that exist; v0: its first
   float s2;
 
-  // p = (exp2(x - lse) - [v = target]) g of a lane's elements of one row, and its terms
+  // p = exp2(x - top) w of a lane's elements of one row, at its target at_hit, and its terms
   template <bool HIT, int MI>
-  __device__ __forceinline__ void row(const f32x4 (&x)[MI], float ref, float w, int hit, u32x2 (&out)[PL][MI]) const {
-    const float one = DT == TMS_DTYPE_F16 && PL == 1 ? (float)(1 << kP16) : 1.f;
+  __device__ __forceinline__ void row(const f32x4 (&x)[MI], float ref, float w, int hit, float at_hit, u32x2 (&out)[PL][MI]) const {
 #pragma unroll
     for (int i = 0; i < MI; i++) {
       float p[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s2, -ref));
-        if constexpr (HIT) p[e] -= hit == 16 * i + e ? one : 0.f;
-        p[e] *= w;
+        p[e] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i][e], s2, -ref)) * w;
+        if constexpr (HIT) p[e] = hit == 16 * i + e ? at_hit : p[e];
       }
 #pragma unroll
       for (int t = 0; t < PL; t++) {
@@ -142,14 +180,14 @@ struct ProbEpilogue {
     for (int j = 0; j < NI; j++) {
       const int r = n + 16 * j + c;
       const bool in = r < rows;
-      const float ref = in ? lse2[r] : __builtin_inff(), w = in ? g_row[r] : 0.f;
+      const float ref = in ? top[r] : __builtin_inff(), w = in ? g_row[r] : 0.f;
       const int hit = in ? target[r] - v0 - (m + 4 * g) : -1;  // its place among this lane's 16 i + e
       f32x4 x[MI];
 #pragma unroll
       for (int i = 0; i < MI; i++) x[i] = acc[i][j];
       u32x2 out[PL][MI];
-      if (__ballot(hit >= 0 && hit < 16 * MI) != 0ull) row<true>(x, ref, w, hit, out);
-      else row<false>(x, ref, w, hit, out);
+      if (__ballot(hit >= 0 && hit < 16 * MI) != 0ull) row<true>(x, ref, w, hit, in ? hit_row[r] : 0.f, out);
+      else row<false>(x, ref, w, hit, 0.f, out);
 #pragma unroll
       for (int t = 0; t < PL; t++) {
 #pragma unroll
@@ -252,12 +290,6 @@ struct WeightEpilogue {
 
 // ---------------------------------------------------------------- rows
 
-__device__ __forceinline__ float element(const void* p, int64_t i, int dt) {
-  if (dt == TMS_DTYPE_F32) return ((const float*)p)[i];
-  if (dt == TMS_DTYPE_F16) return (float)((const _Float16*)p)[i];
-  return (float)((const __bf16*)p)[i];
-}
-
 // Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms: three of
 // a float, 16-bit elements as they are; eight a thread. With `ref`, rows without a gradient
 // become zeros: what stands in them (NaN included) takes no part. 8000 rows of 256 floats: 5 us,
@@ -315,24 +347,27 @@ __device__ __forceinline__ RowStat join_stats(RowStat a, RowStat b) {
   return {t, a.sum * __builtin_amdgcn_exp2f(a.top - ref) + b.sum * __builtin_amdgcn_exp2f(b.top - ref)};
 }
 
-// Joins a row's blocks, and forms its target's logit from the inputs; LANES lanes a row. A
-// target outside the vocabulary (and not ignored) makes the row NaN. With `loss` and one
-// workgroup, that goes over all rows and then reduces them as the kernel below does: a call
-// of a few rows is bound by its launches. Bound by the latency of a row's statistics and, in
-// turn, its dot product: 1024 rows of 128 blocks 6 us, 8192 of 1024 24 us (67 MB read).
+// Joins a row's blocks and its target's exponential; LANES lanes a row. Writes what the backward
+// pass takes, [row] each: the largest logit, 1 over the sum of exp2 relative to it, and in the
+// place of hit_sum the others' share. A target outside the vocabulary (and not ignored) makes the
+// row NaN. With `loss` and one workgroup, that goes over all rows and then reduces them as the
+// kernel below does: a call of a few rows is bound by its launches. Bound by the latency of a
+// row's statistics: 1024 rows of 128 blocks 5 us, 8192 of 1024 20 us (67 MB read).
 template <int LANES>
-__global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int32_t blocks, int32_t rows, const void* H, const void* W,
-                                                       int dt, int32_t V, int32_t d, const int64_t* target, int64_t ignore, float s2,
-                                                       float* lse2, float* rows_loss, float* loss, float* count, int mean) {
+__global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int32_t blocks, int32_t rows, int32_t V, const int64_t* target,
+                                                       int64_t ignore, float s2, float* top, float* inv_sum, float* hit_sum,
+                                                       float* rows_loss, float* loss, float* count, int mean) {
   constexpr int ROWS = 256 / LANES;
   __shared__ RowStat stats[4];
-  __shared__ float dots[4];
   const int lane = threadIdx.x % LANES;
   double all = 0;
   int kept_rows = 0;
   for (int row0 = blockIdx.x * ROWS; row0 < rows; row0 += gridDim.x * ROWS) {
     const int row = row0 + threadIdx.x / LANES;
     const bool in = row < rows;
+    const int64_t t = in ? target[row] : ignore;
+    const bool kept = t != ignore, fine = t >= 0 && t < V;
+    const float hit = lane == 0 && kept && fine ? hit_sum[row] : 0.f;
     RowStat r = {-__builtin_inff(), 0.f};
     for (int b = lane; in && b < blocks; b += 8 * LANES) {  // eight loads at a time
       RowStat x[8];
@@ -344,47 +379,25 @@ __global__ __launch_bounds__(256) void lce_join_kernel(const RowStat* parts, int
 #pragma unroll
       for (int i = 0; i < 8; i++) r = join_stats(r, x[i]);
     }
-    const int64_t t = in ? target[row] : ignore;
-    const bool kept = t != ignore, fine = t >= 0 && t < V;
-    float dot = 0.f;
-    if (kept && fine) {
-      if (dt != TMS_DTYPE_F32 && d % 8 == 0) {  // then rows begin at 16 bytes
-        for (int k = lane * 8; k < d; k += LANES * 8) {
-          const u32x4 h = *(const u32x4*)((const uint16_t*)H + (int64_t)row * d + k), w = *(const u32x4*)((const uint16_t*)W + t * d + k);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const uint32_t a = h[e], c = w[e];
-            if (dt == TMS_DTYPE_F16) {
-              dot += (float)__builtin_bit_cast(_Float16, (uint16_t)a) * (float)__builtin_bit_cast(_Float16, (uint16_t)c);
-              dot += (float)__builtin_bit_cast(_Float16, (uint16_t)(a >> 16)) * (float)__builtin_bit_cast(_Float16, (uint16_t)(c >> 16));
-            } else {
-              dot += __builtin_bit_cast(float, a << 16) * __builtin_bit_cast(float, c << 16);
-              dot += __builtin_bit_cast(float, a & 0xffff0000u) * __builtin_bit_cast(float, c & 0xffff0000u);
-            }
-          }
-        }
-      } else {
-        for (int k = lane; k < d; k += LANES) dot += element(H, (int64_t)row * d + k, dt) * element(W, t * d + k, dt);
-      }
-    }
-#pragma unroll
-    for (int o = (LANES < 64 ? LANES : 64) / 2; o >= 1; o >>= 1) {
-      r = join_stats(r, RowStat{__shfl_xor(r.top, o), __shfl_xor(r.sum, o)});
-      dot += __shfl_xor(dot, o);
-    }
+    for (int o = (LANES < 64 ? LANES : 64) / 2; o >= 1; o >>= 1) r = join_stats(r, RowStat{__shfl_xor(r.top, o), __shfl_xor(r.sum, o)});
     if constexpr (LANES > 64) {
       __syncthreads();  // the last row's are read
-      if ((threadIdx.x & 63) == 0) stats[threadIdx.x >> 6] = r, dots[threadIdx.x >> 6] = dot;
+      if ((threadIdx.x & 63) == 0) stats[threadIdx.x >> 6] = r;
       __syncthreads();
-      r = stats[0], dot = dots[0];
+      r = stats[0];
 #pragma unroll
-      for (int w = 1; w < 4; w++) r = join_stats(r, stats[w]), dot += dots[w];
+      for (int w = 1; w < 4; w++) r = join_stats(r, stats[w]);
     }
-    float lse = r.top + log2f(r.sum);
-    if (kept && !fine) lse = __builtin_nanf("");
-    const float x = kept ? (lse - dot * s2) * kLn2 : 0.f;
+    const float y = __builtin_fmaf(hit, s2, -r.top);  // of the target, as every other exponent is formed
+    float sum = r.sum + __builtin_amdgcn_exp2f(y), x = 0.f;
+    if (kept && !fine) r.top = sum = __builtin_nanf("");
+    // Near the top the loss is log(1 + rest); away from it, at least ln 2, a sum of two positive numbers.
+    if (kept) x = !fine ? sum : y > -1.f ? log1pf(r.sum * __builtin_amdgcn_exp2f(-y)) : (log2f(sum) - y) * kLn2;
     if (in && lane == 0) {
-      lse2[row] = lse;
+      top[row] = r.top;
+      inv_sum[row] = 1.f / sum;
+      hit_sum[row] = r.sum / sum;
       if (rows_loss) rows_loss[row] = x;
     }
     all += (double)x;
@@ -428,35 +441,40 @@ __global__ __launch_bounds__(1024) void lce_reduce_kernel(const float* rows_loss
   }
 }
 
-// What the backward kernels take for each row: g / u, its reference for exp2 and its target;
-// and u with the factor of both gradients' sums. One workgroup, 9 us for 8192 rows.
-__global__ __launch_bounds__(1024) void lce_rows_kernel(const float* lse2, const int64_t* target, int64_t ignore, int32_t V, int32_t rows,
-                                                        const float* grad, int per_row, const float* count, float up, float scale,
-                                                        float* g, float* ref, int32_t* hit, float* factor) {
+// What the backward kernels take for each row: g / u over its sum of exp2, its reference for
+// exp2, its target and what P is there; and u with the factor of both gradients' sums. P is held
+// times 2^up. One workgroup, 12 us for 8192 rows.
+__global__ __launch_bounds__(1024) void lce_rows_kernel(const float* top, const float* inv_sum, const float* others, const int64_t* target,
+                                                        int64_t ignore, int32_t V, int32_t rows, const float* grad, int per_row,
+                                                        const float* count, int up, float scale, float* g, float* ref, int32_t* hit,
+                                                        float* at_hit, float* factor) {
   __shared__ float tops[16];
   float unit = 1.f;
   if (per_row) {
-    float top = 0.f;
+    float most = 0.f;
     for (int i = threadIdx.x; i < rows; i += 1024)
-      if (target[i] != ignore) top = fmaxf(top, fabsf(grad[i]));
+      if (target[i] != ignore) most = fmaxf(most, fabsf(grad[i]));
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    for (int o = 32; o >= 1; o >>= 1) most = fmaxf(most, __shfl_xor(most, o));
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = most;
     __syncthreads();
-    for (int w = 0; w < 16; w++) top = fmaxf(top, tops[w]);
-    int e = (int)((__builtin_bit_cast(uint32_t, top) >> 23) & 0xffu) + 1;  // 2^(e - 127) > top
-    e = top == 0.f || e > 252 ? 127 : e < 2 ? 2 : e;  // an infinite factor stays as it is
+    for (int w = 0; w < 16; w++) most = fmaxf(most, tops[w]);
+    int e = (int)((__builtin_bit_cast(uint32_t, most) >> 23) & 0xffu) + 1;  // 2^(e - 127) > most
+    e = most == 0.f || e > 252 ? 127 : e < 2 ? 2 : e;  // an infinite factor stays as it is
     unit = __builtin_bit_cast(float, (uint32_t)e << 23);
   } else {
     const float all = *grad / (count ? *count : 1.f);
     if (all != 0.f && fabsf(all) < 1e38f) unit = all;
   }
-  if (threadIdx.x == 0) *factor = unit * scale * exp2f(-up);
+  const float held = (float)(1 << up);
+  if (threadIdx.x == 0) *factor = unit * scale / held;
   for (int i = threadIdx.x; i < rows; i += 1024) {
     const int64_t t = target[i];
     const bool kept = t != ignore;
-    g[i] = !kept ? 0.f : (per_row ? grad[i] : *grad / (count ? *count : 1.f)) / unit;
-    ref[i] = kept ? lse2[i] - up : __builtin_inff();
+    const float w = !kept ? 0.f : (per_row ? grad[i] : *grad / (count ? *count : 1.f)) / unit * held;
+    g[i] = kept ? w * inv_sum[i] : 0.f;
+    at_hit[i] = kept ? -w * others[i] : 0.f;
+    ref[i] = kept ? top[i] : __builtin_inff();
     hit[i] = kept && t >= 0 && t < V ? (int32_t)t : -1;
   }
 }
@@ -531,7 +549,7 @@ struct Carve {
   }
 };
 struct LceSpace {
-  int64_t h, w, parts, loss, g, ref, hit, factor, p, sums, bytes;
+  int64_t h, w, parts, loss, g, ref, hit, at_hit, factor, p, sums, bytes;
 };
 static LceSpace lce_space(int64_t N, int64_t V, int64_t d, int dtype, bool backward, bool terms) {
   LceSpace s = {};
@@ -548,6 +566,7 @@ static LceSpace lce_space(int64_t N, int64_t V, int64_t d, int dtype, bool backw
     s.g = c.take(N * 4);
     s.ref = c.take(N * 4);
     s.hit = c.take(N * 4);
+    s.at_hit = c.take(N * 4);
     s.factor = c.take(4);
     s.p = c.take(p.rows_p * p.piece * 2 * planes(dtype));
     s.sums = c.take(p.splits * N * dp * 4);
@@ -606,7 +625,8 @@ static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64
     if ((rc = run_terms(W, dtype, ws + s.w, V, d, dp, nullptr, st))) return rc;
   }
   const GemmArgs a = logits_args(h, w, N, V, V, dp, dtype);
-  LseEpilogue e = {(RowStat*)(ws + s.parts), (int32_t)N, (int32_t)V, s2};
+  float *top = stats, *inv_sum = stats + N, *hit_sum = stats + 2 * N, *count = stats + 3 * N;
+  LseEpilogue e = {(RowStat*)(ws + s.parts), target, hit_sum, (int32_t)N, (int32_t)V, s2};
   const int size = logits_size(N, V, dp, dtype);
   rc = with_size<PL>(size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, false, false>(a, e, st, "train_gemm_kernel (lse)"); });
   if (rc) return rc;
@@ -617,30 +637,32 @@ static int lce_forward(const void* H, int64_t N, int64_t d, const void* W, int64
   // Few rows of many blocks take a workgroup each, many rows sixteen lanes each, which read
   // sixteen rows' neighbouring statistics together.
   if (N <= 1024)
-    hipLaunchKernelGGL(lce_join_kernel<256>, dim3(alone ? 1u : (unsigned)N), dim3(256), 0, st, parts, blocks, (int32_t)N, H, W, dtype, (int32_t)V,
-                       (int32_t)d, target, ignore, s2, stats, rows_loss, alone ? loss : nullptr, stats + N, reduction == TMS_REDUCE_MEAN ? 1 : 0);
+    hipLaunchKernelGGL(lce_join_kernel<256>, dim3(alone ? 1u : (unsigned)N), dim3(256), 0, st, parts, blocks, (int32_t)N, (int32_t)V, target,
+                       ignore, s2, top, inv_sum, hit_sum, rows_loss, alone ? loss : nullptr, count, reduction == TMS_REDUCE_MEAN ? 1 : 0);
   else
-    hipLaunchKernelGGL(lce_join_kernel<16>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, parts, blocks, (int32_t)N, H, W, dtype, (int32_t)V,
-                       (int32_t)d, target, ignore, s2, stats, rows_loss, nullptr, nullptr, 0);
+    hipLaunchKernelGGL(lce_join_kernel<16>, dim3((unsigned)((N + 15) / 16)), dim3(256), 0, st, parts, blocks, (int32_t)N, (int32_t)V, target,
+                       ignore, s2, top, inv_sum, hit_sum, rows_loss, nullptr, nullptr, 0);
   if ((rc = check_launch("lce_join_kernel")) || rows || alone) return rc;
   hipLaunchKernelGGL(lce_reduce_kernel, dim3(1), dim3(1024), 0, st, rows_loss, target, ignore, (int32_t)N, reduction == TMS_REDUCE_MEAN ? 1 : 0,
-                     loss, stats + N);
+                     loss, count);
   return check_launch("lce_reduce_kernel");
 }
 
 template <int DT, int PL, int OUT>
 static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int64_t V, int dtype, const int64_t* target, int64_t ignore,
-                        float scale, int reduction, const float* stats, const float* grad, uint8_t* ws, const LceSpace& s, bool terms,
+                        float scale, float s2, int reduction, const float* stats, const float* grad, uint8_t* ws, const LceSpace& s, bool terms,
                         void* dH, void* dW, hipStream_t st) {
   const LcePlan p = lce_plan(N, V, d, planes(dtype));
-  const float up = DT == TMS_DTYPE_F16 ? (float)kP16 : 0.f;
+  const int up = DT == TMS_DTYPE_F16 ? kP16 : 0;
   float *g = (float*)(ws + s.g), *ref = (float*)(ws + s.ref), *factor = (float*)(ws + s.factor), *sums = (float*)(ws + s.sums);
+  float* at_hit = (float*)(ws + s.at_hit);
   int32_t* hit = (int32_t*)(ws + s.hit);
   uint16_t *h = (uint16_t*)(ws + s.h), *P = (uint16_t*)(ws + s.p);
   const void* w = terms ? ws + s.w : W;
   int rc;
-  hipLaunchKernelGGL(lce_rows_kernel, dim3(1), dim3(1024), 0, st, stats, target, ignore, (int32_t)V, (int32_t)N, grad,
-                     reduction == TMS_REDUCE_NONE ? 1 : 0, reduction == TMS_REDUCE_MEAN ? stats + N : nullptr, up, scale, g, ref, hit, factor);
+  hipLaunchKernelGGL(lce_rows_kernel, dim3(1), dim3(1024), 0, st, stats, stats + N, stats + 2 * N, target, ignore, (int32_t)V, (int32_t)N, grad,
+                     reduction == TMS_REDUCE_NONE ? 1 : 0, reduction == TMS_REDUCE_MEAN ? stats + 3 * N : nullptr, up, scale, g, ref, hit, at_hit,
+                     factor);
   if ((rc = check_launch("lce_rows_kernel"))) return rc;
   if ((rc = run_terms(H, dtype, h, N, d, p.dp, ref, st))) return rc;
   if (terms && (rc = run_terms(W, dtype, ws + s.w, V, d, p.dp, nullptr, st))) return rc;
@@ -650,7 +672,7 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
     GemmArgs a = logits_args(h, (const uint16_t*)w + v0 * p.dp, N, nv, V, p.dp, dtype);
     rc = with_size<PL>(p.size_p, [&](auto z) {
       using Z = decltype(z);
-      const ProbEpilogue<DT, PL, Z::MI> e = {P, ref, g, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, scale * kLog2e};
+      const ProbEpilogue<DT, PL, Z::MI> e = {P, ref, g, at_hit, hit, pplane, (int32_t)p.piece, (int32_t)N, (int32_t)nv, (int32_t)v0, s2};
       return run_gemm<DT, PL, Z::MI, Z::NI, false, false>(a, e, st, "train_gemm_kernel (P)");
     });
     if (rc) return rc;
@@ -703,6 +725,8 @@ static int lce_backward(const void* H, int64_t N, int64_t d, const void* W, int6
 
 using namespace tms;
 
+extern "C" int64_t tms_lce_stats(int64_t N) { return N < 0 ? 0 : 3 * N + 1; }
+
 extern "C" int64_t tms_lce_workspace_size(int64_t N, int64_t d, int64_t V, int dtype, int backward) {
   if (N <= 0 || d < 0 || V <= 0) return 0;
   return lce_space(N, V, d, dtype, backward != 0, dtype == TMS_DTYPE_F32 || d % 8 != 0 || d == 0).bytes;
@@ -732,7 +756,7 @@ extern "C" int tms_linear_cross_entropy(const void* hidden, int64_t N, int64_t d
   bool terms = false;
   if (N > 0) {
     if ((rc = lce_workspace(fn, hidden, weight, N, d, V, dtype, false, ws, workspace_bytes, terms, s))) return rc;
-    const float s2 = (float)(*scale * 1.4426950408889634);
+    const float s2 = (float)(*scale * kLog2e);
     if (dtype == TMS_DTYPE_F16) rc = lce_forward<TMS_DTYPE_F16, 1>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
     else if (dtype == TMS_DTYPE_BF16) rc = lce_forward<TMS_DTYPE_BF16, 1>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
     else rc = lce_forward<TMS_DTYPE_BF16, 3>(hidden, N, d, weight, V, dtype, target, ignore_index, s2, reduction, ws, s, terms, loss, stats, st);
@@ -757,10 +781,10 @@ extern "C" int tms_linear_cross_entropy_grad(const void* hidden, int64_t N, int6
   if ((rc = lce_workspace(fn, hidden, weight, N, d, V, dtype, true, workspace, workspace_bytes, terms, s))) return rc;
   const hipStream_t st = (hipStream_t)stream;
   uint8_t* ws = (uint8_t*)workspace;
-  const float sc = (float)*scale;
+  const float sc = (float)*scale, s2 = (float)(*scale * kLog2e);  // s2: the forward pass's
   if (dtype == TMS_DTYPE_F16)
-    return lce_backward<TMS_DTYPE_F16, 1, TMS_DTYPE_F16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
+    return lce_backward<TMS_DTYPE_F16, 1, TMS_DTYPE_F16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, s2, reduction, stats, grad, ws, s, terms, dH, dW, st);
   if (dtype == TMS_DTYPE_BF16)
-    return lce_backward<TMS_DTYPE_BF16, 1, TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
-  return lce_backward<TMS_DTYPE_BF16, 3, TMS_DTYPE_F32>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, reduction, stats, grad, ws, s, terms, dH, dW, st);
+    return lce_backward<TMS_DTYPE_BF16, 1, TMS_DTYPE_BF16>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, s2, reduction, stats, grad, ws, s, terms, dH, dW, st);
+  return lce_backward<TMS_DTYPE_BF16, 3, TMS_DTYPE_F32>(hidden, N, d, weight, V, dtype, target, ignore_index, sc, s2, reduction, stats, grad, ws, s, terms, dH, dW, st);
 }
