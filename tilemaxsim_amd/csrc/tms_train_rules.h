@@ -32,7 +32,7 @@ inline double gemm_us(int size, int64_t m, int64_t n, int64_t steps, int64_t spl
 inline int64_t gemm_steps(int64_t k, int planes) { return up_to(k, 64) / 64 * (planes == 3 ? 4 : 1); }
 inline int gemm_largest(int planes) { return planes == 3 ? kGemm128 : kGemm256; }
 
-inline int gemm_size(int64_t m, int64_t n, int64_t steps, int largest = kGemm256) {
+inline int gemm_size(int64_t m, int64_t n, int64_t steps, int largest = kGemm256) {  // largest: the largest tile to take
   int best = largest;
   for (int s = best + 1; s < kGemmSizes; s++)
     if (gemm_us(s, m, n, steps, 1) < gemm_us(best, m, n, steps, 1)) best = s;
@@ -42,7 +42,7 @@ inline int gemm_size(int64_t m, int64_t n, int64_t steps, int largest = kGemm256
 // How linear cross entropy's backward pass goes over the vocabulary.
 struct LcePlan {
   int64_t dp;      // width of a row of terms
-  int64_t rows_p;  // rows of P: N up to a multiple of 256 (64 for up to 64 rows)
+  int64_t rows_p;  // rows of P: N up to a multiple of 256 (64 for up to 64 rows), whole tiles of size_p
   int64_t piece;   // columns of P, a multiple of 256
   int splits;      // of the vocabulary in dH's product
   int size_p, size_h, size_w;  // tiles of the three products
@@ -86,7 +86,8 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
     p.dp = dp;
     p.rows_p = rows_p;
     p.piece = (tiles + n - 1) / n * 256;
-    p.size_p = gemm_size(p.piece, N, steps_d, largest);
+    // P's product stores whole tiles: none taller than P, whatever the times say.
+    p.size_p = gemm_size(p.piece, N, steps_d, rows_p % gemm_side(largest) == 0 ? largest : kGemm64);
     p.size_w = gemm_size(dp, p.piece, steps_n, largest);
     const double us = gemm_us(p.size_p, p.piece, N, steps_d, 1) + gemm_us(p.size_w, dp, p.piece, steps_n, 1) + lce_split(p, N, p.piece, planes);
     const double all = us * (double)((tiles * 256 + p.piece - 1) / p.piece);
