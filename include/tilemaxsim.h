@@ -418,8 +418,8 @@ int tms_linear_cross_entropy_grad(const void* hidden, int64_t N, int64_t d, cons
  * the sum of squares (TMS_NORM_2, summed in 64 bits) or the largest absolute value
  * (TMS_NORM_INF), written to `norm` (one float of device memory).
  * tms_grad_clip also writes dst[i] = src[i] * min(1, *max_norm / (norm + 1e-6)), in dst's
- * dtype; dst may be src (then of one dtype), and must not overlap another source. A NaN or
- * infinite norm gives what that factor gives. *max_norm is read during the call, from the host.
+ * dtype; dst may be src (then of one dtype); one that overlaps another tensor's dst or src, or its
+ * own in part, is refused (TMS_ERR_INVALID). A NaN or infinite norm gives what that factor gives. *max_norm is read during the call, from the host.
  * `workspace`: tms_grad_workspace_size(count) bytes of device memory, 8-byte aligned.
  */
 #define TMS_NORM_INF 0

@@ -1,0 +1,43 @@
+"""CPU tests: calls of the training operators that would give a wrong result are refused, before
+any HIP call."""
+import ctypes
+
+import pytest
+from test_training_host import F16, F32, Grad, call, numbers
+
+KB = 1 << 10
+
+
+def clip(*entries):
+    """What the call says of these tensors; without a workspace, so that one it takes ends there."""
+    table, most = (Grad * len(entries))(*entries), numbers(1.0)[0]
+    return call("tms_grad_clip", ctypes.addressof(table), len(entries), 2, ctypes.addressof(most), None, 0, 16, None)
+
+
+IN_PLACE = Grad(4096 * KB, 4096 * KB, 256, F32, F32)  # 1 KB
+
+
+@pytest.mark.parametrize("entries", [
+    (IN_PLACE, IN_PLACE),  # one tensor twice, as tied weights are gathered module by module
+    (IN_PLACE, Grad(64, 64, 4, F16, F16), Grad(4097 * KB - 4, 4097 * KB - 4, 1, F32, F32)),  # its last element alone
+    (IN_PLACE, Grad(4096 * KB - 8, 4096 * KB - 8, 5, F16, F16)),  # and its first one, of another dtype
+    (Grad(64 * KB, 128 * KB, 256, F32, F32), Grad(192 * KB, 128 * KB, 256, F32, F32)),  # two gradients into one tensor
+    (Grad(64 * KB, 128 * KB, 256, F32, F32), Grad(128 * KB + 512, 256 * KB, 4, F32, F32)),  # into another one's gradient
+    (Grad(128 * KB + 512, 256 * KB, 4, F32, F32), Grad(64 * KB, 128 * KB, 256, F32, F32)),
+    (Grad(64 * KB, 64 * KB + 4, 256, F32, F32),),  # into itself, one element on
+    (Grad(64 * KB, 64 * KB, 256, F32, F16),),  # into itself in another dtype
+    tuple(Grad(k * KB, k * KB, 4, F32, F32) for k in (9, 2, 7, 5, 2, 8)),  # in no order
+    tuple(Grad((500 - k) * KB, (500 - k) * KB, 256, F32, F32) for k in range(300)) + (Grad(300 * KB, 300 * KB, 1, F32, F32),)])
+def test_overlapping_tensors_are_not_clipped(entries):
+    rc, msg = clip(*entries)
+    assert rc == 1 and "overlap" in msg and "tms_grad_clip" in msg
+
+
+@pytest.mark.parametrize("entries", [
+    (IN_PLACE, Grad(4097 * KB, 4097 * KB, 256, F32, F32), Grad(4095 * KB, 4095 * KB, 256, F32, F32)),  # end to end
+    (IN_PLACE, Grad(4096 * KB, 4096 * KB, 0, F32, F32)),  # an empty one takes no place
+    (Grad(64 * KB, 128 * KB, 256, F32, F32), Grad(64 * KB, 192 * KB, 256, F32, F32)),  # one gradient into two tensors
+    (Grad(64 * KB, 128 * KB, 256, F16, F32), Grad(64 * KB + 512, 129 * KB, 256, F16, F32))])
+def test_neighbours_and_shared_sources_are_taken(entries):
+    rc, msg = clip(*entries)
+    assert rc == 1 and "workspace" in msg

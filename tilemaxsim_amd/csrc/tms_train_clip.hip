@@ -23,6 +23,10 @@
 // an order of magnitude more fp64 FMAs than memory brings elements.
 #include <math.h>
 
+#include <algorithm>
+#include <memory>
+#include <new>
+
 #include "tms_common.h"
 
 namespace tms {
@@ -276,6 +280,50 @@ static int check_tensors(const char* fn, const tms_grad_tensor* tensors, int64_t
   return TMS_OK;
 }
 
+static int64_t dtype_size(int dt) { return dt == TMS_DTYPE_F32 ? 4 : 2; }
+
+// Refuses what two workgroups would write, or one write and another read: a tensor that is scaled
+// and overlaps another one's memory, or its own source other than as a whole. The written ranges
+// and the ones only read, each in order of their addresses (a model's mostly are already), are
+// gone through together, each against the range that reaches furthest so far.
+static int check_overlap(const char* fn, const tms_grad_tensor* tensors, int64_t count) {
+  struct Range {
+    uintptr_t begin, end;
+    int64_t tensor;
+    bool operator<(const Range& o) const { return begin < o.begin; }
+  };
+  Range few[512];
+  std::unique_ptr<Range[]> many;
+  Range* written = few;
+  if (2 * count > 512) {
+    many.reset(new (std::nothrow) Range[2 * (size_t)count]);
+    written = many.get();
+    if (!written) return fail(TMS_ERR_INVALID, "%s: no memory to look %lld tensors over", fn, (long long)count);
+  }
+  Range* read = written + count;
+  int64_t nw = 0, nr = 0;
+  for (int64_t i = 0; i < count; i++) {
+    const tms_grad_tensor& s = tensors[i];
+    if (s.n == 0) continue;
+    const uintptr_t src = (uintptr_t)s.src, dst = (uintptr_t)s.dst;
+    written[nw++] = {dst, dst + (uintptr_t)(s.n * dtype_size(s.dst_dtype)), i};
+    if (src != dst || s.src_dtype != s.dst_dtype) read[nr++] = {src, src + (uintptr_t)(s.n * dtype_size(s.src_dtype)), i};
+  }
+  if (!std::is_sorted(written, written + nw)) std::sort(written, written + nw);
+  if (!std::is_sorted(read, read + nr)) std::sort(read, read + nr);
+  Range far = {}, far_written = {};  // of all, and of those written
+  for (int64_t w = 0, r = 0; w < nw || r < nr;) {
+    const bool writes = r == nr || (w < nw && written[w].begin <= read[r].begin);
+    const Range& x = writes ? written[w++] : read[r++];
+    const Range& other = writes ? far : far_written;
+    if (x.begin < other.end)
+      return fail(TMS_ERR_INVALID, "%s: tensors %lld and %lld overlap, and one of them is written", fn, (long long)other.tensor, (long long)x.tensor);
+    if (x.end > far.end) far = x;
+    if (writes) far_written = x;  // written ranges that passed do not overlap: the last one reaches furthest
+  }
+  return TMS_OK;
+}
+
 static int norm_partials(const tms_grad_tensor* tensors, int64_t count, int norm_type, Partial* ws, hipStream_t st,
                          int& n) {
   ClipTable tab;
@@ -325,7 +373,7 @@ extern "C" int tms_grad_clip(const tms_grad_tensor* tensors, int64_t count, int 
                              void* workspace, int64_t workspace_bytes, float* norm, void* stream) {
   const char* fn = "tms_grad_clip";
   int rc = check_tensors(fn, tensors, count, norm_type, true);
-  if (rc) return rc;
+  if (rc || (rc = check_overlap(fn, tensors, count))) return rc;
   if (!max_norm || !(*max_norm >= 0)) return fail(TMS_ERR_INVALID, "%s: max_norm must be a number of at least 0", fn);
   if (!norm || !workspace || workspace_bytes < tms_grad_workspace_size(count))
     return fail(TMS_ERR_INVALID, "%s: NULL norm, or a workspace below tms_grad_workspace_size", fn);

@@ -61,6 +61,14 @@ def _table(src: list, dst: list) -> array:
     return words
 
 
+def _apart(fn: str, ts: list) -> None:
+    """Strided tensors are written through copies of their own, one after another: two of one
+    address would take each other's place."""
+    at = [t.data_ptr() for t in ts if t.numel()]
+    if len(set(at)) != len(at):
+        raise ValueError(f"{fn}: two of the tensors overlap")
+
+
 def _workspace(lib, count: int, dev: torch.device) -> torch.Tensor:
     return torch.empty(lib.tms_grad_workspace_size(count) // 8, dtype=torch.float64, device=dev)
 
@@ -95,14 +103,16 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, error_if_n
     """Scale all gradients by ``min(1, max_norm / (norm + 1e-6))``, their norm taken together.
 
     Args:
-        tensors: as for :func:`grad_norm`; changed in place, unless ``out`` is given.
+        tensors: as for :func:`grad_norm`; changed in place, unless ``out`` is given. No two that
+            share memory: a tied weight's gradient is listed once (ValueError otherwise).
         max_norm: the norm to clip to (at least 0).
         norm_type: 2.0 or ``inf``.
         error_if_nonfinite: wait for the norm, and raise RuntimeError on a NaN or infinite
             one, before anything is scaled. Without it such a norm goes into the factor
             (an infinite one gives 0, NaN stays NaN), and nothing waits.
         out: tensors of the same sizes, one for each of ``tensors``, that take the scaled
-            gradients (in their own dtype: bf16 gradients into an optimizer's fp32 ones).
+            gradients (in their own dtype: bf16 gradients into an optimizer's fp32 ones). None
+            may share memory with another one or with a gradient other than its own.
 
     Returns:
         The norm before clipping, a float32 scalar on the gradients' device.
@@ -138,14 +148,16 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, error_if_n
     ws = _workspace(lib, len(ts), dev)
     src = [t if t.is_contiguous() else t.contiguous() for t in ts]
     dst = src if to is ts else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in to]
+    copies = [(o, d) for o, d in zip(to, dst) if o is not d]  # strided tensors' own elements
+    if copies:
+        _apart(fn, to)  # contiguous ones the library looks over
     table = _table(src, dst)
     limit = ctypes.c_double(max_norm)
     status = _lib.launch(dev, lib.tms_grad_clip, table.buffer_info()[0], len(src), code, ctypes.addressof(limit),
                          ws.data_ptr(), 8 * ws.numel(), norm.data_ptr())
     if status:
         _lib.check(status)
-    for o, d in zip(to, dst):
-        if o is not d:
-            o.copy_(d)  # a strided tensor's own elements
+    for o, d in copies:
+        o.copy_(d)
     torch.autograd.graph.increment_version([o for o in to if not o.is_inference()])
     return norm
