@@ -3,6 +3,7 @@ any HIP call."""
 import ctypes
 
 import pytest
+import torch
 from test_training_host import F16, F32, Grad, call, numbers
 
 KB = 1 << 10
@@ -41,3 +42,24 @@ def test_overlapping_tensors_are_not_clipped(entries):
 def test_neighbours_and_shared_sources_are_taken(entries):
     rc, msg = clip(*entries)
     assert rc == 1 and "workspace" in msg
+
+
+def test_parameters_are_not_gradients():
+    """``clip_grad_norm_(model.parameters(), 1.0)`` would scale the parameters."""
+    import tilemaxsim_amd as tms
+    model = torch.nn.Linear(3, 2)
+    before = [p.detach().clone() for p in model.parameters()]
+    for given in (model.parameters(), list(model.parameters()), model.weight):
+        with pytest.raises(ValueError, match="their gradients"):
+            tms.clip_grad_norm_(given, 1.0)
+    g = [torch.ones(2, 3), torch.ones(2)]
+    with pytest.raises(ValueError, match="their gradients"):
+        tms.clip_grad_norm_(model.parameters(), 1.0, out=g)
+    with pytest.raises(ValueError, match="their gradients"):
+        tms.clip_grad_norm_(g, 1.0, out=list(model.parameters()))
+    assert all(torch.equal(p, b) for p, b in zip(model.parameters(), before))
+    # gradients that are a graph's (create_graph) are clipped, as any
+    x = torch.ones(3, requires_grad=True)
+    grad, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    with pytest.raises(ValueError, match="no CPU path"):
+        tms.clip_grad_norm_([grad], 1.0)
