@@ -63,3 +63,17 @@ def test_parameters_are_not_gradients():
     grad, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
     with pytest.raises(ValueError, match="no CPU path"):
         tms.clip_grad_norm_([grad], 1.0)
+
+
+def test_a_norm_without_a_graph_is_not_taken_for_one():
+    """A gradient penalty through ``grad_norm`` would train nothing."""
+    import tilemaxsim_amd as tms
+    x = torch.ones(3, requires_grad=True)
+    grad, = torch.autograd.grad((x ** 3).sum(), x, create_graph=True)
+    for t in (x, grad):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            tms.grad_norm([torch.ones(2), t])
+        with torch.no_grad(), pytest.raises(ValueError, match="no CPU path"):
+            tms.grad_norm([t])
+        with pytest.raises(ValueError, match="no CPU path"):
+            tms.grad_norm([t.detach()])

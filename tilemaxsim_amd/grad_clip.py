@@ -30,6 +30,11 @@ def _not_parameters(fn: str, ts: list) -> None:
         raise ValueError(f"{fn}: got parameters (leaves that require a gradient); pass their gradients, [p.grad for p in parameters]")
 
 
+def _no_graph(fn: str, ts: list) -> None:
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{fn}: the norm is not differentiable, and a tensor requires a gradient; detach the tensors, or call it under torch.no_grad()")
+
+
 def _list(fn: str, tensors, of_a_graph=None) -> tuple[list, list]:
     """The tensors, and their dtypes; where any requires a gradient, `of_a_graph` may refuse them."""
     ts = [tensors] if isinstance(tensors, torch.Tensor) else [t for t in tensors if t is not None]
@@ -91,11 +96,13 @@ def grad_norm(tensors, norm_type: float = 2.0) -> torch.Tensor:
 
     Args:
         tensors: gradients (float16, bfloat16 or float32, any mix, one device); None entries
-            are passed over, as parameters without a gradient leave them.
+            are passed over, as parameters without a gradient leave them. The norm has no
+            gradient of its own: with gradients enabled, tensors that require one are
+            refused (RuntimeError).
         norm_type: 2.0, or ``inf`` for the largest absolute value.
     """
     code = _norm_type("grad_norm", norm_type)
-    ts, kinds = _list("grad_norm", tensors)
+    ts, kinds = _list("grad_norm", tensors, _no_graph)
     _on_one_gpu("grad_norm", ts)
     ts = [t if t.is_contiguous() else t.contiguous() for t in ts]
     if not ts:
