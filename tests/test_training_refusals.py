@@ -77,3 +77,25 @@ def test_a_norm_without_a_graph_is_not_taken_for_one():
             tms.grad_norm([t])
         with pytest.raises(ValueError, match="no CPU path"):
             tms.grad_norm([t.detach()])
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be lost."""
+    import tilemaxsim_amd as tms
+    from torch.autograd import forward_ad
+    Q, D, H, W, t = torch.ones(2, 4, 32), torch.ones(3, 5, 32), torch.ones(3, 8), torch.ones(10, 8), torch.tensor([0, 1, 2])
+    with forward_ad.dual_level():
+        def dual(x):
+            return forward_ad.make_dual(x, torch.ones_like(x))
+        calls = [lambda: tms.maxsim_pairs(dual(Q), D), lambda: tms.maxsim_pairs(Q, dual(D)), lambda: tms.linear_cross_entropy(dual(H), W, t),
+                 lambda: tms.linear_cross_entropy(H, dual(W), t), lambda: tms.grad_norm([H, dual(W)]),
+                 lambda: tms.clip_grad_norm_([dual(H)], 1.0)]
+        for f in calls:
+            with pytest.raises(NotImplementedError, match="forward mode"):
+                f()
+        with pytest.raises(ValueError, match="no CPU path"):
+            tms.maxsim_pairs(Q, D)
+    # the same through torch.func, whose tensors are dual ones inside
+    for f, x in ((lambda q: tms.maxsim_pairs(q, D), Q), (lambda w: tms.linear_cross_entropy(H, w, t), W)):
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            torch.func.jvp(f, (x,), (torch.ones_like(x),))

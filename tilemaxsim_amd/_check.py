@@ -6,6 +6,7 @@ device check, so each error is raised the same way on a machine without a GPU.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -43,6 +44,14 @@ def same_device(**tensors: torch.Tensor) -> torch.device:
 def embedding_dtype(name: str, t: torch.Tensor) -> None:
     if t.dtype not in (torch.float16, torch.bfloat16, torch.float32):
         raise TypeError(f"{name} must be float16, bfloat16 or float32 (got {t.dtype})")
+
+
+def no_tangents(fn: str, tensors) -> None:
+    """Differentiable calls have a backward pass only: a dual tensor's tangent would be lost."""
+    if getattr(forward_ad, "_current_level", 0) < 0:  # torch's own count; none entered: no tensor has one
+        return
+    if any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{fn}: automatic differentiation in forward mode (a dual tensor was given)")
 
 
 def contiguous(name: str, t: torch.Tensor) -> None:

@@ -105,6 +105,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     _check.tensor("hidden", hidden)
     _check.tensor("weight", weight)
     _check.tensor("target", target)
+    _check.no_tangents(fn, (hidden, weight))
     if weight.dim() != 2 or hidden.dim() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError(f"{fn}: hidden must be (..., d) and weight (V, d), got {tuple(hidden.shape)} and {tuple(weight.shape)}")
     if target.shape != hidden.shape[:-1]:

@@ -42,6 +42,7 @@ def _list(fn: str, tensors, of_a_graph=None) -> tuple[list, list]:
     if not all(issubclass(k, torch.Tensor) for k in set(map(type, ts))):
         bad = next(t for t in ts if not isinstance(t, torch.Tensor))
         raise TypeError(f"{fn}: expected tensors, got {type(bad).__name__}")
+    _check.no_tangents(fn, ts)
     kinds = [t.dtype for t in ts]
     for kind in set(kinds):
         if kind not in _lib.DTYPE_CODES:

@@ -111,6 +111,7 @@ def maxsim_pairs(Qs: torch.Tensor, D: torch.Tensor, D_mask: torch.Tensor | None 
     """
     _check.tensor("Qs", Qs)
     _check.tensor("D", D)
+    _check.no_tangents("maxsim_pairs", (Qs, D))
     if Qs.dim() != 3 or D.dim() not in (3, 4):
         raise ValueError("maxsim_pairs: Qs must be (nQ, Nq, d), and D (B, Nd, d) or (nQ, nway, Nd, d), got "
                          f"{tuple(Qs.shape)} and {tuple(D.shape)}")
