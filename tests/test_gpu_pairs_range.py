@@ -1,4 +1,5 @@
-"""``maxsim_pairs`` at the ends of its range: the longest documents."""
+"""``maxsim_pairs`` at the ends of its range: the longest documents, queries with no documents of
+their own."""
 import math
 
 import numpy as np
@@ -55,3 +56,17 @@ def test_longest_documents(cuda, dtype, Nd):
     lim = (B + 2) * 2.0 ** -24 * aQ
     lim = lim + ROUND[dtype] * (dQ.abs() + lim) + TINY[dtype]
     assert bool(((gQ.view(nQ * Nq, d).double() - dQ).abs() <= lim).all())
+
+
+@gpu
+@pytest.mark.parametrize("nQ", [0, 3])
+def test_no_own_documents(cuda, nQ):
+    """Queries with none of their own documents: no scores, and backward gives zeros."""
+    import tilemaxsim_amd as tms
+    Q = torch.ones(nQ, 4, 64, device="cuda", dtype=torch.float16, requires_grad=True)
+    D = torch.ones(nQ, 0, 7, 64, device="cuda", dtype=torch.float16, requires_grad=True)
+    s = tms.maxsim_pairs(Q, D)
+    assert s.shape == (nQ, 0) and s.dtype == torch.float32
+    dQ, dD = torch.autograd.grad(s, (Q, D), torch.ones_like(s))
+    assert dQ.shape == Q.shape and bool((dQ == 0).all()) and dD.shape == D.shape
+    assert tms.maxsim_pairs(Q.detach(), D.detach()).shape == (nQ, 0)

@@ -24,13 +24,21 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _forward(Q, D, qmask, dmask, nway, keep):
+def _documents(Q, D):
+    """The documents of all queries and of each one's own (0: every query with every document),
+    as the library counts them; and the scores' columns."""
+    if D.dim() == 3:
+        return D.shape[0], 0, D.shape[0]
+    return Q.shape[0] * D.shape[1], D.shape[1], D.shape[1]
+
+
+def _forward(Q, D, qmask, dmask, keep):
     nQ, Nq, d = Q.shape
     Nd = D.shape[-2]
-    B = D.shape[0] if nway == 0 else nQ * nway
+    B, nway, columns = _documents(Q, D)
     lib = _lib.load()
     code = _lib.dtype_code(D.dtype)
-    scores = torch.empty(nQ, nway or B, dtype=torch.float32, device=D.device)
+    scores = torch.empty(nQ, columns, dtype=torch.float32, device=D.device)
     positions = None
     if keep:
         positions = torch.empty(lib.tms_pairs_positions(nQ, Nq, B, nway), dtype=torch.int16, device=D.device)
@@ -47,10 +55,9 @@ def _forward(Q, D, qmask, dmask, nway, keep):
 
 class _Pairs(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, Q, D, qmask, dmask, nway):
-        scores, positions = _forward(Q, D, qmask, dmask, nway, True)
+    def forward(ctx, Q, D, qmask, dmask):
+        scores, positions = _forward(Q, D, qmask, dmask, True)
         ctx.save_for_backward(Q, D, positions)
-        ctx.nway = nway
         return scores
 
     @staticmethod
@@ -58,9 +65,8 @@ class _Pairs(torch.autograd.Function):
     def backward(ctx, grad):
         Q, D, positions = ctx.saved_tensors
         nQ, Nq, d = Q.shape
-        nway = ctx.nway
         Nd = D.shape[-2]
-        B = D.shape[0] if nway == 0 else nQ * nway
+        B, nway, _ = _documents(Q, D)
         lib = _lib.load()
         grad = grad.contiguous()
         dQ = torch.empty_like(Q) if ctx.needs_input_grad[0] else None
@@ -72,7 +78,7 @@ class _Pairs(torch.autograd.Function):
                              _lib.ptr(dQ), _lib.ptr(dD))
         if status:
             _lib.check(status)
-        return dQ, dD, None, None, None
+        return dQ, dD, None, None
 
 
 def _mask(name: str, mask, shape):
@@ -134,10 +140,7 @@ def maxsim_pairs(Qs: torch.Tensor, D: torch.Tensor, D_mask: torch.Tensor | None 
     if dmask is not None:
         given["D_mask"] = dmask
     _check.same_device(**given)
-    nway = D.shape[1] if D.dim() == 4 else 0
-    if D.dim() == 4 and nway == 0:
-        return torch.empty(Qs.shape[0], 0, dtype=torch.float32, device=D.device)
     Qs, D = _aligned(Qs), _aligned(D)
     if torch.is_grad_enabled() and (Qs.requires_grad or D.requires_grad):
-        return _Pairs.apply(Qs, D, qmask, dmask, nway)
-    return _forward(Qs, D, qmask, dmask, nway, False)[0]
+        return _Pairs.apply(Qs, D, qmask, dmask)
+    return _forward(Qs, D, qmask, dmask, False)[0]
