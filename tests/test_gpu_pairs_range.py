@@ -1,5 +1,5 @@
-"""``maxsim_pairs`` at the ends of its range: the longest documents, queries with no documents of
-their own."""
+"""``maxsim_pairs`` at the ends of its range: the longest documents, the most documents, queries
+with no documents of their own."""
 import math
 
 import numpy as np
@@ -56,6 +56,33 @@ def test_longest_documents(cuda, dtype, Nd):
     lim = (B + 2) * 2.0 ** -24 * aQ
     lim = lim + ROUND[dtype] * (dQ.abs() + lim) + TINY[dtype]
     assert bool(((gQ.view(nQ * Nq, d).double() - dQ).abs() <= lim).all())
+
+
+@gpu
+def test_most_documents(cuda):
+    """More than 2^24 documents with a workgroup each: a launch's threads along one axis end at
+    2^32. One token a document, so the scores are dot products on the grid, exact in fp32."""
+    import tilemaxsim_amd as tms
+    B, d = (1 << 24) + 77, 32
+    rng = np.random.default_rng(2)
+    Q = _grid(rng, 1, 1, d).half().cuda().requires_grad_(True)
+    D = _grid(rng, 4096, d).half().cuda().repeat(-(-B // 4096), 1)[:B].view(B, 1, d).contiguous()
+    D[-1] = D[0] + D[1]  # the last one unlike the others
+    D.requires_grad_(True)
+    print(f"pairs of {B} documents", flush=True)
+    s = tms.maxsim_pairs(Q, D)
+    with torch.no_grad():
+        want = (D[:, 0].float() * Q[0, 0].float()).sum(1)  # (a matrix product of so many rows ends at the same 2^32)
+        G = torch.zeros(1, B, device="cuda")
+        G[0, ::1001] = 0.5
+        G[0, -3:] = -2.0
+    assert torch.equal(s[0].detach(), want)
+    gQ, gD = torch.autograd.grad(s, (Q, D), G)
+    assert torch.equal(gD[:, 0], (G[0, :, None] * Q[0, 0].float()).half())
+    terms = G[0, :, None].double() * D[:, 0].double()
+    ref, sums = terms.sum(0), terms.abs().sum(0)
+    lim = (B / 1001 + 600) * 2.0 ** -24 * sums
+    assert bool(((gQ[0, 0].double() - ref).abs() <= lim + ROUND["fp16"] * (ref.abs() + lim)).all())
 
 
 @gpu

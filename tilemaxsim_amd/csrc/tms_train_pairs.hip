@@ -36,6 +36,14 @@ __device__ __forceinline__ int64_t arg_at(const PairsArgs& a, int q, int64_t b) 
   return (a.nway ? b : b * a.nQ + q) * a.nqp;
 }
 
+// Workgroups beyond what one axis of a launch takes (2^32 threads) stand in further rows of it.
+constexpr int64_t kAxisGroups = 1 << 21;
+__device__ __forceinline__ int64_t workgroup() { return (int64_t)blockIdx.z * gridDim.x + blockIdx.x; }
+static dim3 grid_of(int64_t groups, unsigned y) {
+  const int64_t rows = (groups + kAxisGroups - 1) / kAxisGroups;
+  return dim3((unsigned)((groups + rows - 1) / rows), y, (unsigned)rows);
+}
+
 // Running maximum and its token over one 16-token tile: lane (c, g) sees query token c
 // against tokens base + 4 g + i. A strict comparison keeps the first of equal ones, as
 // tokens rise; the maximum keeps a NaN, which has to reach the loss. Three VALU instructions
@@ -118,7 +126,8 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
   __shared__ Best joined[4][32];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int r = lane & 15, g = lane >> 4;
-  const int64_t b = blockIdx.x;
+  const int64_t b = workgroup();
+  if (b >= a.B) return;
   const int q = a.nway ? (int)(b / a.nway) : (int)blockIdx.y;
   const int64_t drow = b * a.nd, qrow = (int64_t)q * a.nq;
   const int64_t width = (int64_t)a.d * 2;
@@ -573,7 +582,8 @@ __global__ __launch_bounds__(256) void pairs_grad_d_kernel(PairsGradArgs a) {
   float* weight = (float*)(count + 16 * 256);         // G of the run's blocks
   __shared__ int totals[4], cuts[5];
   const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-  const int64_t b = blockIdx.x;
+  const int64_t b = workgroup();
+  if (b >= a.B) return;
   const int col = (int)blockIdx.y * 128 + 2 * lane;
   const bool in = col < a.d;
   const uint32_t at_col = (uint32_t)((in ? col : 0) * (int)sizeof(T));
@@ -784,7 +794,9 @@ __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {
   constexpr int LD = 4;  // 16-byte loads a thread and stage: 64 KB
   extern __shared__ __attribute__((aligned(16))) uint8_t docs[];  // [2][tokens + 1][ROW]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int split = (int)(blockIdx.x % a.splits), group = (int)(blockIdx.x / a.splits);
+  const int64_t id = workgroup();
+  const int split = (int)(id % a.splits), group = (int)(id / a.splits);
+  if (group * 16 >= a.blocks) return;
   const int kb = group * 16 + wave;
   const bool mine = kb < a.blocks;
   const int q = mine ? kb / a.nbq : 0;
@@ -898,9 +910,11 @@ __global__ __launch_bounds__(512) void pairs_grad_q_few_kernel(PairsGradArgs a) 
   typedef typename El<DT>::T T;
   __shared__ float sums[8][8][128];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int split = (int)(blockIdx.x % a.splits), unit = (int)(blockIdx.x / a.splits);
+  const int64_t id = workgroup();
+  const int split = (int)(id % a.splits), unit = (int)(id / a.splits);
   const int groups = (a.nq + 7) / 8;
   const int q = unit / groups, i0 = (unit - q * groups) * 8;
+  if (q >= a.nQ) return;
   const int col = (int)blockIdx.y * 128 + 2 * lane;
   const int64_t first = a.nway ? (int64_t)q * a.nway : 0, n = a.nway ? a.nway : a.B;
   const int64_t e0 = (int64_t)split * a.chunk, e1 = e0 + a.chunk < n ? e0 + a.chunk : n;
@@ -1019,7 +1033,7 @@ static int check_pairs(const char* fn, int64_t nQ, int64_t nq, int64_t d, int64_
 
 template <int DT, int KS, int PL>
 static int run_direct(const PairsArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)a.B, a.nway ? 1u : (unsigned)a.nQ);
+  const dim3 grid = grid_of(a.B, a.nway ? 1u : (unsigned)a.nQ);
   hipLaunchKernelGGL((pairs_direct_kernel<DT, KS, PL>), grid, dim3(256), 0, st, a);
   return check_launch("pairs_direct_kernel");
 }
@@ -1115,7 +1129,7 @@ static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
     const int n = a.nway ? a.nbq : a.blocks;
     a.run = n < 1 ? 1 : n < kRun ? n : kRun;
     const size_t lds = (size_t)a.run * 32 * 6 + 16 * 256 * 2 + (size_t)a.run * 4;
-    const dim3 grid((unsigned)a.B, (unsigned)((a.d + 127) / 128));
+    const dim3 grid = grid_of(a.B, (unsigned)((a.d + 127) / 128));
     const bool pair = a.d % 2 == 0 && (int64_t)a.nQ * a.nq * a.d * (int64_t)sizeof(typename El<DT>::T) < ((int64_t)1 << 32) && (uintptr_t)a.Q % 8 == 0 && (uintptr_t)a.dD % 8 == 0;
     if (pair) hipLaunchKernelGGL((pairs_grad_d_kernel<DT, true>), grid, dim3(256), lds, st, a);
     else hipLaunchKernelGGL((pairs_grad_d_kernel<DT, false>), grid, dim3(256), lds, st, a);
@@ -1133,12 +1147,12 @@ static int run_grads(PairsGradArgs a, const GradQ& form, hipStream_t st) {
       a.tokens = stages > 0 ? (a.nd + stages - 1) / stages : 0;
       const size_t lds = 2 * (size_t)(a.tokens + 1) * 128 * es;
       const bool whole = a.d * es % 16 == 0 && (uintptr_t)a.D % 16 == 0;
-      const dim3 grid((unsigned)((a.blocks + 15) / 16 * a.splits), cols);
+      const dim3 grid = grid_of((int64_t)(a.blocks + 15) / 16 * a.splits, cols);
       if (whole) hipLaunchKernelGGL((pairs_grad_q_kernel<DT, true>), grid, dim3(1024), lds, st, a);
       else hipLaunchKernelGGL((pairs_grad_q_kernel<DT, false>), grid, dim3(1024), lds, st, a);
       if ((rc = check_launch("pairs_grad_q_kernel"))) return rc;
     } else {
-      hipLaunchKernelGGL(pairs_grad_q_few_kernel<DT>, dim3((unsigned)((int64_t)a.nQ * ((a.nq + 7) / 8) * a.splits), cols), dim3(512), 0, st, a);
+      hipLaunchKernelGGL(pairs_grad_q_few_kernel<DT>, grid_of((int64_t)a.nQ * ((a.nq + 7) / 8) * a.splits, cols), dim3(512), 0, st, a);
       if ((rc = check_launch("pairs_grad_q_few_kernel"))) return rc;
     }
     if (a.splits > 1) {
