@@ -120,18 +120,24 @@ struct GemmTile {
 
 // Tile numbers in the order of the launch: each XCD takes a run of its own (workgroups go to
 // the XCDs in turn), and a run goes over four m tiles for each n tile, so that the workgroups
-// that an XCD holds at a time share rows of both operands in its L2.
+// that an XCD holds at a time share rows of both operands in its L2. One axis of a launch takes
+// 2^32 threads: workgroups beyond kAxisTiles (a multiple of 8) stand in further rows of it.
+constexpr int kAxisTiles = 1 << 22;
 __device__ __forceinline__ bool gemm_tile_of(const GemmArgs& a, int& m, int& n) {
   const int total = a.tm * a.tn, each = (total + 7) / 8;
-  const int id = ((int)blockIdx.x % 8) * each + (int)blockIdx.x / 8;
-  if ((int)blockIdx.x / 8 >= each || id >= total) return false;
+  const int at = (int)blockIdx.z * kAxisTiles + (int)blockIdx.x;
+  const int id = (at % 8) * each + at / 8;
+  if (at / 8 >= each || id >= total) return false;
   const int wide = 4 * a.tn, first = id / wide * 4, in = id % wide;
   const int rows = a.tm - first < 4 ? a.tm - first : 4;
   m = first + in % rows;
   n = in / rows;
   return true;
 }
-static inline unsigned gemm_grid(int tm, int tn) { return (unsigned)(((int64_t)tm * tn + 7) / 8 * 8); }
+static inline dim3 gemm_grid(int tm, int tn, int splits) {
+  const int64_t n = ((int64_t)tm * tn + 7) / 8 * 8;
+  return dim3((unsigned)(n < kAxisTiles ? n : kAxisTiles), (unsigned)splits, (unsigned)((n + kAxisTiles - 1) / kAxisTiles));
+}
 
 template <bool V>
 struct More {
@@ -260,11 +266,12 @@ template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi>
 static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what) {
   a.tm = (a.M + 32 * MI - 1) / (32 * MI);
   a.tn = (a.N + 64 * NI - 1) / (64 * NI);
+  if ((int64_t)a.tm * a.tn > 1 << 30) return fail(TMS_ERR_UNSUPPORTED, "%s: %d x %d tiles are too many", what, a.tm, a.tn);
   const int steps = (a.K + 63) / 64;
   a.per = (steps + a.splits - 1) / a.splits;
   size_t lds = 2 * (size_t)(32 * MI + 64 * NI) * 128;
   if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
-  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi>), dim3(gemm_grid(a.tm, a.tn), (unsigned)a.splits), dim3(kGemmThreads),
+  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);
   return check_launch(what);
 }
