@@ -1,5 +1,5 @@
 """``maxsim_pairs`` at the ends of its range: the longest documents, the most documents, queries
-with no documents of their own."""
+with no documents of their own; and fp32 embeddings whose 24 bits all count."""
 import math
 
 import numpy as np
@@ -97,3 +97,85 @@ def test_no_own_documents(cuda, nQ):
     dQ, dD = torch.autograd.grad(s, (Q, D), torch.ones_like(s))
     assert dQ.shape == Q.shape and bool((dQ == 0).all()) and dD.shape == D.shape
     assert tms.maxsim_pairs(Q.detach(), D.detach()).shape == (nQ, 0)
+
+
+def _terms(x):
+    """A float32 as three bf16 terms, largest first, in float64."""
+    out, left = [], torch.from_numpy(x)
+    for _ in range(3):
+        t = left.bfloat16().float()
+        out.append(t.double().numpy())
+        left = left - t
+    return out
+
+
+def _hot(rng, rows, d, spread):
+    """Rows with one element that is not zero, of 24 random bits, at places in turn; and the places."""
+    at = (np.arange(rows) * 13 + spread) % d  # every place: 13 divides no d here
+    x = np.zeros((rows, d), dtype=np.float32)
+    x[np.arange(rows), at] = (1 + rng.random(rows)).astype(np.float32)
+    return x, at
+
+
+# A product of two such rows is the product of two numbers: six products of terms, in fp32. The
+# three that are left out are below 2^-24 of it together, and the six sums round 2^-24 each.
+PRODUCT = 2.0 ** -21
+
+
+def test_the_bound_sees_every_term():
+    """In float64: the six products of terms lie within the bound, any five that lack one with a
+    third term do not."""
+    rng = np.random.default_rng(0)
+    a, b = ((1 + rng.random(500)).astype(np.float32) for _ in range(2))
+    ta, tb = _terms(a), _terms(b)
+    exact = a.astype(np.float64) * b.astype(np.float64)
+    six = [(2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)]
+
+    def off(pairs):
+        return np.abs(sum(ta[i] * tb[j] for i, j in pairs) - exact) / exact
+    assert (off(six) < PRODUCT / 4).all()
+    for gone in six:
+        assert (off([p for p in six if p != gone]) > PRODUCT).mean() > 0.3, gone
+
+
+@gpu
+@pytest.mark.parametrize("nQ,Nq,B,Nd,d,own", [(2, 3, 3, 140, 32, False), (2, 5, 2, 200, 64, False), (1, 4, 5, 300, 96, True), (3, 2, 4, 400, 128, False),
+                                              (2, 3, 3, 260, 77, False), (2, 3, 2, 620, 200, False), (9, 5, 100, 200, 64, False),
+                                              (20, 3, 60, 400, 128, False), (40, 2, 50, 310, 77, False)])
+def test_all_bits_of_fp32(cuda, nQ, Nq, B, Nd, d, own):
+    """Scores and gradients of embeddings of 24 bits, in every form of the kernels."""
+    import tilemaxsim_amd as tms
+    rng = np.random.default_rng(nQ + B + d)
+    docs = nQ * B if own else B
+    q, qat = _hot(rng, nQ * Nq, d, 1)
+    x, xat = _hot(rng, docs * Nd, d, 0)
+    live = rng.random(docs * Nd) < 0.98
+    G = rng.standard_normal((nQ, B)).astype(np.float32)
+    scores = np.zeros((nQ, B))
+    dQ, dD = np.zeros(q.shape), np.zeros(x.shape)
+    q64, x64 = q.astype(np.float64), x.astype(np.float64)
+    for i in range(nQ):
+        for b in range(B):
+            rows = np.arange(Nd) + (i * B + b if own else b) * Nd
+            for k in range(i * Nq, (i + 1) * Nq):
+                sim = np.where(live[rows], np.where(xat[rows] == qat[k], x64[rows, qat[k]] * q64[k, qat[k]], 0.0), -np.inf)
+                best = rows[int(np.argmax(sim))]
+                second = np.partition(sim, -2)[-2]
+                assert sim.max() > 0 and second < sim.max() * (1 - 4 * PRODUCT)  # which one wins is not in doubt
+                scores[i, b] += sim.max()
+                dQ[k] += G[i, b].astype(np.float64) * x64[best]
+                dD[best] += G[i, b].astype(np.float64) * q64[k]
+    shape = (nQ, B, Nd) if own else (B, Nd)
+    print(f"pairs of 24 bits nQ={nQ} Nq={Nq} B={B} Nd={Nd} d={d} own={own}", flush=True)
+    Q, D = (torch.from_numpy(v).cuda().requires_grad_(True) for v in (q.reshape(nQ, Nq, d), x.reshape(*shape, d)))
+    mask = torch.from_numpy(live.reshape(shape)).cuda()
+    s = tms.maxsim_pairs(Q, D, mask)
+    assert torch.equal(s.detach(), tms.maxsim_pairs(Q.detach(), D.detach(), mask))
+    gQ, gD = torch.autograd.grad(s, (Q, D), torch.from_numpy(G).cuda())
+    far = np.abs(s.detach().cpu().double().numpy() - scores) / scores
+    assert far.max() <= PRODUCT + Nq * 2.0 ** -24, far.max()
+    n = np.abs(G).max()
+    for name, got, ref, terms in (("dQ", gQ, dQ, B), ("dD", gD, dD, nQ * Nq)):
+        lim = (terms + 4) * 2.0 ** -24 * terms * n * 2
+        got = got.cpu().double().numpy().reshape(ref.shape)
+        assert ((got != 0) <= (ref != 0)).all() and np.abs(got - ref).max() <= lim, name
