@@ -19,9 +19,11 @@
 //    lane l receives element l % 4 of lanes l / 4, 4 + l / 4, 8 + l / 4 and 12 + l / 4, so no
 //    transposed copy of anything is made.
 //
-// Tiles of 256 x 256 reach 1.33 to 1.37 PFLOP/s at 4096^3 to 8192^3 in bf16 (the library's product
-// 1.13 to 1.45), bound by the matrix cores at the clock that they hold and the operands' way
-// through LDS. Smaller ones are bound by that way: 10 TB/s into LDS over the chip.
+// Tiles of 256 x 256 with their epilogues, 8192^3 in bf16, random data: 1.30 PFLOP/s with k inside,
+// 1.22 outside in one operand, 1.20 in both (the library's products: 1.61, 1.41, 1.21); 4096^3, one
+// round of workgroups: 1.16, 1.01, 0.91. At 8192 x 131072 x 768 the matrix cores are busy for 40 to 54 %
+// of the cycles, at 1.9 to 2.2 GHz (power), and waves wait for operands for a third to a half of
+// theirs. Smaller tiles are bound by the operands' way: 10 TB/s into LDS over the chip.
 //
 // A 16 x 16 block of sums has lane (c, g) hold column n = c and rows m = 4 g + i: what is
 // reduced over m stays in a lane, and four neighbouring m are one store.
@@ -202,8 +204,9 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
   // The products of the fragments; `next`: the next step's loads, which go out once some of the
   // products are issued (behind the loads, a product would wait for all of the wave's LDS
   // reads together): a quarter of them, or an eighth with k outside in both operands (8192^3 in
-  // bf16, an eighth / a quarter: 1.13 / 1.15 PFLOP/s with k inside, 1.23 / 1.29 outside in one, 1.29 /
-  // 1.21 in both). The scheduler would otherwise move products behind the wait for the loads.
+  // bf16, an eighth / a quarter: 1.25 / 1.28 PFLOP/s with k inside, 1.21 / 1.19 outside in both; outside
+  // in one, 1.24 / 1.22 on one card and 1.23 / 1.29 on another). The scheduler would otherwise move
+  // products behind the wait for the loads.
   constexpr int kBefore = AO && BO ? MI / 4 : MI / 2;
   auto multiply = [&](auto&& next) {
     auto products = [&](int ks, int i0, int i1) {

@@ -16,8 +16,8 @@
 // sum of exp2 relative to it, and the others' share of that sum (all but the target's): with
 // rest = sum over v != t of exp(x[v] - x[t]), the loss is log(1 + rest) and P at the target
 // -rest / (1 + rest). Neither is a difference of two numbers of the logits' size, or of a
-// softmax near 1 and 1, so a row that is nearly right keeps its digits. (From one log-sum-exp
-// a row, a loss of 2e-3 at logits near 300 was 1e-2 of itself off, and P at the target as much.)
+// softmax near 1 and 1, so a row that is nearly right keeps its digits. (From one log-sum-exp a
+// row, a loss of 2e-11 came out as 1.3e-6, others below zero, and P at the target as far off.)
 //
 // Precision. Logits, maxima, sums, and the sums of both gradients are fp32. P is rounded to
 // the inputs' type, as the matrix cores take it (bf16: 2^-9 of each term; fp16: 2^-12, and P is
@@ -26,9 +26,10 @@
 // with a P of 32 bits (512 x 8000 x 256 in fp16, rows of W with ten times their spread in
 // common: 2.3e-4, 1.2e-3 without). dW has both roundings, P's and its own: where a word is the
 // target of one row, 1.4 times the error of the second alone (1024 x 16384 x 128, unit vectors:
-// 2.9e-4 against 2.2e-4 in fp16). fp32 inputs are three bf16 terms, and so is their P. P is times g[n] / u before it is rounded, for both gradients, and their
-// sums are times u: u is what a reduction gives every row alike (the ratio is 1), or a power
-// of two above the largest |g| of rows with their own.
+// 2.9e-4 against 2.2e-4 in fp16). fp32 inputs are three bf16 terms, and so is their P. P is times
+// g[n] / u before it is rounded, for both gradients, and their sums are times u: u is what a
+// reduction gives every row alike (the ratio is 1), or a power of two above the largest |g| of
+// rows with their own.
 #include <math.h>
 
 #include "tms_train_gemm.h"
@@ -46,8 +47,8 @@ struct RowStat {
 
 // The forward pass's statistics, from the sums in registers: a lane has four rows of the
 // vocabulary for each of its hidden rows, and a wave one RowStat a hidden row and tile. 8192 x
-// 131072 x 768 in bf16: 1.44 ms, 1.15 PFLOP/s, bound by the matrix cores and, with twelve steps
-// a tile, by the 6 us in 25 that a tile's first loads and its exponentials take.
+// 131072 x 768 in bf16: 1.38 to 1.46 ms, 1.19 to 1.13 PFLOP/s; the matrix cores are busy for 54 % of
+// it, at 1.9 GHz, and with twelve steps a tile its first loads and its exponentials take 6 us in 25.
 struct LseEpilogue {
   static constexpr int kRowBytes = 0;
   RowStat* parts;  // [block of the vocabulary][rows]
@@ -124,7 +125,8 @@ struct LseEpilogue {
 // P of one piece: [plane][row][ldp]; rows and columns that do not exist are zero. A lane holds
 // four neighbouring columns of a row, so a wave's rows pass through its LDS and leave as whole
 // lines (eight-byte stores left half-written lines: a quarter more time). 8192 x 65,536 of them
-// at d = 768 in bf16: 0.85 ms, 0.98 PFLOP/s, bound like the statistics' product; 1 GB leaves with it.
+// at d = 768 in bf16: 0.79 to 0.82 ms, 1.05 to 1.0 PFLOP/s, bound like the statistics' product (matrix
+// cores busy for 47 %); 1 GB leaves with it.
 template <int DT, int PL, int MIV>
 struct ProbEpilogue {
   static constexpr int kRowBytes = MIV * 32 + 16;  // 16 more: the rows of four lanes fall on other banks
@@ -208,8 +210,8 @@ struct ProbEpilogue {
 };
 
 // Sums of dH: [split][row][d], added to from the second piece on. A piece of 65,536 at 8192 rows
-// of 768 in bf16, five splits: 0.93 ms, 0.89 PFLOP/s, bound by the product (two rounds of 480 workgroups)
-// and 250 MB of sums read and written.
+// of 768 in bf16, five splits: 0.89 to 0.92 ms, 0.92 to 0.9 PFLOP/s: 480 workgroups are two rounds, the second
+// not full (matrix cores busy for 40 %), and 250 MB of sums are read and written.
 struct SumEpilogue {
   static constexpr int kRowBytes = 0;
   float* out;
@@ -254,7 +256,7 @@ __device__ __forceinline__ float from16(uint16_t x) {
 }
 
 // dW of one piece, finished: times *factor, in the inputs' type. 65,536 rows of 768 over 8192 in
-// bf16: 0.75 ms, 1.1 PFLOP/s (three whole rounds of workgroups; pieces half as large take one and a half).
+// bf16: 0.69 to 0.72 ms, 1.2 PFLOP/s (three whole rounds of workgroups; pieces half as large take one and a half).
 template <int OUT>
 struct WeightEpilogue {
   static constexpr int kRowBytes = 0;
@@ -493,7 +495,7 @@ __global__ __launch_bounds__(1024) void lce_rows_kernel(const float* top, const 
 // rounding to 16 bits took off its element at the target, times the target's row: that element is
 // as large as all others of its row together, and what the vocabulary's rows have in common
 // cancels between the two. Four elements of a row a thread (rows of sums and of w are whole
-// multiples of four), eight splits' loads at a time. 8192 x 768, five splits: 26 us, 5.3 TB/s.
+// multiples of four), eight splits' loads at a time. 8192 x 768, five splits: 31 us, 4.9 TB/s.
 template <int OUT>
 __global__ __launch_bounds__(256) void lce_hidden_kernel(const float* sums, int splits, int64_t split, int32_t rows, int32_t d, int32_t dp,
                                                          const float* factor, const uint16_t* w, const int32_t* hit, const float* at_hit,

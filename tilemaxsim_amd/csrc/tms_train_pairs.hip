@@ -234,8 +234,8 @@ __global__ __launch_bounds__(256) void pairs_direct_kernel(PairsArgs a) {
 // their maxima twelve VALU instructions of 4 cycles (POS: with positions), or two without; a
 // wave issues in order, so the maxima of one block are put between the MFMAs of the next.
 // 64 queries x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 315 us with positions (with
-// one block after the other 80 more), 250 without, bound by the SIMDs' issue of the two:
-// neither overlaps the other there. (32 x 32 products, which overlap half of it, take 365 and
+// one block after the other 80 more), 250 without, bound by the SIMDs' issue of the two, which
+// do not overlap there: products 38 % of the cycles, other VALU work 44 %. (32 x 32 products, which overlap half of it, take 365 and
 // 274: documents then end on 32 tokens, and the registers do not hold the next fragments.)
 template <int DT, int KS, int NB, int PL, bool POS>
 __global__ __launch_bounds__(512, 2) void pairs_shared_kernel(PairsArgs a) {
@@ -556,9 +556,10 @@ __device__ __forceinline__ f32x2 two(const uint8_t* p) {
 // document and 128 columns (two a lane). The sort is a counting sort in LDS, four bits of the
 // token at a time: a thread counts and places its own run of maxima, so equal tokens keep their
 // order. Then each wave takes a quarter of the sorted maxima, cut between tokens, with the
-// rows of the next eight in flight while eight are added: 20 cycles of VALU work a maximum.
-// 64 queries of 32 tokens x 4096 documents of 60 to 180 tokens, d = 128, 16 bits: 164 us, bound by
-// issue. (Products with a matrix of ones made from the positions cost a multiply-add for each
+// rows of the next eight in flight while eight are added. 64 queries of 32 tokens x 4096
+// documents of 60 to 180 tokens, d = 128, 16 bits: 158 us; 7.2 vector and 3.7 scalar instructions a
+// maximum with the sort's, the vector units busy for 63 % of it. The rest is waits of the sort
+// (LDS, half of its cycles conflicts, and barriers) and for rows. (Products with a matrix of ones made from the positions cost a multiply-add for each
 // column, token and query block as well: 560 us.)
 // More than kRun blocks are sorted in runs; the sums stand in memory between them, in fp32.
 constexpr int kRun = 128;  // blocks of 32 maxima: 32 KB of LDS
@@ -782,10 +783,12 @@ __device__ __forceinline__ void put_q(const PairsGradArgs& a, int split, int64_t
 // a lane) in registers, walk the same run of documents. A document's tokens come to LDS
 // once for the 512 query tokens, while the one before is added up: each query token reads the
 // row that answered it, 256 bytes in one wave's access. A lane finds its token's row, and the
-// wave takes the rows from the lanes one after another: four VALU instructions a token.
-// Where there is none, a row of zeros stands in. The runs' sums are joined by the kernel
-// below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, 16 bits: 155 us (with the
-// positions through the scalar unit 278), bound by issue; the join takes 10 us.
+// wave takes the rows from the lanes one after another: 6.1 vector and 4.7 scalar instructions a
+// maximum in all. Where there is none, a row of zeros stands in. The runs' sums are joined by
+// the kernel below, in order. 64 queries of 32 tokens x 4096 documents, d = 128, 16 bits: 155 us
+// (with the positions through the scalar unit 278): the vector units busy for 53 % of it, the waves, four
+// a SIMD, waiting for 48 % of theirs, at a barrier a document; padding is loaded too, a third of
+// the bytes. The join takes 11 us.
 // WHOLE: rows in pieces of 16 bytes, on their way in registers meanwhile; others element by element.
 template <int DT, bool WHOLE>
 __global__ __launch_bounds__(1024) void pairs_grad_q_kernel(PairsGradArgs a) {

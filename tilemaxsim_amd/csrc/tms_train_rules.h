@@ -14,8 +14,8 @@ inline int64_t gemm_side(int size) { return size == kGemm256 ? 256 : size == kGe
 // Microseconds of a product of m x n tiles over `steps` 64-steps of k, `splits` times: the
 // rounds of workgroups that the 256 CUs take, each as long as its steps and what surrounds
 // them. Measured in bf16 (4096 deep, a step of one, two and four workgroups a CU): 256 x 256
-// 1.58; 128 x 128 0.87, 1.05; 64 x 64 0.64, 0.68, 0.95. The large tile does 1.35 PFLOP/s once
-// it fills the chip; below that, the smaller ones do the same work on more CUs.
+// 1.58; 128 x 128 0.87, 1.05; 64 x 64 0.64, 0.68, 0.95. The large tile's steps alone make 1.36
+// PFLOP/s once they fill the chip; below that, the smaller ones do the same work on more CUs.
 inline double gemm_us(int size, int64_t m, int64_t n, int64_t steps, int64_t splits) {
   const int64_t side = gemm_side(size);
   const int64_t groups = up_to(m, side) / side * (up_to(n, side) / side) * splits, each = (steps + splits - 1) / splits;
@@ -28,7 +28,7 @@ inline double gemm_us(int size, int64_t m, int64_t n, int64_t steps, int64_t spl
 
 // Products of rows of three bf16 terms take six products a 64-step with seven tiles' loads:
 // as long as four steps. Their largest tile is 128 x 128: 256 x 256 has no registers for the
-// fragments that the next product shares (4096 x 32000 x 1024: 1.23 PFLOP/s against 1.31).
+// fragments that the next product shares (4096 x 32000 x 1024, k inside: 1.23 PFLOP/s against 1.32).
 inline int64_t gemm_steps(int64_t k, int planes) { return up_to(k, 64) / 64 * (planes == 3 ? 4 : 1); }
 inline int gemm_largest(int planes) { return planes == 3 ? kGemm128 : kGemm256; }
 
