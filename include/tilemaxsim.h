@@ -438,6 +438,42 @@ int tms_grad_clip(const tms_grad_tensor* tensors, int64_t count, int norm_type, 
                   void* workspace, int64_t workspace_bytes, float* norm, void* stream);
 
 /*
+ * Training and encoding: attention over packed texts. No reference counterpart. All of it is read
+ * from the HOST during the call. q is (tokens, heads, width), k and v (tokens, kv_heads, width), of
+ * one fp16, bf16 or fp32 dtype; width 32, 64, 96 or 128; heads a multiple of kv_heads (head h reads
+ * keys h / (heads / kv_heads)); 16-byte aligned, with strides (in elements) of whole 16 bytes. Text b
+ * is tokens offsets[b] .. offsets[b + 1] (device memory, texts + 1 of them, ascending, within
+ * [0, tokens]: what lies outside is taken as the nearest bound; if they descend, some rows' results are undefined,
+ * and no memory outside the tensors is touched). A token attends to its own text: to all of it, or, with
+ * `prefix` (device memory, one a text), to the text's first prefix[b] tokens and those up to itself.
+ * The score of two tokens is x = scale <q, k>; with cap > 0, cap tanh(x / cap); with `slopes`
+ * (device memory, one a head), less slope |i - j|.
+ * out (tokens, heads, width) contiguous; tokens of no text come out as zeros. For the backward pass
+ * low (out's shape and dtype; NULL in fp32) takes what out's rounding left, and lse (heads, tokens)
+ * the logarithms to base 2 of the rows' sums of exponentials; both may be NULL where there is none.
+ * The gradients: from grad (tokens, heads, width) contiguous, to dq (as out), dk and dv (tokens, kv_heads,
+ * width), contiguous, of the inputs' dtype; any of the three may be NULL. Sums are fp32 in one order.
+ * workspace: heads * tokens floats of device memory, 16-byte aligned.
+ */
+typedef struct tms_attention {
+  const void* q;
+  const void* k;
+  const void* v;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head;
+  const int64_t* offsets;
+  const int64_t* prefix;
+  const float* slopes;
+  int64_t texts, tokens, heads, kv_heads, width;
+  double scale, cap;
+  int64_t dtype;
+} tms_attention;
+int64_t tms_attention_workspace_size(int64_t tokens, int64_t heads);
+int tms_packed_attention(const tms_attention* attention, void* out, void* low, float* lse, void* stream);
+int tms_packed_attention_grad(const tms_attention* attention, const void* out, const void* low, const float* lse,
+                              const void* grad, void* workspace, int64_t workspace_bytes, void* dq, void* dk, void* dv,
+                              void* stream);
+
+/*
  * Measurement helper, not part of the scoring path and with no counterpart in the
  * reference: reads `bytes` (a multiple of 8 KiB) of `buf` once with a read-only
  * streaming kernel and writes one XOR word per thread to `sink`

@@ -54,6 +54,12 @@ def no_tangents(fn: str, tensors) -> None:
         raise NotImplementedError(f"{fn}: automatic differentiation in forward mode (a dual tensor was given)")
 
 
+def aligned(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous, and at an address the kernels' 16-byte loads take."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def contiguous(name: str, t: torch.Tensor) -> None:
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous (row-major); call .contiguous() first")

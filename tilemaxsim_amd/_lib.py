@@ -99,11 +99,16 @@ SIGNATURES = {
     "tms_grad_workspace_size": [_i64],
     "tms_grad_norm": [_c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tms_grad_clip": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "tms_attention_workspace_size": [_i64, _i64],
+    "tms_packed_attention": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
+    "tms_packed_attention_grad": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
+                                  _c_void_p, _c_void_p],
 }
 RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
             "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64,
-            "tms_lce_workspace_size": ctypes.c_int64, "tms_lce_stats": ctypes.c_int64}
+            "tms_lce_workspace_size": ctypes.c_int64, "tms_lce_stats": ctypes.c_int64,
+            "tms_attention_workspace_size": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()
