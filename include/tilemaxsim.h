@@ -474,6 +474,24 @@ int tms_packed_attention_grad(const tms_attention* attention, const void* out, c
                               void* stream);
 
 /*
+ * Training and encoding: the gated projection of a feed-forward block, h = act(x w_gate^T) * (x w_up^T).
+ * No reference counterpart. x (N, d), w_gate and w_up (F, d), h (N, F), of one fp16, bf16 or fp32
+ * dtype, contiguous, 16-byte aligned, any N, d and F. The gradients: from grad (N, F) to dx (N, d) and
+ * dw_gate, dw_up (F, d), of that dtype, any of which may be NULL; with N = 0 or F = 0 nothing is
+ * written. Sums are fp32 in one order. workspace: tms_gated_workspace_size bytes of device memory
+ * (backward = 0 or 1), 256-byte aligned; its contents need not stay between the two calls.
+ */
+#define TMS_ACT_SILU 0
+#define TMS_ACT_GELU 1
+#define TMS_ACT_GELU_TANH 2
+int64_t tms_gated_workspace_size(int64_t N, int64_t d, int64_t F, int dtype, int backward);
+int tms_gated_linear(const void* x, int64_t N, int64_t d, const void* w_gate, const void* w_up, int64_t F, int dtype,
+                     int activation, void* workspace, int64_t workspace_bytes, void* h, void* stream);
+int tms_gated_linear_grad(const void* x, int64_t N, int64_t d, const void* w_gate, const void* w_up, int64_t F, int dtype,
+                          int activation, const void* grad, void* workspace, int64_t workspace_bytes, void* dx,
+                          void* dw_gate, void* dw_up, void* stream);
+
+/*
  * Measurement helper, not part of the scoring path and with no counterpart in the
  * reference: reads `bytes` (a multiple of 8 KiB) of `buf` once with a read-only
  * streaming kernel and writes one XOR word per thread to `sink`

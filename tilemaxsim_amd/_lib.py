@@ -37,6 +37,9 @@ TMS_NORM_2 = 2
 TMS_REDUCE_NONE = 0
 TMS_REDUCE_SUM = 1
 TMS_REDUCE_MEAN = 2
+TMS_ACT_SILU = 0
+TMS_ACT_GELU = 1
+TMS_ACT_GELU_TANH = 2
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -103,12 +106,16 @@ SIGNATURES = {
     "tms_packed_attention": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "tms_packed_attention_grad": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
                                   _c_void_p, _c_void_p],
+    "tms_gated_workspace_size": [_i64, _i64, _i64, _int, _int],
+    "tms_gated_linear": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "tms_gated_linear_grad": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p, _c_void_p, _i64, _c_void_p,
+                              _c_void_p, _c_void_p, _c_void_p],
 }
 RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
             "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64,
             "tms_lce_workspace_size": ctypes.c_int64, "tms_lce_stats": ctypes.c_int64,
-            "tms_attention_workspace_size": ctypes.c_int64}
+            "tms_attention_workspace_size": ctypes.c_int64, "tms_gated_workspace_size": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

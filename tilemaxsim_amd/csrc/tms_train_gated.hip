@@ -1,0 +1,576 @@
+// The gated projection of a feed-forward block, both products and what joins them in one kernel:
+//
+//   g = x Wg^T,  u = x Wu^T,  h = act(g) u
+//   dg = dh u act'(g),  du = dh act(g)
+//   dx = dg Wg + du Wu,  dWg = dg^T x,  dWu = du^T x
+//
+// The forward pass is one matrix product whose tiles take 16 rows of Wg and 16 of Wu in turn, so
+// that a wave has g and u of the same places in its registers. The backward pass forms them
+// again (4 N F d operations, where keeping them would write and read 8 N F bytes in 16 bits: at d =
+// 768 as long), with an epilogue that leaves dg and du side by side, (N, 2 F), in 16 bits; two more
+// products take them to dx (k over both, and over Wg and Wu one behind the other) and to both
+// weights' gradients (their rows one behind the other).
+//
+// Few tokens (16 N at most) take a kernel of their own: bound by reading the weights once, which
+// needs every CU to have some of them on their way.
+//
+// Precision. g, u, the activation and all sums are fp32; dg and du are rounded to the inputs' type
+// between two products (fp32: three bf16 terms, six products of them), as a product of them
+// would take them. In fp16 they are held times a power of two that brings the largest |dh| to 1 to 2: gradients
+// as small as a mean over many tokens leaves them keep their digits.
+#include <math.h>
+
+#include "tms_train_terms.h"
+
+namespace tms {
+
+enum GatedAct { kSilu = TMS_ACT_SILU, kGelu = TMS_ACT_GELU, kGeluTanh = TMS_ACT_GELU_TANH };
+
+// act(g), and with DERIVATIVE its derivative. FINE: for fp32 results.
+//   silu: g s(g), s the logistic function;  gelu: g Phi(g), Phi the normal distribution's function;
+//   gelu_tanh: g s(2 sqrt(2 / pi) (g + 0.044715 g^3)), as (1 + tanh z) / 2 = s(2 z)
+template <bool FINE, bool DERIVATIVE>
+__device__ __forceinline__ float gated_act(int act, float g, float& slope) {
+  if (act == kGelu) {  // uniform
+    const float phi = 0.5f * erfcf(-0.7071067811865476f * g);
+    if constexpr (DERIVATIVE) slope = __builtin_fmaf(g, 0.3989422804014327f * expf(-0.5f * g * g), phi);
+    return g * phi;
+  }
+  constexpr float k0 = 1.5957691216057308f, k1 = 0.044715f * 1.5957691216057308f;
+  const float z = act == kSilu ? g : g * __builtin_fmaf(k1, g * g, k0);
+  float s;
+  if constexpr (FINE) s = 1.f / (1.f + expf(-z));
+  else s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
+  const float y = g * s;
+  if constexpr (DERIVATIVE) {
+    const float dz = act == kSilu ? 1.f : __builtin_fmaf(3.f * k1, g * g, k0);
+    // s + g s (1 - s) dz; where s is 0 or 1, the second term is 0, also if y dz has overflowed
+    slope = __builtin_fmaf(s == 0.f || s == 1.f ? 0.f : y * dz, 1.f - s, s);
+  }
+  return y;
+}
+
+// Eight (four) elements at an element's alignment: rows of an odd F begin anywhere.
+template <class T, int N, int ALIGN = sizeof(T)>
+struct __attribute__((packed, aligned(ALIGN))) GatedVec {
+  T v[N];
+};
+
+// h, from the sums of 16 rows of Wg and 16 of Wu in turn: whole lines of a token's row, through the wave's LDS.
+template <int OUT, int MIV>
+struct GatedEpilogue {
+  static constexpr int NP = MIV / 2;
+  static constexpr int kRowBytes = OUT == TMS_DTYPE_F32 ? 0 : NP * 32 + 16;
+  void* out;
+  int32_t rows, F, act;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t* lds) const {
+    static_assert(MI == MIV, "rows of the wave's LDS");
+    constexpr bool FINE = OUT == TMS_DTYPE_F32;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
+    float none;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      if constexpr (FINE) {
+        const int row = n + 16 * j + c;
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          const int f = f0 + 16 * p + 4 * g;
+          GatedVec<float, 4> y;
+#pragma unroll
+          for (int e = 0; e < 4; e++) y.v[e] = gated_act<FINE, false>(act, acc[2 * p][j][e], none) * acc[2 * p + 1][j][e];
+          float* to = (float*)out + (int64_t)row * F + f;
+          if (row >= rows) continue;
+          if (f + 4 <= F) *(GatedVec<float, 4>*)to = y;
+          else
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (f + e < F) to[e] = y.v[e];
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < NP; p++) {
+          uint16_t y[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) y[e] = to16<OUT>(gated_act<FINE, false>(act, acc[2 * p][j][e], none) * acc[2 * p + 1][j][e]);
+          *(u32x2*)(lds + c * kRowBytes + p * 32 + g * 8) = u32x2{(uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16};
+        }
+        wave_meets();
+        constexpr int PIECES = NP * 2, ROWS = 64 / PIECES;
+#pragma unroll
+        for (int k = 0; k < (16 + ROWS - 1) / ROWS; k++) {
+          const int rr = k * ROWS + lane / PIECES, f = f0 + lane % PIECES * 8, row = n + 16 * j + rr;
+          const u32x4 v = *(const u32x4*)(lds + (rr & 15) * kRowBytes + lane % PIECES * 16);
+          uint16_t* to = (uint16_t*)out + (int64_t)row * F + f;
+          if (rr < 16 && row < rows) {
+            if (f + 8 <= F) *(GatedVec<uint32_t, 4, 2>*)to = GatedVec<uint32_t, 4, 2>{{v[0], v[1], v[2], v[3]}};
+            else
+#pragma unroll
+              for (int e = 0; e < 8; e++)
+                if (f + e < F) to[e] = (uint16_t)(v[e / 2] >> (16 * (e & 1)));
+          }
+        }
+        wave_meets();
+      }
+    }
+  }
+};
+
+// dg and du, [plane][token][2 half]: dg in columns from 0, du from half on; zeros from F up to the next
+// multiple of 32 (what follows is not read, or not used).
+template <int DT, int PL, int MIV>
+struct GatedGradEpilogue {
+  static constexpr int NP = MIV / 2;
+  static constexpr int kRowBytes = NP * 32 + 16;
+  const void* grad;     // (rows, F), of the inputs' type
+  uint16_t* P;
+  const float* factor;  // fp16: what they are held times
+  int64_t plane;
+  int32_t rows, F, half, act;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t* lds) const {
+    static_assert(MI == MIV, "rows of the wave's LDS");
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
+    float held = 1.f;
+    if constexpr (DT == TMS_DTYPE_F16) held = *factor;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int row = n + 16 * j + c;
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
+        const int f = f0 + 16 * p + 4 * g;
+        float dh[4] = {0.f, 0.f, 0.f, 0.f};
+        if (row < rows) {
+          const int64_t at = (int64_t)row * F + f;
+          if constexpr (PL > 1) {
+            const float* from = (const float*)grad + at;
+            if (f + 4 <= F) {
+              const GatedVec<float, 4> v = *(const GatedVec<float, 4>*)from;
+#pragma unroll
+              for (int e = 0; e < 4; e++) dh[e] = v.v[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; e++) dh[e] = f + e < F ? from[e] : 0.f;
+            }
+          } else {
+            const uint16_t* from = (const uint16_t*)grad + at;
+            if (f + 4 <= F) {
+              const GatedVec<uint16_t, 4> v = *(const GatedVec<uint16_t, 4>*)from;
+#pragma unroll
+              for (int e = 0; e < 4; e++) dh[e] = from16<DT>(v.v[e]);
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; e++) dh[e] = f + e < F ? from16<DT>(from[e]) : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float slope;
+          const float y = gated_act<(PL > 1), true>(act, acc[2 * p][j][e], slope);
+          const float d = dh[e] * held;
+          const bool in = f + e < F;
+          acc[2 * p][j][e] = in ? d * acc[2 * p + 1][j][e] * slope : 0.f;
+          acc[2 * p + 1][j][e] = in ? d * y : 0.f;
+        }
+      }
+#pragma unroll
+      for (int which = 0; which < 2; which++)
+#pragma unroll
+        for (int t = 0; t < PL; t++) {
+#pragma unroll
+          for (int p = 0; p < NP; p++) {
+            uint16_t b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float x = acc[2 * p + which][j][e];
+              b[e] = to16<DT>(x);
+              if constexpr (PL > 1) acc[2 * p + which][j][e] = x - from16<DT>(b[e]);
+            }
+            *(u32x2*)(lds + c * kRowBytes + p * 32 + g * 8) = u32x2{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
+          }
+          wave_meets();
+          constexpr int PIECES = NP * 2, ROWS = 64 / PIECES;
+#pragma unroll
+          for (int k = 0; k < (16 + ROWS - 1) / ROWS; k++) {
+            const int rr = k * ROWS + lane / PIECES, f = f0 + lane % PIECES * 8, r = n + 16 * j + rr;
+            const u32x4 v = *(const u32x4*)(lds + (rr & 15) * kRowBytes + lane % PIECES * 16);
+            if (rr < 16 && r < rows && f < half) *(u32x4*)(P + t * plane + (int64_t)r * (2 * half) + which * half + f) = v;
+          }
+          wave_meets();
+        }
+    }
+  }
+};
+
+// Rows of a gradient, finished: times *factor (NULL: 1), in the inputs' type; row n from `half` on
+// is row n - half of the second output.
+template <int OUT>
+struct GatedRowsEpilogue {
+  static constexpr int kRowBytes = 0;
+  void *out, *out2;
+  const float* factor;
+  int32_t rows, half, d;  // rows: of each output
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t*) const {
+    typedef typename std::conditional<OUT == TMS_DTYPE_F32, float, uint16_t>::type T;
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    const float k = factor ? *factor : 1.f;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      int row = n + 16 * j + c;
+      T* to = (T*)out;
+      if (row >= half) to = (T*)out2, row -= half;
+      if (row >= rows || to == nullptr) continue;
+      to += (int64_t)row * d;
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+        const int col = m + 16 * i + 4 * g;
+        GatedVec<T, 4> v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if constexpr (OUT == TMS_DTYPE_F32) v.v[e] = acc[i][j][e] * k;
+          else v.v[e] = to16<OUT>(acc[i][j][e] * k);
+        }
+        if (col + 4 <= d) *(GatedVec<T, 4>*)(to + col) = v;
+        else
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (col + e < d) to[col + e] = v.v[e];
+      }
+    }
+  }
+};
+
+// The largest |dh| of fp16 (its bits are ordered like its value; NaN above all), a part a workgroup.
+__global__ __launch_bounds__(256) void gated_most_kernel(const uint16_t* x, int64_t n, uint32_t* parts) {
+  __shared__ uint32_t lds[4];
+  uint32_t most = 0;
+  const int64_t whole = n / 8;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < whole; k += (int64_t)gridDim.x * 256) {
+    const u32x4 v = *(const u32x4*)(x + k * 8);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const uint32_t lo = v[e] & 0x7fffu, hi = v[e] >> 16 & 0x7fffu;
+      most = lo > most ? lo : most;
+      most = hi > most ? hi : most;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x < n % 8) {
+    const uint32_t y = x[whole * 8 + threadIdx.x] & 0x7fffu;
+    most = y > most ? y : most;
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t y = __shfl_xor(most, o);
+    most = y > most ? y : most;
+  }
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < 4; w++) most = lds[w] > most ? lds[w] : most;
+    parts[blockIdx.x] = most;
+  }
+}
+// factor[0]: the power of two that brings it to 1 to 2 (1 for zeros, infinities and NaN); factor[1]: its reciprocal.
+__global__ __launch_bounds__(64) void gated_factor_kernel(const uint32_t* parts, int n, float* factor) {
+  uint32_t most = 0;
+  for (int i = threadIdx.x; i < n; i += 64) most = parts[i] > most ? parts[i] : most;
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    const uint32_t y = __shfl_xor(most, o);
+    most = y > most ? y : most;
+  }
+  if (threadIdx.x != 0) return;
+  int e = 0;
+  if (most != 0 && most < 0x7c00u) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, from16<TMS_DTYPE_F16>((uint16_t)most));
+    e = (int)(bits >> 23) - 127;
+  }
+  factor[0] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
+  factor[1] = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+}
+
+// ---------------------------------------------------------------- few tokens
+
+constexpr int kFewWaves = 8;
+constexpr int kFewTokens = 64;
+
+// Eight rows of Wg and eight of Wu are one operand's 16 rows; the waves share k, 32 in turn, and add
+// up through LDS. fp32 goes through the fp32 matrix instructions as it is.
+template <int DT, int NI>
+__global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x, int32_t N, int32_t d, const void* wg, const void* wu, int32_t F,
+                                                                   int32_t act, int32_t whole, void* out) {
+  typedef typename std::conditional<DT == TMS_DTYPE_F32, float, uint16_t>::type T;
+  __shared__ f32x4 parts[kFewWaves][NI][64];
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int f0 = (int)blockIdx.x * 8;
+  const int fr = f0 + (c & 7) < F ? f0 + (c & 7) : F - 1;
+  const T* w = (const T*)(c < 8 ? wg : wu) + (int64_t)fr * d;
+  const T* xs[NI];
+#pragma unroll
+  for (int j = 0; j < NI; j++) xs[j] = (const T*)x + (int64_t)(16 * j + c < N ? 16 * j + c : N - 1) * d;
+  f32x4 acc[NI];
+#pragma unroll
+  for (int j = 0; j < NI; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto eight = [&](const T* p, int k) {  // elements k .. k + 8 of a row, zeros behind its end
+    GatedVec<T, 8> v;
+    if (whole ? k < d : k + 8 <= d) {
+      v = *(const GatedVec<T, 8>*)(p + k);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) v.v[e] = k + e < d ? p[k + e] : (T)0;
+    }
+    return v;
+  };
+#pragma unroll 4
+  for (int k0 = wave * 32; k0 < d; k0 += kFewWaves * 32) {
+    const GatedVec<T, 8> a = eight(w, k0 + 8 * g);
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const GatedVec<T, 8> b = eight(xs[j], k0 + 8 * g);
+      if constexpr (DT == TMS_DTYPE_F32) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc[j], 0, 0, 0);
+      } else {
+        acc[j] = mfma16x16x32<DT>(__builtin_bit_cast(u32x4, a), __builtin_bit_cast(u32x4, b), acc[j]);
+      }
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NI; j++) parts[wave][j][lane] = acc[j];
+  __syncthreads();
+  // thread (c, g, j) with g < 2: token 16 j + c, columns f0 + 4 g ..; g from lanes 32 on has u's
+  for (int i = threadIdx.x; i < 32 * NI; i += kFewWaves * 64) {
+    const int j = i / 32, l = i % 32, row = 16 * j + (l & 15), f = f0 + 4 * (l >> 4);
+    f32x4 gate = {0.f, 0.f, 0.f, 0.f}, up = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < kFewWaves; v++) {
+      const f32x4 a = parts[v][j][l], b = parts[v][j][l + 32];
+#pragma unroll
+      for (int e = 0; e < 4; e++) gate[e] += a[e], up[e] += b[e];
+    }
+    if (row >= N) continue;
+    float none;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const float y = gated_act<(DT == TMS_DTYPE_F32), false>(act, gate[e], none) * up[e];
+      if (f + e < F) {
+        if constexpr (DT == TMS_DTYPE_F32) ((float*)out)[(int64_t)row * F + f + e] = y;
+        else ((uint16_t*)out)[(int64_t)row * F + f + e] = to16<DT>(y);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host
+
+struct GatedSpace {
+  int64_t x, wg, wu, p, parts, factor, bytes;
+};
+constexpr int kMostParts = 256;
+
+static bool gated_few(int64_t N, bool backward) { return !backward && N <= kFewTokens; }
+static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool backward) {
+  GatedSpace s = {};
+  Carve c;
+  if (gated_few(N, backward)) return s;
+  const int64_t dp = up_to(d, 8);
+  if (dtype == TMS_DTYPE_F32 || d % 8) {
+    s.x = c.take(N * dp * 2 * planes(dtype));
+    s.wg = c.take(F * dp * 2 * planes(dtype));
+    s.wu = c.take(F * dp * 2 * planes(dtype));
+  }
+  if (backward) {
+    s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype));
+    s.parts = c.take(kMostParts * 4);
+    s.factor = c.take(8);
+  }
+  s.bytes = c.at;
+  return s;
+}
+
+static int check_gated(const char* fn, const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, bool backward,
+                       const void* ws, int64_t bytes, GatedSpace& s) {
+  if (N < 0 || d < 0 || F < 0) return fail(TMS_ERR_INVALID, "%s: negative size", fn);
+  if (dtype != TMS_DTYPE_F16 && dtype != TMS_DTYPE_BF16 && dtype != TMS_DTYPE_F32)
+    return fail(TMS_ERR_UNSUPPORTED, "%s: dtype must be fp16, bf16 or fp32", fn);
+  if (act != TMS_ACT_SILU && act != TMS_ACT_GELU && act != TMS_ACT_GELU_TANH) return fail(TMS_ERR_INVALID, "%s: unknown activation %d", fn, act);
+  if (d == 0) return fail(TMS_ERR_INVALID, "%s: rows of no elements", fn);
+  if (d > 65536 || N > (1 << 24) || F > (1 << 24)) return fail(TMS_ERR_UNSUPPORTED, "%s: sizes up to d = 65536, N = F = 2^24", fn);
+  if (N == 0 || F == 0) return TMS_OK;
+  if (!x || !wg || !wu) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  const uintptr_t all = (uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu;
+  if (all % 16) return fail(TMS_ERR_INVALID, "%s: x and the weights must be 16-byte aligned", fn);
+  s = gated_space(N, d, F, dtype, backward);
+  if (s.bytes > 0 && (!ws || (uintptr_t)ws % 256 || bytes < s.bytes))
+    return fail(TMS_ERR_INVALID, "%s: a workspace of %lld bytes is needed, 256-byte aligned", fn, (long long)s.bytes);
+  return TMS_OK;
+}
+
+// The operands as the products take them.
+struct GatedOperands {
+  const uint16_t *x, *wg, *wu;
+};
+static int gated_operands(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, uint8_t* ws, const GatedSpace& s,
+                          GatedOperands& o, hipStream_t st) {
+  o = {(const uint16_t*)x, (const uint16_t*)wg, (const uint16_t*)wu};
+  if (dtype != TMS_DTYPE_F32 && d % 8 == 0) return TMS_OK;
+  const int64_t dp = up_to(d, 8);
+  o = {(const uint16_t*)(ws + s.x), (const uint16_t*)(ws + s.wg), (const uint16_t*)(ws + s.wu)};
+  int rc = run_terms(x, dtype, ws + s.x, N, d, dp, nullptr, st);
+  if (rc || (rc = run_terms(wg, dtype, ws + s.wg, F, d, dp, nullptr, st))) return rc;
+  return run_terms(wu, dtype, ws + s.wu, F, d, dp, nullptr, st);
+}
+
+// g and u: m over rows of Wg and Wu in turn, n over tokens.
+static GemmArgs gated_args(const GatedOperands& o, int64_t N, int64_t F, int64_t dp) {
+  GemmArgs a = {};
+  a.A = o.wg;
+  a.A2 = o.wu;
+  a.B = o.x;
+  a.aplane = F * dp;
+  a.bplane = N * dp;
+  a.lda = a.ldb = (int32_t)dp;
+  a.M = (int32_t)(2 * F);
+  a.N = (int32_t)N;
+  a.K = (int32_t)dp;
+  a.splits = 1;
+  return a;
+}
+
+template <int DT>
+static int gated_few_rows(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int act, void* h, hipStream_t st) {
+  const dim3 grid((unsigned)((F + 7) / 8)), threads(kFewWaves * 64);
+  const int whole = d % 8 == 0;
+  auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, threads, 0, st, x, (int32_t)N, (int32_t)d, wg, wu, (int32_t)F, (int32_t)act, whole, h); };
+  if (N <= 16) go(gated_few_kernel<DT, 1>);
+  else if (N <= 32) go(gated_few_kernel<DT, 2>);
+  else go(gated_few_kernel<DT, 4>);
+  return check_launch("gated_few_kernel");
+}
+
+template <int DT, int PL, int OUT>
+static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, uint8_t* ws, const GatedSpace& s,
+                         void* h, hipStream_t st) {
+  if (gated_few(N, false)) return gated_few_rows<OUT>(x, N, d, wg, wu, F, act, h, st);
+  GatedOperands o;
+  int rc = gated_operands(x, N, d, wg, wu, F, dtype, ws, s, o, st);
+  if (rc) return rc;
+  const int64_t dp = up_to(d, 8);
+  const GemmArgs a = gated_args(o, N, F, dp);
+  return with_size<PL>(gemm_size(2 * F, N, gemm_steps(dp, PL), gemm_largest(PL)), [&](auto z) {
+    using Z = decltype(z);
+    const GatedEpilogue<OUT, Z::MI> e = {h, (int32_t)N, (int32_t)F, (int32_t)act};
+    return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (gated)");
+  });
+}
+
+template <int DT, int PL, int OUT>
+static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, const void* grad, uint8_t* ws,
+                          const GatedSpace& s, void* dx, void* dwg, void* dwu, hipStream_t st) {
+  GatedOperands o;
+  int rc = gated_operands(x, N, d, wg, wu, F, dtype, ws, s, o, st);
+  if (rc) return rc;
+  const int64_t dp = up_to(d, 8), half = up_to(F, 64), plane = N * 2 * half;
+  uint16_t* P = (uint16_t*)(ws + s.p);
+  float* factor = nullptr;
+  if (DT == TMS_DTYPE_F16) {
+    factor = (float*)(ws + s.factor);
+    const int64_t groups = (N * F / 8 + 255) / 256;
+    const int parts = (int)(groups < 1 ? 1 : groups > kMostParts ? kMostParts : groups);
+    hipLaunchKernelGGL(gated_most_kernel, dim3(parts), dim3(256), 0, st, (const uint16_t*)grad, N * F, (uint32_t*)(ws + s.parts));
+    if ((rc = check_launch("gated_most_kernel"))) return rc;
+    hipLaunchKernelGGL(gated_factor_kernel, dim3(1), dim3(64), 0, st, (const uint32_t*)(ws + s.parts), parts, factor);
+    if ((rc = check_launch("gated_factor_kernel"))) return rc;
+  }
+  const float* back = factor ? factor + 1 : nullptr;
+  const GemmArgs a = gated_args(o, N, F, dp);
+  rc = with_size<PL>(gemm_size(2 * F, N, gemm_steps(dp, PL), gemm_largest(PL)), [&](auto z) {
+    using Z = decltype(z);
+    const GatedGradEpilogue<DT, PL, Z::MI> e = {grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
+    return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (dg, du)");
+  });
+  if (rc) return rc;
+  if (dx) {  // m over d, n over tokens, k over F columns of dg and du and the rows of Wg and Wu
+    GemmArgs b = {};
+    b.A = o.wg;
+    b.A2 = o.wu;
+    b.B = P;
+    b.aplane = F * dp;
+    b.bplane = plane;
+    b.lda = (int32_t)dp;
+    b.ldb = b.K = (int32_t)(2 * half);
+    b.M = (int32_t)dp;
+    b.N = (int32_t)N;
+    b.half = (int32_t)half;
+    b.real = (int32_t)F;
+    b.splits = 1;
+    const GatedRowsEpilogue<OUT> e = {dx, nullptr, back, (int32_t)N, 0x7fffffff, (int32_t)d};
+    rc = with_size<PL>(gemm_size(dp, N, gemm_steps(2 * half, PL), gemm_largest(PL)), [&](auto z) {
+      return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, false, kPairDepth>(b, e, st, "train_gemm_kernel (dx)");
+    });
+    if (rc) return rc;
+  }
+  if (dwg || dwu) {  // m over d, n over F columns of dg and du, k over tokens
+    GemmArgs b = {};
+    b.A = o.x;
+    b.B = P;
+    b.aplane = N * dp;
+    b.bplane = plane;
+    b.lda = (int32_t)dp;
+    b.ldb = b.N = (int32_t)(2 * half);
+    b.M = (int32_t)dp;
+    b.K = (int32_t)N;
+    b.splits = 1;
+    const GatedRowsEpilogue<OUT> e = {dwg, dwu, back, (int32_t)F, (int32_t)half, (int32_t)d};
+    rc = with_size<PL>(gemm_size(dp, 2 * half, gemm_steps(N, PL), gemm_largest(PL)), [&](auto z) {
+      return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, true>(b, e, st, "train_gemm_kernel (dWg, dWu)");
+    });
+  }
+  return rc;
+}
+
+}  // namespace tms
+
+using namespace tms;
+
+extern "C" int64_t tms_gated_workspace_size(int64_t N, int64_t d, int64_t F, int dtype, int backward) {
+  if (N <= 0 || d <= 0 || F <= 0) return 0;
+  return gated_space(N, d, F, dtype, backward != 0).bytes;
+}
+
+extern "C" int tms_gated_linear(const void* x, int64_t N, int64_t d, const void* w_gate, const void* w_up, int64_t F, int dtype, int activation,
+                                void* workspace, int64_t workspace_bytes, void* h, void* stream) {
+  const char* fn = "tms_gated_linear";
+  GatedSpace s = {};
+  const int rc = check_gated(fn, x, N, d, w_gate, w_up, F, dtype, activation, false, workspace, workspace_bytes, s);
+  if (rc || N == 0 || F == 0) return rc;
+  if (!h) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  if ((uintptr_t)h % 16) return fail(TMS_ERR_INVALID, "%s: h must be 16-byte aligned", fn);
+  const hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = (uint8_t*)workspace;
+  if (dtype == TMS_DTYPE_F16) return gated_forward<TMS_DTYPE_F16, 1, TMS_DTYPE_F16>(x, N, d, w_gate, w_up, F, dtype, activation, ws, s, h, st);
+  if (dtype == TMS_DTYPE_BF16) return gated_forward<TMS_DTYPE_BF16, 1, TMS_DTYPE_BF16>(x, N, d, w_gate, w_up, F, dtype, activation, ws, s, h, st);
+  return gated_forward<TMS_DTYPE_BF16, 3, TMS_DTYPE_F32>(x, N, d, w_gate, w_up, F, dtype, activation, ws, s, h, st);
+}
+
+extern "C" int tms_gated_linear_grad(const void* x, int64_t N, int64_t d, const void* w_gate, const void* w_up, int64_t F, int dtype, int activation,
+                                     const void* grad, void* workspace, int64_t workspace_bytes, void* dx, void* dw_gate, void* dw_up, void* stream) {
+  const char* fn = "tms_gated_linear_grad";
+  GatedSpace s = {};
+  const int rc = check_gated(fn, x, N, d, w_gate, w_up, F, dtype, activation, true, workspace, workspace_bytes, s);
+  if (rc || N == 0 || F == 0 || (!dx && !dw_gate && !dw_up)) return rc;  // no rows or columns: the caller's zeros
+  if (!grad) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
+  if (((uintptr_t)grad | (uintptr_t)dx | (uintptr_t)dw_gate | (uintptr_t)dw_up) % 16) return fail(TMS_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
+  const hipStream_t st = (hipStream_t)stream;
+  uint8_t* ws = (uint8_t*)workspace;
+  if (dtype == TMS_DTYPE_F16)
+    return gated_backward<TMS_DTYPE_F16, 1, TMS_DTYPE_F16>(x, N, d, w_gate, w_up, F, dtype, activation, grad, ws, s, dx, dw_gate, dw_up, st);
+  if (dtype == TMS_DTYPE_BF16)
+    return gated_backward<TMS_DTYPE_BF16, 1, TMS_DTYPE_BF16>(x, N, d, w_gate, w_up, F, dtype, activation, grad, ws, s, dx, dw_gate, dw_up, st);
+  return gated_backward<TMS_DTYPE_BF16, 3, TMS_DTYPE_F32>(x, N, d, w_gate, w_up, F, dtype, activation, grad, ws, s, dx, dw_gate, dw_up, st);
+}

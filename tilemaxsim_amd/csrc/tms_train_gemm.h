@@ -46,7 +46,13 @@ struct GemmArgs {
   int32_t M, N, K;         // k inside: K is a multiple of 8, or zeros follow it up to one; outside: M (N) is
   int32_t splits, per;     // splits of k, 64-steps each
   int32_t tm, tn;          // tiles
+  const uint16_t* A2;      // the second A of a pair (GemmPair)
+  int32_t half, real;      // kPairDepth: the k at which it begins, a multiple of 64; how many of them each A has
 };
+
+// Two matrices in the place of A: 16 rows of one and 16 of the other in turn (M counts both; the
+// epilogue has them as neighbouring blocks of one wave), or one behind the other along k.
+enum GemmPair { kSingle = 0, kPairRows = 1, kPairDepth = 2 };
 
 constexpr int kGemmThreads = 512;
 
@@ -65,6 +71,7 @@ struct GemmTile {
 
   // Units go to the waves in turn: wave w loads units w, w + 8, ...: k inside, rows 8 unit ..;
   // outside, k 8 (unit % 8) .. of columns 64 (unit / 8) ..
+  template <bool PAIR = false>
   __device__ __forceinline__ void init(int ld, int limit, int lane, int wave) {  // limit: rows (columns) that exist
     const int r = lane >> 3, slot = lane & 7;
     if constexpr (OUTER) {
@@ -79,7 +86,8 @@ struct GemmTile {
       kk = 8 * (slot ^ r);
 #pragma unroll
       for (int i = 0; i < L; i++) {
-        const int row = (i * 8 + wave) * 8 + r;
+        // of a pair, blocks of 16 rows in turn: a wave's units are all of one matrix
+        const int row = PAIR ? (2 * i + (wave >> 2)) * 16 + (wave & 1) * 8 + r : (i * 8 + wave) * 8 + r;
         off[i] = 2u * (uint32_t)((row < limit ? row : limit - 1) * ld + kk);
       }
     }
@@ -147,7 +155,7 @@ struct More {
 };
 
 // PL: planes of both operands, 1 or 3.
-template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi>
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi, int PAIR = kSingle>
 __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
   constexpr int BM = 32 * MI, BN = 64 * NI;
   constexpr int ASZ = BM * 128, BSZ = BN * 128;
@@ -160,21 +168,36 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
 
   GemmTile<BM, AO> ta;
   GemmTile<BN, BO> tb;
-  ta.init(a.lda, a.M - m0, lane, wave);
+  static_assert(PAIR != kPairRows || !AO, "rows in turn have k inside");
+  static_assert(PAIR != kPairDepth || (AO && !BO), "one behind the other along k: k outside, and inside of B");
+  ta.template init<PAIR == kPairRows>(a.lda, PAIR == kPairRows ? (a.M - m0) / 2 : a.M - m0, lane, wave);
   tb.init(a.ldb, a.N - n0, lane, wave);
   const int k0 = (int)blockIdx.y * a.per;
   const int steps_all = (a.K + 63) / 64;
   const int nk = k0 + a.per < steps_all ? a.per : steps_all - k0;
-  const uint16_t* A = a.A + (AO ? (int64_t)m0 : (int64_t)m0 * a.lda);
+  const uint16_t* A = (PAIR == kPairRows && (wave >> 1 & 1) ? a.A2 : a.A) + (AO ? (int64_t)m0 : (int64_t)(PAIR == kPairRows ? m0 / 2 : m0) * a.lda);
   const uint16_t* B = a.B + (BO ? (int64_t)n0 : (int64_t)n0 * a.ldb);
   uint8_t* const lds_a = gemm_mem;
   uint8_t* const lds_b = gemm_mem + 2 * ASZ;
   auto load_a = [&](int buf, int step, int plane) {
-    const int64_t k = (int64_t)(k0 + step) * 64;
+    int64_t k = (int64_t)(k0 + step) * 64;
+    if constexpr (PAIR == kPairDepth) {
+      const uint16_t* from = A;
+      if (k >= a.half) {
+        from = a.A2 + m0;
+        k -= a.half;
+      }
+      ta.load(from + plane * a.aplane + k * a.lda, a.real - (int)k, lds_a + buf * ASZ, wave);
+      return;
+    }
     ta.load(A + plane * a.aplane + (AO ? k * a.lda : k), a.K - (int)k, lds_a + buf * ASZ, wave);
   };
   auto load_b = [&](int buf, int step, int plane) {
     const int64_t k = (int64_t)(k0 + step) * 64;
+    if constexpr (PAIR == kPairDepth) {  // columns behind the last one that each A has a row for are not read
+      tb.load(B + plane * a.bplane + k, a.real - (int)(k >= a.half ? k - a.half : k), lds_b + buf * BSZ, wave);
+      return;
+    }
     tb.load(B + plane * a.bplane + (BO ? k * a.ldb : k), a.K - (int)k, lds_b + buf * BSZ, wave);
   };
   auto meet = [&]() {  // this wave's loads are in LDS, then everyone's
@@ -265,7 +288,7 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
   epi(acc, m0 + wm * MI * 16, n0 + wn * NI * 16, (int)blockIdx.y, gemm_mem + wave * (NI * 16 * Epi::kRowBytes));
 }
 
-template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi>
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, int PAIR = kSingle, class Epi>
 static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what) {
   a.tm = (a.M + 32 * MI - 1) / (32 * MI);
   a.tn = (a.N + 64 * NI - 1) / (64 * NI);
@@ -274,7 +297,7 @@ static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what
   a.per = (steps + a.splits - 1) / a.splits;
   size_t lds = 2 * (size_t)(32 * MI + 64 * NI) * 128;
   if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
-  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
+  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi, PAIR>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);
   return check_launch(what);
 }
