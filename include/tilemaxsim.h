@@ -492,6 +492,53 @@ int tms_gated_linear_grad(const void* x, int64_t N, int64_t d, const void* w_gat
                           void* dw_gate, void* dw_up, void* stream);
 
 /*
+ * Training: an AdamW step over `count` tensors. No reference counterpart. `tensors` and `state` are HOST
+ * memory, read during the call. With g' = g * min(1, max_norm / (norm + 1e-6)) (norm: one float of device
+ * memory, as tms_grad_norm leaves it; NULL: g' = g), t the tensor's step and lr (or *lr_at, a float of
+ * device memory, where that is not NULL):
+ *   m = beta1 m + (1 - beta1) g',  v = beta2 v + (1 - beta2) g'^2,
+ *   p = p (1 - lr decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps)
+ * p, g and copy (NULL, or what takes the new p) are fp16, bf16 or fp32, of n elements, at any alignment to the
+ * element; no two that are written may overlap, nor one of them a gradient. steps[index] (device memory) counts
+ * a tensor's steps: the call adds one and uses it. Its states are n elements from `at` on, a multiple of
+ * TMS_ADAMW_BLOCK, of m and v (`size` elements); tensors come in the order of their places and counters.
+ * bits = 32: m and v are floats. bits = 8: bytes, with m_exp and v_exp the exponents of blocks of
+ * TMS_ADAMW_BLOCK (size / TMS_ADAMW_BLOCK of them). A code c of v stands for the fp32 number with the bits
+ * (c + 8 (v_exp - 30)) << 20, one of m (its magnitude, the low seven bits; the high one is the sign) for
+ * (c + 8 (m_exp - 14)) << 20; 0 for zero, the largest magnitude for NaN. What is cut off goes by a hash of the
+ * step and the place, so that codes are right in the mean, and the same in every run.
+ * m, v and factors (device memory, 16 bytes a counter, the call's own) are 16-byte aligned.
+ * tms_adamw_moments writes the `size` numbers that 8-bit states stand for.
+ */
+#define TMS_ADAMW_BLOCK 128
+typedef struct tms_adamw_tensor {
+  void* p;
+  const void* g;
+  void* copy;
+  int64_t n;
+  int64_t at;
+  int32_t index;
+  int32_t p_dtype;
+  int32_t g_dtype;
+  int32_t copy_dtype;
+} tms_adamw_tensor;
+typedef struct tms_adamw {
+  void* m;
+  void* v;
+  uint8_t* m_exp;
+  uint8_t* v_exp;
+  int64_t* steps;
+  void* factors;
+  const float* norm;
+  const float* lr_at;
+  int64_t size, counters, bits;
+  double lr, beta1, beta2, eps, decay, max_norm;
+} tms_adamw;
+int tms_adamw_step(const tms_adamw_tensor* tensors, int64_t count, const tms_adamw* state, void* stream);
+int tms_adamw_moments(const uint8_t* m, const uint8_t* m_exp, const uint8_t* v, const uint8_t* v_exp, int64_t size,
+                      float* mean, float* square, void* stream);
+
+/*
  * Measurement helper, not part of the scoring path and with no counterpart in the
  * reference: reads `bytes` (a multiple of 8 KiB) of `buf` once with a read-only
  * streaming kernel and writes one XOR word per thread to `sink`

@@ -40,6 +40,7 @@ TMS_REDUCE_MEAN = 2
 TMS_ACT_SILU = 0
 TMS_ACT_GELU = 1
 TMS_ACT_GELU_TANH = 2
+TMS_ADAMW_BLOCK = 128  # elements of 8-bit states that share an exponent
 
 _c_void_p = ctypes.c_void_p
 _i64 = ctypes.c_int64
@@ -110,6 +111,8 @@ SIGNATURES = {
     "tms_gated_linear": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tms_gated_linear_grad": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _int, _int, _c_void_p, _c_void_p, _i64, _c_void_p,
                               _c_void_p, _c_void_p, _c_void_p],
+    "tms_adamw_step": [_c_void_p, _i64, _c_void_p, _c_void_p],
+    "tms_adamw_moments": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _c_void_p],
 }
 RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": ctypes.c_int64,
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
