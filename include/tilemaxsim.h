@@ -449,11 +449,13 @@ int tms_grad_clip(const tms_grad_tensor* tensors, int64_t count, int norm_type, 
  * The score of two tokens is x = scale <q, k>; with cap > 0, cap tanh(x / cap); with `slopes`
  * (device memory, one a head), less slope |i - j|.
  * out (tokens, heads, width) contiguous; tokens of no text come out as zeros. For the backward pass
- * low (out's shape and dtype; NULL in fp32) takes what out's rounding left, and lse (heads, tokens)
- * the logarithms to base 2 of the rows' sums of exponentials; both may be NULL where there is none.
+ * low (out's shape and dtype; NULL in fp32) takes what out's rounding left, and stats
+ * (tms_attention_stats floats) the logarithms to base 2 of the rows' sums of exponentials, by head and token,
+ * and the norms that say how far a bias lets tokens see. Both may be NULL where there is no backward pass;
+ * with stats, long texts under a bias are taken only as far as their P are not 0 in fp32.
  * The gradients: from grad (tokens, heads, width) contiguous, to dq (as out), dk and dv (tokens, kv_heads,
  * width), contiguous, of the inputs' dtype; any of the three may be NULL. Sums are fp32 in one order.
- * workspace: heads * tokens floats of device memory, 16-byte aligned.
+ * workspace: tms_attention_workspace_size bytes of device memory, 256-byte aligned. Tensors are 16-byte aligned.
  */
 typedef struct tms_attention {
   const void* q;
@@ -467,9 +469,10 @@ typedef struct tms_attention {
   double scale, cap;
   int64_t dtype;
 } tms_attention;
-int64_t tms_attention_workspace_size(int64_t tokens, int64_t heads);
-int tms_packed_attention(const tms_attention* attention, void* out, void* low, float* lse, void* stream);
-int tms_packed_attention_grad(const tms_attention* attention, const void* out, const void* low, const float* lse,
+int64_t tms_attention_stats(int64_t tokens, int64_t heads, int64_t kv_heads);
+int64_t tms_attention_workspace_size(int64_t texts, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t width);
+int tms_packed_attention(const tms_attention* attention, void* out, void* low, float* stats, void* stream);
+int tms_packed_attention_grad(const tms_attention* attention, const void* out, const void* low, const float* stats,
                               const void* grad, void* workspace, int64_t workspace_bytes, void* dq, void* dk, void* dv,
                               void* stream);
 

@@ -286,6 +286,54 @@ def test_long_text(cuda):
         check(*qkv, offsets, G, f"long {dt}", prefix=0)
 
 
+@pytest.mark.parametrize("D,dt", [(32, torch.bfloat16), (64, torch.bfloat16), (64, torch.float16), (96, torch.float16), (128, torch.bfloat16)],
+                         ids=str)
+@pytest.mark.parametrize("kind", ["plain", "prefix", "bias", "cap"])
+def test_tiles_of_128(cuda, kind, D, dt):
+    """Texts and heads enough for a wave to take 32 rows; a steep bias lets tokens see a part of their text only."""
+    H = 24
+    qkv, offsets, G = make([2901, 60, 37], H, H, D, dt, seed=9, behind=2)
+    how = {}
+    if kind in ("prefix", "cap"):
+        how["prefix"] = torch.tensor([700, 0, 37])
+    if kind == "bias":
+        how["slopes"] = torch.exp2(3 - torch.arange(H, device="cuda") / 2.0)
+        qkv, offsets, G = make([2901, 160], H, H, D, dt, seed=9, behind=2)
+    if kind == "cap":
+        how["cap"] = 6.0
+    check(*qkv, offsets, G, f"wide {kind} {D} {dt}", **how)
+
+
+@pytest.mark.parametrize("slope", [0.0, -0.01, 1.0, math.inf])
+def test_reach(cuda, slope):
+    """A bias of any slope over a long text; norms that are not finite leave nothing out. An infinite
+    slope makes a token's own distance a NaN, as 0 times infinity is."""
+    import tilemaxsim_amd as tms
+    (q, k, v), offsets, G = make([1500], 2, 1, 64, torch.bfloat16, seed=2, behind=3)
+    slopes = torch.tensor([slope, 0.3], device="cuda")
+    if math.isinf(slope):
+        out = tms.packed_attention(q, k, v, offsets, slopes=slopes)
+        assert bool(torch.isnan(out[:1500, 0]).all())
+        return
+    check(q, k, v, offsets, G, f"slope {slope}", slopes=slopes)
+    want = tms.packed_attention(q, k, v, offsets, slopes=slopes)
+    with torch.no_grad():
+        k2 = k.clone()
+        k2[1501:] = math.nan  # in rows of no text
+        want, off = reference(q, k, v, offsets, G, slopes=slopes)
+        close([tms.packed_attention(q, k2, v, offsets, slopes=slopes)], want, off, "NaN norms")
+
+
+@pytest.mark.parametrize("H,KV", [(12, 1), (10, 2), (7, 1)])
+@pytest.mark.parametrize("dt", DT, ids=str)
+def test_heads_shared_by_workgroups(cuda, H, KV, dt):
+    """Few tiles of keys with many heads each: their sums come in parts."""
+    qkv, offsets, G = make([130, 600, 1], H, KV, 32, dt, seed=H)
+    check(*qkv, offsets, G, f"parts {H} {KV} {dt}", prefix=0)
+    qkv, offsets, G = make([64] * 90, H, KV, 32, dt, seed=H)
+    check(*qkv, offsets, G, f"fewer parts {H} {KV} {dt}", slopes=torch.linspace(0, 1, H, device="cuda"))
+
+
 def test_streams_and_graphs(cuda):
     """Another stream than the tensors' own; a captured forward and backward pass follows its inputs, replay by replay."""
     import tilemaxsim_amd as tms

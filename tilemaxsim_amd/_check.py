@@ -56,7 +56,8 @@ def no_tangents(fn: str, tensors) -> None:
 
 def aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous, and at an address the kernels' 16-byte loads take."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 

@@ -103,7 +103,8 @@ SIGNATURES = {
     "tms_grad_workspace_size": [_i64],
     "tms_grad_norm": [_c_void_p, _i64, _int, _c_void_p, _i64, _c_void_p, _c_void_p],
     "tms_grad_clip": [_c_void_p, _i64, _int, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
-    "tms_attention_workspace_size": [_i64, _i64],
+    "tms_attention_stats": [_i64, _i64, _i64],
+    "tms_attention_workspace_size": [_i64, _i64, _i64, _i64, _i64],
     "tms_packed_attention": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p],
     "tms_packed_attention_grad": [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p,
                                   _c_void_p, _c_void_p],
@@ -118,7 +119,8 @@ RESTYPES = {"tms_topk_workspace_size": ctypes.c_int64, "tms_set_rerank_limit": c
             "tms_pairs_workspace_size": ctypes.c_int64, "tms_pairs_positions": ctypes.c_int64,
             "tms_pairs_grad_workspace_size": ctypes.c_int64, "tms_grad_workspace_size": ctypes.c_int64,
             "tms_lce_workspace_size": ctypes.c_int64, "tms_lce_stats": ctypes.c_int64,
-            "tms_attention_workspace_size": ctypes.c_int64, "tms_gated_workspace_size": ctypes.c_int64}
+            "tms_attention_workspace_size": ctypes.c_int64, "tms_attention_stats": ctypes.c_int64,
+             "tms_gated_workspace_size": ctypes.c_int64}
 
 _lib = None
 _lock = threading.Lock()

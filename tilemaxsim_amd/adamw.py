@@ -6,8 +6,8 @@ reference does not train).
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 from array import array
 
 import torch
@@ -17,11 +17,7 @@ from . import _check, _lib
 BLOCK = _lib.TMS_ADAMW_BLOCK
 
 
-class _State(ctypes.Structure):
-    """tms_adamw"""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("m", "v", "m_exp", "v_exp", "steps", "factors", "norm", "lr_at")]
-                + [(n, ctypes.c_int64) for n in ("size", "counters", "bits")]
-                + [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "decay", "max_norm")])
+_pack = struct.Struct("@8P3q6d").pack  # tms_adamw
 
 
 class AdamWState:
@@ -104,10 +100,6 @@ class AdamWState:
         return [flat[a:a + n].view(s) for a, n, s in zip(self.places, self.sizes, self.shapes)]
 
 
-def _words(ints: list) -> array:
-    return array("q", ints)
-
-
 def _scalar(fn: str, name: str, t: torch.Tensor, dev: torch.device) -> torch.Tensor:
     if t.numel() != 1 or t.dtype != torch.float32:
         raise ValueError(f"{fn}: {name} must be one float32 number, got {tuple(t.shape)} {t.dtype}")
@@ -121,18 +113,18 @@ def _kinds(fn: str, name: str, ts: list, dev: torch.device) -> list:
     if not all(issubclass(k, torch.Tensor) for k in set(map(type, ts))):
         bad = next(t for t in ts if not isinstance(t, torch.Tensor))
         raise TypeError(f"{fn}: {name} must be tensors, got {type(bad).__name__}")
-    kinds = [t.dtype for t in ts]
-    for kind in set(kinds):
-        if kind not in _lib.DTYPE_CODES:
-            raise TypeError(f"{fn}: {name} must be float16, bfloat16 or float32 (got {kind})")
+    try:
+        kinds = [_lib.DTYPE_CODES[t.dtype] for t in ts]
+    except KeyError as e:
+        raise TypeError(f"{fn}: {name} must be float16, bfloat16 or float32 (got {e.args[0]})") from None
     if {t.get_device() for t in ts} - {dev.index}:
         bad = next(t for t in ts if t.device != dev)
         raise ValueError(f"{fn}: {name} must be on {dev}, where the states are (got {bad.device})")
-    return [_lib.DTYPE_CODES[k] for k in kinds]
+    return kinds
 
 
 def _shapes_match(fn: str, name: str, ts: list, shapes: list) -> None:
-    if [tuple(t.shape) for t in ts] != shapes:
+    if [t.shape for t in ts] != shapes:  # torch.Size is a tuple
         i = next(i for i, (t, s) in enumerate(zip(ts, shapes)) if tuple(t.shape) != s)
         raise ValueError(f"{fn}: {name}[{i}] is {tuple(ts[i].shape)}, the states are for {shapes[i]}")
 
@@ -194,9 +186,11 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
     _check.no_tangents(fn, [*ps, *gs])
     _shapes_match(fn, "parameters", ps, shapes)
     _shapes_match(fn, "gradients", gs, shapes)
-    given = [] if cs is None else [(i, c) for i, c in enumerate(cs) if c is not None]
-    c_kinds = _kinds(fn, "copies", [c for _, c in given], dev)
-    _shapes_match(fn, "copies", [c for _, c in given], [shapes[i] for i, _ in given])
+    given, c_kinds = [], []
+    if cs is not None:
+        given = [(i, c) for i, c in enumerate(cs) if c is not None]
+        c_kinds = _kinds(fn, "copies", [c for _, c in given], dev)
+        _shapes_match(fn, "copies", [c for _, c in given], [shapes[i] for i, _ in given])
     if not ps:
         return
     if isinstance(lr, torch.Tensor):
@@ -216,21 +210,21 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
     g_from = whole(gs)
     n = len(ps)
     words = array("q", bytes(56 * n))  # tms_adamw_tensor entries
-    words[0::7] = _words([t.data_ptr() for t in p_to])
-    words[1::7] = _words([t.data_ptr() for t in g_from])
-    words[3::7] = _words(sizes)
-    words[4::7] = _words(places)
-    words[5::7] = _words([i | k << 32 for i, k in zip(indexes, p_kinds)])
-    words[6::7] = _words(g_kinds)
+    words[0::7] = array("q", [t.data_ptr() for t in p_to])
+    words[1::7] = array("q", [t.data_ptr() for t in g_from])
+    words[3::7] = array("q", sizes)
+    words[4::7] = array("q", places)
+    words[5::7] = array("q", [i | k << 32 for i, k in zip(indexes, p_kinds)])
+    words[6::7] = array("q", g_kinds)
     for (i, _), c, k in zip(given, c_to, c_kinds):
         words[7 * i + 2] = c.data_ptr()
         words[7 * i + 6] |= k << 32
     factors = torch.empty(4 * len(state.shapes), dtype=torch.float32, device=dev)
     host_lr = 0.0 if isinstance(lr, torch.Tensor) else lr
-    s = _State(state.m.data_ptr(), state.v.data_ptr(), _lib.ptr(state.m_exp), _lib.ptr(state.v_exp), state.steps.data_ptr(),
-               factors.data_ptr(), _lib.ptr(norm), lr.data_ptr() if isinstance(lr, torch.Tensor) else None, state.size, len(state.shapes),
-               state.bits, host_lr, beta1, beta2, eps, weight_decay, max_norm or 0.0)
-    status = _lib.launch(dev, _lib.load().tms_adamw_step, words.buffer_info()[0], n, ctypes.addressof(s))
+    described = _pack(state.m.data_ptr(), state.v.data_ptr(), _lib.ptr(state.m_exp) or 0, _lib.ptr(state.v_exp) or 0,
+                      state.steps.data_ptr(), factors.data_ptr(), _lib.ptr(norm) or 0, lr.data_ptr() if isinstance(lr, torch.Tensor) else 0,
+                      state.size, len(state.shapes), state.bits, host_lr, beta1, beta2, eps, weight_decay, max_norm or 0.0)
+    status = _lib.launch(dev, _lib.load().tms_adamw_step, words.buffer_info()[0], n, described)
     if status:
         _lib.check(status)
     for t, d in back:

@@ -6,8 +6,8 @@ train).
 """
 from __future__ import annotations
 
-import ctypes
 import math
+import struct
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -15,57 +15,57 @@ from torch.autograd.function import once_differentiable
 from . import _check, _lib
 
 WIDTHS = (32, 64, 96, 128)
+MOST_STRIDE = 1 << 22  # elements between tokens that the kernels read in place
 
 
-class _Attention(ctypes.Structure):
-    """tms_attention"""
-    _fields_ = ([(n, ctypes.c_void_p) for n in ("q", "k", "v")]
-                + [(n, ctypes.c_int64) for n in ("q_token", "q_head", "k_token", "k_head", "v_token", "v_head")]
-                + [(n, ctypes.c_void_p) for n in ("offsets", "prefix", "slopes")]
-                + [(n, ctypes.c_int64) for n in ("texts", "tokens", "heads", "kv_heads", "width")]
-                + [("scale", ctypes.c_double), ("cap", ctypes.c_double), ("dtype", ctypes.c_int64)])
+_pack = struct.Struct("@3P6q3P5q2dq").pack  # tms_attention
 
 
-def _describe(q, k, v, offsets, prefix, slopes, scale, cap) -> _Attention:
+def _describe(q, k, v, offsets, prefix, slopes, scale, cap) -> bytes:
     T, H, D = q.shape
-    return _Attention(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
-                      offsets.data_ptr(), _lib.ptr(prefix), _lib.ptr(slopes), offsets.numel() - 1, T, H, k.shape[1], D, scale, cap,
-                      _lib.dtype_code(q.dtype))
+    qt, qh, _ = q.stride()
+    kt, kh, _ = k.stride()
+    vt, vh, _ = v.stride()
+    return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, offsets.data_ptr(),
+                 0 if prefix is None else prefix.data_ptr(), 0 if slopes is None else slopes.data_ptr(), offsets.shape[0] - 1, T, H,
+                 k.shape[1], D, scale, cap, _lib.DTYPE_CODES[q.dtype])
 
 
 def _forward(q, k, v, offsets, prefix, slopes, scale, cap, train):
     lib = _lib.load()
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     low = torch.empty_like(out) if train and q.dtype != torch.float32 else None
-    lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if train else None
+    stats = None
+    if train or slopes is not None:
+        stats = torch.empty(lib.tms_attention_stats(q.shape[0], q.shape[1], k.shape[1]), dtype=torch.float32, device=q.device)
     given = _describe(q, k, v, offsets, prefix, slopes, scale, cap)
-    status = _lib.launch(q.device, lib.tms_packed_attention, ctypes.addressof(given), out.data_ptr(), _lib.ptr(low), _lib.ptr(lse))
+    status = _lib.launch(q.device, lib.tms_packed_attention, given, out.data_ptr(), _lib.ptr(low), _lib.ptr(stats))
     if status:
         _lib.check(status)
-    return out, low, lse
+    return out, low, stats
 
 
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, prefix, slopes, scale, cap):
-        out, low, lse = _forward(q, k, v, offsets, prefix, slopes, scale, cap, True)
-        ctx.save_for_backward(q, k, v, offsets, prefix, slopes, out, low, lse)
+        out, low, stats = _forward(q, k, v, offsets, prefix, slopes, scale, cap, True)
+        ctx.save_for_backward(q, k, v, offsets, prefix, slopes, out, low, stats)
         ctx.args = scale, cap
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        q, k, v, offsets, prefix, slopes, out, low, lse = ctx.saved_tensors
+        q, k, v, offsets, prefix, slopes, out, low, stats = ctx.saved_tensors
         lib = _lib.load()
         grad = _check.aligned(grad)
         dq, dk, dv = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if need else None
                       for x, need in zip((q, k, v), ctx.needs_input_grad))
-        nbytes = lib.tms_attention_workspace_size(q.shape[0], q.shape[1])
+        nbytes = lib.tms_attention_workspace_size(offsets.shape[0] - 1, *q.shape[:2], *k.shape[1:])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
         given = _describe(q, k, v, offsets, prefix, slopes, *ctx.args)
-        status = _lib.launch(q.device, lib.tms_packed_attention_grad, ctypes.addressof(given), out.data_ptr(), _lib.ptr(low),
-                             lse.data_ptr(), grad.data_ptr(), _lib.ptr(ws), nbytes, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv))
+        status = _lib.launch(q.device, lib.tms_packed_attention_grad, given, out.data_ptr(), _lib.ptr(low),
+                             stats.data_ptr(), grad.data_ptr(), _lib.ptr(ws), nbytes, _lib.ptr(dq), _lib.ptr(dk), _lib.ptr(dv))
         if status:
             _lib.check(status)
         return dq, dk, dv, None, None, None, None, None
@@ -74,7 +74,8 @@ class _PackedAttention(torch.autograd.Function):
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """As it is where the kernels read it so (whole rows of a head, at 16-byte steps), else a copy."""
     step = 16 // t.element_size()
-    if t.stride(2) == 1 and t.stride(0) % step == 0 and t.stride(1) % step == 0 and t.data_ptr() % 16 == 0:
+    token, head, one = t.stride()
+    if one == 1 and token % step == 0 and head % step == 0 and token <= MOST_STRIDE and t.data_ptr() % 16 == 0:
         return t
     return _check.aligned(t)
 
@@ -82,6 +83,39 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 def _integers(fn: str, name: str, t: torch.Tensor) -> None:
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
         raise TypeError(f"{fn}: {name} must be an integer tensor (got {t.dtype})")
+
+
+def _usual(q, k, v, offsets) -> bool:
+    """Whether the tensors are what a model has in hand, one dtype on one GPU with int64 offsets there,
+    and need none of the checks below (which cost a small call as much as its kernel)."""
+    if not (isinstance(q, torch.Tensor) and isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor) and isinstance(offsets, torch.Tensor)):
+        return False
+    if not (q.is_cuda and q.dtype is k.dtype and q.dtype is v.dtype and q.dtype in _lib.DTYPE_CODES and offsets.dtype is torch.int64
+            and q.dim() == 3 and k.dim() == 3 and offsets.dim() == 1):
+        return False
+    (T, H, D), shape, dev = q.shape, k.shape, q.get_device()
+    return (shape == v.shape and shape[0] == T and shape[2] == D and D in WIDTHS and H > 0 and shape[1] > 0 and H % shape[1] == 0
+            and offsets.shape[0] > 0 and k.get_device() == dev and v.get_device() == dev and offsets.get_device() == dev)
+
+
+def _checked(fn: str, q, k, v, offsets) -> None:
+    for name, t in (("q", q), ("k", k), ("v", v), ("offsets", offsets)):
+        _check.tensor(name, t)
+    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"{fn}: q must be (T, H, D), k and v (T, KV, D), got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
+    T, H, D = q.shape
+    if k.shape[1] == 0 or H == 0 or H % k.shape[1]:
+        raise ValueError(f"{fn}: {H} query heads cannot share {k.shape[1]} heads of keys")
+    if offsets.dim() != 1 or offsets.numel() == 0:
+        raise ValueError(f"{fn}: offsets must be (B + 1,), got {tuple(offsets.shape)}")
+    _integers(fn, "offsets", offsets)
+    _check.embedding_dtype("q", q)
+    if k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError(f"{fn}: q is {q.dtype}, k is {k.dtype}, v is {v.dtype}")
+    if D not in WIDTHS:
+        raise NotImplementedError(f"{fn}: heads of {', '.join(map(str, WIDTHS))} elements (got {D})")
+    if offsets.device.type == "cpu" and (bool((offsets[1:] < offsets[:-1]).any()) or int(offsets[0]) < 0 or int(offsets[-1]) > T):
+        raise ValueError(f"{fn}: offsets must ascend within [0, {T}]")
 
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets: torch.Tensor, *, prefix=None,
@@ -112,24 +146,12 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     inputs' type between two products. Every sum has one order.
     """
     fn = "packed_attention"
-    for name, t in (("q", q), ("k", k), ("v", v), ("offsets", offsets)):
-        _check.tensor(name, t)
+    usual = _usual(q, k, v, offsets)
+    if not usual:
+        _checked(fn, q, k, v, offsets)
     _check.no_tangents(fn, (q, k, v))
-    if q.dim() != 3 or k.dim() != 3 or v.shape != k.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"{fn}: q must be (T, H, D), k and v (T, KV, D), got {tuple(q.shape)}, {tuple(k.shape)} and {tuple(v.shape)}")
-    T, H, D = q.shape
-    if k.shape[1] == 0 or H == 0 or H % k.shape[1]:
-        raise ValueError(f"{fn}: {H} query heads cannot share {k.shape[1]} heads of keys")
-    if offsets.dim() != 1 or offsets.numel() == 0:
-        raise ValueError(f"{fn}: offsets must be (B + 1,), got {tuple(offsets.shape)}")
-    _integers(fn, "offsets", offsets)
-    B = offsets.numel() - 1
-    _check.embedding_dtype("q", q)
-    if k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError(f"{fn}: q is {q.dtype}, k is {k.dtype}, v is {v.dtype}")
-    if D not in WIDTHS:
-        raise NotImplementedError(f"{fn}: heads of {', '.join(map(str, WIDTHS))} elements (got {D})")
-    scale = 1 / math.sqrt(D) if scale is None else float(scale)
+    H, B = q.shape[1], offsets.shape[0] - 1
+    scale = 1 / math.sqrt(q.shape[2]) if scale is None else float(scale)
     if not 0 < scale < 1e30:
         raise ValueError(f"{fn}: scale must be positive and finite (got {scale})")
     if cap is not None and not 0 < (cap := float(cap)) < 1e30:
@@ -146,27 +168,23 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
             raise ValueError(f"{fn}: slopes must be ({H},) float32, got {tuple(slopes.shape)} {slopes.dtype}")
         if slopes.requires_grad:
             raise NotImplementedError(f"{fn}: a gradient of the slopes")
-    if offsets.device.type == "cpu":
-        if bool((offsets[1:] < offsets[:-1]).any()) or int(offsets[0]) < 0 or int(offsets[-1]) > T:
-            raise ValueError(f"{fn}: offsets must ascend within [0, {T}]")
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        _check.on_gpu(name, t)
-    given = {"q": q, "k": k, "v": v}
-    if slopes is not None:
-        given["slopes"] = slopes
-    if isinstance(prefix, torch.Tensor) and prefix.device.type != "cpu":
-        given["prefix"] = prefix
-    if offsets.device.type != "cpu":
-        given["offsets"] = offsets
-    dev = _check.same_device(**given)
-    offsets = offsets.to(dev, torch.int64).contiguous()
+    if not usual:
+        for name, t in (("q", q), ("k", k), ("v", v)):
+            _check.on_gpu(name, t)
+        _check.same_device(q=q, k=k, v=v)
+    dev = q.device
+    for name, t in (("slopes", slopes), ("prefix", prefix), ("offsets", offsets)):  # the latter two may come from the host
+        if isinstance(t, torch.Tensor) and t.device != dev and (t.is_cuda or name == "slopes"):
+            raise ValueError(f"{fn}: {name} is on {t.device}, q on {dev}")
+    if not usual or not offsets.is_contiguous():
+        offsets = offsets.to(dev, torch.int64).contiguous()
     if isinstance(prefix, torch.Tensor):
         prefix = prefix.to(dev, torch.int64).contiguous()
     elif prefix is not None:
         prefix = torch.full((B,), prefix, dtype=torch.int64, device=dev)
-    slopes = None if slopes is None else slopes.contiguous()
+    if slopes is not None:
+        slopes = slopes.contiguous()
     q, k, v = _rows(q), _rows(k), _rows(v)
-    args = (q, k, v, offsets, prefix, slopes, scale, cap or 0.0)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _PackedAttention.apply(*args)
-    return _forward(*args, False)[0]
+        return _PackedAttention.apply(q, k, v, offsets, prefix, slopes, scale, cap or 0.0)
+    return _forward(q, k, v, offsets, prefix, slopes, scale, cap or 0.0, False)[0]

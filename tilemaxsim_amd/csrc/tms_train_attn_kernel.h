@@ -39,14 +39,20 @@
 #include <math.h>
 
 #include "tms_common.h"
+#include "tms_train_rules.h"
 
 namespace tms {
 
 typedef short attn_s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 attn_f16x2 __attribute__((ext_vector_type(2)));
 
 constexpr int kAttnThreads = 256;
 constexpr float kAttnLog2e = 1.4426950408889634f;
+constexpr float kAttnNothing = 160.f;  // so many powers of two below, exp2 is 0
+constexpr float kAttnSlack = 8.f;  // powers of two that P may stand above its reference in the forward pass
 constexpr int kAttnP16 = 15;  // fp16: P times 2^15 in the backward pass
+
+constexpr int kAttnNorms = 64;  // numbers a head
 
 struct AttnArgs {
   const void *q, *k, *v;
@@ -55,7 +61,8 @@ struct AttnArgs {
   const int64_t* prefix;           // B, or NULL: a text sees all of itself
   const float* slopes;             // H, or NULL
   int64_t T;
-  int32_t B, H, KV, slots;
+  int32_t B, H, KV, many, slots;  // many: heads that share keys
+  int32_t parts;                  // workgroups that share a tile's heads in the kernel for dk and dv
   float scale, cap;  // cap 0: none
   void* out;         // (T, H, D)
   void* low;         // what out's rounding left, of out's type, or NULL
@@ -63,7 +70,9 @@ struct AttnArgs {
   // backward
   const void* grad;  // (T, H, D)
   float* delta;      // (H, T)
+  float* sums;       // [part][dk, dv][T, KV, D], where parts > 1
   void *dq, *dk, *dv;
+  float* norms;  // [H + KV][kAttnNorms]: largest squares of rows of q and k; or NULL
 };
 
 template <int DT>
@@ -111,7 +120,8 @@ __device__ __forceinline__ typename AttnType<DT>::Frag attn_pack(f32x4 lo, f32x4
         const f32x2 v = {a, b};
         r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2));
       } else {
-        r[i] = (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)a) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)b) << 16;
+        const f32x2 v = {a, b};
+        r[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(v, attn_f16x2));
       }
     }
   }
@@ -157,20 +167,40 @@ struct AttnTile {
     const int64_t x = a.offsets[i - 1];
     return (int32_t)(x < 0 ? 0 : x > a.T ? a.T : x);
   }
-  __device__ __forceinline__ void find(const AttnArgs& a, int w, int rows) {
+  template <int ROWS>
+  __device__ __forceinline__ void find(const AttnArgs& a, int w) {
     const int lane = threadIdx.x & 63;
     int lo = 0, n = a.B + 2;
-    while (n > 1) {  // 64 candidates at a time
+    while (n > 255) {  // 64 candidates at a time
       const int step = (n + 63) / 64, i = lane * step;
-      const bool in = i < n;
-      const uint64_t hit = __ballot(in && (lane == 0 || offset(a, lo + i) / rows + lo + i <= w));
+      const uint64_t hit = __ballot(i < n && (lane == 0 || offset(a, lo + i) / ROWS + lo + i <= w));
       const int at = (63 - __builtin_clzll(hit)) * step;  // the last one at or before w
       lo += at;
       n = n - at < step ? n - at : step;
     }
-    text = __builtin_amdgcn_readfirstlane(lo);
-    begin = __builtin_amdgcn_readfirstlane(offset(a, text));
-    end = __builtin_amdgcn_readfirstlane(offset(a, text + 1));
+    // four a lane, and the one behind the last: one round trip, and both ends of the text's rows are at hand
+    int v[4], hits = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = lo + lane * 4 + k <= a.B + 2 ? offset(a, lo + lane * 4 + k) : 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int i = lane * 4 + k;
+      hits += __builtin_popcountll(__ballot(i < n && (i == 0 || v[k] / ROWS + lo + i <= w)));
+    }
+    auto value = [&](int i) {  // uniform i
+      int x = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const int y = __builtin_amdgcn_readlane(v[k], i / 4);
+        x = i % 4 == k ? y : x;
+      }
+      return x;
+    };
+    hits = hits < 1 ? 1 : hits > n ? n : hits;
+    text = lo + hits - 1;
+    begin = value(hits - 1);
+    end = value(hits);
+    constexpr int rows = ROWS;
     const int64_t at = (int64_t)begin + (int64_t)(w - (begin / rows + text)) * rows;
     if (at < begin || at >= end) {
       text = -1;
@@ -187,14 +217,28 @@ struct AttnTile {
   }
 };
 
-// Which tile and head a workgroup takes: each XCD (workgroups go to the eight in turn) takes a run of its
-// own, head by head, so that the tiles of a long text that read the same keys share an L2.
+// Which tile and head a workgroup takes. Workgroups go to the eight XCDs in turn. Each XCD takes a run of its
+// own, head by head: the tiles of a long text read the same keys through one L2 (2048 tokens, 8 heads
+// of 64, forward and backward: 98 us, 124 without). Where heads differ in how far they reach, each XCD takes
+// every eighth group of four neighbouring tiles instead, and so its share of each head (two texts of
+// 8192 under biases of 2^-0.7 to 2^-8: 1,533 us, 2,019 in runs, as long as the XCD with the flattest ones).
+constexpr int kAttnGroup = 4;
+static inline int64_t attn_grid(int64_t slots, int64_t heads) {
+  return ((slots + kAttnGroup - 1) / kAttnGroup * heads + 7) / 8 * 8 * kAttnGroup;
+}
 __device__ __forceinline__ bool attn_place(const AttnArgs& a, int heads, int& slot, int& head) {
-  const int64_t total = (int64_t)a.slots * heads, each = (total + 7) / 8;
-  const int64_t at = blockIdx.x % 8 * each + blockIdx.x / 8;
-  if (blockIdx.x / 8 >= each || at >= total) return false;
-  head = (int)(at / a.slots);
-  slot = (int)(at - (int64_t)head * a.slots);
+  const uint32_t slots = (uint32_t)a.slots, xcd = blockIdx.x % 8, i = blockIdx.x / 8;
+  if (a.norms != nullptr) {
+    const uint32_t groups = (slots + kAttnGroup - 1) / kAttnGroup, unit = i / kAttnGroup * 8 + xcd;
+    if (unit >= groups * (uint32_t)heads) return false;
+    head = (int)(unit / groups);
+    slot = (int)((unit - (uint32_t)head * groups) * kAttnGroup + i % kAttnGroup);
+    return slot < a.slots;
+  }
+  const uint32_t total = slots * (uint32_t)heads, each = (total + 7) / 8, at = xcd * each + i;
+  if (i >= each || at >= total) return false;
+  head = (int)(at / slots);
+  slot = (int)(at - (uint32_t)head * slots);
   return true;
 }
 
@@ -217,13 +261,29 @@ struct AttnRows {
     if constexpr (ES == 4) row = line, col = panel * 32 + p * 4;
     else row = 2 * line + (p >> 2), col = panel * 32 + (p & 3) * 8;
   }
+  uint32_t off[kLoads];  // bytes from the tile's first row: 64 rows are less than 2^32 apart
+  __device__ __forceinline__ void init(int64_t stride) {
+#pragma unroll
+    for (int i = 0; i < kLoads; i++) {
+      int row, col;
+      piece(i * kAttnThreads + (int)threadIdx.x, row, col);
+      off[i] = (uint32_t)(row * (int)stride + col) * (uint32_t)ES;
+    }
+  }
+  // Rows from `first` (uniform) on.
   __device__ __forceinline__ void load(const typename Ty::E* base, int64_t stride, int first, int limit) {
+    const uint8_t* at = (const uint8_t*)(base + first * stride);
+    if (first + R <= limit) {
+#pragma unroll
+      for (int i = 0; i < kLoads; i++) held[i] = *(const u32x4*)(at + off[i]);
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < kLoads; i++) {
       int row, col;
       piece(i * kAttnThreads + (int)threadIdx.x, row, col);
       held[i] = u32x4{0u, 0u, 0u, 0u};
-      if (first + row < limit) held[i] = *(const u32x4*)(base + (int64_t)(first + row) * stride + col);
+      if (first + row < limit) held[i] = *(const u32x4*)(at + off[i]);
     }
   }
   __device__ __forceinline__ void store(uint8_t* lds) const {
@@ -274,40 +334,127 @@ __device__ __forceinline__ void attn_own(const typename AttnType<DT>::E* base, i
   for (int ks = 0; ks < D / 32; ks++) f[ks] = *(const Frag*)(base + row_elems + ks * 32 + 8 * g);
 }
 
-// A score in powers of two from the sum of products, and (under a cap) its derivative's factor.
+// What a score takes besides the products: nothing, a bias, or a cap (and perhaps a bias).
+enum AttnKind { kAttnPlain = 0, kAttnBias = 1, kAttnCap = 2 };
+
+// Scores x from sums of products s, as y with x log2(e) = unit y + shift: y = s - lean |i - j|, or under
+// a cap y = cap log2(e) tanh(s scale / cap) - lean |i - j| with a unit of 1. The unit goes into the exponent's
+// one FMA. Without a cap, a bias costs next to nothing in tiles that lie on one side of a wave's own rows:
+// there it is a part of the tile's row, which the products' sums begin with, and a part of
+// the wave's own row, which is in the shift.
+template <int DT, int KIND>
 struct AttnScore {
-  float c1, cap2, inv_cap, slope2;  // scale log2(e), cap log2(e), scale / cap, slope log2(e)
+  float unit, cap2, inv_cap, lean;
+  int side = 2;  // of the tile: its rows before the wave's (-1), behind them (1), or both (0)
+  f32x4 begin[KIND == kAttnBias ? AttnType<DT>::kRows / 16 : 1];  // -lean of rows 16 b + 4 g + e by side
+
   __device__ __forceinline__ void init(const AttnArgs& a, int head) {
-    c1 = a.scale * kAttnLog2e;
+    unit = KIND == kAttnCap ? 1.f : a.scale * kAttnLog2e;
     cap2 = a.cap * kAttnLog2e;
-    inv_cap = a.cap > 0.f ? a.scale / a.cap : 0.f;
-    slope2 = a.slopes ? a.slopes[head] * kAttnLog2e : 0.f;
+    inv_cap = KIND == kAttnCap ? a.scale / a.cap * (DT == TMS_DTYPE_F32 ? 1.f : 2.f * kAttnLog2e) : 0.f;
+    lean = a.slopes ? a.slopes[head] * (KIND == kAttnCap ? kAttnLog2e : 1.f / a.scale) : 0.f;
+    side = 2;
   }
-  template <int DT>
-  __device__ __forceinline__ static float tanh_of(float z) {
-    if constexpr (DT == TMS_DTYPE_F32) return tanhf(z);
-    // 1 - 2 / (1 + e^2z): to 2^-22 or so of the cap, where the operands have 2^-9 or 2^-12
-    return __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * (2.f * kAttnLog2e))), 1.f);
-  }
-  template <int DT>
-  __device__ __forceinline__ float operator()(float s, int far, float* factor) const {
-    float x;
-    if (cap2 > 0.f) {  // uniform
-      const float t = tanh_of<DT>(s * inv_cap);
-      x = t * cap2;
-      if (factor) *factor = __builtin_fmaf(-t, t, 1.f);
-    } else {
-      x = s * c1;
-      if (factor) *factor = 1.f;
+  // The tile of rows from `first` on, against the wave's own from `own` up to `own_end`.
+  __device__ __forceinline__ void tile(int first, int own, int own_end, int g) {
+    if constexpr (KIND == kAttnBias) {
+      const int now = first + AttnType<DT>::kRows <= own ? -1 : first >= own_end ? 1 : 0;
+      if (now == side) return;
+      side = now;
+#pragma unroll
+      for (int b = 0; b < AttnType<DT>::kRows / 16; b++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) begin[b][e] = lean * (float)(-now * (16 * b + 4 * g + e));
     }
-    return __builtin_fmaf(-slope2, (float)(far < 0 ? -far : far), x);
   }
+  __device__ __forceinline__ f32x4 start(int b) const {
+    if constexpr (KIND == kAttnBias) return begin[b];
+    return f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // What the scores of the wave's own row `own` have in common with the tile from `first` on.
+  __device__ __forceinline__ float shift(int own, int first) const {
+    if constexpr (KIND == kAttnBias) return unit * lean * (float)(side * (own - first));
+    return 0.f;
+  }
+  // Whether the bias has to be taken off element by element.
+  __device__ __forceinline__ bool single() const { return (KIND == kAttnCap && lean != 0.f) || (KIND == kAttnBias && side == 0); }
+  // Under a cap, y from s, and kSlope times the derivative's factor, 1 - tanh^2. In 16 bits tanh z is taken as
+  // 1 - 2 r with r = 1 / (1 + e^2z), to 2^-22 or so of the cap, where the operands have 2^-9 or 2^-12.
+  static constexpr float kSlope = KIND == kAttnCap && DT != TMS_DTYPE_F32 ? 0.25f : 1.f;
+  __device__ __forceinline__ float capped(float s, float& slope) const {
+    if constexpr (DT == TMS_DTYPE_F32) {
+      const float t = tanhf(s * inv_cap);
+      slope = __builtin_fmaf(-t, t, 1.f);
+      return t * cap2;
+    }
+    const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * inv_cap));  // inv_cap has 2 log2(e) in it
+    slope = __builtin_fmaf(-r, r, r);  // (1 - t^2) / 4
+    return __builtin_fmaf(-2.f * cap2, r, cap2);
+  }
+  // far: i - j, or its negative.
+  __device__ __forceinline__ float biased(float y, float far) const { return __builtin_fmaf(-lean, fabsf(far), y); }
 };
+
+// How far from a token its keys can matter under a bias alone (T without one). With |q|, |k| the largest
+// norms, scores but for the bias lie within scale |q| |k| of 0, and a row's largest is at least its own
+// token's: P of a token n away is at most exp(2 scale |q| |k| - slope n), and 0 in fp32 where that is
+// below 2^-160. Where a norm is not finite, nothing is left out.
+__device__ __forceinline__ int attn_reach(const AttnArgs& a, int head) {
+  if (a.norms == nullptr) return (int)a.T;
+  const int lane = threadIdx.x & 63;
+  float q = a.norms[head * kAttnNorms + lane], k = a.norms[(a.H + head / a.many) * kAttnNorms + lane];
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) {
+    q = __builtin_elementwise_maximum(q, __shfl_xor(q, o));
+    k = __builtin_elementwise_maximum(k, __shfl_xor(k, o));
+  }
+  const float far = (kAttnNothing + 2.f * kAttnLog2e * a.scale * sqrtf(q) * sqrtf(k) * 1.001f) / (a.slopes[head] * kAttnLog2e);
+  const int reach = far >= 0.f && far < (float)a.T ? (int)far + 1 : (int)a.T;  // no slope, a negative one, NaN: all
+  return __builtin_amdgcn_readfirstlane(reach);
+}
+
+// The larger of the two; NaN if either is.
+__device__ __forceinline__ float attn_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The largest over the four lanes that have a column's rows, in all of them.
+__device__ __forceinline__ float attn_cross_max(float m) {
+  const auto p = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, m), false, false);
+  m = attn_max(__builtin_bit_cast(float, (unsigned)p[0]), __builtin_bit_cast(float, (unsigned)p[1]));
+  const auto q = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, m), __builtin_bit_cast(unsigned, m), false, false);
+  return attn_max(__builtin_bit_cast(float, (unsigned)q[0]), __builtin_bit_cast(float, (unsigned)q[1]));
+}
+
+// ---------------------------------------------------------------- norms
+
+// The largest squared norms of q's and k's rows: 16 lanes a row, a part of the tokens a workgroup.
+template <int DT, int D>
+__global__ __launch_bounds__(kAttnThreads) void attn_norms_kernel(AttnArgs a) {
+  typedef typename AttnType<DT>::E E;
+  constexpr int EACH = D / 16;
+  __shared__ float lds[kAttnThreads / 64];
+  const int head = blockIdx.x / kAttnNorms, part = blockIdx.x % kAttnNorms;
+  const bool of_q = head < a.H;
+  const E* base = of_q ? (const E*)a.q + head * a.qh : (const E*)a.k + (head - a.H) * a.kh;
+  const int64_t stride = of_q ? a.qt : a.kt;
+  float most = 0.f;
+  for (int64_t row = part * 16 + (int)threadIdx.x / 16; row < a.T; row += 16 * kAttnNorms) {
+    const E* x = base + row * stride + (threadIdx.x & 15) * EACH;
+    float s = 0.f;
+#pragma unroll
+    for (int e = 0; e < EACH; e++) s = __builtin_fmaf(attn_float<DT>(x[e]), attn_float<DT>(x[e]), s);
+    most = attn_max(most, row_sum16(s));
+  }
+#pragma unroll
+  for (int o = 32; o >= 1; o >>= 1) most = attn_max(most, __shfl_xor(most, o));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x == 0) a.norms[blockIdx.x] = attn_max(attn_max(lds[0], lds[1]), attn_max(lds[2], lds[3]));
+}
 
 // ---------------------------------------------------------------- forward
 
-// GENERAL: with a cap or a bias. NB: blocks of 16 queries a wave.
-template <int DT, int D, int NB, bool GENERAL>
+// NB: blocks of 16 queries a wave.
+template <int DT, int D, int NB, int KIND>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs a) {
   typedef AttnRows<DT, D> Rows;
   typedef typename AttnType<DT>::E E;
@@ -317,7 +464,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
   int slot, head;
   if (!attn_place(a, a.H, slot, head)) return;
   AttnTile t;
-  t.find(a, slot, BQ);
+  t.find<BQ>(a, slot);
   if (t.text < 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int row0 = t.first + wave * 16 * NB;
@@ -333,10 +480,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
   for (int j = 0; j < NB; j++) top[j] = NEG, sum[j] = 0.f;
 
   if (t.real) {
-    const int kvh = head / (a.H / a.KV);
+    const int kvh = head / a.many;
     const E* K = (const E*)a.k + kvh * a.kh;
     const E* V = (const E*)a.v + kvh * a.vh;
-    AttnScore score;
+    AttnScore<DT, KIND> score;
     score.init(a, head);
     Frag q[NB][KS];
     int sees[NB];  // a row's last visible key, plus one
@@ -351,15 +498,22 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
     else least = t.prefix_end;
     // keys that any of the workgroup's rows sees, and any of this wave's
     const int last = t.first + BQ < t.end ? t.first + BQ : t.end;
-    const int keys = last > t.prefix_end ? last : t.prefix_end;
+    int keys = last > t.prefix_end ? last : t.prefix_end, key0 = t.begin;
+    if constexpr (KIND == kAttnBias) {
+      const int reach = attn_reach(a, head);
+      if (t.first - reach > key0) key0 += (t.first - reach - key0) / R * R;
+      if (last + reach < keys) keys = last + reach;
+    }
     int mine = row0 + 16 * NB < t.end ? row0 + 16 * NB : t.end;
     mine = row0 >= t.end ? t.begin : mine > t.prefix_end ? mine : t.prefix_end;
 
     Rows rk, rv;
-    rk.load(K, a.kt, t.begin, keys);
-    rv.load(V, a.vt, t.begin, keys);
+    rk.init(a.kt);
+    rv.init(a.vt);
+    rk.load(K, a.kt, key0, keys);
+    rv.load(V, a.vt, key0, keys);
     int buf = 0;
-    for (int k0 = t.begin; k0 < keys; k0 += R) {
+    for (int k0 = key0; k0 < keys; k0 += R) {
       uint8_t* lk = attn_mem + buf * 2 * Rows::kBytes;
       uint8_t* lv = lk + Rows::kBytes;
       rk.store(lk);
@@ -374,10 +528,11 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
       if (k0 >= mine) continue;  // uniform in the wave
 
       f32x4 s[KB][NB];
+      score.tile(k0, row0, row0 + 16 * NB, g);
 #pragma unroll
       for (int b = 0; b < KB; b++) {
 #pragma unroll
-        for (int j = 0; j < NB; j++) s[b][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < NB; j++) s[b][j] = score.start(b);
 #pragma unroll
         for (int ks = 0; ks < KS; ks++) {
           const Frag f = Rows::row_frag(lk, b, ks, c, g);
@@ -385,14 +540,23 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
           for (int j = 0; j < NB; j++) s[b][j] = attn_mfma<DT>(f, q[j][ks], s[b][j]);
         }
       }
-      if constexpr (GENERAL) {
+      if constexpr (KIND == kAttnCap) {
+        float none;
 #pragma unroll
         for (int b = 0; b < KB; b++)
 #pragma unroll
           for (int j = 0; j < NB; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-              s[b][j][e] = score.template operator()<DT>(s[b][j][e], row0 + 16 * j + c - (k0 + 16 * b + 4 * g + e), nullptr);
+            for (int e = 0; e < 4; e++) s[b][j][e] = score.capped(s[b][j][e], none);
+      }
+      if (score.single()) {
+        const float near = (float)(row0 + c - k0 - 4 * g);
+#pragma unroll
+        for (int b = 0; b < KB; b++)
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[b][j][e] = score.biased(s[b][j][e], near + (float)(16 * j - 16 * b - e));
       }
       if (k0 + R > least) {  // some row does not see all of the tile
 #pragma unroll
@@ -402,18 +566,27 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
 #pragma unroll
             for (int e = 0; e < 4; e++) s[b][j][e] = k0 + 16 * b + 4 * g + e < sees[j] ? s[b][j][e] : NEG;
       }
-      Frag p[NB][R / 32];
+      // A row's reference follows its maximum when that has left it by kAttnSlack: not at every tile of a bias
+      // that favours what comes next.
+      float m[NB], shift[NB];
+      bool over = false, some = false;
 #pragma unroll
       for (int j = 0; j < NB; j++) {
-        float m = NEG;
+        m[j] = NEG;
 #pragma unroll
         for (int b = 0; b < KB; b++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) m = fmaxf(m, s[b][j][e]);
-        m = cross_row_max(m);
-        if constexpr (!GENERAL) m *= score.c1;
-        if (__ballot(m > top[j]) != 0ull) {
-          const float up = fmaxf(m, top[j]);
+          for (int e = 0; e < 4; e += 2) m[j] = attn_max(attn_max(s[b][j][e], s[b][j][e + 1]), m[j]);
+        shift[j] = score.shift(row0 + 16 * j + c, k0);
+        m[j] = __builtin_fmaf(attn_cross_max(m[j]), score.unit, shift[j]);
+        over |= m[j] > top[j] + kAttnSlack;
+        some |= !(m[j] < top[j] - kAttnNothing);
+      }
+      if (__ballot(some) == 0ull) continue;  // every P of the tile is 0, as far behind as it is by its bias
+      if (__ballot(over) != 0ull) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+          const float up = fmaxf(m[j], top[j]);
           const float k = up == NEG ? 1.f : __builtin_amdgcn_exp2f(top[j] - up);
           top[j] = up;
           sum[j] *= k;
@@ -422,28 +595,31 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
 #pragma unroll
             for (int e = 0; e < 4; e++) acc[d][j][e] *= k;
         }
-        const float ref = top[j] == NEG ? 0.f : top[j];
-#pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float x;
-            if constexpr (GENERAL) x = s[b][j][e] - ref;
-            else x = __builtin_fmaf(s[b][j][e], score.c1, -ref);
-            s[b][j][e] = __builtin_amdgcn_exp2f(x);
-            sum[j] += s[b][j][e];
-          }
-#pragma unroll
-        for (int h = 0; h < R / 32; h++) p[j][h] = attn_pack<DT>(s[2 * h][j], s[2 * h + 1][j]);
       }
+      float ref[NB];
 #pragma unroll
-      for (int h = 0; h < R / 32; h++)
+      for (int j = 0; j < NB; j++) ref[j] = (top[j] == NEG ? 0.f : top[j]) - shift[j];
+#pragma unroll
+      for (int h = 0; h < R / 32; h++) {  // 32 keys at a time
+        Frag p[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+#pragma unroll
+          for (int b = 2 * h; b < 2 * h + 2; b++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              s[b][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j][e], score.unit, -ref[j]));
+              sum[j] += s[b][j][e];
+            }
+          p[j] = attn_pack<DT>(s[2 * h][j], s[2 * h + 1][j]);
+        }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           const Frag f = Rows::col_frag(lv, h, d, c, g);
 #pragma unroll
-          for (int j = 0; j < NB; j++) acc[d][j] = attn_mfma<DT>(f, p[j][h], acc[d][j]);
+          for (int j = 0; j < NB; j++) acc[d][j] = attn_mfma<DT>(f, p[j], acc[d][j]);
         }
+      }
     }
   }
 
@@ -477,23 +653,30 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
 // ---------------------------------------------------------------- backward
 
 // Sums of products of dS in fp16: dS is held times a power of two a column, which goes down
-// when a larger one comes. `most`: the largest |dS| of this round in the column.
+// when a larger one comes.
 struct AttnRange {
   float held = 0x1p100f;
+  // Two blocks of dS on their way to fp16; j: their column of sums.
   template <int DB, int NB>
-  __device__ __forceinline__ void follow(float most, f32x4 (&acc)[DB][NB], int j) {
-    most = cross_row_max(most);
-    if (__ballot(most * held > 32768.f) == 0ull) return;
-    const int e = (int)((__builtin_bit_cast(uint32_t, most) >> 23) & 0xffu);  // most < 2^(e - 126)
-    int s = 14 + 126 - e;
-    s = s < -100 ? -100 : s > 100 ? 100 : s;
-    const float to = most * held > 32768.f ? __builtin_bit_cast(float, (uint32_t)(s + 127) << 23) : held;
-    const float k = to / held;
-    held = to;
+  __device__ __forceinline__ void follow(f32x4& x, f32x4& y, f32x4 (&acc)[DB][NB], int j) {
+    float most = 0.f;
 #pragma unroll
-    for (int d = 0; d < DB; d++)
+    for (int e = 0; e < 4; e++) most = attn_max(attn_max(fabsf(x[e]), fabsf(y[e])), most);
+    most = attn_cross_max(most);
+    if (__ballot(most * held > 32768.f) != 0ull) {
+      const int e = (int)((__builtin_bit_cast(uint32_t, most) >> 23) & 0xffu);  // most < 2^(e - 126)
+      int s = 14 + 126 - e;
+      s = s < -100 ? -100 : s > 100 ? 100 : s;
+      const float to = most * held > 32768.f ? __builtin_bit_cast(float, (uint32_t)(s + 127) << 23) : held;
+      const float k = to / held;
+      held = to;
 #pragma unroll
-      for (int i = 0; i < 4; i++) acc[d][j][i] *= k;
+      for (int d = 0; d < DB; d++)
+#pragma unroll
+        for (int i = 0; i < 4; i++) acc[d][j][i] *= k;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] *= held, y[i] *= held;
   }
 };
 
@@ -512,17 +695,17 @@ __device__ __forceinline__ void attn_store(void* out, int64_t at, const f32x4 (&
 }
 
 // delta and dq: a workgroup has a tile of queries and goes over their keys.
-template <int DT, int D, int NB, bool GENERAL>
+template <int DT, int D, int NB, int KIND>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   typedef AttnRows<DT, D> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
-  constexpr int R = Rows::R, KB = R / 16, DB = D / 16, KS = D / 32, BQ = 64 * NB;
+  constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BQ = 64 * NB;
   extern __shared__ __attribute__((aligned(1024))) uint8_t attn_mem[];
   int slot, head;
   if (!attn_place(a, a.H, slot, head)) return;
   AttnTile t;
-  t.find(a, slot, BQ);
+  t.find<BQ>(a, slot);
   if (t.text < 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int row0 = t.first + wave * 16 * NB;
@@ -535,10 +718,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   AttnRange range[NB];
 
   if (t.real) {
-    const int kvh = head / (a.H / a.KV);
+    const int kvh = head / a.many;
     const E* K = (const E*)a.k + kvh * a.kh;
     const E* V = (const E*)a.v + kvh * a.vh;
-    AttnScore score;
+    AttnScore<DT, KIND> score;
     score.init(a, head);
     Frag q[NB][KS], go[NB][KS];
     int sees[NB];
@@ -568,15 +751,22 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
     }
     const int least = row0 + 1 > t.prefix_end ? row0 + 1 : t.prefix_end;
     const int last = t.first + BQ < t.end ? t.first + BQ : t.end;
-    const int keys = last > t.prefix_end ? last : t.prefix_end;
+    int keys = last > t.prefix_end ? last : t.prefix_end, key0 = t.begin;
+    if constexpr (KIND == kAttnBias) {
+      const int reach = attn_reach(a, head);
+      if (t.first - reach > key0) key0 += (t.first - reach - key0) / R * R;
+      if (last + reach < keys) keys = last + reach;
+    }
     int mine = row0 + 16 * NB < t.end ? row0 + 16 * NB : t.end;
     mine = row0 >= t.end ? t.begin : mine > t.prefix_end ? mine : t.prefix_end;
 
     Rows rk, rv;
-    rk.load(K, a.kt, t.begin, keys);
-    rv.load(V, a.vt, t.begin, keys);
+    rk.init(a.kt);
+    rv.init(a.vt);
+    rk.load(K, a.kt, key0, keys);
+    rv.load(V, a.vt, key0, keys);
     int buf = 0;
-    for (int k0 = t.begin; k0 < keys; k0 += R) {
+    for (int k0 = key0; k0 < keys; k0 += R) {
       uint8_t* lk = attn_mem + buf * 2 * Rows::kBytes;
       uint8_t* lv = lk + Rows::kBytes;
       rk.store(lk);
@@ -589,86 +779,102 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       buf ^= 1;
       if (k0 >= mine) continue;
+      float ref[NB];
+      score.tile(k0, row0, row0 + 16 * NB, g);
+#pragma unroll
+      for (int j = 0; j < NB; j++) ref[j] = score.shift(row0 + 16 * j + c, k0) - lse[j];
       const bool part = k0 + R > least;
-
-      f32x4 s[KB][NB];
-      float most[NB];
+      const float near = (float)(row0 + c - k0 - 4 * g);
 #pragma unroll
-      for (int j = 0; j < NB; j++) most[j] = 0.f;
+      for (int h = 0; h < R / 32; h++) {  // 32 keys at a time
+        f32x4 s[2][NB];
 #pragma unroll
-      for (int b = 0; b < KB; b++) {
-        f32x4 dp[NB];
-#pragma unroll
-        for (int j = 0; j < NB; j++) s[b][j] = dp[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-          const Frag fk = Rows::row_frag(lk, b, ks, c, g), fv = Rows::row_frag(lv, b, ks, c, g);
+        for (int i = 0; i < 2; i++) {
+          const int b = 2 * h + i;
+          f32x4 dp[NB];
 #pragma unroll
           for (int j = 0; j < NB; j++) {
-            s[b][j] = attn_mfma<DT>(fk, q[j][ks], s[b][j]);
-            dp[j] = attn_mfma<DT>(fv, go[j][ks], dp[j]);
+            s[i][j] = score.start(b);
+            dp[j] = f32x4{-delta[j], -delta[j], -delta[j], -delta[j]};
           }
-        }
 #pragma unroll
-        for (int j = 0; j < NB; j++)
+          for (int ks = 0; ks < KS; ks++) {
+            const Frag fk = Rows::row_frag(lk, b, ks, c, g), fv = Rows::row_frag(lv, b, ks, c, g);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            float x, f = 1.f;
-            if constexpr (GENERAL) x = score.template operator()<DT>(s[b][j][e], row0 + 16 * j + c - (k0 + 16 * b + 4 * g + e), &f) - lse[j];
-            else x = __builtin_fmaf(s[b][j][e], score.c1, -lse[j]);
-            float y = __builtin_amdgcn_exp2f(x) * (dp[j][e] - delta[j]);
-            if constexpr (GENERAL) y *= f;
-            if (part) y = k0 + 16 * b + 4 * g + e < sees[j] ? y : 0.f;
-            s[b][j][e] = y;
-            if constexpr (DT == TMS_DTYPE_F16) most[j] = fmaxf(most[j], fabsf(y));
+            for (int j = 0; j < NB; j++) {
+              s[i][j] = attn_mfma<DT>(fk, q[j][ks], s[i][j]);
+              dp[j] = attn_mfma<DT>(fv, go[j][ks], dp[j]);
+            }
           }
-      }
-      Frag ds[NB][R / 32];
+          if constexpr (KIND == kAttnCap) {
 #pragma unroll
-      for (int j = 0; j < NB; j++) {
-        if constexpr (DT == TMS_DTYPE_F16) {
-          range[j].follow(most[j], acc, j);
+            for (int j = 0; j < NB; j++)
 #pragma unroll
-          for (int b = 0; b < KB; b++)
+              for (int e = 0; e < 4; e++) {
+                float f;
+                s[i][j][e] = score.capped(s[i][j][e], f);
+                dp[j][e] *= f;
+              }
+          }
+          if (score.single()) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[b][j][e] *= range[j].held;
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[i][j][e] = score.biased(s[i][j][e], near + (float)(16 * j - 16 * b - e));
+          }
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][e], score.unit, ref[j])) * dp[j][e];
         }
+        if (part) {
 #pragma unroll
-        for (int h = 0; h < R / 32; h++) ds[j][h] = attn_pack<DT>(s[2 * h][j], s[2 * h + 1][j]);
-      }
+          for (int i = 0; i < 2; i++)
 #pragma unroll
-      for (int h = 0; h < R / 32; h++)
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[i][j][e] = k0 + 32 * h + 16 * i + 4 * g + e < sees[j] ? s[i][j][e] : 0.f;
+        }
+        Frag ds[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+          if constexpr (DT == TMS_DTYPE_F16) range[j].follow(s[0][j], s[1][j], acc, j);
+          ds[j] = attn_pack<DT>(s[0][j], s[1][j]);
+        }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           const Frag f = Rows::col_frag(lk, h, d, c, g);
 #pragma unroll
-          for (int j = 0; j < NB; j++) acc[d][j] = attn_mfma<DT>(f, ds[j][h], acc[d][j]);
+          for (int j = 0; j < NB; j++) acc[d][j] = attn_mfma<DT>(f, ds[j], acc[d][j]);
         }
+      }
     }
   }
 #pragma unroll
   for (int j = 0; j < NB; j++) {
     const int row = row0 + 16 * j + c;
     if (row >= t.end) continue;
-    const float f = !t.real ? 0.f : DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale;
+    const float f = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND>::kSlope;
     if (a.dq) attn_store<DT>(a.dq, ((int64_t)row * a.H + head) * D, acc, j, f, g);
   }
 }
 
 // dk and dv: a workgroup has a tile of keys and goes over the queries that see them, head by head of
 // those that share the keys.
-template <int DT, int D, int NB, bool GENERAL>
+template <int DT, int D, int NB, int KIND>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
   typedef AttnRows<DT, D> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
-  constexpr int R = Rows::R, QB = R / 16, DB = D / 16, KS = D / 32, BK = 64 * NB;
+  constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BK = 64 * NB;
   extern __shared__ __attribute__((aligned(1024))) uint8_t attn_mem[];
   float* const stats = (float*)(attn_mem + 4 * Rows::kBytes);  // [buffer][lse, delta][R]
   int slot, kvh;
-  if (!attn_place(a, a.KV, slot, kvh)) return;
+  if (!attn_place(a, a.KV * a.parts, slot, kvh)) return;
+  const int part_of = kvh % a.parts;
+  kvh /= a.parts;
   AttnTile t;
-  t.find(a, slot, BK);
+  t.find<BK>(a, slot);
   if (t.text < 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int key0 = t.first + wave * 16 * NB;
@@ -691,24 +897,37 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
       from[j] = key < t.prefix_end ? t.begin : key;
     }
     // the first row that sees any key of the workgroup, and any of this wave's; the first one that sees all of the wave's
-    const int rows = t.first < t.prefix_end ? t.begin : t.first;
+    int rows = t.first < t.prefix_end ? t.begin : t.first, rows_end = t.end;
     const int mine = key0 >= t.end ? 0x7fffffff : key0 < t.prefix_end ? t.begin : key0;
     const int all = key0 + 16 * NB <= t.prefix_end || t.prefix_end == t.end ? t.begin : key0 + 16 * NB - 1;
-    const int many = a.H / a.KV, tiles = (t.end - rows + R - 1) / R, total = tiles * many;
+    const int head0 = kvh * a.many + part_of * a.many / a.parts, heads = kvh * a.many + (part_of + 1) * a.many / a.parts - head0;
+    if constexpr (KIND == kAttnBias) {  // as far as the farthest of the heads reaches
+      int reach = 0;
+      for (int h = 0; h < heads; h++) {
+        const int of = attn_reach(a, head0 + h);
+        reach = of > reach ? of : reach;
+      }
+      const int last = t.first + BK < t.end ? t.first + BK : t.end;
+      if (t.first - reach > rows) rows = t.first - reach;
+      if (last + reach < rows_end) rows_end = last + reach;
+    }
+    const int tiles = (rows_end - rows + R - 1) / R, total = tiles * heads;
 
     Rows rq, rg;
+    rq.init(a.qt);
+    rg.init((int64_t)a.H * D);
     float st = 0.f;  // a thread's share of the tile's statistics: lse (the first R), delta (the next)
     auto load = [&](int n) {
-      const int head = kvh * many + n / tiles, r0 = rows + n % tiles * R;
-      rq.load((const E*)a.q + head * a.qh, a.qt, r0, t.end);
-      rg.load((const E*)a.grad + (int64_t)head * D, (int64_t)a.H * D, r0, t.end);
+      const int head = head0 + n / tiles, r0 = rows + n % tiles * R;
+      rq.load((const E*)a.q + head * a.qh, a.qt, r0, rows_end);
+      rg.load((const E*)a.grad + (int64_t)head * D, (int64_t)a.H * D, r0, rows_end);
       if ((int)threadIdx.x < 2 * R) {
         const int r = r0 + (int)threadIdx.x % R;
         const float* from_ = (int)threadIdx.x < R ? a.lse : a.delta;
-        st = r < t.end ? from_[(int64_t)head * a.T + r] : (int)threadIdx.x < R ? __builtin_inff() : 0.f;
+        st = -(r < rows_end ? from_[(int64_t)head * a.T + r] : (int)threadIdx.x < R ? __builtin_inff() : 0.f);
       }
     };
-    AttnScore score;
+    AttnScore<DT, KIND> score;
     load(0);
     int buf = 0;
     for (int n = 0; n < total; n++) {
@@ -723,74 +942,91 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
       __builtin_amdgcn_sched_barrier(0);
       buf ^= 1;
       const int r0 = rows + n % tiles * R;
-      if (n % tiles == 0) score.init(a, kvh * many + n / tiles);
+      if (n % tiles == 0) score.init(a, head0 + n / tiles);
       if (r0 + R <= mine) continue;  // uniform in the wave
       const bool part = r0 < all;
-
-      f32x4 p[QB][NB], s[QB][NB];
-      float most[NB];
+      const float near = (float)(r0 + 4 * g - key0 - c);
+      score.tile(r0, key0, key0 + 16 * NB, g);
+      float shift[NB];
 #pragma unroll
-      for (int j = 0; j < NB; j++) most[j] = 0.f;
+      for (int j = 0; j < NB; j++) shift[j] = score.shift(key0 + 16 * j + c, r0);
 #pragma unroll
-      for (int b = 0; b < QB; b++) {
-        f32x4 dp[NB];
+      for (int h = 0; h < R / 32; h++) {  // 32 rows at a time
+        f32x4 p[2][NB], s[2][NB];
 #pragma unroll
-        for (int j = 0; j < NB; j++) s[b][j] = dp[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ks++) {
-          const Frag fq = Rows::row_frag(lq, b, ks, c, g), fg = Rows::row_frag(lg, b, ks, c, g);
+        for (int i = 0; i < 2; i++) {
+          const int b = 2 * h + i;
+          const f32x4 lse = *(const f32x4*)(ls + 16 * b + 4 * g), delta = *(const f32x4*)(ls + R + 16 * b + 4 * g);  // both negated
+          f32x4 dp[NB];
 #pragma unroll
           for (int j = 0; j < NB; j++) {
-            s[b][j] = attn_mfma<DT>(fq, k[j][ks], s[b][j]);
-            dp[j] = attn_mfma<DT>(fg, v[j][ks], dp[j]);
+            s[i][j] = score.start(b);
+            dp[j] = delta;
           }
-        }
-        const f32x4 lse = *(const f32x4*)(ls + 16 * b + 4 * g), delta = *(const f32x4*)(ls + R + 16 * b + 4 * g);
 #pragma unroll
-        for (int j = 0; j < NB; j++)
+          for (int ks = 0; ks < KS; ks++) {
+            const Frag fq = Rows::row_frag(lq, b, ks, c, g), fg = Rows::row_frag(lg, b, ks, c, g);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int row = r0 + 16 * b + 4 * g + e;
-            float x, f = 1.f;
-            if constexpr (GENERAL) x = score.template operator()<DT>(s[b][j][e], row - (key0 + 16 * j + c), &f) - lse[e];
-            else x = __builtin_fmaf(s[b][j][e], score.c1, -lse[e]);
-            float y = __builtin_amdgcn_exp2f(x);
-            if (part) y = row >= from[j] ? y : 0.f;
-            float z = y * (dp[j][e] - delta[e]);
-            if constexpr (GENERAL) z *= f;
-            if (part) z = row >= from[j] ? z : 0.f;
-            p[b][j][e] = DT == TMS_DTYPE_F16 ? y * (float)(1 << kAttnP16) : y;
-            s[b][j][e] = z;
-            if constexpr (DT == TMS_DTYPE_F16) most[j] = fmaxf(most[j], fabsf(z));
+            for (int j = 0; j < NB; j++) {
+              s[i][j] = attn_mfma<DT>(fq, k[j][ks], s[i][j]);
+              dp[j] = attn_mfma<DT>(fg, v[j][ks], dp[j]);
+            }
           }
-      }
-      Frag pf[NB][R / 32], sf[NB][R / 32];
+          if constexpr (KIND == kAttnCap) {
 #pragma unroll
-      for (int j = 0; j < NB; j++) {
-        if constexpr (DT == TMS_DTYPE_F16) {
-          range[j].follow(most[j], dk, j);
+            for (int j = 0; j < NB; j++)
 #pragma unroll
-          for (int b = 0; b < QB; b++)
+              for (int e = 0; e < 4; e++) {
+                float f;
+                s[i][j][e] = score.capped(s[i][j][e], f);
+                dp[j][e] *= f;
+              }
+          }
+          if (score.single()) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[b][j][e] *= range[j].held;
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) s[i][j][e] = score.biased(s[i][j][e], near + (float)(16 * b + e - 16 * j));
+          }
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              const float ref = KIND == kAttnBias ? lse[e] + shift[j] : lse[e];
+              const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][e], score.unit, ref));
+              s[i][j][e] = y * dp[j][e];
+              p[i][j][e] = DT == TMS_DTYPE_F16 ? y * (float)(1 << kAttnP16) : y;
+            }
         }
+        if (part) {
 #pragma unroll
-        for (int h = 0; h < R / 32; h++) {
-          pf[j][h] = attn_pack<DT>(p[2 * h][j], p[2 * h + 1][j]);
-          sf[j][h] = attn_pack<DT>(s[2 * h][j], s[2 * h + 1][j]);
+          for (int i = 0; i < 2; i++)
+#pragma unroll
+            for (int j = 0; j < NB; j++)
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                const bool in = r0 + 32 * h + 16 * i + 4 * g + e >= from[j];
+                p[i][j][e] = in ? p[i][j][e] : 0.f;
+                s[i][j][e] = in ? s[i][j][e] : 0.f;
+              }
         }
-      }
+        Frag pf[NB], sf[NB];
 #pragma unroll
-      for (int h = 0; h < R / 32; h++)
+        for (int j = 0; j < NB; j++) {
+          if constexpr (DT == TMS_DTYPE_F16) range[j].follow(s[0][j], s[1][j], dk, j);
+          pf[j] = attn_pack<DT>(p[0][j], p[1][j]);
+          sf[j] = attn_pack<DT>(s[0][j], s[1][j]);
+        }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           const Frag fg = Rows::col_frag(lg, h, d, c, g), fq = Rows::col_frag(lq, h, d, c, g);
 #pragma unroll
           for (int j = 0; j < NB; j++) {
-            dv[d][j] = attn_mfma<DT>(fg, pf[j][h], dv[d][j]);
-            dk[d][j] = attn_mfma<DT>(fq, sf[j][h], dk[d][j]);
+            dv[d][j] = attn_mfma<DT>(fg, pf[j], dv[d][j]);
+            dk[d][j] = attn_mfma<DT>(fq, sf[j], dk[d][j]);
           }
         }
+      }
     }
   }
 #pragma unroll
@@ -798,10 +1034,39 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     const int key = key0 + 16 * j + c;
     if (key >= t.end) continue;
     const int64_t at = ((int64_t)key * a.KV + kvh) * D;
-    const float fk = !t.real ? 0.f : DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale;
+    const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND>::kSlope;
     const float fv = !t.real ? 0.f : DT == TMS_DTYPE_F16 ? 1.f / (float)(1 << kAttnP16) : 1.f;
+    if (a.parts > 1) {
+      const int64_t one = a.T * a.KV * D;
+      attn_store<TMS_DTYPE_F32>(a.sums + 2 * part_of * one, at, dk, j, fk, g);
+      attn_store<TMS_DTYPE_F32>(a.sums + (2 * part_of + 1) * one, at, dv, j, fv, g);
+      continue;
+    }
     if (a.dk) attn_store<DT>(a.dk, at, dk, j, fk, g);
     if (a.dv) attn_store<DT>(a.dv, at, dv, j, fv, g);
+  }
+}
+
+// dk and dv from the parts' sums, in their order: four elements a thread.
+template <int DT>
+__global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const float* sums, int parts, int64_t n, void* dk, void* dv) {
+  typedef typename AttnType<DT>::E E;
+  struct __attribute__((packed, aligned(4 * sizeof(E)))) Four { E x[4]; };
+  for (int64_t i = (int64_t)blockIdx.x * kAttnThreads + threadIdx.x; i < n / 2; i += (int64_t)gridDim.x * kAttnThreads) {
+    const bool second = i >= n / 4;
+    E* to = (E*)(second ? dv : dk);
+    if (to == nullptr) continue;
+    const int64_t at = (second ? i - n / 4 : i) * 4;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int p = 0; p < parts; p++) {
+      const f32x4 y = *(const f32x4*)(sums + (2 * p + second) * n + at);
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] += y[e];
+    }
+    Four o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) o.x[e] = attn_round<DT>(x[e]);
+    *(Four*)(to + at) = o;
   }
 }
 
@@ -809,25 +1074,27 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
 
 enum AttnPass { kAttnForward = 0, kAttnDq = 1, kAttnDkv = 2 };
 
-static inline int64_t attn_slots(int64_t T, int64_t B, int64_t rows) { return T / rows + B + 2; }
-
-template <int DT, int D, int NB, bool GENERAL>
+template <int DT, int D, int NB, int KIND>
 static int attn_launch(AttnArgs a, AttnPass pass, hipStream_t st) {
   typedef AttnRows<DT, D> Rows;
   a.slots = (int32_t)attn_slots(a.T, a.B, 64 * NB);
-  const int64_t total = (int64_t)a.slots * (pass == kAttnDkv ? a.KV : a.H), grid = (total + 7) / 8 * 8;
+  const int64_t grid = attn_grid(a.slots, pass == kAttnDkv ? a.KV * a.parts : a.H);  // below 2^23
   size_t lds = 4 * (size_t)Rows::kBytes;
   if (pass == kAttnForward) {
-    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, GENERAL>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
+    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
     return check_launch("attn_forward_kernel");
   }
   if (pass == kAttnDq) {
-    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, GENERAL>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
+    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
     return check_launch("attn_dq_kernel");
   }
   lds += 4 * Rows::R * sizeof(float);
-  hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, GENERAL>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
-  return check_launch("attn_dkv_kernel");
+  hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
+  int rc = check_launch("attn_dkv_kernel");
+  if (rc || a.parts == 1) return rc;
+  const int64_t n = a.T * a.KV * D, groups = (n / 2 + kAttnThreads - 1) / kAttnThreads;
+  hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(kAttnThreads), 0, st, a.sums, a.parts, n, a.dk, a.dv);
+  return check_launch("attn_join_kernel");
 }
 
 // One of these for each dtype, in a file of its own.
@@ -835,11 +1102,26 @@ int attn_run_f16(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 int attn_run_bf16(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 int attn_run_f32(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 
+template <int DT, int D, int NB>
+static int attn_run_nb(const AttnArgs& a, AttnPass pass, hipStream_t st) {
+  if (a.cap > 0.f) return attn_launch<DT, D, NB, kAttnCap>(a, pass, st);
+  if (a.slopes) return attn_launch<DT, D, NB, kAttnBias>(a, pass, st);
+  return attn_launch<DT, D, NB, kAttnPlain>(a, pass, st);
+}
 template <int DT, int D>
 static int attn_run_d(const AttnArgs& a, AttnPass pass, hipStream_t st) {
-  constexpr int NB = 1;
-  if (a.cap > 0.f || a.slopes) return attn_launch<DT, D, NB, true>(a, pass, st);
-  return attn_launch<DT, D, NB, false>(a, pass, st);
+  if (a.norms && pass == kAttnForward) {
+    hipLaunchKernelGGL((attn_norms_kernel<DT, D>), dim3((unsigned)((a.H + a.KV) * kAttnNorms)), dim3(kAttnThreads), 0, st, a);
+    const int rc = check_launch("attn_norms_kernel");
+    if (rc) return rc;
+  }
+  if constexpr (DT != TMS_DTYPE_F32) {
+    if (pass != kAttnDkv && attn_wide(a.T, a.B, a.H)) return attn_run_nb<DT, D, 2>(a, pass, st);
+    if constexpr (D < 128) {  // 128 has no registers for two blocks' keys, values and both their gradients
+      if (pass == kAttnDkv && attn_wide(a.T, a.B, (int64_t)a.KV * a.parts)) return attn_run_nb<DT, D, 2>(a, pass, st);
+    }
+  }
+  return attn_run_nb<DT, D, 1>(a, pass, st);
 }
 template <int DT>
 static int attn_run(const AttnArgs& a, int D, AttnPass pass, hipStream_t st) {

@@ -96,4 +96,29 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   return best;
 }
 
+// Attention over packed texts (tms_train_attn_kernel.h). Numbers that tiles of `rows` rows may have: those of
+// B texts, and of what stands before and behind them.
+inline int64_t attn_slots(int64_t T, int64_t B, int64_t rows) { return T / rows + B + 2; }
+
+// Whether a wave takes 32 queries (or keys) and not 16: each row that passes through LDS then serves twice
+// as many, but tiles of 128 rows fill short texts badly, and few of them the chip. 16,384 tokens, 8 heads of
+// 64 in bf16, forward and both backward kernels, 16 / 32: texts of 128 tokens 27, 29, 32 / 35, 38, 44 us; of 512
+// 43, 48, 71 / 44, 48, 55; of 8192 414, 477, 657 / 363, 412, 526; heads of 128, texts of 512: 79, 88 / 62, 73.
+// One text of 2048 tokens: 28, 29, 40 / 36, 42, 50.
+inline bool attn_wide(int64_t T, int64_t B, int64_t heads) { return T >= 512 * B && T / 128 * heads >= 512; }
+
+// Workgroups that share the heads of a tile of keys (a divisor of how many those are), where there are
+// fewer than two a CU without. Their sums, in fp32, are joined by another kernel.
+inline int64_t attn_parts(int64_t T, int64_t B, int64_t kv_heads, int64_t many) {
+  const int64_t groups = attn_slots(T, B, 64) * kv_heads;
+  int64_t parts = (512 + groups - 1) / groups;
+  parts = parts < 1 ? 1 : parts > many ? many : parts;
+  while (many % parts) parts++;
+  return parts;
+}
+
+// Whether keys beyond a bias's reach are looked for: texts so long that they may be, or the norms' kernel (2 x 8192
+// tokens, 12 heads of 64: 10 us) is lost.
+inline bool attn_reaches(int64_t T, int64_t B) { return T >= 512 * B; }
+
 }  // namespace tms
