@@ -29,25 +29,39 @@ enum GatedAct { kSilu = TMS_ACT_SILU, kGelu = TMS_ACT_GELU, kGeluTanh = TMS_ACT_
 // act(g), and with DERIVATIVE its derivative. FINE: for fp32 results.
 //   silu: g s(g), s the logistic function;  gelu: g Phi(g), Phi the normal distribution's function;
 //   gelu_tanh: g s(2 sqrt(2 / pi) (g + 0.044715 g^3)), as (1 + tanh z) / 2 = s(2 z)
-template <bool FINE, bool DERIVATIVE>
-__device__ __forceinline__ float gated_act(int act, float g, float& slope) {
-  if (act == kGelu) {  // uniform
+template <int ACT, bool FINE, bool DERIVATIVE>
+__device__ __forceinline__ float gated_act(float g, float& slope) {
+  if constexpr (ACT == kGelu) {
     const float phi = 0.5f * erfcf(-0.7071067811865476f * g);
     if constexpr (DERIVATIVE) slope = __builtin_fmaf(g, 0.3989422804014327f * expf(-0.5f * g * g), phi);
     return g * phi;
   }
   constexpr float k0 = 1.5957691216057308f, k1 = 0.044715f * 1.5957691216057308f;
-  const float z = act == kSilu ? g : g * __builtin_fmaf(k1, g * g, k0);
+  const float z = ACT == kSilu ? g : g * __builtin_fmaf(k1, g * g, k0);
   float s;
   if constexpr (FINE) s = 1.f / (1.f + expf(-z));
   else s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f));
   const float y = g * s;
   if constexpr (DERIVATIVE) {
-    const float dz = act == kSilu ? 1.f : __builtin_fmaf(3.f * k1, g * g, k0);
-    // s + g s (1 - s) dz; where s is 0 or 1, the second term is 0, also if y dz has overflowed
-    slope = __builtin_fmaf(s == 0.f || s == 1.f ? 0.f : y * dz, 1.f - s, s);
+    const float dz = ACT == kSilu ? 1.f : __builtin_fmaf(3.f * k1, g * g, k0);
+    // s + g s (1 - s) dz; where s is 0 or 1, the second term is 0, also if the square in dz has overflowed
+    if constexpr (ACT == kSilu) slope = __builtin_fmaf(y, 1.f - s, s);
+    else slope = __builtin_fmaf(s == 0.f || s == 1.f ? 0.f : y * dz, 1.f - s, s);
   }
   return y;
+}
+
+template <int A>
+struct ActOf {
+  static constexpr int value = A;
+};
+// f of the activation's type: a branch an epilogue, not one an element, whose code (64 times erfc's) would not stay
+// in the instruction cache (16384 x 1024 x 4096 forward: 292 us so).
+template <class F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  if (act == kSilu) f(ActOf<kSilu>());
+  else if (act == kGelu) f(ActOf<kGelu>());
+  else f(ActOf<kGeluTanh>());
 }
 
 // Eight (four) elements at an element's alignment: rows of an odd F begin anywhere.
@@ -66,6 +80,10 @@ struct GatedEpilogue {
 
   template <int MI, int NI>
   __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t* lds) const {
+    with_act(act, [&](auto a) { finish<decltype(a)::value>(acc, m, n, lds); });
+  }
+  template <int ACT, int MI, int NI>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NI], int m, int n, uint8_t* lds) const {
     static_assert(MI == MIV, "rows of the wave's LDS");
     constexpr bool FINE = OUT == TMS_DTYPE_F32;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
@@ -79,7 +97,7 @@ struct GatedEpilogue {
           const int f = f0 + 16 * p + 4 * g;
           GatedVec<float, 4> y;
 #pragma unroll
-          for (int e = 0; e < 4; e++) y.v[e] = gated_act<FINE, false>(act, acc[2 * p][j][e], none) * acc[2 * p + 1][j][e];
+          for (int e = 0; e < 4; e++) y.v[e] = gated_act<ACT, FINE, false>(acc[2 * p][j][e], none) * acc[2 * p + 1][j][e];
           float* to = (float*)out + (int64_t)row * F + f;
           if (row >= rows) continue;
           if (f + 4 <= F) *(GatedVec<float, 4>*)to = y;
@@ -93,7 +111,7 @@ struct GatedEpilogue {
         for (int p = 0; p < NP; p++) {
           uint16_t y[4];
 #pragma unroll
-          for (int e = 0; e < 4; e++) y[e] = to16<OUT>(gated_act<FINE, false>(act, acc[2 * p][j][e], none) * acc[2 * p + 1][j][e]);
+          for (int e = 0; e < 4; e++) y[e] = to16<OUT>(gated_act<ACT, FINE, false>(acc[2 * p][j][e], none) * acc[2 * p + 1][j][e]);
           *(u32x2*)(lds + c * kRowBytes + p * 32 + g * 8) = u32x2{(uint32_t)y[0] | (uint32_t)y[1] << 16, (uint32_t)y[2] | (uint32_t)y[3] << 16};
         }
         wave_meets();
@@ -131,49 +149,52 @@ struct GatedGradEpilogue {
 
   template <int MI, int NI>
   __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t* lds) const {
+    with_act(act, [&](auto a) { finish<decltype(a)::value>(acc, m, n, lds); });
+  }
+  template <int ACT, int MI, int NI>
+  __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NI], int m, int n, uint8_t* lds) const {
     static_assert(MI == MIV, "rows of the wave's LDS");
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
+    typedef typename std::conditional<(PL > 1), float, uint16_t>::type T;
     float held = 1.f;
     if constexpr (DT == TMS_DTYPE_F16) held = *factor;
-#pragma unroll
-    for (int j = 0; j < NI; j++) {
+    // The dh of the next 16 tokens are on their way while these are used: one by one, their latencies would take
+    // as long as a third of the product.
+    const bool whole = n + 16 * NI <= rows && f0 + 16 * NP <= F;
+    auto load = [&](int j, GatedVec<T, 4>(&to)[NP]) {
       const int row = n + 16 * j + c;
+      const T* from = (const T*)grad + (int64_t)row * F + f0 + 4 * g;
 #pragma unroll
       for (int p = 0; p < NP; p++) {
-        const int f = f0 + 16 * p + 4 * g;
-        float dh[4] = {0.f, 0.f, 0.f, 0.f};
-        if (row < rows) {
-          const int64_t at = (int64_t)row * F + f;
-          if constexpr (PL > 1) {
-            const float* from = (const float*)grad + at;
-            if (f + 4 <= F) {
-              const GatedVec<float, 4> v = *(const GatedVec<float, 4>*)from;
+        if (whole) {
+          to[p] = *(const GatedVec<T, 4>*)(from + 16 * p);
+        } else {
 #pragma unroll
-              for (int e = 0; e < 4; e++) dh[e] = v.v[e];
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; e++) dh[e] = f + e < F ? from[e] : 0.f;
-            }
-          } else {
-            const uint16_t* from = (const uint16_t*)grad + at;
-            if (f + 4 <= F) {
-              const GatedVec<uint16_t, 4> v = *(const GatedVec<uint16_t, 4>*)from;
-#pragma unroll
-              for (int e = 0; e < 4; e++) dh[e] = from16<DT>(v.v[e]);
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; e++) dh[e] = f + e < F ? from16<DT>(from[e]) : 0.f;
-            }
-          }
+          for (int e = 0; e < 4; e++) to[p].v[e] = row < rows && f0 + 16 * p + 4 * g + e < F ? from[16 * p + e] : (T)0;
         }
+      }
+    };
+    GatedVec<T, 4> dhs[2][NP];
+    load(0, dhs[0]);
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      if (j + 1 < NI) load(j + 1, dhs[(j + 1) & 1]);
+#pragma unroll
+      for (int p = 0; p < NP; p++) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          float slope;
-          const float y = gated_act<(PL > 1), true>(act, acc[2 * p][j][e], slope);
-          const float d = dh[e] * held;
-          const bool in = f + e < F;
-          acc[2 * p][j][e] = in ? d * acc[2 * p + 1][j][e] * slope : 0.f;
-          acc[2 * p + 1][j][e] = in ? d * y : 0.f;
+          float d, slope;
+          if constexpr (PL > 1) d = dhs[j & 1][p].v[e];
+          else d = from16<DT>(dhs[j & 1][p].v[e]);
+          if constexpr (DT == TMS_DTYPE_F16) d *= held;
+          const float y = gated_act<ACT, (PL > 1), true>(acc[2 * p][j][e], slope);
+          acc[2 * p][j][e] = d * acc[2 * p + 1][j][e] * slope;
+          acc[2 * p + 1][j][e] = d * y;
+        }
+        if (!whole) {  // columns behind F come from some row of the weights
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+            if (f0 + 16 * p + 4 * g + e >= F) acc[2 * p][j][e] = acc[2 * p + 1][j][e] = 0.f;
         }
       }
 #pragma unroll
@@ -244,6 +265,70 @@ struct GatedRowsEpilogue {
     }
   }
 };
+
+// The same rows as sums of a part of k, [split][row][dp].
+struct GatedSumEpilogue {
+  static constexpr int kRowBytes = 0;
+  float* out;
+  int64_t split;  // elements of one
+  int32_t rows, dp;
+
+  template <int MI, int NI>
+  __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int s, uint8_t*) const {
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < NI; j++) {
+      const int row = n + 16 * j + c;
+      if (row >= rows) continue;
+#pragma unroll
+      for (int i = 0; i < MI; i++) {
+        const int col = m + 16 * i + 4 * g;
+        if (col < dp) *(f32x4*)(out + s * split + (int64_t)row * dp + col) = acc[i][j];
+      }
+    }
+  }
+};
+
+// The splits' sums, in order, as GatedRowsEpilogue finishes rows; four elements a thread.
+template <int OUT>
+__global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int splits, int64_t split, int32_t all, int32_t half, int32_t rows, int32_t d,
+                                                         int32_t dp, const float* factor, void* out, void* out2) {
+  typedef typename std::conditional<OUT == TMS_DTYPE_F32, float, uint16_t>::type T;
+  const int quads = (d + 3) / 4;
+  const int64_t n = (int64_t)all * quads;
+  const float k = factor ? *factor : 1.f;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / quads;
+    const int col = (int)(i - row * quads) * 4;
+    const bool second = row >= half;
+    const int64_t r = second ? row - half : row;
+    T* to = (T*)(second ? out2 : out);
+    if (r >= rows || to == nullptr) continue;
+    const float* from = sums + row * dp + col;
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; s += 4) {
+      f32x4 y[4];
+#pragma unroll
+      for (int v = 0; v < 4; v++) y[v] = s + v < splits ? *(const f32x4*)(from + (s + v) * split) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int v = 0; v < 4; v++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] += y[v][e];
+    }
+    GatedVec<T, 4> o;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if constexpr (OUT == TMS_DTYPE_F32) o.v[e] = x[e] * k;
+      else o.v[e] = to16<OUT>(x[e] * k);
+    }
+    to += r * d + col;
+    if (col + 4 <= d) *(GatedVec<T, 4>*)to = o;
+    else
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (col + e < d) to[e] = o.v[e];
+  }
+}
 
 // The largest |dh| of fp16 (its bits are ordered like its value; NaN above all), a part a workgroup.
 __global__ __launch_bounds__(256) void gated_most_kernel(const uint16_t* x, int64_t n, uint32_t* parts) {
@@ -354,22 +439,25 @@ __global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x
       for (int e = 0; e < 4; e++) gate[e] += a[e], up[e] += b[e];
     }
     if (row >= N) continue;
-    float none;
+    with_act(act, [&](auto a) {
+      float none;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const float y = gated_act<(DT == TMS_DTYPE_F32), false>(act, gate[e], none) * up[e];
-      if (f + e < F) {
-        if constexpr (DT == TMS_DTYPE_F32) ((float*)out)[(int64_t)row * F + f + e] = y;
-        else ((uint16_t*)out)[(int64_t)row * F + f + e] = to16<DT>(y);
+      for (int e = 0; e < 4; e++) {
+        const float y = gated_act<decltype(a)::value, (DT == TMS_DTYPE_F32), false>(gate[e], none) * up[e];
+        if (f + e < F) {
+          if constexpr (DT == TMS_DTYPE_F32) ((float*)out)[(int64_t)row * F + f + e] = y;
+          else ((uint16_t*)out)[(int64_t)row * F + f + e] = to16<DT>(y);
+        }
       }
-    }
+    });
   }
 }
 
 // ---------------------------------------------------------------- host
 
 struct GatedSpace {
-  int64_t x, wg, wu, p, parts, factor, bytes;
+  int64_t x, wg, wu, p, parts, factor, sums, bytes;
+  GemmSplit dx, dw;  // how the gradients' products go
 };
 constexpr int kMostParts = 256;
 
@@ -388,6 +476,11 @@ static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool b
     s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype));
     s.parts = c.take(kMostParts * 4);
     s.factor = c.take(8);
+    const int64_t half = up_to(F, 64);
+    s.dx = gemm_split(dp, N, 2 * half, planes(dtype));
+    s.dw = gemm_split(dp, 2 * half, N, planes(dtype));
+    const int64_t one = s.dx.splits > 1 ? s.dx.splits * N : 0, other = s.dw.splits > 1 ? s.dw.splits * 2 * half : 0;
+    s.sums = c.take((one > other ? one : other) * dp * 4);  // one product after the other
   }
   s.bytes = c.at;
   return s;
@@ -415,15 +508,35 @@ static int check_gated(const char* fn, const void* x, int64_t N, int64_t d, cons
 struct GatedOperands {
   const uint16_t *x, *wg, *wu;
 };
+// x and both weights as rows of terms, in one launch.
+struct GatedTerms {
+  const void* src[3];
+  uint16_t* dst[3];
+  int64_t rows[3];
+};
+template <bool F32>
+__global__ __launch_bounds__(256) void gated_terms_kernel(GatedTerms t, int32_t d, int32_t dp) {
+  const int which = blockIdx.y;
+  const bool whole = d == dp && (uintptr_t)t.src[which] % 16 == 0;
+  const int eights = dp / 8;
+  const int64_t n = t.rows[which] * eights;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int64_t row = k / eights;
+    terms_of_eight<F32>(t.src[which], t.dst[which], k, row, (int)(k - row * eights) * 8, d, t.rows[which] * dp, whole, true);
+  }
+}
 static int gated_operands(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, uint8_t* ws, const GatedSpace& s,
                           GatedOperands& o, hipStream_t st) {
   o = {(const uint16_t*)x, (const uint16_t*)wg, (const uint16_t*)wu};
   if (dtype != TMS_DTYPE_F32 && d % 8 == 0) return TMS_OK;
   const int64_t dp = up_to(d, 8);
-  o = {(const uint16_t*)(ws + s.x), (const uint16_t*)(ws + s.wg), (const uint16_t*)(ws + s.wu)};
-  int rc = run_terms(x, dtype, ws + s.x, N, d, dp, nullptr, st);
-  if (rc || (rc = run_terms(wg, dtype, ws + s.wg, F, d, dp, nullptr, st))) return rc;
-  return run_terms(wu, dtype, ws + s.wu, F, d, dp, nullptr, st);
+  uint16_t *px = (uint16_t*)(ws + s.x), *pg = (uint16_t*)(ws + s.wg), *pu = (uint16_t*)(ws + s.wu);
+  o = {px, pg, pu};
+  const GatedTerms t = {{x, wg, wu}, {px, pg, pu}, {N, F, F}};
+  const dim3 grid(blocks_for((N > F ? N : F) * dp / 8), 3);
+  if (dtype == TMS_DTYPE_F32) hipLaunchKernelGGL(gated_terms_kernel<true>, grid, dim3(256), 0, st, t, (int32_t)d, (int32_t)dp);
+  else hipLaunchKernelGGL(gated_terms_kernel<false>, grid, dim3(256), 0, st, t, (int32_t)d, (int32_t)dp);
+  return check_launch("gated_terms_kernel");
 }
 
 // g and u: m over rows of Wg and Wu in turn, n over tokens.
@@ -469,6 +582,23 @@ static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, co
   });
 }
 
+// A product to rows of d elements, at once or in splits.
+template <int DT, int PL, int OUT, bool BO, int PAIR>
+static int gated_rows(GemmArgs b, GemmSplit plan, int64_t all, int64_t half, int64_t rows, int64_t d, int64_t dp, const float* factor, float* sums, void* out,
+                      void* out2, const char* what, hipStream_t st) {
+  b.splits = plan.splits;
+  if (plan.splits == 1) {
+    const GatedRowsEpilogue<OUT> e = {out, out2, factor, (int32_t)rows, (int32_t)half, (int32_t)d};
+    return with_size<PL>(plan.size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, BO, PAIR>(b, e, st, what); });
+  }
+  const GatedSumEpilogue e = {sums, all * dp, (int32_t)all, (int32_t)dp};
+  const int rc = with_size<PL>(plan.size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, BO, PAIR>(b, e, st, what); });
+  if (rc) return rc;
+  hipLaunchKernelGGL(gated_join_kernel<OUT>, dim3(blocks_for(all * ((d + 3) / 4))), dim3(256), 0, st, sums, plan.splits, all * dp, (int32_t)all,
+                     (int32_t)half, (int32_t)rows, (int32_t)d, (int32_t)dp, factor, out, out2);
+  return check_launch("gated_join_kernel");
+}
+
 template <int DT, int PL, int OUT>
 static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, const void* grad, uint8_t* ws,
                           const GatedSpace& s, void* dx, void* dwg, void* dwu, hipStream_t st) {
@@ -508,11 +638,7 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.N = (int32_t)N;
     b.half = (int32_t)half;
     b.real = (int32_t)F;
-    b.splits = 1;
-    const GatedRowsEpilogue<OUT> e = {dx, nullptr, back, (int32_t)N, 0x7fffffff, (int32_t)d};
-    rc = with_size<PL>(gemm_size(dp, N, gemm_steps(2 * half, PL), gemm_largest(PL)), [&](auto z) {
-      return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, false, kPairDepth>(b, e, st, "train_gemm_kernel (dx)");
-    });
+    rc = gated_rows<DT, PL, OUT, false, kPairDepth>(b, s.dx, N, 0x7fffffff, N, d, dp, back, (float*)(ws + s.sums), dx, nullptr, "train_gemm_kernel (dx)", st);
     if (rc) return rc;
   }
   if (dwg || dwu) {  // m over d, n over F columns of dg and du, k over tokens
@@ -525,11 +651,7 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.ldb = b.N = (int32_t)(2 * half);
     b.M = (int32_t)dp;
     b.K = (int32_t)N;
-    b.splits = 1;
-    const GatedRowsEpilogue<OUT> e = {dwg, dwu, back, (int32_t)F, (int32_t)half, (int32_t)d};
-    rc = with_size<PL>(gemm_size(dp, 2 * half, gemm_steps(N, PL), gemm_largest(PL)), [&](auto z) {
-      return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, true>(b, e, st, "train_gemm_kernel (dWg, dWu)");
-    });
+    rc = gated_rows<DT, PL, OUT, true, kSingle>(b, s.dw, 2 * half, half, F, d, dp, back, (float*)(ws + s.sums), dwg, dwu, "train_gemm_kernel (dWg, dWu)", st);
   }
   return rc;
 }

@@ -96,6 +96,27 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   return best;
 }
 
+// Tiles and splits of k of a product of m x n whose sums go to 16 bits at once, or through fp32 and another kernel where that
+// is shorter: splits fill the chip where tiles are few. A split's sums are written and read at about 4 TB/s, and the
+// second kernel takes 4 us. (500 x 256 over 1408 in three terms: 53 us whole, 17 in eight splits.)
+struct GemmSplit {
+  int size, splits;
+};
+inline GemmSplit gemm_split(int64_t m, int64_t n, int64_t k, int planes) {
+  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
+  const int64_t steps = gemm_steps(k, planes);
+  GemmSplit best = {};
+  double least = 1e30;
+  for (int s : kSplits) {
+    if (s > 1 && s * 2 > up_to(k, 64) / 64) break;
+    for (int size = gemm_largest(planes); size < kGemmSizes; size++) {
+      const double us = gemm_us(size, m, n, steps, s) + (s > 1 ? (double)s * (double)m * (double)n * 8 / 4e6 + 4.0 : 0.0);
+      if (us < least) least = us, best = {size, s};
+    }
+  }
+  return best;
+}
+
 // Attention over packed texts (tms_train_attn_kernel.h). Numbers that tiles of `rows` rows may have: those of
 // B texts, and of what stands before and behind them.
 inline int64_t attn_slots(int64_t T, int64_t B, int64_t rows) { return T / rows + B + 2; }

@@ -27,10 +27,49 @@ __device__ __forceinline__ float from16(uint16_t x) {
   return __builtin_bit_cast(float, (uint32_t)x << 16);
 }
 
-// Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms: three of
-// a float, 16-bit elements as they are; eight a thread. With `ref`, rows without a gradient
-// become zeros: what stands in them (NaN included) takes no part. 8000 rows of 256 floats: 5 us,
-// bound by the launch.
+// Eight elements from column c of a row of d as 16-bit terms (three of a float, 16-bit elements as they
+// are), zeros behind d; piece k of the output. `whole`: rows of whole 16-byte pieces. Not `on`: zeros.
+template <bool F32>
+__device__ __forceinline__ void terms_of_eight(const void* src, uint16_t* dst, int64_t k, int64_t row, int c, int32_t d, int64_t plane, bool whole, bool on) {
+  const int64_t at = row * d + c;
+  if constexpr (F32) {
+    float x[8];
+    if (whole) {
+      const f32x4 lo = ((const f32x4*)((const float*)src + at))[0], hi = ((const f32x4*)((const float*)src + at))[1];
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] = on ? lo[e] : 0.f, x[4 + e] = on ? hi[e] : 0.f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) x[e] = on && c + e < d ? ((const float*)src)[at + e] : 0.f;
+    }
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+      u32x4 out;
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const __bf16 t = (__bf16)x[e];
+        const uint32_t bits = __builtin_bit_cast(uint16_t, t);
+        out[e / 2] = e % 2 ? out[e / 2] | bits << 16 : bits;
+        x[e] -= (float)t;
+      }
+      *(u32x4*)(dst + p * plane + k * 8) = out;
+    }
+  } else {
+    u32x4 out = {0u, 0u, 0u, 0u};
+    if (on && whole) {
+      out = *(const u32x4*)((const uint16_t*)src + at);
+    } else if (on) {
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (c + e < d) out[e / 2] |= (uint32_t)((const uint16_t*)src)[at + e] << (16 * (e % 2));
+    }
+    *(u32x4*)(dst + k * 8) = out;
+  }
+}
+
+// Rows of d elements as rows of dp (a multiple of 8, zeros behind d) of 16-bit terms, eight a thread.
+// With `ref`, rows without a gradient become zeros: what stands in them (NaN included) takes no part.
+// 8000 rows of 256 floats: 5 us, bound by the launch.
 template <bool F32>
 __global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, uint16_t* dst, int64_t rows, int32_t d, int32_t dp, int64_t plane,
                                                         const float* ref) {
@@ -39,42 +78,7 @@ __global__ __launch_bounds__(256) void lce_terms_kernel(const void* src, uint16_
   const bool whole = d == dp && (uintptr_t)src % 16 == 0;  // pieces of eight in 16-byte loads (d = 0: dp = 8, nothing to load)
   for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
     const int64_t row = n >> 32 ? k / eights : (int64_t)((uint32_t)k / eights);
-    const int c = (int)(k - row * eights) * 8;
-    const bool on = !ref || ref[row] != __builtin_inff();
-    const int64_t at = row * d + c;
-    if constexpr (F32) {
-      float x[8];
-      if (whole) {
-        const f32x4 lo = ((const f32x4*)((const float*)src + at))[0], hi = ((const f32x4*)((const float*)src + at))[1];
-#pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = on ? lo[e] : 0.f, x[4 + e] = on ? hi[e] : 0.f;
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = on && c + e < d ? ((const float*)src)[at + e] : 0.f;
-      }
-#pragma unroll
-      for (int p = 0; p < 3; p++) {
-        u32x4 out;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-          const __bf16 t = (__bf16)x[e];
-          const uint32_t bits = __builtin_bit_cast(uint16_t, t);
-          out[e / 2] = e % 2 ? out[e / 2] | bits << 16 : bits;
-          x[e] -= (float)t;
-        }
-        *(u32x4*)(dst + p * plane + k * 8) = out;
-      }
-    } else {
-      u32x4 out = {0u, 0u, 0u, 0u};
-      if (on && whole) {
-        out = *(const u32x4*)((const uint16_t*)src + at);
-      } else if (on) {
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (c + e < d) out[e / 2] |= (uint32_t)((const uint16_t*)src)[at + e] << (16 * (e % 2));
-      }
-      *(u32x4*)(dst + k * 8) = out;
-    }
+    terms_of_eight<F32>(src, dst, k, row, (int)(k - row * eights) * 8, d, plane, whole, !ref || ref[row] != __builtin_inff());
   }
 }
 
