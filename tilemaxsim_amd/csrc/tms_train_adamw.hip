@@ -8,7 +8,7 @@
 // written and g read once, and what a 16-bit model reads of p is written in the same pass.
 //
 // The tensor list goes in the kernel arguments, kAdamTensors of them a launch, and a workgroup takes whole
-// chunks of kAdamChunk elements, as gradient clipping does. A first small kernel counts the
+// chunks of them, as gradient clipping does. A first small kernel counts the
 // steps and leaves each tensor's factors, which need powers in 64 bits.
 //
 // States of all tensors stand in flat buffers, each tensor's at a multiple of 128 elements. In
@@ -32,10 +32,16 @@ namespace tms {
 
 constexpr int kAdamTensors = 64;
 constexpr int kAdamThreads = 256;
-constexpr int kAdamVec = 8;
-constexpr int kAdamBlock = TMS_ADAMW_BLOCK;  // elements that share an exponent: 16 lanes of eight
-constexpr int kAdamRounds = 4;
-constexpr int kAdamChunk = kAdamThreads * kAdamVec * kAdamRounds;  // 8,192
+constexpr int kAdamBlock = TMS_ADAMW_BLOCK;  // elements that share an exponent
+// Elements a thread takes at once: with fp32 states four, so that a wave's accesses are whole lines (336 M parameters:
+// 1,815 us, 5.19 TB/s; with eight, in halves of lines, 1,890); with 8-bit ones eight, which share more of a
+// block's work (109 M with bf16 gradients and copies: 380 us, 400 with four).
+template <bool SMALL>
+constexpr int kAdamVec = SMALL ? 8 : 4;
+// Elements that a workgroup takes at a time, or 2,048 where those would be fewer than four workgroups a CU
+// (98,432 elements, a projection head: 10 us in chunks of 8,192, 5 in smaller ones).
+constexpr int kAdamChunk = 8192, kAdamSmallChunk = 2048;
+constexpr int64_t kAdamFewChunks = 1024;
 
 struct AdamTensor {
   void* p;
@@ -49,7 +55,7 @@ struct AdamTensor {
 };
 struct AdamTable {
   AdamTensor t[kAdamTensors];
-  int32_t count, chunks;
+  int32_t count, chunks, chunk;  // chunk: elements of one
 };
 static_assert(sizeof(AdamTable) <= 3600, "kernel arguments");
 
@@ -116,46 +122,48 @@ template <>
 struct AdamElem<TMS_DTYPE_BF16> {
   typedef __bf16 T;
 };
-template <class T>
-struct __attribute__((packed, aligned(sizeof(T)))) AdamVec {  // eight elements at an element's alignment
-  T v[kAdamVec];
+template <class T, int N>
+struct __attribute__((packed, aligned(sizeof(T)))) AdamVec {  // N elements at an element's alignment
+  T v[N];
 };
 
-// Eight elements (or the `here` first of them) from `at` on.
-template <int DT>
-__device__ __forceinline__ void adam_get(const void* p, int64_t at, int here, float (&x)[kAdamVec]) {
+// N elements (or the `here` first of them) from `at` on.
+template <int DT, int N>
+__device__ __forceinline__ void adam_get(const void* p, int64_t at, int here, float (&x)[N]) {
   typedef typename AdamElem<DT>::T T;
   const T* from = (const T*)p + at;
-  if (here == kAdamVec) {
-    const AdamVec<T> v = *(const AdamVec<T>*)from;
+  if (here == N) {
+    const AdamVec<T, N> v = *(const AdamVec<T, N>*)from;
 #pragma unroll
-    for (int i = 0; i < kAdamVec; i++) x[i] = (float)v.v[i];
+    for (int i = 0; i < N; i++) x[i] = (float)v.v[i];
   } else {
 #pragma unroll
-    for (int i = 0; i < kAdamVec; i++) x[i] = i < here ? (float)from[i] : 0.f;
+    for (int i = 0; i < N; i++) x[i] = i < here ? (float)from[i] : 0.f;
   }
 }
-template <int DT>
-__device__ __forceinline__ void adam_put(void* p, int64_t at, int here, const float (&x)[kAdamVec]) {
+template <int DT, int N>
+__device__ __forceinline__ void adam_put(void* p, int64_t at, int here, const float (&x)[N]) {
   typedef typename AdamElem<DT>::T T;
   T* to = (T*)p + at;
-  if (here == kAdamVec) {
-    AdamVec<T> v;
+  if (here == N) {
+    AdamVec<T, N> v;
 #pragma unroll
-    for (int i = 0; i < kAdamVec; i++) v.v[i] = (T)x[i];
-    *(AdamVec<T>*)to = v;
+    for (int i = 0; i < N; i++) v.v[i] = (T)x[i];
+    *(AdamVec<T, N>*)to = v;
   } else {
 #pragma unroll
-    for (int i = 0; i < kAdamVec; i++)
+    for (int i = 0; i < N; i++)
       if (i < here) to[i] = (T)x[i];
   }
 }
-__device__ __forceinline__ void adam_get_typed(int dt, const void* p, int64_t at, int here, float (&x)[kAdamVec]) {
+template <int N>
+__device__ __forceinline__ void adam_get_typed(int dt, const void* p, int64_t at, int here, float (&x)[N]) {
   if (dt == TMS_DTYPE_F32) adam_get<TMS_DTYPE_F32>(p, at, here, x);
   else if (dt == TMS_DTYPE_F16) adam_get<TMS_DTYPE_F16>(p, at, here, x);
   else adam_get<TMS_DTYPE_BF16>(p, at, here, x);
 }
-__device__ __forceinline__ void adam_put_typed(int dt, void* p, int64_t at, int here, const float (&x)[kAdamVec]) {
+template <int N>
+__device__ __forceinline__ void adam_put_typed(int dt, void* p, int64_t at, int here, const float (&x)[N]) {
   if (dt == TMS_DTYPE_F32) adam_put<TMS_DTYPE_F32>(p, at, here, x);
   else if (dt == TMS_DTYPE_F16) adam_put<TMS_DTYPE_F16>(p, at, here, x);
   else adam_put<TMS_DTYPE_BF16>(p, at, here, x);
@@ -198,23 +206,27 @@ __device__ __forceinline__ uint32_t adam_encode(float x, int exp, uint32_t dithe
   return (uint32_t)c;
 }
 
-// The largest of 16 lanes' numbers, in all of them.
-__device__ __forceinline__ uint32_t adam_row_max(uint32_t x) {
+// The exponent of the largest finite |x| of a block: of eight in each of 16 lanes, which all get it.
+__device__ __forceinline__ int adam_block_exp(const float (&v)[8]) {
+  uint32_t x = 0;
   auto up = [&](uint32_t y) { x = y > x ? y : x; };
+#pragma unroll
+  for (int i = 0; i < 8; i++) {
+    const uint32_t a = __builtin_bit_cast(uint32_t, v[i]) & 0x7fffffffu;
+    up(a < 0x7f800000u ? a : 0u);
+  }
   up((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xB1, 0xf, 0xf, true));   // lane ^ 1
   up((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4E, 0xf, 0xf, true));   // lane ^ 2
   up((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x141, 0xf, 0xf, true));  // the other quad of each half
   up((uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x140, 0xf, 0xf, true));  // the other half
-  return x;
+  return (int)(x >> 23);
 }
-__device__ __forceinline__ int adam_block_exp(const float (&x)[kAdamVec]) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int i = 0; i < kAdamVec; i++) {
-    const uint32_t a = __builtin_bit_cast(uint32_t, x[i]) & 0x7fffffffu;
-    most = a < 0x7f800000u && a > most ? a : most;
-  }
-  return (int)(adam_row_max(most) >> 23);
+
+// The root to 2^-23 of it (the correctly rounded one, and a division in the place of the reciprocal below, would
+// take as many instructions as the rest of a step); the instruction takes no subnormal numbers.
+__device__ __forceinline__ float adam_root(float x) {
+  const bool low = x < 0x1p-96f;
+  return __builtin_amdgcn_sqrtf(low ? x * 0x1p64f : x) * (low ? 0x1p-32f : 1.f);
 }
 
 // ---------------------------------------------------------------- the step
@@ -222,6 +234,7 @@ __device__ __forceinline__ int adam_block_exp(const float (&x)[kAdamVec]) {
 template <bool SMALL>
 __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab, AdamArgs a) {
 #pragma clang fp contract(off)
+  constexpr int N = kAdamVec<SMALL>;
   float c = 1.f;
   if (a.norm) {
     c = a.max_norm / (*a.norm + 1e-6f);
@@ -237,15 +250,14 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab,
     const AdamTensor& t = tab.t[lo];
     const AdamFactors f = a.factors[t.index];
     const int tp = t.types & 0xff, tg = t.types >> 8 & 0xff, tc = t.types >> 16;
-    const int64_t begin = (int64_t)(chunk - t.first) * kAdamChunk;
-#pragma unroll
-    for (int r = 0; r < kAdamRounds; r++) {
-      const int64_t at = begin + (r * kAdamThreads + (int)threadIdx.x) * kAdamVec, in = t.at + at;
+    const int64_t begin = (int64_t)(chunk - t.first) * tab.chunk;
+    for (int r = (int)threadIdx.x * N; r < tab.chunk; r += kAdamThreads * N) {
+      const int64_t at = begin + r, in = t.at + at;
       const int64_t left = t.n - at;
       // whole blocks of states exist behind a tensor's end: lanes there keep to the exchange below
       if (left + kAdamBlock <= 0) break;
-      const int here = left >= kAdamVec ? kAdamVec : left > 0 ? (int)left : 0;
-      float p[kAdamVec], g[kAdamVec], m[kAdamVec], v[kAdamVec];
+      const int here = left >= N ? N : left > 0 ? (int)left : 0;
+      float p[N], g[N], m[N], v[N];
       adam_get_typed(tp, t.p, at, here, p);
       adam_get_typed(tg, t.g, at, here, g);
       if constexpr (SMALL) {
@@ -258,7 +270,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab,
           ev = a.v_exp[in / kAdamBlock];
         }
 #pragma unroll
-        for (int i = 0; i < kAdamVec; i++) {
+        for (int i = 0; i < N; i++) {
           m[i] = adam_decode<127>(cm[i / 4] >> (8 * (i % 4)) & 0xffu, em);
           v[i] = adam_decode<255>(cv[i / 4] >> (8 * (i % 4)) & 0xffu, ev);
         }
@@ -267,11 +279,11 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab,
         adam_get<TMS_DTYPE_F32>(a.v, in, here, v);
       }
 #pragma unroll
-      for (int i = 0; i < kAdamVec; i++) {
+      for (int i = 0; i < N; i++) {
         const float x = g[i] * c;
         m[i] = a.b1 * m[i] + a.n1 * x;
         v[i] = a.b2 * v[i] + a.n2 * x * x;
-        p[i] = f.keep * p[i] - f.step * m[i] / (sqrtf(v[i]) * f.root + a.eps);
+        p[i] = f.keep * p[i] - f.step * m[i] * __builtin_amdgcn_rcpf(adam_root(v[i]) * f.root + a.eps);
         if (i >= here) m[i] = v[i] = 0.f;
       }
       if (here > 0) {
@@ -283,7 +295,7 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab,
         const uint32_t key = adam_mix(f.key + (uint32_t)(in >> 32) * 0x9e3779b1u);
         u32x2 cm = {0u, 0u}, cv = {0u, 0u};
 #pragma unroll
-        for (int i = 0; i < kAdamVec; i++) {
+        for (int i = 0; i < N; i++) {
           const uint32_t mixed = adam_mix((uint32_t)(in + i) ^ key);
           cm[i / 4] |= adam_encode<127>(m[i], em, mixed & 0xffffu) << (8 * (i % 4));
           cv[i / 4] |= adam_encode<255>(v[i], ev, mixed >> 16) << (8 * (i % 4));
@@ -304,23 +316,20 @@ __global__ __launch_bounds__(kAdamThreads) void adamw_step_kernel(AdamTable tab,
   }
 }
 
-// The numbers that 8-bit states stand for: eight a thread.
+// The numbers that 8-bit states stand for: four a thread, whole lines a store.
 __global__ __launch_bounds__(256) void adamw_decode_kernel(const uint8_t* m, const uint8_t* m_exp, const uint8_t* v, const uint8_t* v_exp, int64_t n,
                                                            float* mean, float* square) {
-  for (int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8; k < n; k += (int64_t)gridDim.x * 2048) {
-    const u32x2 cm = *(const u32x2*)(m + k), cv = *(const u32x2*)(v + k);
+  for (int64_t k = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; k < n; k += (int64_t)gridDim.x * 1024) {
+    const uint32_t cm = *(const uint32_t*)(m + k), cv = *(const uint32_t*)(v + k);
     const int em = m_exp[k / kAdamBlock], ev = v_exp[k / kAdamBlock];
-    f32x4 x[2], y[2];
+    f32x4 x, y;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-      x[i / 4][i % 4] = adam_decode<127>(cm[i / 4] >> (8 * (i % 4)) & 0xffu, em);
-      y[i / 4][i % 4] = adam_decode<255>(cv[i / 4] >> (8 * (i % 4)) & 0xffu, ev);
+    for (int i = 0; i < 4; i++) {
+      x[i] = adam_decode<127>(cm >> (8 * i) & 0xffu, em);
+      y[i] = adam_decode<255>(cv >> (8 * i) & 0xffu, ev);
     }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-      *(f32x4*)(mean + k + 4 * h) = x[h];
-      *(f32x4*)(square + k + 4 * h) = y[h];
-    }
+    *(f32x4*)(mean + k) = x;
+    *(f32x4*)(square + k) = y;
   }
 }
 
@@ -355,7 +364,7 @@ static int check_adamw(const char* fn, const tms_adamw_tensor* tensors, int64_t 
     end = t.at + (t.n + kAdamBlock - 1) / kAdamBlock * kAdamBlock;
     if (i % kAdamTensors == 0) chunks = 0;
     if (t.n > ((int64_t)1 << 43)) return fail(TMS_ERR_UNSUPPORTED, "%s: tensor %lld is too large", fn, (long long)i);
-    chunks += (t.n + kAdamChunk - 1) / kAdamChunk;
+    chunks += (t.n + kAdamSmallChunk - 1) / kAdamSmallChunk;
     if (chunks > 0x7fffffff) return fail(TMS_ERR_UNSUPPORTED, "%s: tensor %lld is too large", fn, (long long)i);
   }
   if (end > s->size) return fail(TMS_ERR_INVALID, "%s: the last tensor's block of states ends behind them", fn);
@@ -401,8 +410,12 @@ extern "C" int tms_adamw_step(const tms_adamw_tensor* tensors, int64_t count, co
   a.b1 = (float)state->beta1, a.n1 = (float)(1 - state->beta1);
   a.b2 = (float)state->beta2, a.n2 = (float)(1 - state->beta2);
   a.eps = (float)state->eps;
+  int64_t all = 0;
+  for (int64_t i = 0; i < count; i++) all += (tensors[i].n + kAdamChunk - 1) / kAdamChunk;
+  AdamTable tab;
+  tab.chunk = all < kAdamFewChunks ? kAdamSmallChunk : kAdamChunk;
+  const int64_t chunk = tab.chunk;
   for (int64_t i = 0; i < count;) {
-    AdamTable tab;
     tab.count = 0;
     int64_t chunks = 0;
     const int64_t end = i + kAdamTensors < count ? i + kAdamTensors : count;
@@ -410,7 +423,7 @@ extern "C" int tms_adamw_step(const tms_adamw_tensor* tensors, int64_t count, co
       const tms_adamw_tensor& t = tensors[i];
       if (t.n == 0) continue;
       tab.t[tab.count++] = {t.p, t.g, t.copy, t.n, t.at, (int32_t)chunks, t.index, t.p_dtype | t.g_dtype << 8 | t.copy_dtype << 16};
-      chunks += (t.n + kAdamChunk - 1) / kAdamChunk;
+      chunks += (t.n + chunk - 1) / chunk;
     }
     tab.chunks = (int32_t)chunks;
     if (chunks == 0) continue;
@@ -429,8 +442,8 @@ extern "C" int tms_adamw_moments(const uint8_t* m, const uint8_t* m_exp, const u
   if (size == 0) return TMS_OK;
   if (!m || !m_exp || !v || !v_exp || !mean || !square) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
   if (((uintptr_t)m | (uintptr_t)v | (uintptr_t)mean | (uintptr_t)square) % 16) return fail(TMS_ERR_INVALID, "%s: tensors must be 16-byte aligned", fn);
-  const int64_t groups = (size / 8 + 255) / 256;
-  hipLaunchKernelGGL(adamw_decode_kernel, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(256), 0, (hipStream_t)stream, m, m_exp, v, v_exp, size,
+  const int64_t groups = (size / 4 + 255) / 256;
+  hipLaunchKernelGGL(adamw_decode_kernel, dim3((unsigned)(groups < (1 << 20) ? groups : (1 << 20))), dim3(256), 0, (hipStream_t)stream, m, m_exp, v, v_exp, size,
                      mean, square);
   return check_launch("adamw_decode_kernel");
 }
