@@ -83,9 +83,6 @@ def _checked(fn: str, x, w_gate, w_up) -> None:
     _check.embedding_dtype("x", x)
     if w_gate.dtype != x.dtype or w_up.dtype != x.dtype:
         raise TypeError(f"{fn}: x is {x.dtype}, w_gate is {w_gate.dtype}, w_up is {w_up.dtype}")
-    for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up)):
-        _check.on_gpu(name, t)
-    _check.same_device(x=x, w_gate=w_gate, w_up=w_up)
 
 
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, activation: str = "silu") -> torch.Tensor:
@@ -104,12 +101,17 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
     inputs' type (float32: three bf16 terms) before the products that they go into.
     """
     fn = "gated_linear"
-    if not _usual(x, w_gate, w_up):
+    usual = _usual(x, w_gate, w_up)
+    if not usual:
         _checked(fn, x, w_gate, w_up)
     _check.no_tangents(fn, (x, w_gate, w_up))
     act = _ACTIVATIONS.get(activation)
     if act is None:
         raise ValueError(f"{fn}: activation must be one of {', '.join(_ACTIVATIONS)} (got {activation!r})")
+    if not usual:
+        for name, t in (("x", x), ("w_gate", w_gate), ("w_up", w_up)):
+            _check.on_gpu(name, t)
+        _check.same_device(x=x, w_gate=w_gate, w_up=w_up)
     flat = x.dim() == 2
     rows = _check.aligned(x if flat else x.reshape(x.numel() // x.shape[-1], x.shape[-1]))
     wg, wu = _check.aligned(w_gate), _check.aligned(w_up)
