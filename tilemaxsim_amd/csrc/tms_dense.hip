@@ -182,7 +182,7 @@ void keep_error(char* to, int n) { snprintf(to, (size_t)n, "%s", g_err); }
 
 extern "C" {
 
-int tms_version(void) { return 101; }
+int tms_version(void) { return 102; }
 
 const char* tms_last_error(void) { return tms::g_err; }
 
