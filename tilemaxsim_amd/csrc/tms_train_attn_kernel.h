@@ -49,7 +49,6 @@ typedef _Float16 attn_f16x2 __attribute__((ext_vector_type(2)));
 constexpr int kAttnThreads = 256;
 constexpr float kAttnLog2e = 1.4426950408889634f;
 constexpr float kAttnNothing = 160.f;  // so many powers of two below, exp2 is 0
-constexpr float kAttnSlack = 8.f;  // powers of two that P may stand above its reference in the forward pass
 constexpr int kAttnP16 = 15;  // fp16: P times 2^15 in the backward pass
 
 constexpr int kAttnNorms = 64;  // numbers a head
@@ -566,8 +565,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
 #pragma unroll
             for (int e = 0; e < 4; e++) s[b][j][e] = k0 + 16 * b + 4 * g + e < sees[j] ? s[b][j][e] : NEG;
       }
-      // A row's reference follows its maximum when that has left it by kAttnSlack: not at every tile of a bias
-      // that favours what comes next.
+      // A row's reference is its maximum so far, so that its largest P is 1 and not rounded: rows that look at few keys
+      // have their error from the others.
       float m[NB], shift[NB];
       bool over = false, some = false;
 #pragma unroll
@@ -579,7 +578,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
           for (int e = 0; e < 4; e += 2) m[j] = attn_max(attn_max(s[b][j][e], s[b][j][e + 1]), m[j]);
         shift[j] = score.shift(row0 + 16 * j + c, k0);
         m[j] = __builtin_fmaf(attn_cross_max(m[j]), score.unit, shift[j]);
-        over |= m[j] > top[j] + kAttnSlack;
+        over |= m[j] > top[j];
         some |= !(m[j] < top[j] - kAttnNothing);
       }
       if (__ballot(some) == 0ull) continue;  // every P of the tile is 0, as far behind as it is by its bias
@@ -694,8 +693,11 @@ __device__ __forceinline__ void attn_store(void* out, int64_t at, const f32x4 (&
   }
 }
 
-// delta and dq: a workgroup has a tile of queries and goes over their keys.
-template <int DT, int D, int NB, int KIND>
+// delta and dq: a workgroup has a tile of queries and goes over their keys. SHORT: texts of one tile of keys
+// have their delta from P and dP, before dS is formed: where few keys share a row, o's own error (P is
+// rounded there) would be as large as that of dS's rounding. (For all: 128 documents of 32 to 300 tokens take 70 us
+// and not 62.)
+template <int DT, int D, int NB, int KIND, bool SHORT>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   typedef AttnRows<DT, D> Rows;
   typedef typename AttnType<DT>::E E;
@@ -726,6 +728,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
     Frag q[NB][KS], go[NB][KS];
     int sees[NB];
     float lse[NB], delta[NB];
+    const bool alone = SHORT && t.end - t.begin <= R;  // all keys in one tile
 #pragma unroll
     for (int j = 0; j < NB; j++) {
       const int row = row0 + 16 * j + c, in = row < t.end ? row : t.end - 1;
@@ -734,6 +737,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       attn_own<DT, D>((const E*)a.grad, at, g, go[j]);
       lse[j] = a.lse[(int64_t)head * a.T + in];
       sees[j] = in + 1 > t.prefix_end ? in + 1 : t.prefix_end;
+      delta[j] = 0.f;
+      if (alone) continue;
       Frag o[KS], low[KS];
       attn_own<DT, D>((const E*)a.out, at, g, o);
       if constexpr (DT != TMS_DTYPE_F32) attn_own<DT, D>((const E*)a.low, at, g, low);
@@ -785,47 +790,74 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       for (int j = 0; j < NB; j++) ref[j] = score.shift(row0 + 16 * j + c, k0) - lse[j];
       const bool part = k0 + R > least;
       const float near = (float)(row0 + c - k0 - 4 * g);
+      // Block b of the tile: P (p) and dP less delta (dp), under a cap times its slope if `sloped`.
+      auto block = [&](int b, bool sloped, f32x4(&p)[NB], f32x4(&dp)[NB]) {
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+          p[j] = score.start(b);
+          dp[j] = f32x4{-delta[j], -delta[j], -delta[j], -delta[j]};
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+          const Frag fk = Rows::row_frag(lk, b, ks, c, g), fv = Rows::row_frag(lv, b, ks, c, g);
+#pragma unroll
+          for (int j = 0; j < NB; j++) {
+            p[j] = attn_mfma<DT>(fk, q[j][ks], p[j]);
+            dp[j] = attn_mfma<DT>(fv, go[j][ks], dp[j]);
+          }
+        }
+        if constexpr (KIND == kAttnCap) {
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              float f;
+              p[j][e] = score.capped(p[j][e], f);
+              if (sloped) dp[j][e] *= f;
+            }
+        }
+        if (score.single()) {
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) p[j][e] = score.biased(p[j][e], near + (float)(16 * j - 16 * b - e));
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) p[j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[j][e], score.unit, ref[j]));
+      };
+      if (alone) {
+        float all[NB];
+#pragma unroll
+        for (int j = 0; j < NB; j++) all[j] = 0.f;
+#pragma unroll
+        for (int b = 0; b < R / 16; b++) {
+          f32x4 p[NB], dp[NB];
+          block(b, false, p, dp);
+#pragma unroll
+          for (int j = 0; j < NB; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) all[j] += k0 + 16 * b + 4 * g + e < sees[j] ? p[j][e] * dp[j][e] : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+          delta[j] = cross_row_sum(all[j]);
+          const int row = row0 + 16 * j + c;
+          if (g == 0 && row < t.end) a.delta[(int64_t)head * a.T + row] = delta[j];
+        }
+      }
 #pragma unroll
       for (int h = 0; h < R / 32; h++) {  // 32 keys at a time
         f32x4 s[2][NB];
 #pragma unroll
         for (int i = 0; i < 2; i++) {
-          const int b = 2 * h + i;
           f32x4 dp[NB];
-#pragma unroll
-          for (int j = 0; j < NB; j++) {
-            s[i][j] = score.start(b);
-            dp[j] = f32x4{-delta[j], -delta[j], -delta[j], -delta[j]};
-          }
-#pragma unroll
-          for (int ks = 0; ks < KS; ks++) {
-            const Frag fk = Rows::row_frag(lk, b, ks, c, g), fv = Rows::row_frag(lv, b, ks, c, g);
-#pragma unroll
-            for (int j = 0; j < NB; j++) {
-              s[i][j] = attn_mfma<DT>(fk, q[j][ks], s[i][j]);
-              dp[j] = attn_mfma<DT>(fv, go[j][ks], dp[j]);
-            }
-          }
-          if constexpr (KIND == kAttnCap) {
-#pragma unroll
-            for (int j = 0; j < NB; j++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                float f;
-                s[i][j][e] = score.capped(s[i][j][e], f);
-                dp[j][e] *= f;
-              }
-          }
-          if (score.single()) {
-#pragma unroll
-            for (int j = 0; j < NB; j++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) s[i][j][e] = score.biased(s[i][j][e], near + (float)(16 * j - 16 * b - e));
-          }
+          block(2 * h + i, true, s[i], dp);
 #pragma unroll
           for (int j = 0; j < NB; j++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[i][j][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][e], score.unit, ref[j])) * dp[j][e];
+            for (int e = 0; e < 4; e++) s[i][j][e] *= dp[j][e];
         }
         if (part) {
 #pragma unroll
@@ -1074,27 +1106,32 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const float* su
 
 enum AttnPass { kAttnForward = 0, kAttnDq = 1, kAttnDkv = 2 };
 
-template <int DT, int D, int NB, int KIND>
-static int attn_launch(AttnArgs a, AttnPass pass, hipStream_t st) {
+template <int DT, int D, int NB, int KIND, AttnPass PASS>
+static int attn_launch(AttnArgs a, hipStream_t st) {
   typedef AttnRows<DT, D> Rows;
   a.slots = (int32_t)attn_slots(a.T, a.B, 64 * NB);
-  const int64_t grid = attn_grid(a.slots, pass == kAttnDkv ? a.KV * a.parts : a.H);  // below 2^23
-  size_t lds = 4 * (size_t)Rows::kBytes;
-  if (pass == kAttnForward) {
-    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
+  const dim3 grid((unsigned)attn_grid(a.slots, PASS == kAttnDkv ? a.KV * a.parts : a.H)), threads(kAttnThreads);  // below 2^23
+  constexpr size_t lds = 4 * (size_t)Rows::kBytes;
+  if constexpr (PASS == kAttnForward) {
+    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, KIND>), grid, threads, lds, st, a);
     return check_launch("attn_forward_kernel");
-  }
-  if (pass == kAttnDq) {
-    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
+  } else if constexpr (PASS == kAttnDq) {
+    if constexpr (NB == 1) {
+      if (attn_short(a.T, a.B)) {
+        hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, true>), grid, threads, lds, st, a);
+        return check_launch("attn_dq_kernel");
+      }
+    }
+    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, false>), grid, threads, lds, st, a);
     return check_launch("attn_dq_kernel");
+  } else {
+    hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND>), grid, threads, lds + 4 * Rows::R * sizeof(float), st, a);
+    const int rc = check_launch("attn_dkv_kernel");
+    if (rc || a.parts == 1) return rc;
+    const int64_t n = a.T * a.KV * D, groups = (n / 2 + kAttnThreads - 1) / kAttnThreads;
+    hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)(groups < 65536 ? groups : 65536)), threads, 0, st, a.sums, a.parts, n, a.dk, a.dv);
+    return check_launch("attn_join_kernel");
   }
-  lds += 4 * Rows::R * sizeof(float);
-  hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND>), dim3((unsigned)grid), dim3(kAttnThreads), lds, st, a);
-  int rc = check_launch("attn_dkv_kernel");
-  if (rc || a.parts == 1) return rc;
-  const int64_t n = a.T * a.KV * D, groups = (n / 2 + kAttnThreads - 1) / kAttnThreads;
-  hipLaunchKernelGGL(attn_join_kernel<DT>, dim3((unsigned)(groups < 65536 ? groups : 65536)), dim3(kAttnThreads), 0, st, a.sums, a.parts, n, a.dk, a.dv);
-  return check_launch("attn_join_kernel");
 }
 
 // One of these for each dtype, in a file of its own.
@@ -1102,11 +1139,26 @@ int attn_run_f16(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 int attn_run_bf16(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 int attn_run_f32(const AttnArgs& a, int D, AttnPass pass, hipStream_t st);
 
-template <int DT, int D, int NB>
-static int attn_run_nb(const AttnArgs& a, AttnPass pass, hipStream_t st) {
-  if (a.cap > 0.f) return attn_launch<DT, D, NB, kAttnCap>(a, pass, st);
-  if (a.slopes) return attn_launch<DT, D, NB, kAttnBias>(a, pass, st);
-  return attn_launch<DT, D, NB, kAttnPlain>(a, pass, st);
+// Whether a pass has the registers for two blocks of 16 of its own rows: dk and dv need keys, values and both
+// gradients (96 under a bias, with spills: 585 us, 320 with one block), dq queries, their gradients and sums.
+template <int DT, int D, int KIND>
+constexpr bool attn_two(AttnPass pass) {
+  if (DT == TMS_DTYPE_F32) return false;
+  if (pass == kAttnDkv) return D <= 64 || (D == 96 && KIND == kAttnPlain);
+  return pass == kAttnForward || D < 128 || KIND == kAttnPlain;
+}
+template <int DT, int D, int KIND, AttnPass PASS>
+static int attn_run_pass(const AttnArgs& a, hipStream_t st) {
+  if constexpr (attn_two<DT, D, KIND>(PASS)) {
+    if (attn_wide(a.T, a.B, PASS == kAttnDkv ? (int64_t)a.KV * a.parts : a.H)) return attn_launch<DT, D, 2, KIND, PASS>(a, st);
+  }
+  return attn_launch<DT, D, 1, KIND, PASS>(a, st);
+}
+template <int DT, int D, int KIND>
+static int attn_run_kind(const AttnArgs& a, AttnPass pass, hipStream_t st) {
+  if (pass == kAttnForward) return attn_run_pass<DT, D, KIND, kAttnForward>(a, st);
+  if (pass == kAttnDq) return attn_run_pass<DT, D, KIND, kAttnDq>(a, st);
+  return attn_run_pass<DT, D, KIND, kAttnDkv>(a, st);
 }
 template <int DT, int D>
 static int attn_run_d(const AttnArgs& a, AttnPass pass, hipStream_t st) {
@@ -1115,13 +1167,9 @@ static int attn_run_d(const AttnArgs& a, AttnPass pass, hipStream_t st) {
     const int rc = check_launch("attn_norms_kernel");
     if (rc) return rc;
   }
-  if constexpr (DT != TMS_DTYPE_F32) {
-    if (pass != kAttnDkv && attn_wide(a.T, a.B, a.H)) return attn_run_nb<DT, D, 2>(a, pass, st);
-    if constexpr (D < 128) {  // 128 has no registers for two blocks' keys, values and both their gradients
-      if (pass == kAttnDkv && attn_wide(a.T, a.B, (int64_t)a.KV * a.parts)) return attn_run_nb<DT, D, 2>(a, pass, st);
-    }
-  }
-  return attn_run_nb<DT, D, 1>(a, pass, st);
+  if (a.cap > 0.f) return attn_run_kind<DT, D, kAttnCap>(a, pass, st);
+  if (a.slopes) return attn_run_kind<DT, D, kAttnBias>(a, pass, st);
+  return attn_run_kind<DT, D, kAttnPlain>(a, pass, st);
 }
 template <int DT>
 static int attn_run(const AttnArgs& a, int D, AttnPass pass, hipStream_t st) {
