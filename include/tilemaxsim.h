@@ -446,7 +446,7 @@ int tms_grad_clip(const tms_grad_tensor* tensors, int64_t count, int norm_type, 
  * [0, tokens]: what lies outside is taken as the nearest bound; if they descend, some rows' results are undefined,
  * and no memory outside the tensors is touched). A token attends to its own text: to all of it, or, with
  * `prefix` (device memory, one a text), to the text's first prefix[b] tokens and those up to itself.
- * The score of two tokens is x = scale <q, k>; with cap > 0, cap tanh(x / cap); with `slopes`
+ * The score of two tokens is x = scale <q, k>; with a cap, cap tanh(x / cap) (0: none; both from 1e-15 to 1e15); with `slopes`
  * (device memory, one a head), less slope |i - j|.
  * out (tokens, heads, width) contiguous; tokens of no text come out as zeros. For the backward pass
  * low (out's shape and dtype; NULL in fp32) takes what out's rounding left, and stats
@@ -479,7 +479,7 @@ int tms_packed_attention_grad(const tms_attention* attention, const void* out, c
 /*
  * Training and encoding: the gated projection of a feed-forward block, h = act(x w_gate^T) * (x w_up^T).
  * No reference counterpart. x (N, d), w_gate and w_up (F, d), h (N, F), of one fp16, bf16 or fp32
- * dtype, contiguous, 16-byte aligned, any N, d and F. The gradients: from grad (N, F) to dx (N, d) and
+ * dtype, contiguous, 16-byte aligned, any N up to 2^24, d up to 65,536 and F up to 2^20. The gradients: from grad (N, F) to dx (N, d) and
  * dw_gate, dw_up (F, d), of that dtype, any of which may be NULL; with N = 0 or F = 0 nothing is
  * written. Sums are fp32 in one order. workspace: tms_gated_workspace_size bytes of device memory
  * (backward = 0 or 1), 256-byte aligned; its contents need not stay between the two calls.

@@ -39,6 +39,7 @@ REFUSED = [
     (dict(dtype=3), 2, "dtype"), (dict(width=48), 2, "32, 64, 96 or 128"), (dict(width=256), 2, "256"),
     (dict(heads=0), 1, "share"), (dict(kv_heads=0), 1, "share"), (dict(heads=5), 1, "share"),
     (dict(scale=0.0), 1, "scale"), (dict(scale=-1.0), 1, "scale"), (dict(scale=NAN), 1, "scale"), (dict(scale=INF), 1, "scale"),
+    (dict(scale=1e-16), 1, "scale"), (dict(scale=1e16), 1, "scale"), (dict(cap=1e-16), 1, "cap"), (dict(cap=1e16), 1, "cap"),
     (dict(cap=-1.0), 1, "cap"), (dict(cap=NAN), 1, "cap"), (dict(cap=INF), 1, "cap"),
     (dict(tokens=1 << 31), 2, "too many"), (dict(texts=1 << 31), 2, "too many"), (dict(tokens=1 << 29), 2, "too many"),
     (dict(texts=1 << 23), 2, "too many"), (dict(heads=1 << 17, kv_heads=1), 2, "too many"),
@@ -110,7 +111,7 @@ Q, K, O = bf(10, 4, 64), bf(10, 2, 64), torch.tensor([0, 4, 10])
     (dict(offsets=torch.tensor([0, 11])), ValueError, "ascend"), (dict(offsets=torch.tensor([-1, 10])), ValueError, "ascend"),
     (dict(offsets=torch.tensor([0, 6, 4])), ValueError, "ascend"),
     (dict(scale=0.0), ValueError, "scale"), (dict(scale=-1), ValueError, "scale"), (dict(scale=NAN), ValueError, "scale"),
-    (dict(cap=0.0), ValueError, "cap"), (dict(cap=-2.0), ValueError, "cap"), (dict(cap=INF), ValueError, "cap"),
+    (dict(cap=0.0), ValueError, "cap"), (dict(cap=-2.0), ValueError, "cap"), (dict(cap=INF), ValueError, "cap"), (dict(cap=1e-16), ValueError, "cap"), (dict(scale=1e16), ValueError, "scale"),
     (dict(prefix=True), TypeError, "prefix"), (dict(prefix=1.5), TypeError, "prefix"), (dict(prefix=torch.tensor([1.0, 2.0])), TypeError, "prefix"),
     (dict(prefix=torch.tensor([1])), ValueError, "prefix"),
     (dict(slopes=torch.zeros(3)), ValueError, "slopes"), (dict(slopes=torch.zeros(4).half()), ValueError, "slopes"),
@@ -130,7 +131,7 @@ GATED = dict(x=256, N=100, d=64, w_gate=256, w_up=256, F=32, dtype=BF16, activat
 GATED_REFUSED = [
     (dict(N=-1), 1, "negative"), (dict(d=-1), 1, "negative"), (dict(F=-1), 1, "negative"), (dict(dtype=4), 2, "dtype"),
     (dict(activation=3), 1, "activation"), (dict(d=0), 1, "no elements"), (dict(d=65537), 2, "65536"), (dict(N=(1 << 24) + 1), 2, "2^24"),
-    (dict(F=(1 << 24) + 1), 2, "2^24"), (dict(x=None), 1, "NULL"), (dict(w_gate=None), 1, "NULL"), (dict(w_up=None), 1, "NULL"),
+    (dict(F=(1 << 20) + 1), 2, "2^20"), (dict(x=None), 1, "NULL"), (dict(w_gate=None), 1, "NULL"), (dict(w_up=None), 1, "NULL"),
     (dict(x=264), 1, "16-byte"), (dict(w_gate=258), 1, "16-byte"), (dict(w_up=8), 1, "16-byte"),
     (dict(d=77, ws=None), 1, "workspace"), (dict(dtype=F32, ws=None), 1, "workspace"), (dict(d=77, ws=272), 1, "256-byte"),
     (dict(d=77, ws_bytes=10), 1, "workspace")]

@@ -4,7 +4,8 @@ Tolerances, for each element, from the arithmetic. u is half a step of the input
 nothing is rounded between the products), e = 2^-23 for a rounding of an fp32 sum (twice half a step).
  * A score: sums of D products, 3 roundings more, in natural units: ex = e (D + 6) scale <|q|, |k|> +
    3 e |x|, and under a cap what tanh is off by, cap 2^-20 (16-bit kernels: from an exponential and a
-   reciprocal of 2^-22 each; fp32: 2^-21). P is then off by rp = 2 max ex + e (n + 4) of itself (its sum is, too), and by u more when
+   reciprocal of 2^-22 each; fp32: 2^-21); of |x| and not of the cap in caps above 64, 2^-16 of it (where it is formed so, |x| is
+   at least 2^-4 of the cap; below, it is off by 2^-22 of itself). P is then off by rp = 2 max ex + e (n + 4) of itself (its sum is, too), and by u more when
    it is rounded; in fp16 also by 2^-25 of the row's largest P, where it is below fp16's normal numbers.
  * out: (u + rp) sum P |v| + u |out|, and dv likewise with |do| in the place of |v|.
  * dP: e (D + 1) <|do|, |v|>. delta: from an out before its rounding, (u + rp + u^2) sum P <|do|, |v|> + e (D + 1) of that.
@@ -69,7 +70,7 @@ def reference(q, k, v, offsets, G, prefix=None, scale=None, cap=None, slopes=Non
             if cap:
                 t = torch.tanh(x / cap)
                 x, slope = cap * t, 1 - t * t
-                ex = ex + cap * 2.0 ** (-21 if dt == torch.float32 else -20)
+                ex = ex + (x.abs() * 2.0 ** -16 if cap > 64 else cap * 2.0 ** (-21 if dt == torch.float32 else -20))
             if slopes is not None:
                 x = x - float(slopes[h]) * (i[:, None] - i[None, :]).abs()
             ex = torch.where(sees, ex + 3 * E * x.abs(), 0.0)
@@ -302,6 +303,14 @@ def test_tiles_of_128(cuda, kind, D, dt):
     if kind == "cap":
         how["cap"] = 6.0
     check(*qkv, offsets, G, f"wide {kind} {D} {dt}", **how)
+
+
+@pytest.mark.parametrize("dt", DT, ids=str)
+@pytest.mark.parametrize("cap", [0.5, 64.0, 65.0, 300.0, 1e5, 1e12])
+def test_caps(cuda, cap, dt):
+    """A cap far above the scores changes nothing, one below flattens them."""
+    (q, k, v), offsets, G = make([90, 33], 2, 2, 64, dt, seed=4, scale=4.0)
+    out, _ = check(q, k, v, offsets, G, f"cap {cap} {dt}", cap=cap)
 
 
 @pytest.mark.parametrize("slope", [0.0, -0.01, 1.0, math.inf])

@@ -133,8 +133,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         prefix: None (a token attends to its whole text), or one integer a text, (B,) or a number
             for all: its first ``prefix`` tokens are seen by all of it, the others by themselves and
             those behind them. 0: causal.
-        scale: multiplies the products of q and k (positive; default ``1 / sqrt(D)``).
-        cap: scores become ``cap * tanh(score / cap)`` (positive; None: as they are).
+        scale: multiplies the products of q and k (1e-15 to 1e15; default ``1 / sqrt(D)``).
+        cap: scores become ``cap * tanh(score / cap)`` (1e-15 to 1e15; None: as they are).
         slopes: (H,) float32: a score is lessened by ``slope * |i - j|`` for tokens i and j
             (after the cap). They have no gradient.
 
@@ -152,10 +152,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
     _check.no_tangents(fn, (q, k, v))
     H, B = q.shape[1], offsets.shape[0] - 1
     scale = 1 / math.sqrt(q.shape[2]) if scale is None else float(scale)
-    if not 0 < scale < 1e30:
-        raise ValueError(f"{fn}: scale must be positive and finite (got {scale})")
-    if cap is not None and not 0 < (cap := float(cap)) < 1e30:
-        raise ValueError(f"{fn}: cap must be positive and finite (got {cap})")
+    if not 1e-15 <= scale <= 1e15:
+        raise ValueError(f"{fn}: scale must be from 1e-15 to 1e15 (got {scale})")
+    if cap is not None and not 1e-15 <= (cap := float(cap)) <= 1e15:
+        raise ValueError(f"{fn}: cap must be from 1e-15 to 1e15 (got {cap})")
     if isinstance(prefix, torch.Tensor):
         _integers(fn, "prefix", prefix)
         if tuple(prefix.shape) != (B,):

@@ -17,8 +17,8 @@ static int check_attention(const char* fn, const tms_attention* p, AttnArgs& a) 
     return fail(TMS_ERR_UNSUPPORTED, "%s: heads of 32, 64, 96 or 128 elements (got %lld)", fn, (long long)p->width);
   if (p->heads == 0 || p->kv_heads == 0 || p->heads % p->kv_heads)
     return fail(TMS_ERR_INVALID, "%s: %lld heads do not share %lld", fn, (long long)p->heads, (long long)p->kv_heads);
-  if (!(p->scale > 0) || !(p->scale < 1e30)) return fail(TMS_ERR_INVALID, "%s: scale must be positive and finite", fn);
-  if (!(p->cap >= 0) || !(p->cap < 1e30)) return fail(TMS_ERR_INVALID, "%s: cap must be positive and finite, or 0 for none", fn);
+  if (!(p->scale >= 1e-15) || !(p->scale <= 1e15)) return fail(TMS_ERR_INVALID, "%s: scale must be from 1e-15 to 1e15", fn);
+  if (p->cap != 0 && (!(p->cap >= 1e-15) || !(p->cap <= 1e15))) return fail(TMS_ERR_INVALID, "%s: cap must be from 1e-15 to 1e15, or 0 for none", fn);
   if (p->tokens > ((int64_t)1 << 31) - (1 << 16) || p->texts > ((int64_t)1 << 31) - (1 << 16) || p->heads > (1 << 16) ||
       attn_grid(attn_slots(p->tokens, p->texts, 64), p->heads) >= kAttnMostTiles)
     return fail(TMS_ERR_UNSUPPORTED, "%s: %lld tokens of %lld heads in %lld texts are too many", fn, (long long)p->tokens, (long long)p->heads, (long long)p->texts);

@@ -333,6 +333,12 @@ __device__ __forceinline__ void attn_own(const typename AttnType<DT>::E* base, i
   for (int ks = 0; ks < D / 32; ks++) f[ks] = *(const Frag*)(base + row_elems + ks * 32 + 8 * g);
 }
 
+constexpr float kAttnCoarse = 64.f;  // 2^-22 of it: 1.5e-5 of a score
+template <bool V>
+struct AttnYes {
+  static constexpr bool value = V;
+};
+
 // What a score takes besides the products: nothing, a bias, or a cap (and perhaps a bias).
 enum AttnKind { kAttnPlain = 0, kAttnBias = 1, kAttnCap = 2 };
 
@@ -378,8 +384,11 @@ struct AttnScore {
   // Whether the bias has to be taken off element by element.
   __device__ __forceinline__ bool single() const { return (KIND == kAttnCap && lean != 0.f) || (KIND == kAttnBias && side == 0); }
   // Under a cap, y from s, and kSlope times the derivative's factor, 1 - tanh^2. In 16 bits tanh z is taken as
-  // 1 - 2 r with r = 1 / (1 + e^2z), to 2^-22 or so of the cap, where the operands have 2^-9 or 2^-12.
+  // 1 - 2 r with r = 1 / (1 + e^2z), to 2^-22 or so of the cap, where the operands have 2^-9 or 2^-12. A cap above
+  // kAttnCoarse takes the series z (1 - z^2 / 3 + 2 z^4 / 15) up to |z| = 2^-4 (the next term, 17 z^6 / 315, is
+  // below 2^-28 there), as scores far below their cap would have its error: FINE.
   static constexpr float kSlope = KIND == kAttnCap && DT != TMS_DTYPE_F32 ? 0.25f : 1.f;
+  template <bool FINE>
   __device__ __forceinline__ float capped(float s, float& slope) const {
     if constexpr (DT == TMS_DTYPE_F32) {
       const float t = tanhf(s * inv_cap);
@@ -388,7 +397,28 @@ struct AttnScore {
     }
     const float r = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(s * inv_cap));  // inv_cap has 2 log2(e) in it
     slope = __builtin_fmaf(-r, r, r);  // (1 - t^2) / 4
-    return __builtin_fmaf(-2.f * cap2, r, cap2);
+    float y = __builtin_fmaf(-2.f * cap2, r, cap2);
+    if constexpr (FINE) {
+      const float z = s * inv_cap * (0.5f / kAttnLog2e), zz = z * z;
+      y = zz < 0x1p-8f ? z * cap2 * __builtin_fmaf(zz, __builtin_fmaf(zz, 2.f / 15.f, -1.f / 3.f), 1.f) : y;
+    }
+    return y;
+  }
+  // y of all of a wave's s, and (with dp) their factors: f(place, slope) for each.
+  template <int N, class F>
+  __device__ __forceinline__ void cap_all(f32x4 (&s)[N], F&& f) const {
+    auto all = [&](auto fine) {
+#pragma unroll
+      for (int j = 0; j < N; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float slope;
+          s[j][e] = capped<decltype(fine)::value>(s[j][e], slope);
+          f(j, e, slope);
+        }
+    };
+    if (cap2 > kAttnCoarse * kAttnLog2e) all(AttnYes<true>());  // uniform
+    else all(AttnYes<false>());
   }
   // far: i - j, or its negative.
   __device__ __forceinline__ float biased(float y, float far) const { return __builtin_fmaf(-lean, fabsf(far), y); }
@@ -540,13 +570,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
         }
       }
       if constexpr (KIND == kAttnCap) {
-        float none;
 #pragma unroll
-        for (int b = 0; b < KB; b++)
-#pragma unroll
-          for (int j = 0; j < NB; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[b][j][e] = score.capped(s[b][j][e], none);
+        for (int b = 0; b < KB; b++) score.cap_all(s[b], [](int, int, float) {});
       }
       if (score.single()) {
         const float near = (float)(row0 + c - k0 - 4 * g);
@@ -807,14 +832,9 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
           }
         }
         if constexpr (KIND == kAttnCap) {
-#pragma unroll
-          for (int j = 0; j < NB; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              float f;
-              p[j][e] = score.capped(p[j][e], f);
-              if (sloped) dp[j][e] *= f;
-            }
+          score.cap_all(p, [&](int j, int e, float slope) {
+            if (sloped) dp[j][e] *= slope;
+          });
         }
         if (score.single()) {
 #pragma unroll
@@ -1004,16 +1024,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
               dp[j] = attn_mfma<DT>(fg, v[j][ks], dp[j]);
             }
           }
-          if constexpr (KIND == kAttnCap) {
-#pragma unroll
-            for (int j = 0; j < NB; j++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                float f;
-                s[i][j][e] = score.capped(s[i][j][e], f);
-                dp[j][e] *= f;
-              }
-          }
+          if constexpr (KIND == kAttnCap) score.cap_all(s[i], [&](int j, int e, float slope) { dp[j][e] *= slope; });
           if (score.single()) {
 #pragma unroll
             for (int j = 0; j < NB; j++)

@@ -493,7 +493,8 @@ static int check_gated(const char* fn, const void* x, int64_t N, int64_t d, cons
     return fail(TMS_ERR_UNSUPPORTED, "%s: dtype must be fp16, bf16 or fp32", fn);
   if (act != TMS_ACT_SILU && act != TMS_ACT_GELU && act != TMS_ACT_GELU_TANH) return fail(TMS_ERR_INVALID, "%s: unknown activation %d", fn, act);
   if (d == 0) return fail(TMS_ERR_INVALID, "%s: rows of no elements", fn);
-  if (d > 65536 || N > (1 << 24) || F > (1 << 24)) return fail(TMS_ERR_UNSUPPORTED, "%s: sizes up to d = 65536, N = F = 2^24", fn);
+  // 256 rows of dg and du side by side are less than 2^31 bytes: the product's offsets in a tile have 32 bits
+  if (d > 65536 || N > (1 << 24) || F > (1 << 20)) return fail(TMS_ERR_UNSUPPORTED, "%s: sizes up to d = 65536, N = 2^24, F = 2^20", fn);
   if (N == 0 || F == 0) return TMS_OK;
   if (!x || !wg || !wu) return fail(TMS_ERR_INVALID, "%s: NULL pointer", fn);
   const uintptr_t all = (uintptr_t)x | (uintptr_t)wg | (uintptr_t)wu;
