@@ -78,14 +78,24 @@ template <int DT>
 struct AttnType {
   typedef uint16_t E;
   typedef u32x4 Frag;  // eight elements
-  static constexpr int kRows = 64;  // rows of a tile that passes through LDS
 };
 template <>
 struct AttnType<TMS_DTYPE_F32> {
   typedef float E;
   typedef u32x8 Frag;
-  static constexpr int kRows = 32;
 };
+
+enum AttnPass { kAttnForward = 0, kAttnDq = 1, kAttnDkv = 2 };
+
+// Rows of a tile that passes through LDS: 64, but for rows so wide that two workgroups fill a CU's LDS with them,
+// where 32 leave room for another one (37 texts of 1 to 701 tokens, 8 heads of 128, forward and dq: 62 and 74
+// us with 64, 52 and 65 with 32; a wave of 32 queries needs fewer of them at a time: texts of 8192, 565 and 668).
+template <int DT, int D, int NB>
+constexpr int attn_rows(AttnPass pass) {
+  if (DT == TMS_DTYPE_F32) return 32;
+  if (D < 128 || pass == kAttnDkv || (pass == kAttnForward && NB == 2)) return 64;
+  return 32;
+}
 
 // One product of 16 x 16 over 32: lane (c, g) gives eight elements of row (column) c each; which k
 // they are is the caller's, the same for both operands.
@@ -243,11 +253,11 @@ __device__ __forceinline__ bool attn_place(const AttnArgs& a, int heads, int& sl
 
 // Rows of D elements in LDS, and the way there: from memory to registers, and (after the wait that
 // the store makes) to LDS. Rows from `limit` on are zeros.
-template <int DT, int D>
+template <int DT, int D, int R_>
 struct AttnRows {
   typedef AttnType<DT> Ty;
   typedef typename Ty::Frag Frag;
-  static constexpr int R = Ty::kRows, ES = sizeof(typename Ty::E);
+  static constexpr int R = R_, ES = sizeof(typename Ty::E);
   static constexpr int kBytes = R * D * ES;
   static constexpr int kPanel = R * 32 * ES;                 // bytes of 32 columns
   static constexpr int kLoads = kBytes / 16 / kAttnThreads;  // 16-byte pieces a thread
@@ -347,11 +357,11 @@ enum AttnKind { kAttnPlain = 0, kAttnBias = 1, kAttnCap = 2 };
 // one FMA. Without a cap, a bias costs next to nothing in tiles that lie on one side of a wave's own rows:
 // there it is a part of the tile's row, which the products' sums begin with, and a part of
 // the wave's own row, which is in the shift.
-template <int DT, int KIND>
+template <int DT, int KIND, int R>
 struct AttnScore {
   float unit, cap2, inv_cap, lean;
   int side = 2;  // of the tile: its rows before the wave's (-1), behind them (1), or both (0)
-  f32x4 begin[KIND == kAttnBias ? AttnType<DT>::kRows / 16 : 1];  // -lean of rows 16 b + 4 g + e by side
+  f32x4 begin[KIND == kAttnBias ? R / 16 : 1];  // -lean of rows 16 b + 4 g + e by side
 
   __device__ __forceinline__ void init(const AttnArgs& a, int head) {
     unit = KIND == kAttnCap ? 1.f : a.scale * kAttnLog2e;
@@ -363,11 +373,11 @@ struct AttnScore {
   // The tile of rows from `first` on, against the wave's own from `own` up to `own_end`.
   __device__ __forceinline__ void tile(int first, int own, int own_end, int g) {
     if constexpr (KIND == kAttnBias) {
-      const int now = first + AttnType<DT>::kRows <= own ? -1 : first >= own_end ? 1 : 0;
+      const int now = first + R <= own ? -1 : first >= own_end ? 1 : 0;
       if (now == side) return;
       side = now;
 #pragma unroll
-      for (int b = 0; b < AttnType<DT>::kRows / 16; b++)
+      for (int b = 0; b < R / 16; b++)
 #pragma unroll
         for (int e = 0; e < 4; e++) begin[b][e] = lean * (float)(-now * (16 * b + 4 * g + e));
     }
@@ -485,7 +495,7 @@ __global__ __launch_bounds__(kAttnThreads) void attn_norms_kernel(AttnArgs a) {
 // NB: blocks of 16 queries a wave.
 template <int DT, int D, int NB, int KIND>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs a) {
-  typedef AttnRows<DT, D> Rows;
+  typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnForward)> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
   constexpr int R = Rows::R, KB = R / 16, DB = D / 16, KS = D / 32, BQ = 64 * NB;
@@ -512,7 +522,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
     const int kvh = head / a.many;
     const E* K = (const E*)a.k + kvh * a.kh;
     const E* V = (const E*)a.v + kvh * a.vh;
-    AttnScore<DT, KIND> score;
+    AttnScore<DT, KIND, R> score;
     score.init(a, head);
     Frag q[NB][KS];
     int sees[NB];  // a row's last visible key, plus one
@@ -724,7 +734,7 @@ __device__ __forceinline__ void attn_store(void* out, int64_t at, const f32x4 (&
 // and not 62.)
 template <int DT, int D, int NB, int KIND, bool SHORT>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
-  typedef AttnRows<DT, D> Rows;
+  typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDq)> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
   constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BQ = 64 * NB;
@@ -748,7 +758,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
     const int kvh = head / a.many;
     const E* K = (const E*)a.k + kvh * a.kh;
     const E* V = (const E*)a.v + kvh * a.vh;
-    AttnScore<DT, KIND> score;
+    AttnScore<DT, KIND, R> score;
     score.init(a, head);
     Frag q[NB][KS], go[NB][KS];
     int sees[NB];
@@ -906,7 +916,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   for (int j = 0; j < NB; j++) {
     const int row = row0 + 16 * j + c;
     if (row >= t.end) continue;
-    const float f = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND>::kSlope;
+    const float f = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
     if (a.dq) attn_store<DT>(a.dq, ((int64_t)row * a.H + head) * D, acc, j, f, g);
   }
 }
@@ -915,7 +925,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
 // those that share the keys.
 template <int DT, int D, int NB, int KIND>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
-  typedef AttnRows<DT, D> Rows;
+  typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDkv)> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
   constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BK = 64 * NB;
@@ -979,7 +989,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
         st = -(r < rows_end ? from_[(int64_t)head * a.T + r] : (int)threadIdx.x < R ? __builtin_inff() : 0.f);
       }
     };
-    AttnScore<DT, KIND> score;
+    AttnScore<DT, KIND, R> score;
     load(0);
     int buf = 0;
     for (int n = 0; n < total; n++) {
@@ -1077,7 +1087,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     const int key = key0 + 16 * j + c;
     if (key >= t.end) continue;
     const int64_t at = ((int64_t)key * a.KV + kvh) * D;
-    const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND>::kSlope;
+    const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
     const float fv = !t.real ? 0.f : DT == TMS_DTYPE_F16 ? 1.f / (float)(1 << kAttnP16) : 1.f;
     if (a.parts > 1) {
       const int64_t one = a.T * a.KV * D;
@@ -1115,11 +1125,9 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const float* su
 
 // ---------------------------------------------------------------- launches
 
-enum AttnPass { kAttnForward = 0, kAttnDq = 1, kAttnDkv = 2 };
-
 template <int DT, int D, int NB, int KIND, AttnPass PASS>
 static int attn_launch(AttnArgs a, hipStream_t st) {
-  typedef AttnRows<DT, D> Rows;
+  typedef AttnRows<DT, D, attn_rows<DT, D, NB>(PASS)> Rows;
   a.slots = (int32_t)attn_slots(a.T, a.B, 64 * NB);
   const dim3 grid((unsigned)attn_grid(a.slots, PASS == kAttnDkv ? a.KV * a.parts : a.H)), threads(kAttnThreads);  // below 2^23
   constexpr size_t lds = 4 * (size_t)Rows::kBytes;
