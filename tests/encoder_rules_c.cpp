@@ -1,4 +1,4 @@
-// The rules of attention and of split products (tms_train_rules.h), for test_encoder_host.py.
+// The rules of attention, of few tokens and of split products (tms_train_rules.h), for test_encoder_host.py.
 #include "tms_train_rules.h"
 
 using namespace tms;
@@ -11,3 +11,4 @@ extern "C" void gemm_split_of(int64_t m, int64_t n, int64_t k, int planes, int64
   out[0] = s.size;
   out[1] = s.splits;
 }
+extern "C" int gated_few_of(int64_t N, int64_t d, int64_t F, int f32) { return gated_few(N, d, F, f32 != 0); }

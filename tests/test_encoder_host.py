@@ -133,7 +133,7 @@ GATED_REFUSED = [
     (dict(activation=3), 1, "activation"), (dict(d=0), 1, "no elements"), (dict(d=65537), 2, "65536"), (dict(N=(1 << 24) + 1), 2, "2^24"),
     (dict(F=(1 << 20) + 1), 2, "2^20"), (dict(x=None), 1, "NULL"), (dict(w_gate=None), 1, "NULL"), (dict(w_up=None), 1, "NULL"),
     (dict(x=264), 1, "16-byte"), (dict(w_gate=258), 1, "16-byte"), (dict(w_up=8), 1, "16-byte"),
-    (dict(d=77, ws=None), 1, "workspace"), (dict(dtype=F32, ws=None), 1, "workspace"), (dict(d=77, ws=272), 1, "256-byte"),
+    (dict(d=77, ws=None), 1, "workspace"), (dict(dtype=F32, N=200, ws=None), 1, "workspace"), (dict(d=77, ws=272), 1, "256-byte"),
     (dict(d=77, ws_bytes=10), 1, "workspace")]
 
 
@@ -161,7 +161,7 @@ def test_gated_sizes():
     assert size(1000, 64, 32, BF16, 0) == 0 and size(1000, 77, 32, BF16, 0) > 0
     for dtype in (F16, BF16, F32):
         assert size(FEW_TOKENS, 77, 33, dtype, 0) == 0  # the Python layer asks for none
-    assert size(FEW_TOKENS + 1, 77, 33, F32, 0) > 0
+    assert size(FEW_TOKENS + 1, 77, 33, BF16, 0) > 0 and size(129, 77, 33, F32, 0) > 0
     assert size(1000, 64, 100, BF16, 1) >= 1000 * 2 * 128 * 2
 
 
@@ -323,6 +323,7 @@ def rules(tmp_path_factory):
     lib.attn_slots_of.argtypes = [i64] * 3
     lib.attn_wide_of.argtypes = [i64] * 3
     lib.attn_parts_of.argtypes = [i64] * 4
+    lib.gated_few_of.argtypes = [i64, i64, i64, ctypes.c_int]
     lib.gemm_split_of.argtypes = [i64, i64, i64, ctypes.c_int, ctypes.POINTER(i64)]
     return lib
 
@@ -350,6 +351,16 @@ def test_parts_divide_the_heads(rules):
         if rules.attn_slots_of(T, B, 64) * kv >= 512:
             assert parts == 1
     assert rules.attn_wide_of(16384, 2, 12) and not rules.attn_wide_of(16384, 128, 12) and not rules.attn_wide_of(2048, 1, 8)
+
+
+def test_few_tokens(rules):
+    """More tokens or larger weights never bring the kernel of few tokens back; a single token always has it."""
+    sizes = [(8, 8), (768, 2048), (1024, 2816), (2048, 5504), (4096, 11008), (65536, 1 << 20)]
+    for f32 in (0, 1):
+        few = [[rules.gated_few_of(N, d, F, f32) for d, F in sizes] for N in range(1, 140)]
+        assert all(few[0]) and not any(few[128])
+        assert all(a >= b for row in few for a, b in zip(row, row[1:])) and all(a >= b for one, other in zip(few, few[1:]) for a, b in zip(one, other))
+    assert rules.gated_few_of(64, 1021, 4096, 0) and not rules.gated_few_of(65, 1021, 4096, 0)
 
 
 def test_splits(rules):

@@ -343,6 +343,35 @@ def test_heads_shared_by_workgroups(cuda, H, KV, dt):
     check(*qkv, offsets, G, f"fewer parts {H} {KV} {dt}", slopes=torch.linspace(0, 1, H, device="cuda"))
 
 
+@pytest.mark.parametrize("lens", ["short", "long"])
+@pytest.mark.parametrize("dt", DT, ids=str)
+def test_some_gradients(cuda, dt, lens):
+    """Each gradient by itself, and each pair, has the bits of all three; frozen operands have none."""
+    import tilemaxsim_amd as tms
+    ts, offsets, G = make(LENS[lens], 6, 2, 64, dt, seed=8)
+    how = dict(prefix=4, cap=20.0, slopes=torch.linspace(0, 0.5, 6, device="cuda"))
+    want = torch.autograd.grad(tms.packed_attention(*ts, offsets, **how), ts, G)
+    for some in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        part = [t.detach().requires_grad_(m in some) for m, t in enumerate(ts)]
+        tms.packed_attention(*part, offsets, **how).backward(G)
+        assert all(torch.equal(t.grad, w) if m in some else t.grad is None for m, (t, w) in enumerate(zip(part, want))), some
+        got = torch.autograd.grad(tms.packed_attention(*ts, offsets, **how), [ts[m] for m in some], G)
+        assert all(torch.equal(a, want[m]) for a, m in zip(got, some)), some
+
+
+def test_one_tensor_three_times(cuda):
+    """Queries, keys and values that are the same tensor: its gradient is the three gradients' sum."""
+    import tilemaxsim_amd as tms
+    (x, _, _), offsets, G = make([33, 1, 70], 4, 4, 64, torch.float32, seed=9)
+    parts = [x.detach().clone().requires_grad_(True) for _ in range(3)]
+    a, b, c = torch.autograd.grad(tms.packed_attention(*parts, offsets), parts, G)
+    out = tms.packed_attention(x, x, x, offsets)
+    grad = torch.autograd.grad(out, x, G)[0].double()
+    a, b, c = (t.double() for t in (a, b, c))
+    # two sums of three addends in either order: two roundings each of at most the sum of magnitudes
+    assert bool(((grad - (a + b + c)).abs() <= 4 * 2.0 ** -24 * (a.abs() + b.abs() + c.abs())).all())
+
+
 def test_streams_and_graphs(cuda):
     """Another stream than the tensors' own; a captured forward and backward pass follows its inputs, replay by replay."""
     import tilemaxsim_amd as tms

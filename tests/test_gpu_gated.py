@@ -112,6 +112,29 @@ def test_large_tiles(cuda, N, d, F, dt):
     check(N, d, F, dt, "gelu", seed=3)
 
 
+@pytest.mark.parametrize("dt", DT, ids=str)
+@pytest.mark.parametrize("N,d,F", [(8, 4096, 8193), (9, 4096, 8193), (16, 2048, 8200), (17, 2048, 8200), (33, 1024, 2050), (64, 1024, 2040), (128, 96, 33)])
+def test_few_tokens(cuda, N, d, F, dt):
+    """Both sides of where the kernel of few tokens ends."""
+    check(N, d, F, dt, "silu", seed=5)
+
+
+@pytest.mark.parametrize("N", [3, 200])
+@pytest.mark.parametrize("dt", DT, ids=str)
+def test_some_gradients(cuda, dt, N):
+    """Each gradient by itself, and each pair, has the bits of all three; frozen operands have none."""
+    import tilemaxsim_amd as tms
+    ts, G = make(N, 72, 50, dt, seed=7)
+    want = torch.autograd.grad(tms.gated_linear(*ts), ts, G)
+    for some in ((0,), (1,), (2,), (0, 1), (0, 2), (1, 2)):
+        part = [t.detach().requires_grad_(m in some) for m, t in enumerate(ts)]
+        h = tms.gated_linear(*part)
+        h.backward(G)
+        assert all(torch.equal(t.grad, w) if m in some else t.grad is None for m, (t, w) in enumerate(zip(part, want))), some
+        got = torch.autograd.grad(tms.gated_linear(*ts), [ts[m] for m in some], G)
+        assert all(torch.equal(a, want[m]) for a, m in zip(got, some)), some
+
+
 @pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -20, 2.0 ** 9])
 def test_gradients_of_any_size(cuda, size):
     """fp16's narrow range: gradients as a mean over many tokens, or a loss's scale, leave them."""

@@ -11,8 +11,8 @@
 // products take them to dx (k over both, and over Wg and Wu one behind the other) and to both
 // weights' gradients (their rows one behind the other).
 //
-// Few tokens (16 N at most) take a kernel of their own: bound by reading the weights once, which
-// needs every CU to have some of them on their way.
+// Few tokens take a kernel of their own: bound by reading the weights once, which needs every CU to have
+// some of them on their way.
 //
 // Precision. g, u, the activation and all sums are fp32; dg and du are rounded to the inputs' type
 // between two products (fp32: three bf16 terms, six products of them), as a product of them
@@ -382,22 +382,22 @@ __global__ __launch_bounds__(64) void gated_factor_kernel(const uint32_t* parts,
 // ---------------------------------------------------------------- few tokens
 
 constexpr int kFewWaves = 8;
-constexpr int kFewTokens = 64;
+constexpr int kFewTokens = 64;  // of a workgroup
 
 // Eight rows of Wg and eight of Wu are one operand's 16 rows; the waves share k, 32 in turn, and add
-// up through LDS. fp32 goes through the fp32 matrix instructions as it is.
+// up through LDS. fp32 goes through the fp32 matrix instructions as it is; tokens behind 64 are another row of workgroups.
 template <int DT, int NI>
 __global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x, int32_t N, int32_t d, const void* wg, const void* wu, int32_t F,
                                                                    int32_t act, int32_t whole, void* out) {
   typedef typename std::conditional<DT == TMS_DTYPE_F32, float, uint16_t>::type T;
   __shared__ f32x4 parts[kFewWaves][NI][64];
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int f0 = (int)blockIdx.x * 8;
+  const int f0 = (int)blockIdx.x * 8, n0 = (int)blockIdx.y * kFewTokens;
   const int fr = f0 + (c & 7) < F ? f0 + (c & 7) : F - 1;
   const T* w = (const T*)(c < 8 ? wg : wu) + (int64_t)fr * d;
   const T* xs[NI];
 #pragma unroll
-  for (int j = 0; j < NI; j++) xs[j] = (const T*)x + (int64_t)(16 * j + c < N ? 16 * j + c : N - 1) * d;
+  for (int j = 0; j < NI; j++) xs[j] = (const T*)x + (int64_t)(n0 + 16 * j + c < N ? n0 + 16 * j + c : N - 1) * d;
   f32x4 acc[NI];
 #pragma unroll
   for (int j = 0; j < NI; j++) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -430,7 +430,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x
   __syncthreads();
   // thread (c, g, j) with g < 2: token 16 j + c, columns f0 + 4 g ..; g from lanes 32 on has u's
   for (int i = threadIdx.x; i < 32 * NI; i += kFewWaves * 64) {
-    const int j = i / 32, l = i % 32, row = 16 * j + (l & 15), f = f0 + 4 * (l >> 4);
+    const int j = i / 32, l = i % 32, row = n0 + 16 * j + (l & 15), f = f0 + 4 * (l >> 4);
     f32x4 gate = {0.f, 0.f, 0.f, 0.f}, up = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < kFewWaves; v++) {
@@ -461,11 +461,10 @@ struct GatedSpace {
 };
 constexpr int kMostParts = 256;
 
-static bool gated_few(int64_t N, bool backward) { return !backward && N <= kFewTokens; }
 static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool backward) {
   GatedSpace s = {};
   Carve c;
-  if (gated_few(N, backward)) return s;
+  if (!backward && gated_few(N, d, F, dtype == TMS_DTYPE_F32)) return s;
   const int64_t dp = up_to(d, 8);
   if (dtype == TMS_DTYPE_F32 || d % 8) {
     s.x = c.take(N * dp * 2 * planes(dtype));
@@ -558,7 +557,7 @@ static GemmArgs gated_args(const GatedOperands& o, int64_t N, int64_t F, int64_t
 
 template <int DT>
 static int gated_few_rows(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int act, void* h, hipStream_t st) {
-  const dim3 grid((unsigned)((F + 7) / 8)), threads(kFewWaves * 64);
+  const dim3 grid((unsigned)((F + 7) / 8), (unsigned)((N + kFewTokens - 1) / kFewTokens)), threads(kFewWaves * 64);
   const int whole = d % 8 == 0;
   auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, threads, 0, st, x, (int32_t)N, (int32_t)d, wg, wu, (int32_t)F, (int32_t)act, whole, h); };
   if (N <= 16) go(gated_few_kernel<DT, 1>);
@@ -570,7 +569,7 @@ static int gated_few_rows(const void* x, int64_t N, int64_t d, const void* wg, c
 template <int DT, int PL, int OUT>
 static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, uint8_t* ws, const GatedSpace& s,
                          void* h, hipStream_t st) {
-  if (gated_few(N, false)) return gated_few_rows<OUT>(x, N, d, wg, wu, F, act, h, st);
+  if (gated_few(N, d, F, dtype == TMS_DTYPE_F32)) return gated_few_rows<OUT>(x, N, d, wg, wu, F, act, h, st);
   GatedOperands o;
   int rc = gated_operands(x, N, d, wg, wu, F, dtype, ws, s, o, st);
   if (rc) return rc;

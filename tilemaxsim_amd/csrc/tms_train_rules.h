@@ -117,6 +117,19 @@ inline GemmSplit gemm_split(int64_t m, int64_t n, int64_t k, int planes) {
   return best;
 }
 
+// Whether the gated projection's forward pass takes the kernel of few tokens, whose workgroups read all of x each and
+// eight columns of the weights, or the matrix product's tiles, which need rows of whole 16 bytes. Few / tiles, us, in
+// bf16: 768 x 2048, 16 tokens 4.1 / 6.7, 64 tokens 6.1 / 6.9; 1024 x 2816, 32 tokens 7.9 / 8.3, 33 tokens 9.3 / 8.2;
+// 2048 x 5504, 32 tokens 19 / 21; 4096 x 11008, 1 token 34 / 41, 8 tokens 38 / 41, 16 tokens 46 / 41, 64 tokens
+// 108 / 41. Rows that have to be laid out anew first: 1020 x 4096, 64 tokens 8.5 / 26. fp32, whose tiles take terms:
+// 768 x 2048, 64 tokens 9.8 / 40, and twice that for 128; 4096 x 11008, 222 / 453.
+inline bool gated_few(int64_t N, int64_t d, int64_t F, bool f32) {
+  if (f32) return N <= 128;
+  if (d % 8) return N <= 64;
+  const int64_t weights = 2 * d * F;
+  return N <= 8 || (N <= 16 && weights <= (int64_t)1 << 26) || (N <= 32 && weights <= (int64_t)1 << 25) || (N <= 64 && weights <= (int64_t)1 << 22);
+}
+
 // Attention over packed texts (tms_train_attn_kernel.h). Numbers that tiles of `rows` rows may have: those of
 // B texts, and of what stands before and behind them.
 inline int64_t attn_slots(int64_t T, int64_t B, int64_t rows) { return T / rows + B + 2; }

@@ -9,7 +9,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _check, _lib
 
-FEW_TOKENS = 64  # up to which the forward pass needs no workspace
+FEW_TOKENS = 64  # up to which the forward pass needs no workspace, whatever its rows
 _ACTIVATIONS = {"silu": _lib.TMS_ACT_SILU, "gelu": _lib.TMS_ACT_GELU, "gelu_tanh": _lib.TMS_ACT_GELU_TANH}
 
 
