@@ -263,6 +263,21 @@ def test_layouts(cuda):
     near(state.views(state.m)[0], wm, em, "strided m")
 
 
+def test_one_element_in_two_places(cuda):
+    """Parameters and copies that are expanded, or given twice, are refused, and nothing has changed."""
+    import tilemaxsim_amd as tms
+    p, q = torch.ones(1, 5, device="cuda"), torch.ones(4, 5, device="cuda")
+    for params, copies in (([p.expand(4, 5)], None), ([q], [p.expand(4, 5)]), ([p.expand(4, 5)], [q]), ([q], [q])):
+        state = tms.AdamWState(params)
+        with pytest.raises(ValueError, match="overlap"):
+            tms.adamw_(params, [torch.ones(4, 5, device="cuda")], state, copies=copies)
+        assert not state.steps.any() and not state.m.any() and bool((p == 1).all()) and bool((q == 1).all())
+    q = torch.ones(4, 5, device="cuda").t()  # rows and columns in the other order are no overlap
+    state = tms.AdamWState([q])
+    tms.adamw_([q], [p.expand(4, 5).t()], state)
+    assert int(state.steps) == 1 and bool((q < 1).all())
+
+
 def test_nonfinite(cuda):
     """A NaN or infinite gradient goes into its own element alone, in 8 bits too; a NaN norm into all."""
     import tilemaxsim_amd as tms

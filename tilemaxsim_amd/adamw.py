@@ -137,7 +137,7 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
 
     Args:
         params: float32, float16 or bfloat16 (rounded to their type after the step: a small step may not
-            move them; float32 ones with ``copies`` do not have that). No two may share memory.
+            move them; float32 ones with ``copies`` do not have that). No two may share memory, nor elements of one.
         grads: one for each parameter, of its shape, in any of those types; None: the parameter is left
             as it is, and so are its states and its count.
         state: an :class:`AdamWState` of these parameters; its counts are raised by this call.
@@ -205,8 +205,8 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
     back = [(t, d) for t, d in zip([*ps, *(c for _, c in given)], [*p_to, *c_to]) if t is not d]
     if back:
         at = [t.data_ptr() for t in (*ps, *(c for _, c in given)) if t.numel()]
-        if len(set(at)) != len(at):
-            raise ValueError(f"{fn}: two of the tensors overlap")
+        if len(set(at)) != len(at) or any(s == 0 and n > 1 for t, _ in back for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{fn}: two of the tensors (or elements of one) overlap")
     g_from = whole(gs)
     n = len(ps)
     words = array("q", bytes(56 * n))  # tms_adamw_tensor entries
