@@ -583,7 +583,7 @@ static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, co
   if (rc) return rc;
   const int64_t dp = up_to(d, 8);
   const GemmArgs a = gated_args(o, N, F, dp);
-  return with_size<PL>(gemm_size(2 * F, N, gemm_steps(dp, PL), gemm_largest(PL)), [&](auto z) {
+  return with_size<PL>(product_size(2 * F, N, dp, PL), [&](auto z) {
     using Z = decltype(z);
     const GatedEpilogue<OUT, Z::MI> e = {h, (int32_t)N, (int32_t)F, (int32_t)act};
     return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (gated)");
@@ -627,7 +627,7 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
   }
   const float* back = factor ? factor + 1 : nullptr;
   const GemmArgs a = gated_args(o, N, F, dp);
-  rc = with_size<PL>(gemm_size(2 * F, N, gemm_steps(dp, PL), gemm_largest(PL)), [&](auto z) {
+  rc = with_size<PL>(product_size(2 * F, N, dp, PL), [&](auto z) {
     using Z = decltype(z);
     const GatedGradEpilogue<DT, PL, Z::MI> e = {grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
     return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (dg, du)");

@@ -154,11 +154,16 @@ struct More {
   static constexpr bool value = V;
 };
 
+// Tiles of 64 x 64 of three planes have room for all of a step's tiles at once (96 KB for two steps), and registers for their
+// fragments: one wait a step, and not six.
+constexpr bool gemm_whole(int PL, int MI) { return PL == 3 && MI == 2; }
+
 // PL: planes of both operands, 1 or 3.
 template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi, int PAIR = kSingle>
-__global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
+__global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
   constexpr int BM = 32 * MI, BN = 64 * NI;
-  constexpr int ASZ = BM * 128, BSZ = BN * 128;
+  constexpr bool WHOLE = gemm_whole(PL, MI);
+  constexpr int ASZ = BM * 128, BSZ = BN * 128, HELD = WHOLE ? 3 : 1;  // tiles of each operand in a buffer
   extern __shared__ __attribute__((aligned(1024))) uint8_t gemm_mem[];
   int tm, tn;
   if (!gemm_tile_of(a, tm, tn)) return;
@@ -178,7 +183,7 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
   const uint16_t* A = (PAIR == kPairRows && (wave >> 1 & 1) ? a.A2 : a.A) + (AO ? (int64_t)m0 : (int64_t)(PAIR == kPairRows ? m0 / 2 : m0) * a.lda);
   const uint16_t* B = a.B + (BO ? (int64_t)n0 : (int64_t)n0 * a.ldb);
   uint8_t* const lds_a = gemm_mem;
-  uint8_t* const lds_b = gemm_mem + 2 * ASZ;
+  uint8_t* const lds_b = gemm_mem + 2 * HELD * ASZ;
   auto load_a = [&](int buf, int step, int plane) {
     int64_t k = (int64_t)(k0 + step) * 64;
     if constexpr (PAIR == kPairDepth) {
@@ -211,18 +216,20 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
 #pragma unroll
     for (int j = 0; j < NI; j++) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  u32x4 fa[2][MI], fb[2][NI];
-  auto read_a = [&](int buf) {
+  u32x4 fas[HELD][2][MI], fbs[HELD][2][NI];
+  auto& fa = fas[0];
+  auto& fb = fbs[0];
+  auto read_a = [&](int buf, int to = 0) {
 #pragma unroll
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-      for (int i = 0; i < MI; i++) fa[ks][i] = GemmTile<BM, AO>::frag(lds_a + buf * ASZ, wm * MI + i, ks, lane);
+      for (int i = 0; i < MI; i++) fas[to][ks][i] = GemmTile<BM, AO>::frag(lds_a + buf * ASZ, wm * MI + i, ks, lane);
   };
-  auto read_b = [&](int buf) {
+  auto read_b = [&](int buf, int to = 0) {
 #pragma unroll
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-      for (int j = 0; j < NI; j++) fb[ks][j] = GemmTile<BN, BO>::frag(lds_b + buf * BSZ, wn * NI + j, ks, lane);
+      for (int j = 0; j < NI; j++) fbs[to][ks][j] = GemmTile<BN, BO>::frag(lds_b + buf * BSZ, wn * NI + j, ks, lane);
   };
   // The products of the fragments; `next`: the next step's loads, which go out once some of the
   // products are issued (behind the loads, a product would wait for all of the wave's LDS
@@ -247,13 +254,51 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 ? 2 : 4) void train_gemm_kern
     products(1, 0, MI);
     __builtin_amdgcn_sched_barrier(0);
   };
+  // WHOLE: a step's three tiles of each operand, into buffers 3 buf + plane.
+  auto load_whole = [&](int buf, int t) {
+#pragma unroll
+    for (int plane = 0; plane < 3; plane++) {
+      load_a(3 * buf + plane, t, plane);
+      load_b(3 * buf + plane, t, plane);
+    }
+  };
   if (nk > 0) {
-    load_a(0, 0, PL - 1);
-    load_b(0, 0, 0);
+    if constexpr (WHOLE) {
+      load_whole(0, 0);
+    } else {
+      load_a(0, 0, PL - 1);
+      load_b(0, 0, 0);
+    }
     meet();
   }
   int buf = 0;
+  auto step_whole = [&](int t, auto more) {
+#pragma unroll
+    for (int plane = 0; plane < HELD; plane++) {
+      read_a(3 * buf + plane, plane);
+      read_b(3 * buf + plane, plane);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (decltype(more)::value) load_whole(buf ^ 1, t + 1);
+    __builtin_amdgcn_sched_barrier(0);
+    constexpr int PA[6] = {2, 1, 1, 0, 0, 0}, PB[6] = {0, 0, 1, 1, 2, 0};
+#pragma unroll
+    for (int p = 0; p < 6; p++)
+#pragma unroll
+      for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+        for (int i = 0; i < MI; i++)
+#pragma unroll
+          for (int j = 0; j < NI; j++) acc[i][j] = mfma16x16x32<DT>(fas[PA[p] % HELD][ks][i], fbs[PB[p] % HELD][ks][j], acc[i][j]);
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (decltype(more)::value) meet();
+    buf ^= 1;
+  };
   auto step = [&](int t, auto more) {
+    if constexpr (WHOLE) {
+      step_whole(t, more);
+      return;
+    }
     read_b(PL == 3 ? 0 : buf);
     read_a(buf);
     if constexpr (PL == 3) {  // the fragments of the tile that stays, stay
@@ -295,7 +340,7 @@ static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what
   if ((int64_t)a.tm * a.tn > 1 << 30) return fail(TMS_ERR_UNSUPPORTED, "%s: %d x %d tiles are too many", what, a.tm, a.tn);
   const int steps = (a.K + 63) / 64;
   a.per = (steps + a.splits - 1) / a.splits;
-  size_t lds = 2 * (size_t)(32 * MI + 64 * NI) * 128;
+  size_t lds = 2 * (gemm_whole(PL, MI) ? 3 : 1) * (size_t)(32 * MI + 64 * NI) * 128;
   if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
   hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi, PAIR>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);

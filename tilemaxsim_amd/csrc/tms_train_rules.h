@@ -96,21 +96,35 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   return best;
 }
 
+// Microseconds of a product of m x n over k. Of three planes, tiles of 64 x 64 wait once a 64-step, one workgroup a CU: 0.91
+// each, and 3.8 around them (176 tiles over 256, 768 and 2048 of k: 7.4, 14.6, 33.0; 352 over 1024: 34.6. With a wait a
+// product, 176 over 256: 12.7. Tiles of 128, 176 over 1024: 56.6).
+inline double product_us(int size, int64_t m, int64_t n, int64_t k, int planes, int64_t splits) {
+  if (planes != 3 || size != kGemm64) return gemm_us(size, m, n, gemm_steps(k, planes), splits);
+  const int64_t groups = up_to(m, 64) / 64 * (up_to(n, 64) / 64) * splits, steps = up_to(k, 64) / 64;
+  return (double)((groups + 255) / 256) * ((double)((steps + splits - 1) / splits) * 0.91 + 3.8);
+}
+inline int product_size(int64_t m, int64_t n, int64_t k, int planes) {
+  int best = gemm_largest(planes);
+  for (int s = best + 1; s < kGemmSizes; s++)
+    if (product_us(s, m, n, k, planes, 1) < product_us(best, m, n, k, planes, 1)) best = s;
+  return best;
+}
+
 // Tiles and splits of k of a product of m x n whose sums go to 16 bits at once, or through fp32 and another kernel where that
 // is shorter: splits fill the chip where tiles are few. A split's sums are written and read at about 4 TB/s, and the
-// second kernel takes 4 us. (500 x 256 over 1408 in three terms: 53 us whole, 17 in eight splits.)
+// second kernel takes 4 us. (500 x 256 over 1408 in three terms, a wait a product: 53 us whole, 17 in eight splits.)
 struct GemmSplit {
   int size, splits;
 };
 inline GemmSplit gemm_split(int64_t m, int64_t n, int64_t k, int planes) {
   static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32};
-  const int64_t steps = gemm_steps(k, planes);
   GemmSplit best = {};
   double least = 1e30;
   for (int s : kSplits) {
     if (s > 1 && s * 2 > up_to(k, 64) / 64) break;
     for (int size = gemm_largest(planes); size < kGemmSizes; size++) {
-      const double us = gemm_us(size, m, n, steps, s) + (s > 1 ? (double)s * (double)m * (double)n * 8 / 4e6 + 4.0 : 0.0);
+      const double us = product_us(size, m, n, k, planes, s) + (s > 1 ? (double)s * (double)m * (double)n * 8 / 4e6 + 4.0 : 0.0);
       if (us < least) least = us, best = {size, s};
     }
   }
