@@ -113,7 +113,8 @@ def test_large_tiles(cuda, N, d, F, dt):
 
 
 @pytest.mark.parametrize("dt", DT, ids=str)
-@pytest.mark.parametrize("N,d,F", [(8, 4096, 8193), (9, 4096, 8193), (16, 2048, 8200), (17, 2048, 8200), (33, 1024, 2050), (64, 1024, 2040), (128, 96, 33)])
+@pytest.mark.parametrize("N,d,F", [(1, 4096, 8193), (9, 4096, 8193), (16, 2048, 8200), (16, 2048, 8190), (17, 2048, 8190), (32, 1024, 2040),
+                                   (33, 1024, 2040), (32, 1024, 2050), (64, 1020, 2050), (65, 1020, 2050), (128, 96, 33)])
 def test_few_tokens(cuda, N, d, F, dt):
     """Both sides of where the kernel of few tokens ends."""
     check(N, d, F, dt, "silu", seed=5)

@@ -13,8 +13,8 @@
 //
 // Bound by the matrix cores, the tiles' ends behind them. 16,384 tokens, 1024 x 4096, bf16: forward 270 us (1.02 PFLOP/s), dg
 // and du 322 (their ends form two functions and write 268 MB), dx 274, both weights' gradients 267 and 14 for
-// the join of two splits. 1229 x 768 x 2043 in fp16: 19, 23, 20 + 5 and 20 us, where tiles of 128 fill the
-// chip once and a quarter.
+// the join of two splits. 1229 x 768 x 2043: 16, 22, 18 + 5 and 17 us, where tiles of 128 fill the chip once
+// and a quarter, or less than once (two steps a wait).
 //
 // Few tokens take a kernel of their own: bound by reading the weights once, which needs every CU to have
 // some of them on their way.
@@ -391,7 +391,7 @@ __global__ __launch_bounds__(64) void gated_factor_kernel(const uint32_t* parts,
 constexpr int kFewWaves = 8;
 constexpr int kFewTokens = 64;  // of a workgroup
 
-// Bound by reading the weights: one token, 4096 x 11008 in bf16, 34 us (5.2 TB/s); 768 x 2048, 4 us, the launch and two
+// Bound by reading the weights: 16 tokens, 2048 x 5504 in bf16, 13.4 us (3.4 TB/s); 768 x 2048, 4 us, the launch and two
 // trips to memory. Eight rows of Wg and eight of Wu are one operand's 16 rows; the waves share k, 32 in turn, and add
 // up through LDS. fp32 goes through the fp32 matrix instructions as it is; tokens behind 64 are another row of workgroups.
 template <int DT, int NI>
@@ -574,6 +574,18 @@ static int gated_few_rows(const void* x, int64_t N, int64_t d, const void* wg, c
   return check_launch("gated_few_kernel");
 }
 
+// A product with the tiles of `size`; epi(SizeOf) is its epilogue.
+template <int DT, int PL, bool AO, bool BO, int PAIR, class F>
+static int gated_product(const GemmArgs& a, int size, F&& epi, const char* what, hipStream_t st) {
+  return with_size<PL>(size, [&](auto z) {
+    using Z = decltype(z);
+    if constexpr (PL == 1 && Z::MI < 8) {
+      if (product_deep(size, a.M, a.N, a.splits)) return run_gemm<DT, PL, Z::MI, Z::NI, AO, BO, PAIR, true>(a, epi(z), st, what);
+    }
+    return run_gemm<DT, PL, Z::MI, Z::NI, AO, BO, PAIR>(a, epi(z), st, what);
+  });
+}
+
 template <int DT, int PL, int OUT>
 static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, int act, uint8_t* ws, const GatedSpace& s,
                          void* h, hipStream_t st) {
@@ -583,11 +595,8 @@ static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, co
   if (rc) return rc;
   const int64_t dp = up_to(d, 8);
   const GemmArgs a = gated_args(o, N, F, dp);
-  return with_size<PL>(product_size(2 * F, N, dp, PL), [&](auto z) {
-    using Z = decltype(z);
-    const GatedEpilogue<OUT, Z::MI> e = {h, (int32_t)N, (int32_t)F, (int32_t)act};
-    return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (gated)");
-  });
+  auto epi = [&](auto z) { return GatedEpilogue<OUT, decltype(z)::MI>{h, (int32_t)N, (int32_t)F, (int32_t)act}; };
+  return gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (gated)", st);
 }
 
 // A product to rows of d elements, at once or in splits.
@@ -597,10 +606,10 @@ static int gated_rows(GemmArgs b, GemmSplit plan, int64_t all, int64_t half, int
   b.splits = plan.splits;
   if (plan.splits == 1) {
     const GatedRowsEpilogue<OUT> e = {out, out2, factor, (int32_t)rows, (int32_t)half, (int32_t)d};
-    return with_size<PL>(plan.size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, BO, PAIR>(b, e, st, what); });
+    return gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   }
   const GatedSumEpilogue e = {sums, all * dp, (int32_t)all, (int32_t)dp};
-  const int rc = with_size<PL>(plan.size, [&](auto z) { return run_gemm<DT, PL, decltype(z)::MI, decltype(z)::NI, true, BO, PAIR>(b, e, st, what); });
+  const int rc = gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   if (rc) return rc;
   hipLaunchKernelGGL(gated_join_kernel<OUT>, dim3(blocks_for(all * ((d + 3) / 4))), dim3(256), 0, st, sums, plan.splits, all * dp, (int32_t)all,
                      (int32_t)half, (int32_t)rows, (int32_t)d, (int32_t)dp, factor, out, out2);
@@ -627,11 +636,10 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
   }
   const float* back = factor ? factor + 1 : nullptr;
   const GemmArgs a = gated_args(o, N, F, dp);
-  rc = with_size<PL>(product_size(2 * F, N, dp, PL), [&](auto z) {
-    using Z = decltype(z);
-    const GatedGradEpilogue<DT, PL, Z::MI> e = {grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
-    return run_gemm<DT, PL, Z::MI, Z::NI, false, false, kPairRows>(a, e, st, "train_gemm_kernel (dg, du)");
-  });
+  auto epi = [&](auto z) {
+    return GatedGradEpilogue<DT, PL, decltype(z)::MI>{grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
+  };
+  rc = gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (dg, du)", st);
   if (rc) return rc;
   if (dx) {  // m over d, n over tokens, k over F columns of dg and du and the rows of Wg and Wu
     GemmArgs b = {};

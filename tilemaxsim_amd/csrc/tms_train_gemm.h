@@ -154,16 +154,16 @@ struct More {
   static constexpr bool value = V;
 };
 
-// Tiles of 64 x 64 of three planes have room for all of a step's tiles at once (96 KB for two steps), and registers for their
-// fragments: one wait a step, and not six.
-constexpr bool gemm_whole(int PL, int MI) { return PL == 3 && MI == 2; }
+// Tiles of an operand that a buffer holds, all of them waited for at once: of three planes and 64 x 64 a step's (96 KB for
+// two steps: one wait a step, and not six); DEEP, two steps' (128 x 128: 128 KB, where one workgroup a CU has nothing
+// beside it to fill its waits).
+constexpr int gemm_held(int PL, int MI, bool DEEP) { return PL == 3 ? (MI == 2 ? 3 : 1) : DEEP ? 2 : 1; }
 
 // PL: planes of both operands, 1 or 3.
-template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi, int PAIR = kSingle>
-__global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, class Epi, int PAIR = kSingle, bool DEEP = false>
+__global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_held(PL, MI, DEEP) > 1 ? 2 : 4) void train_gemm_kernel(GemmArgs a, Epi epi) {
   constexpr int BM = 32 * MI, BN = 64 * NI;
-  constexpr bool WHOLE = gemm_whole(PL, MI);
-  constexpr int ASZ = BM * 128, BSZ = BN * 128, HELD = WHOLE ? 3 : 1;  // tiles of each operand in a buffer
+  constexpr int ASZ = BM * 128, BSZ = BN * 128, HELD = gemm_held(PL, MI, DEEP);
   extern __shared__ __attribute__((aligned(1024))) uint8_t gemm_mem[];
   int tm, tn;
   if (!gemm_tile_of(a, tm, tn)) return;
@@ -184,6 +184,8 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
   const uint16_t* B = a.B + (BO ? (int64_t)n0 : (int64_t)n0 * a.ldb);
   uint8_t* const lds_a = gemm_mem;
   uint8_t* const lds_b = gemm_mem + 2 * HELD * ASZ;
+  // A deep step's second half may be behind the last one: zeros.
+  auto behind = [&](int step) { return DEEP && step >= nk; };
   auto load_a = [&](int buf, int step, int plane) {
     int64_t k = (int64_t)(k0 + step) * 64;
     if constexpr (PAIR == kPairDepth) {
@@ -192,18 +194,18 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
         from = a.A2 + m0;
         k -= a.half;
       }
-      ta.load(from + plane * a.aplane + k * a.lda, a.real - (int)k, lds_a + buf * ASZ, wave);
+      ta.load(from + plane * a.aplane + k * a.lda, behind(step) ? 0 : a.real - (int)k, lds_a + buf * ASZ, wave);
       return;
     }
-    ta.load(A + plane * a.aplane + (AO ? k * a.lda : k), a.K - (int)k, lds_a + buf * ASZ, wave);
+    ta.load(A + plane * a.aplane + (AO ? k * a.lda : k), behind(step) ? 0 : a.K - (int)k, lds_a + buf * ASZ, wave);
   };
   auto load_b = [&](int buf, int step, int plane) {
     const int64_t k = (int64_t)(k0 + step) * 64;
     if constexpr (PAIR == kPairDepth) {  // columns behind the last one that each A has a row for are not read
-      tb.load(B + plane * a.bplane + k, a.real - (int)(k >= a.half ? k - a.half : k), lds_b + buf * BSZ, wave);
+      tb.load(B + plane * a.bplane + k, behind(step) ? 0 : a.real - (int)(k >= a.half ? k - a.half : k), lds_b + buf * BSZ, wave);
       return;
     }
-    tb.load(B + plane * a.bplane + (BO ? k * a.ldb : k), a.K - (int)k, lds_b + buf * BSZ, wave);
+    tb.load(B + plane * a.bplane + (BO ? k * a.ldb : k), behind(step) ? 0 : a.K - (int)k, lds_b + buf * BSZ, wave);
   };
   auto meet = [&]() {  // this wave's loads are in LDS, then everyone's
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
@@ -254,17 +256,17 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
     products(1, 0, MI);
     __builtin_amdgcn_sched_barrier(0);
   };
-  // WHOLE: a step's three tiles of each operand, into buffers 3 buf + plane.
-  auto load_whole = [&](int buf, int t) {
+  // Tile h of a buffer that holds several: a plane of step t, or step t + h.
+  auto load_held = [&](int buf, int t) {
 #pragma unroll
-    for (int plane = 0; plane < 3; plane++) {
-      load_a(3 * buf + plane, t, plane);
-      load_b(3 * buf + plane, t, plane);
+    for (int h = 0; h < HELD; h++) {
+      load_a(HELD * buf + h, PL == 3 ? t : t + h, PL == 3 ? h : 0);
+      load_b(HELD * buf + h, PL == 3 ? t : t + h, PL == 3 ? h : 0);
     }
   };
   if (nk > 0) {
-    if constexpr (WHOLE) {
-      load_whole(0, 0);
+    if constexpr (HELD > 1) {
+      load_held(0, 0);
     } else {
       load_a(0, 0, PL - 1);
       load_b(0, 0, 0);
@@ -272,18 +274,18 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
     meet();
   }
   int buf = 0;
-  auto step_whole = [&](int t, auto more) {
+  auto step_held = [&](int t, auto more) {
 #pragma unroll
-    for (int plane = 0; plane < HELD; plane++) {
-      read_a(3 * buf + plane, plane);
-      read_b(3 * buf + plane, plane);
+    for (int h = 0; h < HELD; h++) {
+      read_a(HELD * buf + h, h);
+      read_b(HELD * buf + h, h);
     }
     __builtin_amdgcn_sched_barrier(0);
-    if constexpr (decltype(more)::value) load_whole(buf ^ 1, t + 1);
+    if constexpr (decltype(more)::value) load_held(buf ^ 1, PL == 3 ? t + 1 : t + HELD);
     __builtin_amdgcn_sched_barrier(0);
-    constexpr int PA[6] = {2, 1, 1, 0, 0, 0}, PB[6] = {0, 0, 1, 1, 2, 0};
+    constexpr int PA[6] = {PL == 3 ? 2 : 0, 1, 1, 0, 0, 0}, PB[6] = {0, PL == 3 ? 0 : 1, 1, 1, 2, 0};
 #pragma unroll
-    for (int p = 0; p < 6; p++)
+    for (int p = 0; p < (PL == 3 ? 6 : HELD); p++)
 #pragma unroll
       for (int ks = 0; ks < 2; ks++)
 #pragma unroll
@@ -295,8 +297,8 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
     buf ^= 1;
   };
   auto step = [&](int t, auto more) {
-    if constexpr (WHOLE) {
-      step_whole(t, more);
+    if constexpr (HELD > 1) {
+      step_held(t, more);
       return;
     }
     read_b(PL == 3 ? 0 : buf);
@@ -327,22 +329,24 @@ __global__ __launch_bounds__(kGemmThreads, MI == 8 || gemm_whole(PL, MI) ? 2 : 4
     if constexpr (decltype(more)::value) meet();
     buf ^= 1;
   };
-  for (int t = 0; t + 1 < nk; t++) step(t, More<true>());
-  if (nk > 0) step(nk - 1, More<false>());
+  constexpr int EACH = PL == 1 ? HELD : 1;
+  const int last = nk > 0 ? (nk - 1) / EACH * EACH : 0;
+  for (int t = 0; t < last; t += EACH) step(t, More<true>());
+  if (nk > 0) step(last, More<false>());
   if constexpr (Epi::kRowBytes > 0) __syncthreads();  // the operands' LDS is the epilogue's
   epi(acc, m0 + wm * MI * 16, n0 + wn * NI * 16, (int)blockIdx.y, gemm_mem + wave * (NI * 16 * Epi::kRowBytes));
 }
 
-template <int DT, int PL, int MI, int NI, bool AO, bool BO, int PAIR = kSingle, class Epi>
+template <int DT, int PL, int MI, int NI, bool AO, bool BO, int PAIR = kSingle, bool DEEP = false, class Epi>
 static int run_gemm(GemmArgs a, const Epi& epi, hipStream_t st, const char* what) {
   a.tm = (a.M + 32 * MI - 1) / (32 * MI);
   a.tn = (a.N + 64 * NI - 1) / (64 * NI);
   if ((int64_t)a.tm * a.tn > 1 << 30) return fail(TMS_ERR_UNSUPPORTED, "%s: %d x %d tiles are too many", what, a.tm, a.tn);
   const int steps = (a.K + 63) / 64;
   a.per = (steps + a.splits - 1) / a.splits;
-  size_t lds = 2 * (gemm_whole(PL, MI) ? 3 : 1) * (size_t)(32 * MI + 64 * NI) * 128;
+  size_t lds = 2 * gemm_held(PL, MI, DEEP) * (size_t)(32 * MI + 64 * NI) * 128;
   if (lds < (size_t)8 * NI * 16 * Epi::kRowBytes) lds = (size_t)8 * NI * 16 * Epi::kRowBytes;
-  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi, PAIR>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
+  hipLaunchKernelGGL((train_gemm_kernel<DT, PL, MI, NI, AO, BO, Epi, PAIR, DEEP>), gemm_grid(a.tm, a.tn, a.splits), dim3(kGemmThreads),
                      lds, st, a, epi);
   return check_launch(what);
 }

@@ -96,13 +96,24 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   return best;
 }
 
+// Whether a product of one plane takes two 64-steps with one wait: where there are no more workgroups than LDS then has room
+// for. Rows of weights in turn, bf16, one step a wait / two: 256 tiles of 128 over 2048, 29.5 / 23.6 us; 112 of 64 over 1024, 11.6 /
+// 8.2; 512 of 64 over 4096, 41.8 / 31.0. With k outside, 256 of 128 over 1024: 20.8 / 17.6.
+inline bool product_deep(int size, int64_t m, int64_t n, int64_t splits) {
+  if (size == kGemm256) return false;
+  const int64_t side = gemm_side(size);
+  return up_to(m, side) / side * (up_to(n, side) / side) * splits <= (size == kGemm128 ? 256 : 512);
+}
+
 // Microseconds of a product of m x n over k. Of three planes, tiles of 64 x 64 wait once a 64-step, one workgroup a CU: 0.91
 // each, and 3.8 around them (176 tiles over 256, 768 and 2048 of k: 7.4, 14.6, 33.0; 352 over 1024: 34.6. With a wait a
 // product, 176 over 256: 12.7. Tiles of 128, 176 over 1024: 56.6).
 inline double product_us(int size, int64_t m, int64_t n, int64_t k, int planes, int64_t splits) {
-  if (planes != 3 || size != kGemm64) return gemm_us(size, m, n, gemm_steps(k, planes), splits);
-  const int64_t groups = up_to(m, 64) / 64 * (up_to(n, 64) / 64) * splits, steps = up_to(k, 64) / 64;
-  return (double)((groups + 255) / 256) * ((double)((steps + splits - 1) / splits) * 0.91 + 3.8);
+  const int64_t side = gemm_side(size), groups = up_to(m, side) / side * (up_to(n, side) / side) * splits;
+  const double each = (double)((up_to(k, 64) / 64 + splits - 1) / splits);
+  if (planes == 3 && size == kGemm64) return (double)((groups + 255) / 256) * (each * 0.91 + 3.8);
+  if (planes == 1 && product_deep(size, m, n, splits)) return size == kGemm128 ? each * 0.7 + 5.0 : each * (groups <= 256 ? 0.42 : 0.57) + 3.5;
+  return gemm_us(size, m, n, gemm_steps(k, planes), splits);
 }
 inline int product_size(int64_t m, int64_t n, int64_t k, int planes) {
   int best = gemm_largest(planes);
@@ -133,15 +144,15 @@ inline GemmSplit gemm_split(int64_t m, int64_t n, int64_t k, int planes) {
 
 // Whether the gated projection's forward pass takes the kernel of few tokens, whose workgroups read all of x each and
 // eight columns of the weights, or the matrix product's tiles, which need rows of whole 16 bytes. Few / tiles, us, in
-// bf16: 768 x 2048, 16 tokens 4.1 / 6.7, 64 tokens 6.1 / 6.9; 1024 x 2816, 32 tokens 7.9 / 8.3, 33 tokens 9.3 / 8.2;
-// 2048 x 5504, 32 tokens 19 / 21; 4096 x 11008, 1 token 34 / 41, 8 tokens 38 / 41, 16 tokens 46 / 41, 64 tokens
-// 108 / 41. Rows that have to be laid out anew first: 1020 x 4096, 64 tokens 8.5 / 26. fp32, whose tiles take terms:
-// 768 x 2048, 64 tokens 9.8 / 40, and twice that for 128; 4096 x 11008, 222 / 453.
+// bf16: 768 x 2048, 16 tokens 4.1 / 5.5, 32 tokens 4.7 / 5.5, 64 tokens 6.1 / 5.6; 1024 x 2816, 16 tokens 6.0 / 6.5, 32 tokens
+// 7.9 / 6.5; 2048 x 5504, 16 tokens 13.4 / 14.6; 4096 x 11008, 1 token 34 / 28, 16 tokens 46 / 28. Rows that have to be laid out
+// anew first: 1020 x 4096, 64 tokens 8.7 / 23. fp32, whose tiles take terms: 768 x 2048, 64 tokens 9.7 / 24, 128 tokens
+// 16.5 / 24; 4096 x 11008, 64 tokens 221 / 450.
 inline bool gated_few(int64_t N, int64_t d, int64_t F, bool f32) {
   if (f32) return N <= 128;
   if (d % 8) return N <= 64;
   const int64_t weights = 2 * d * F;
-  return N <= 8 || (N <= 16 && weights <= (int64_t)1 << 26) || (N <= 32 && weights <= (int64_t)1 << 25) || (N <= 64 && weights <= (int64_t)1 << 22);
+  return (N <= 16 && weights <= (int64_t)1 << 25) || (N <= 32 && weights <= (int64_t)1 << 22);
 }
 
 // Attention over packed texts (tms_train_attn_kernel.h). Numbers that tiles of `rows` rows may have: those of
