@@ -278,6 +278,23 @@ def test_one_element_in_two_places(cuda):
     assert int(state.steps) == 1 and bool((q < 1).all())
 
 
+def test_some_copies(cuda):
+    """Copies of some parameters, of several types, and parameters of inference mode: each as by itself, versions counted."""
+    import tilemaxsim_amd as tms
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ps, gs = ([torch.randn(n, generator=g, device="cuda") for n in (5, 300, 77, 1)] for _ in range(2))
+    with torch.inference_mode():
+        ps[3] = ps[3].clone()
+    alone = [p.clone() for p in ps]
+    for p, x in zip(alone, gs):
+        tms.adamw_(p, x, tms.AdamWState(p))
+    copies = [None, torch.empty(300, device="cuda", dtype=torch.float16), torch.empty(77, device="cuda", dtype=torch.bfloat16), None]
+    before = [t._version for t in (*ps[:3], *copies[1:3])]
+    tms.adamw_(ps, gs, tms.AdamWState(ps), copies=copies)
+    assert all(torch.equal(a, b) for a, b in zip(ps, alone)) and all(torch.equal(c, p.to(c.dtype)) for c, p in zip(copies[1:3], ps[1:3]))
+    assert all(t._version > v for t, v in zip((*ps[:3], *copies[1:3]), before))
+
+
 def test_nonfinite(cuda):
     """A NaN or infinite gradient goes into its own element alone, in 8 bits too; a NaN norm into all."""
     import tilemaxsim_amd as tms

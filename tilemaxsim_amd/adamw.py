@@ -18,6 +18,7 @@ BLOCK = _lib.TMS_ADAMW_BLOCK
 
 
 _pack = struct.Struct("@8P3q6d").pack  # tms_adamw
+_pointer, _contiguous = torch.Tensor.data_ptr, torch.Tensor.is_contiguous
 
 
 class AdamWState:
@@ -117,7 +118,7 @@ def _kinds(fn: str, name: str, ts: list, dev: torch.device) -> list:
         kinds = [_lib.DTYPE_CODES[t.dtype] for t in ts]
     except KeyError as e:
         raise TypeError(f"{fn}: {name} must be float16, bfloat16 or float32 (got {e.args[0]})") from None
-    if {t.get_device() for t in ts} - {dev.index}:
+    if set(map(torch.Tensor.get_device, ts)) - {dev.index}:
         bad = next(t for t in ts if t.device != dev)
         raise ValueError(f"{fn}: {name} must be on {dev}, where the states are (got {bad.device})")
     return kinds
@@ -186,11 +187,18 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
     _check.no_tangents(fn, [*ps, *gs])
     _shapes_match(fn, "parameters", ps, shapes)
     _shapes_match(fn, "gradients", gs, shapes)
-    given, c_kinds = [], []
-    if cs is not None:
-        given = [(i, c) for i, c in enumerate(cs) if c is not None]
-        c_kinds = _kinds(fn, "copies", [c for _, c in given], dev)
-        _shapes_match(fn, "copies", [c for _, c in given], [shapes[i] for i, _ in given])
+    given = range(0)  # places in the list of what has a copy
+    if cs is None:
+        cs = []
+    else:
+        given = range(len(cs))
+        if any(c is None for c in cs):
+            given = [i for i in given if cs[i] is not None]
+            cs = [cs[i] for i in given]
+            _shapes_match(fn, "copies", cs, [shapes[i] for i in given])
+        else:
+            _shapes_match(fn, "copies", cs, shapes)
+    c_kinds = _kinds(fn, "copies", cs, dev)
     if not ps:
         return
     if isinstance(lr, torch.Tensor):
@@ -199,26 +207,32 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
         norm = _scalar(fn, "norm", norm, dev)
 
     def whole(ts):  # strided tensors are written through copies of their own
-        return [t if t.is_contiguous() else t.contiguous() for t in ts]
+        return ts if all(map(_contiguous, ts)) else [t if t.is_contiguous() else t.contiguous() for t in ts]
 
-    p_to, c_to = whole(ps), whole([c for _, c in given])
-    back = [(t, d) for t, d in zip([*ps, *(c for _, c in given)], [*p_to, *c_to]) if t is not d]
-    if back:
-        at = [t.data_ptr() for t in (*ps, *(c for _, c in given)) if t.numel()]
+    p_to, c_to, g_from = whole(ps), whole(cs), whole(gs)
+    back = []
+    if p_to is not ps or c_to is not cs:
+        back = [(t, d) for t, d in zip([*ps, *cs], [*p_to, *c_to]) if t is not d]
+        at = [t.data_ptr() for t in (*ps, *cs) if t.numel()]
         if len(set(at)) != len(at) or any(s == 0 and n > 1 for t, _ in back for s, n in zip(t.stride(), t.shape)):
             raise ValueError(f"{fn}: two of the tensors (or elements of one) overlap")
-    g_from = whole(gs)
     n = len(ps)
+    copied, kinds = [0] * n, g_kinds
+    if len(given) == n:
+        copied, kinds = map(_pointer, c_to), [g | c << 32 for g, c in zip(g_kinds, c_kinds)]
+    else:
+        kinds = list(g_kinds)
+        for i, c, k in zip(given, c_to, c_kinds):
+            copied[i] = c.data_ptr()
+            kinds[i] |= k << 32
     words = array("q", bytes(56 * n))  # tms_adamw_tensor entries
-    words[0::7] = array("q", [t.data_ptr() for t in p_to])
-    words[1::7] = array("q", [t.data_ptr() for t in g_from])
+    words[0::7] = array("q", map(_pointer, p_to))
+    words[1::7] = array("q", map(_pointer, g_from))
+    words[2::7] = array("q", copied)
     words[3::7] = array("q", sizes)
     words[4::7] = array("q", places)
     words[5::7] = array("q", [i | k << 32 for i, k in zip(indexes, p_kinds)])
-    words[6::7] = array("q", g_kinds)
-    for (i, _), c, k in zip(given, c_to, c_kinds):
-        words[7 * i + 2] = c.data_ptr()
-        words[7 * i + 6] |= k << 32
+    words[6::7] = array("q", kinds)
     factors = torch.empty(4 * len(state.shapes), dtype=torch.float32, device=dev)
     host_lr = 0.0 if isinstance(lr, torch.Tensor) else lr
     described = _pack(state.m.data_ptr(), state.v.data_ptr(), _lib.ptr(state.m_exp) or 0, _lib.ptr(state.v_exp) or 0,
@@ -229,4 +243,8 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
         _lib.check(status)
     for t, d in back:
         t.copy_(d)
-    torch.autograd.graph.increment_version([t for t in (*ps, *(c for _, c in given)) if not t.is_inference()])
+    changed = [*ps, *cs]
+    try:
+        torch.autograd.graph.increment_version(changed)
+    except RuntimeError:  # inference tensors count no versions
+        torch.autograd.graph.increment_version([t for t in changed if not t.is_inference()])
