@@ -7,7 +7,7 @@ inputs' products of three bf16 terms each are off by as much again.
    reciprocal or erfc and three products), slopes to 2^-20 (1 + |g|).
  * h: |u| (1.13 eg + 2^-20 |a|) + |a| eu, and half a step of its type (u).
  * dg: |dh| (|a'| eu + |u| (0.8 eg + 2^-20 (1 + |g|))), du: |dh| (1.13 eg + 2^-20 |a|); both u of
-   themselves more when they are rounded (16 bits), in fp16 at least 2^-25 of the largest |dh|.
+   themselves more when they are rounded (16 bits; up to 64 tokens to two terms, u^2), in fp16 at least 2^-25 of the largest |dh|.
  * The products of those: their errors with the other operand's magnitude, E (n + 4) of the sum of magnitudes
    over n, u of the result, and half of the type's smallest number.
 """
@@ -45,7 +45,7 @@ def functions(g, act):
 def reference(x, wg, wu, G, act):
     dt = x.dtype
     u_, tiny = U[dt], TINY[dt]
-    held = 0.0 if dt == torch.float32 else u_
+    held = 0.0 if dt == torch.float32 else u_ if x.shape[0] > 64 else u_ * u_
     x, wg, wu, G = (t.detach().double() for t in (x, wg, wu, G))
     (N, d), F = x.shape, wg.shape[0]
     g, u = x @ wg.T, x @ wu.T

@@ -21,7 +21,10 @@
 //
 // Precision. g, u, the activation and all sums are fp32; dg and du are rounded to the inputs' type
 // between two products (fp32: three bf16 terms, six products of them), as a product of them
-// would take them. In fp16 they are held times a power of two that brings the largest |dh| to 1 to 2: gradients
+// would take them. The gradients then have two roundings, and an error of 1.4 times that of one: on average, but
+// in few tokens, where few elements make up the norm, of up to twice. Up to 64 tokens dg and du are therefore
+// two 16-bit terms, which the products take as twice as many tokens (a pass of 2 x 384 x 411 in bf16: 19.4 us, 16.5
+// with one; 64 x 4096 x 8192: 163, 145). In fp16 they are held times a power of two that brings the largest |dh| to 1 to 2: gradients
 // as small as a mean over many tokens leaves them keep their digits.
 #include <math.h>
 
@@ -140,9 +143,9 @@ struct GatedEpilogue {
   }
 };
 
-// dg and du, [plane][token][2 half]: dg in columns from 0, du from half on; zeros from F up to the next
+// dg and du, [term][token][2 half]: dg in columns from 0, du from half on; zeros from F up to the next
 // multiple of 32 (what follows is not read, or not used).
-template <int DT, int PL, int MIV>
+template <int DT, bool F32, int TERMS, int MIV>
 struct GatedGradEpilogue {
   static constexpr int NP = MIV / 2;
   static constexpr int kRowBytes = NP * 32 + 16;
@@ -160,7 +163,7 @@ struct GatedGradEpilogue {
   __device__ __forceinline__ void finish(f32x4 (&acc)[MI][NI], int m, int n, uint8_t* lds) const {
     static_assert(MI == MIV, "rows of the wave's LDS");
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
-    typedef typename std::conditional<(PL > 1), float, uint16_t>::type T;
+    typedef typename std::conditional<F32, float, uint16_t>::type T;
     float held = 1.f;
     if constexpr (DT == TMS_DTYPE_F16) held = *factor;
     // The dh of the next 16 tokens are on their way while these are used: one by one, their latencies would take
@@ -189,10 +192,10 @@ struct GatedGradEpilogue {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           float d, slope;
-          if constexpr (PL > 1) d = dhs[j & 1][p].v[e];
+          if constexpr (F32) d = dhs[j & 1][p].v[e];
           else d = from16<DT>(dhs[j & 1][p].v[e]);
           if constexpr (DT == TMS_DTYPE_F16) d *= held;
-          const float y = gated_act<ACT, (PL > 1), true>(acc[2 * p][j][e], slope);
+          const float y = gated_act<ACT, F32, true>(acc[2 * p][j][e], slope);
           acc[2 * p][j][e] = d * acc[2 * p + 1][j][e] * slope;
           acc[2 * p + 1][j][e] = d * y;
         }
@@ -205,7 +208,7 @@ struct GatedGradEpilogue {
 #pragma unroll
       for (int which = 0; which < 2; which++)
 #pragma unroll
-        for (int t = 0; t < PL; t++) {
+        for (int t = 0; t < TERMS; t++) {
 #pragma unroll
           for (int p = 0; p < NP; p++) {
             uint16_t b[4];
@@ -213,7 +216,8 @@ struct GatedGradEpilogue {
             for (int e = 0; e < 4; e++) {
               const float x = acc[2 * p + which][j][e];
               b[e] = to16<DT>(x);
-              if constexpr (PL > 1) acc[2 * p + which][j][e] = x - from16<DT>(b[e]);
+              if constexpr (F32) acc[2 * p + which][j][e] = x - from16<DT>(b[e]);
+              else if constexpr (TERMS > 1) acc[2 * p + which][j][e] = fabsf(from16<DT>(b[e])) < __builtin_inff() ? x - from16<DT>(b[e]) : 0.f;  // not inf - inf
             }
             *(u32x2*)(lds + c * kRowBytes + p * 32 + g * 8) = u32x2{(uint32_t)b[0] | (uint32_t)b[1] << 16, (uint32_t)b[2] | (uint32_t)b[3] << 16};
           }
@@ -466,6 +470,7 @@ __global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x
 struct GatedSpace {
   int64_t x, wg, wu, p, parts, factor, sums, bytes;
   GemmSplit dx, dw;  // how the gradients' products go
+  int terms;         // of dg and du, as that many times the tokens
 };
 constexpr int kMostParts = 256;
 
@@ -474,19 +479,20 @@ static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool b
   Carve c;
   if (!backward && gated_few(N, d, F, dtype == TMS_DTYPE_F32)) return s;
   const int64_t dp = up_to(d, 8);
+  s.terms = backward && dtype != TMS_DTYPE_F32 && N <= kFewTokens ? 2 : 1;
+  if (dtype == TMS_DTYPE_F32 || d % 8 || s.terms > 1) s.x = c.take(N * dp * 2 * planes(dtype) * s.terms);
   if (dtype == TMS_DTYPE_F32 || d % 8) {
-    s.x = c.take(N * dp * 2 * planes(dtype));
     s.wg = c.take(F * dp * 2 * planes(dtype));
     s.wu = c.take(F * dp * 2 * planes(dtype));
   }
   if (backward) {
-    s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype));
+    s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype) * s.terms);
     s.parts = c.take(kMostParts * 4);
     s.factor = c.take(8);
     const int64_t half = up_to(F, 64);
-    s.dx = gemm_split(dp, N, 2 * half, planes(dtype));
-    s.dw = gemm_split(dp, 2 * half, N, planes(dtype));
-    const int64_t one = s.dx.splits > 1 ? s.dx.splits * N : 0, other = s.dw.splits > 1 ? s.dw.splits * 2 * half : 0;
+    s.dx = gemm_split(dp, N * s.terms, 2 * half, planes(dtype));
+    s.dw = gemm_split(dp, 2 * half, N * s.terms, planes(dtype));
+    const int64_t one = s.dx.splits * s.terms > 1 ? s.dx.splits * s.terms * N : 0, other = s.dw.splits > 1 ? s.dw.splits * 2 * half : 0;
     s.sums = c.take((one > other ? one : other) * dp * 4);  // one product after the other
   }
   s.bytes = c.at;
@@ -516,11 +522,11 @@ static int check_gated(const char* fn, const void* x, int64_t N, int64_t d, cons
 struct GatedOperands {
   const uint16_t *x, *wg, *wu;
 };
-// x and both weights as rows of terms, in one launch.
+// x (twice in a row, where dg and du are two terms) and both weights as rows of terms, in one launch.
 struct GatedTerms {
-  const void* src[3];
-  uint16_t* dst[3];
-  int64_t rows[3];
+  const void* src[4];
+  uint16_t* dst[4];
+  int64_t rows[4];
 };
 template <bool F32>
 __global__ __launch_bounds__(256) void gated_terms_kernel(GatedTerms t, int32_t d, int32_t dp) {
@@ -536,12 +542,25 @@ __global__ __launch_bounds__(256) void gated_terms_kernel(GatedTerms t, int32_t 
 static int gated_operands(const void* x, int64_t N, int64_t d, const void* wg, const void* wu, int64_t F, int dtype, uint8_t* ws, const GatedSpace& s,
                           GatedOperands& o, hipStream_t st) {
   o = {(const uint16_t*)x, (const uint16_t*)wg, (const uint16_t*)wu};
-  if (dtype != TMS_DTYPE_F32 && d % 8 == 0) return TMS_OK;
+  const bool all = dtype == TMS_DTYPE_F32 || d % 8;
+  if (!all && s.terms <= 1) return TMS_OK;
   const int64_t dp = up_to(d, 8);
   uint16_t *px = (uint16_t*)(ws + s.x), *pg = (uint16_t*)(ws + s.wg), *pu = (uint16_t*)(ws + s.wu);
-  o = {px, pg, pu};
-  const GatedTerms t = {{x, wg, wu}, {px, pg, pu}, {N, F, F}};
-  const dim3 grid(blocks_for((N > F ? N : F) * dp / 8), 3);
+  GatedTerms t = {};
+  unsigned n = 0;
+  auto lay = [&](const void* src, uint16_t* dst, int64_t rows) {
+    t.src[n] = src, t.dst[n] = dst, t.rows[n] = rows;
+    n++;
+  };
+  lay(x, px, N);
+  if (s.terms > 1) lay(x, px + N * dp, N);
+  o.x = px;
+  if (all) {
+    lay(wg, pg, F);
+    lay(wu, pu, F);
+    o.wg = pg, o.wu = pu;
+  }
+  const dim3 grid(blocks_for((all && F > N ? F : N) * dp / 8), n);
   if (dtype == TMS_DTYPE_F32) hipLaunchKernelGGL(gated_terms_kernel<true>, grid, dim3(256), 0, st, t, (int32_t)d, (int32_t)dp);
   else hipLaunchKernelGGL(gated_terms_kernel<false>, grid, dim3(256), 0, st, t, (int32_t)d, (int32_t)dp);
   return check_launch("gated_terms_kernel");
@@ -599,19 +618,19 @@ static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, co
   return gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (gated)", st);
 }
 
-// A product to rows of d elements, at once or in splits.
+// A product to rows of d elements, at once or in splits; with terms > 1, of so many times `all` rows, summed.
 template <int DT, int PL, int OUT, bool BO, int PAIR>
-static int gated_rows(GemmArgs b, GemmSplit plan, int64_t all, int64_t half, int64_t rows, int64_t d, int64_t dp, const float* factor, float* sums, void* out,
+static int gated_rows(GemmArgs b, GemmSplit plan, int terms, int64_t all, int64_t half, int64_t rows, int64_t d, int64_t dp, const float* factor, float* sums, void* out,
                       void* out2, const char* what, hipStream_t st) {
   b.splits = plan.splits;
-  if (plan.splits == 1) {
+  if (plan.splits * terms == 1) {
     const GatedRowsEpilogue<OUT> e = {out, out2, factor, (int32_t)rows, (int32_t)half, (int32_t)d};
     return gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   }
-  const GatedSumEpilogue e = {sums, all * dp, (int32_t)all, (int32_t)dp};
+  const GatedSumEpilogue e = {sums, terms * all * dp, (int32_t)(terms * all), (int32_t)dp};
   const int rc = gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   if (rc) return rc;
-  hipLaunchKernelGGL(gated_join_kernel<OUT>, dim3(blocks_for(all * ((d + 3) / 4))), dim3(256), 0, st, sums, plan.splits, all * dp, (int32_t)all,
+  hipLaunchKernelGGL(gated_join_kernel<OUT>, dim3(blocks_for(all * ((d + 3) / 4))), dim3(256), 0, st, sums, plan.splits * terms, all * dp, (int32_t)all,
                      (int32_t)half, (int32_t)rows, (int32_t)d, (int32_t)dp, factor, out, out2);
   return check_launch("gated_join_kernel");
 }
@@ -636,10 +655,14 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
   }
   const float* back = factor ? factor + 1 : nullptr;
   const GemmArgs a = gated_args(o, N, F, dp);
-  auto epi = [&](auto z) {
-    return GatedGradEpilogue<DT, PL, decltype(z)::MI>{grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
+  auto form = [&](auto terms) {
+    auto epi = [&](auto z) {
+      return GatedGradEpilogue<DT, (PL > 1), decltype(terms)::value, decltype(z)::MI>{grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
+    };
+    return gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (dg, du)", st);
   };
-  rc = gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (dg, du)", st);
+  if (PL == 1 && s.terms > 1) rc = form(std::integral_constant<int, PL == 1 ? 2 : PL>());
+  else rc = form(std::integral_constant<int, PL>());
   if (rc) return rc;
   if (dx) {  // m over d, n over tokens, k over F columns of dg and du and the rows of Wg and Wu
     GemmArgs b = {};
@@ -651,10 +674,10 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.lda = (int32_t)dp;
     b.ldb = b.K = (int32_t)(2 * half);
     b.M = (int32_t)dp;
-    b.N = (int32_t)N;
+    b.N = (int32_t)(N * s.terms);
     b.half = (int32_t)half;
     b.real = (int32_t)F;
-    rc = gated_rows<DT, PL, OUT, false, kPairDepth>(b, s.dx, N, 0x7fffffff, N, d, dp, back, (float*)(ws + s.sums), dx, nullptr, "train_gemm_kernel (dx)", st);
+    rc = gated_rows<DT, PL, OUT, false, kPairDepth>(b, s.dx, s.terms, N, 0x7fffffff, N, d, dp, back, (float*)(ws + s.sums), dx, nullptr, "train_gemm_kernel (dx)", st);
     if (rc) return rc;
   }
   if (dwg || dwu) {  // m over d, n over F columns of dg and du, k over tokens
@@ -666,8 +689,8 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.lda = (int32_t)dp;
     b.ldb = b.N = (int32_t)(2 * half);
     b.M = (int32_t)dp;
-    b.K = (int32_t)N;
-    rc = gated_rows<DT, PL, OUT, true, kSingle>(b, s.dw, 2 * half, half, F, d, dp, back, (float*)(ws + s.sums), dwg, dwu, "train_gemm_kernel (dWg, dWu)", st);
+    b.K = (int32_t)(N * s.terms);
+    rc = gated_rows<DT, PL, OUT, true, kSingle>(b, s.dw, 1, 2 * half, half, F, d, dp, back, (float*)(ws + s.sums), dwg, dwu, "train_gemm_kernel (dWg, dWu)", st);
   }
   return rc;
 }
