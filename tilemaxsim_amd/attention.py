@@ -143,7 +143,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
         there, and in other texts, is not seen, NaN included.
 
     Scores, softmax and sums are fp32; probabilities and their gradients are rounded to the
-    inputs' type between two products. Every sum has one order.
+    inputs' type between two products (backward, where texts are short, to two terms of it). Every sum has one order.
     """
     fn = "packed_attention"
     usual = _usual(q, k, v, offsets)

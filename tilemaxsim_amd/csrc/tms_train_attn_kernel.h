@@ -39,7 +39,7 @@
 //
 // Precision. Scores, statistics, sums and gradients are fp32. P and dS are rounded to the
 // inputs' type between two products (2^-9 of each term in bf16, 2^-12 in fp16), as the matrix
-// cores take them. fp16 has no range to spare for gradients: P is held times 2^15, and dS times
+// cores take them; where most texts are short, to two terms in the backward pass. fp16 has no range to spare for gradients: P is held times 2^15, and dS times
 // a power of two for each row (column of sums) that follows the largest |dS| so far. delta is
 // taken from o in two 16-bit terms (2^-17 of it): from o as it is returned, dS would have o's rounding
 // even where P is 1 and dS 0. fp32 goes through the fp32 matrix instructions.
@@ -146,6 +146,8 @@ __device__ __forceinline__ typename AttnType<DT>::Frag attn_pack(f32x4 lo, f32x4
 }
 
 template <int DT>
+__device__ __forceinline__ typename AttnType<DT>::E attn_round(float x);
+template <int DT>
 __device__ __forceinline__ float attn_float(typename AttnType<DT>::E x) {
   if constexpr (DT == TMS_DTYPE_F32) return x;
   else if constexpr (DT == TMS_DTYPE_F16) return (float)__builtin_bit_cast(_Float16, x);
@@ -156,6 +158,16 @@ __device__ __forceinline__ typename AttnType<DT>::E attn_round(float x) {
   if constexpr (DT == TMS_DTYPE_F32) return x;
   else if constexpr (DT == TMS_DTYPE_F16) return __builtin_bit_cast(uint16_t, (_Float16)x);
   else return __builtin_bit_cast(uint16_t, (__bf16)x);
+}
+// What attn_pack's rounding leaves of the values, in the inputs' type.
+template <int DT>
+__device__ __forceinline__ typename AttnType<DT>::Frag attn_rest(f32x4 lo, f32x4 hi) {
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    lo[e] -= attn_float<DT>(attn_round<DT>(lo[e]));
+    hi[e] -= attn_float<DT>(attn_round<DT>(hi[e]));
+  }
+  return attn_pack<DT>(lo, hi);
 }
 // Element e of a fragment.
 template <int DT>
@@ -741,13 +753,16 @@ __device__ __forceinline__ void attn_store(void* out, int64_t at, const f32x4 (&
 // delta and dq: a workgroup has a tile of queries and goes over their keys. SHORT: texts of one tile of keys
 // have their delta from P and dP, before dS is formed: where few keys share a row, o's own error (P is
 // rounded there) would be as large as that of dS's rounding. (For all: 128 documents of 32 to 300 tokens take 70 us
-// and not 62.)
+// and not 62.) And dS goes into its products as two 16-bit terms, as do P and dS in the kernel for dk and dv: where
+// few elements make up a gradient's norm, one rounding more than its own can be twice the error (256 texts of 64, 12 heads of
+// 64: 48 and 61 us, 46 and 58 with one term; 1024 of 16: 74 and 93, 72 and 88).
 template <int DT, int D, int NB, int KIND, bool SHORT>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDq)> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
   constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BQ = 64 * NB;
+  constexpr bool TWO = SHORT && DT != TMS_DTYPE_F32;
   extern __shared__ __attribute__((aligned(1024))) uint8_t attn_mem[];
   int slot, head;
   if (!attn_place(a, a.H, slot, head)) return;
@@ -907,17 +922,21 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
 #pragma unroll
               for (int e = 0; e < 4; e++) s[i][j][e] = k0 + 32 * h + 16 * i + 4 * g + e < sees[j] ? s[i][j][e] : 0.f;
         }
-        Frag ds[NB];
+        Frag ds[NB], rest[NB];
 #pragma unroll
         for (int j = 0; j < NB; j++) {
           if constexpr (DT == TMS_DTYPE_F16) range[j].follow(s[0][j], s[1][j], acc, j);
           ds[j] = attn_pack<DT>(s[0][j], s[1][j]);
+          if constexpr (TWO) rest[j] = attn_rest<DT>(s[0][j], s[1][j]);
         }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
           const Frag f = Rows::col_frag(lk, h, d, c, g);
 #pragma unroll
-          for (int j = 0; j < NB; j++) acc[d][j] = attn_mfma<DT>(f, ds[j], acc[d][j]);
+          for (int j = 0; j < NB; j++) {
+            acc[d][j] = attn_mfma<DT>(f, ds[j], acc[d][j]);
+            if constexpr (TWO) acc[d][j] = attn_mfma<DT>(f, rest[j], acc[d][j]);
+          }
         }
       }
     }
@@ -934,11 +953,12 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
 // dk and dv: a workgroup has a tile of keys and goes over the queries that see them, head by head of
 // those that share the keys. Both gradients' sums are as many registers as the keys and values: more than two
 // workgroups a CU spill (heads of 128, a bound of three: 166 us, 118 with two).
-template <int DT, int D, int NB, int KIND>
+template <int DT, int D, int NB, int KIND, bool SHORT>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDkv)> Rows;
   typedef typename AttnType<DT>::E E;
   typedef typename AttnType<DT>::Frag Frag;
+  constexpr bool TWO = SHORT && DT != TMS_DTYPE_F32;
   constexpr int R = Rows::R, DB = D / 16, KS = D / 32, BK = 64 * NB;
   extern __shared__ __attribute__((aligned(1024))) uint8_t attn_mem[];
   float* const stats = (float*)(attn_mem + 4 * Rows::kBytes);  // [buffer][lse, delta][R]
@@ -1074,12 +1094,16 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
                 s[i][j][e] = in ? s[i][j][e] : 0.f;
               }
         }
-        Frag pf[NB], sf[NB];
+        Frag pf[NB], sf[NB], prest[NB], srest[NB];
 #pragma unroll
         for (int j = 0; j < NB; j++) {
           if constexpr (DT == TMS_DTYPE_F16) range[j].follow(s[0][j], s[1][j], dk, j);
           pf[j] = attn_pack<DT>(p[0][j], p[1][j]);
           sf[j] = attn_pack<DT>(s[0][j], s[1][j]);
+          if constexpr (TWO) {
+            prest[j] = attn_rest<DT>(p[0][j], p[1][j]);
+            srest[j] = attn_rest<DT>(s[0][j], s[1][j]);
+          }
         }
 #pragma unroll
         for (int d = 0; d < DB; d++) {
@@ -1088,6 +1112,10 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
           for (int j = 0; j < NB; j++) {
             dv[d][j] = attn_mfma<DT>(fg, pf[j], dv[d][j]);
             dk[d][j] = attn_mfma<DT>(fq, sf[j], dk[d][j]);
+            if constexpr (TWO) {
+              dv[d][j] = attn_mfma<DT>(fg, prest[j], dv[d][j]);
+              dk[d][j] = attn_mfma<DT>(fq, srest[j], dk[d][j]);
+            }
           }
         }
       }
@@ -1156,7 +1184,13 @@ static int attn_launch(AttnArgs a, hipStream_t st) {
     hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, false>), grid, threads, lds, st, a);
     return check_launch("attn_dq_kernel");
   } else {
-    hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND>), grid, threads, lds + 4 * Rows::R * sizeof(float), st, a);
+    constexpr size_t both = lds + 4 * Rows::R * sizeof(float);
+    bool few = false;
+    if constexpr (NB == 1 && DT != TMS_DTYPE_F32) {
+      few = attn_short(a.T, a.B);
+      if (few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, true>), grid, threads, both, st, a);
+    }
+    if (!few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, false>), grid, threads, both, st, a);
     const int rc = check_launch("attn_dkv_kernel");
     if (rc || a.parts == 1) return rc;
     const int64_t n = a.T * a.KV * D, groups = (n / 2 + kAttnThreads - 1) / kAttnThreads;

@@ -98,7 +98,7 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, acti
 
     Both products, the activation and all sums are fp32, rounded once. The backward pass forms
     both products again instead of keeping them; the gradients of the two are rounded to the
-    inputs' type (float32: three bf16 terms) before the products that they go into.
+    inputs' type (float32: three bf16 terms; up to 64 tokens: two terms) before the products that they go into.
     """
     fn = "gated_linear"
     usual = _usual(x, w_gate, w_up)
