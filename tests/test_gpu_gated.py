@@ -142,6 +142,27 @@ def test_gradients_of_any_size(cuda, size):
     check(200, 64, 96, torch.float16, "silu", seed=4, size=size)
 
 
+@pytest.mark.parametrize("size", [2.0 ** -20, 1.0, 2.0 ** 9])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float16], ids=str)
+def test_gradients_of_few_tokens(cuda, dt, size):
+    """Two terms of dg and du: zeros, one large row among small ones, and infinities that stay where they are."""
+    import tilemaxsim_amd as tms
+    for N in (1, 40, 64):
+        check(N, 64, 96, dt, "gelu", seed=6, size=size)
+    ts, G = make(40, 72, 50, dt, seed=8, size=size)
+    with torch.no_grad():
+        G[1:] *= 2.0 ** -8
+        G[5] = 0
+    grads = torch.autograd.grad(tms.gated_linear(*ts), ts, G)
+    close((tms.gated_linear(*ts).detach(), *grads), reference(*ts, G, "silu"), f"one large row {dt}")
+    with torch.no_grad():
+        G[7, 3] = math.inf
+    again = torch.autograd.grad(tms.gated_linear(*ts), ts, G)
+    keep = torch.arange(50, device="cuda") != 3
+    assert not torch.isfinite(again[0][7]).any() and bool(torch.isfinite(again[0][torch.arange(40, device="cuda") != 7]).all())
+    assert all(not torch.isfinite(w[3]).any() and bool(torch.isfinite(w[keep]).all()) for w in again[1:])
+
+
 def test_empty(cuda):
     import tilemaxsim_amd as tms
     for N, F in ((0, 16), (5, 0), (0, 0)):

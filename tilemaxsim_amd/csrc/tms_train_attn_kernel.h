@@ -27,11 +27,11 @@
 //
 // What bounds them. Long texts: issue. A score takes about seven vector instructions, one of them an exponential,
 // beside its products, and the two take turns rather than overlap. Two texts of 8192 tokens under biases, 12 heads of 64, in
-// bf16: forward 432 us, dq 508, dk and dv 694; vector instructions issue for 56, 41 and 39 % of the time, matrix
+// bf16: forward 434 us, dq 513, dk and dv 701; vector instructions issue for 56, 41 and 39 % of the time, matrix
 // cores are busy for 25, 32 and 31 %, without a bank conflict. Without a bias, 8 heads over texts of 8192 (16,384 tokens):
 // 367, 395 and 521 us in heads of 64 (0.75, 1.05 and 1.06 PFLOP/s, the products formed again counted),
 // 565, 690 and 1,165 in heads of 128 (0.97, 1.2, 0.94). Short texts: the way to a tile's first products. 128 texts
-// of 32 to 300 tokens, 12 heads of 64: 66, 69 and 92 us, where their bytes take 81 for all three at a copy's rate.
+// of 32 to 300 tokens, 12 heads of 64: 67, 71 and 96 us, where their bytes take 81 for all three at a copy's rate.
 //
 // In LDS a row of 32 elements takes 64 bytes (fp32: 128), two rows a line of 128, whose 16-byte
 // pieces stand at p ^ (line % 8): the row fragments (a lane's eight neighbouring elements) and the

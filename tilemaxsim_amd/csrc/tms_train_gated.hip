@@ -6,13 +6,13 @@
 //
 // The forward pass is one matrix product whose tiles take 16 rows of Wg and 16 of Wu in turn, so
 // that a wave has g and u of the same places in its registers. The backward pass forms them
-// again (4 N F d operations, where keeping them would write and read 8 N F bytes in 16 bits: at d =
-// 768 as long), with an epilogue that leaves dg and du side by side, (N, 2 F), in 16 bits; two more
+// again (4 N F d operations, 260 us at 16384 x 1024 x 4096, where keeping them in 16 bits would take 110 of memory's
+// time, 4 N F bytes and one rounding more), with an epilogue that leaves dg and du side by side, (N, 2 F), in 16 bits; two more
 // products take them to dx (k over both, and over Wg and Wu one behind the other) and to both
 // weights' gradients (their rows one behind the other).
 //
-// Bound by the matrix cores, the tiles' ends behind them. 16,384 tokens, 1024 x 4096, bf16: forward 270 us (1.02 PFLOP/s), dg
-// and du 322 (their ends form two functions and write 268 MB), dx 274, both weights' gradients 267 and 14 for
+// Bound by the matrix cores, the tiles' ends behind them. 16,384 tokens, 1024 x 4096, bf16: forward 267 us (1.03 PFLOP/s), dg
+// and du 317 (their ends form two functions and write 268 MB), dx 269, both weights' gradients 273 and 14 for
 // the join of two splits. 1229 x 768 x 2043: 16, 22, 18 + 5 and 17 us, where tiles of 128 fill the chip once
 // and a quarter, or less than once (two steps a wait).
 //
