@@ -39,7 +39,8 @@
 //
 // Precision. Scores, statistics, sums and gradients are fp32. P and dS are rounded to the
 // inputs' type between two products (2^-9 of each term in bf16, 2^-12 in fp16), as the matrix
-// cores take them; where most texts are short, to two terms in the backward pass. fp16 has no range to spare for gradients: P is held times 2^15, and dS times
+// cores take them; where most texts are short, to two terms in the backward pass. fp16 has no range to spare: P is held times 2^15 in all three
+// kernels (a key e^-17 below a row's best is nothing in fp16 as it is, and 16,000 of them half a step of o), and dS times
 // a power of two for each row (column of sums) that follows the largest |dS| so far. delta is
 // taken from o in two 16-bit terms (2^-17 of it): from o as it is returned, dS would have o's rounding
 // even where P is 1 and dS 0. fp32 goes through the fp32 matrix instructions.
@@ -57,7 +58,11 @@ typedef _Float16 attn_f16x2 __attribute__((ext_vector_type(2)));
 constexpr int kAttnThreads = 256;
 constexpr float kAttnLog2e = 1.4426950408889634f;
 constexpr float kAttnNothing = 160.f;  // so many powers of two below, exp2 is 0
-constexpr int kAttnP16 = 15;  // fp16: P times 2^15 in the backward pass
+// P is held times 2^this between two products.
+template <int DT>
+constexpr int attn_up() {
+  return DT == TMS_DTYPE_F16 ? 15 : 0;
+}
 
 constexpr int kAttnNorms = 64;  // numbers a head
 
@@ -654,7 +659,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
       }
       float ref[NB];
 #pragma unroll
-      for (int j = 0; j < NB; j++) ref[j] = (top[j] == NEG ? 0.f : top[j]) - shift[j];
+      for (int j = 0; j < NB; j++) ref[j] = (top[j] == NEG ? 0.f : top[j]) - shift[j] - (float)attn_up<DT>();
 #pragma unroll
       for (int h = 0; h < R / 32; h++) {  // 32 keys at a time
         Frag p[NB];
@@ -688,7 +693,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
     z += __shfl_xor(z, 16);
     z += __shfl_xor(z, 32);
     const float inv = t.real ? 1.f / z : 0.f;
-    if (a.lse && g == 0) a.lse[(int64_t)head * a.T + row] = t.real ? top[j] + log2f(z) : __builtin_inff();
+    if (a.lse && g == 0) a.lse[(int64_t)head * a.T + row] = t.real ? top[j] + (log2f(z) - (float)attn_up<DT>()) : __builtin_inff();
     const int64_t at = ((int64_t)row * a.H + head) * D;
 #pragma unroll
     for (int d = 0; d < DB; d++) {
@@ -1079,7 +1084,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
               const float ref = KIND == kAttnBias ? lse[e] + shift[j] : lse[e];
               const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[i][j][e], score.unit, ref));
               s[i][j][e] = y * dp[j][e];
-              p[i][j][e] = DT == TMS_DTYPE_F16 ? y * (float)(1 << kAttnP16) : y;
+              p[i][j][e] = y * (float)(1 << attn_up<DT>());
             }
         }
         if (part) {
@@ -1127,7 +1132,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     if (key >= t.end) continue;
     const int64_t at = ((int64_t)key * a.KV + kvh) * D;
     const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
-    const float fv = !t.real ? 0.f : DT == TMS_DTYPE_F16 ? 1.f / (float)(1 << kAttnP16) : 1.f;
+    const float fv = !t.real ? 0.f : 1.f / (float)(1 << attn_up<DT>());
     if (a.parts > 1) {
       const int64_t one = a.T * a.KV * D;
       attn_store<TMS_DTYPE_F32>(a.sums + 2 * part_of * one, at, dk, j, fk, g);
