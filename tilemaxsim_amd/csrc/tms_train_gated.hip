@@ -24,8 +24,9 @@
 // would take them. The gradients then have two roundings, and an error of 1.4 times that of one: on average, but
 // in few tokens, where few elements make up the norm, of up to twice. Up to 64 tokens dg and du are therefore
 // two 16-bit terms, which the products take as twice as many tokens (a pass of 2 x 384 x 411 in bf16: 19.4 us, 16.5
-// with one; 64 x 4096 x 8192: 163, 145). In fp16 they are held times a power of two that brings the largest |dh| to 1 to 2: gradients
-// as small as a mean over many tokens leaves them keep their digits.
+// with one; 64 x 4096 x 8192: 163, 145). In fp16 they are held times a power of two that brings a bound of them,
+// from the largest |dh| and the norms of x and of the weights, to 2^14 to 2^15: gradients as small as a mean over many tokens
+// leaves them keep their digits, and a factor beyond fp16's range, as u may be where act(g) is small, does not overflow.
 #include <math.h>
 
 #include "tms_train_terms.h"
@@ -340,54 +341,110 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int 
   }
 }
 
-// The largest |dh| of fp16 (its bits are ordered like its value; NaN above all), a part a workgroup. 1229 x 2043: 4 us,
-// and 2 for the factor.
-__global__ __launch_bounds__(256) void gated_most_kernel(const uint16_t* x, int64_t n, uint32_t* parts) {
-  __shared__ uint32_t lds[4];
-  uint32_t most = 0;
-  const int64_t whole = n / 8;
-  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < whole; k += (int64_t)gridDim.x * 256) {
-    const u32x4 v = *(const u32x4*)(x + k * 8);
+// What fp16's dg and du are bounded by: |dg| <= 1.13 |dh| |u|, |du| <= |dh| |g| (no activation is further from 0 than its
+// argument, or steeper than 1.13), and |g|, |u| <= |x| |w| for the norms of the token's row and the weight's. A workgroup has
+// tokens (their largest |dh| times |x|: `parts`), or four rows of weights at a time (squares of their norms: `parts` from
+// kBoundTokens on). What is not finite is passed over: it makes its own rows what it will. 1229 x 768 x 2043: 6.2 us, 2.7 for
+// the factor.
+constexpr int kBoundTokens = 2048, kBoundWeights = 1024;
+constexpr float kBoundSlope = 1.2f;
+
+__device__ __forceinline__ float gated_finite(float x) { return x < __builtin_inff() ? x : 0.f; }  // 0 for NaN, too
+
+// Thread `t` of `all`'s share of a row of n elements: f(bits) for each.
+template <class F>
+__device__ __forceinline__ void gated_row(const uint16_t* row, int n, int t, int all, F&& f) {
+  for (int k = t * 8; k < n; k += all * 8) {
+    if (k + 8 <= n) {
+      const GatedVec<uint16_t, 8> v = *(const GatedVec<uint16_t, 8>*)(row + k);
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const uint32_t lo = v[e] & 0x7fffu, hi = v[e] >> 16 & 0x7fffu;
-      most = lo > most ? lo : most;
-      most = hi > most ? hi : most;
+      for (int e = 0; e < 8; e++) f(v.v[e]);
+    } else {
+      for (int e = k; e < n; e++) f(row[e]);
     }
   }
-  if (blockIdx.x == 0 && threadIdx.x < n % 8) {
-    const uint32_t y = x[whole * 8 + threadIdx.x] & 0x7fffu;
-    most = y > most ? y : most;
-  }
-#pragma unroll
-  for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t y = __shfl_xor(most, o);
-    most = y > most ? y : most;
-  }
-  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = most;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int w = 1; w < 4; w++) most = lds[w] > most ? lds[w] : most;
-    parts[blockIdx.x] = most;
-  }
 }
-// factor[0]: the power of two that brings it to 1 to 2 (1 for zeros, infinities and NaN); factor[1]: its reciprocal.
-__global__ __launch_bounds__(64) void gated_factor_kernel(const uint32_t* parts, int n, float* factor) {
-  uint32_t most = 0;
-  for (int i = threadIdx.x; i < n; i += 64) most = parts[i] > most ? parts[i] : most;
+__device__ __forceinline__ float gated_square_of(const uint16_t* row, int n, int t, int all) {
+  float s = 0.f;
+  gated_row(row, n, t, all, [&](uint16_t x) {
+    const float y = from16<TMS_DTYPE_F16>(x);
+    s = __builtin_fmaf(y, y, s);
+  });
+  return s;
+}
+__global__ __launch_bounds__(256) void gated_bounds_kernel(const uint16_t* dh, const uint16_t* x, const uint16_t* wg, const uint16_t* wu, int32_t N, int32_t d,
+                                                           int32_t F, int32_t tokens, float* parts) {
+  __shared__ float lds[2][4];
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  float most = 0.f;
+  if ((int)blockIdx.x < tokens) {
+    for (int64_t n = blockIdx.x; n < N; n += tokens) {
+      uint32_t top = 0;
+      gated_row(dh + n * F, F, t, 256, [&](uint16_t y) {
+        const uint32_t a = y & 0x7fffu;
+        top = a < 0x7c00u && a > top ? a : top;
+      });
+      float h = from16<TMS_DTYPE_F16>((uint16_t)top), s = gated_square_of(x + n * d, d, t, 256);
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) {
+        h = fmaxf(h, __shfl_xor(h, o));
+        s += __shfl_xor(s, o);
+      }
+      __syncthreads();  // the last token's have been read
+      if (lane == 0) lds[0][wave] = h, lds[1][wave] = s;
+      __syncthreads();
+      h = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+      s = (lds[1][0] + lds[1][1]) + (lds[1][2] + lds[1][3]);
+      most = fmaxf(most, gated_finite(h * sqrtf(s)));
+    }
+    if (t == 0) parts[blockIdx.x] = most;
+    return;
+  }
+  for (int64_t r = (int64_t)(blockIdx.x - tokens) * 4 + wave; r < 2 * (int64_t)F; r += (int64_t)(gridDim.x - tokens) * 4) {
+    float s = gated_square_of(r < F ? wg + r * d : wu + (r - F) * d, d, lane, 64);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s += __shfl_xor(s, o);
+    most = fmaxf(most, gated_finite(s));
+  }
+  if (lane == 0) lds[0][wave] = most;
+  __syncthreads();
+  if (t == 0) parts[kBoundTokens + (int)blockIdx.x - tokens] = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+}
+// The largest of both kinds of parts in all of the workgroup's threads.
+__device__ __forceinline__ void gated_largest(const float* parts, int tokens, int weights, float& h, float& w) {
+  __shared__ float lds[2][4];
+  h = w = 0.f;
+#pragma unroll
+  for (int k = 0; k < kBoundTokens / 256; k++) {
+    const int i = k * 256 + (int)threadIdx.x;
+    h = fmaxf(h, i < tokens ? parts[i] : 0.f);
+  }
+#pragma unroll
+  for (int k = 0; k < kBoundWeights / 256; k++) {
+    const int i = k * 256 + (int)threadIdx.x;
+    w = fmaxf(w, i < weights ? parts[kBoundTokens + i] : 0.f);
+  }
 #pragma unroll
   for (int o = 32; o >= 1; o >>= 1) {
-    const uint32_t y = __shfl_xor(most, o);
-    most = y > most ? y : most;
+    h = fmaxf(h, __shfl_xor(h, o));
+    w = fmaxf(w, __shfl_xor(w, o));
   }
-  if (threadIdx.x != 0) return;
-  int e = 0;
-  if (most != 0 && most < 0x7c00u) {
-    const uint32_t bits = __builtin_bit_cast(uint32_t, from16<TMS_DTYPE_F16>((uint16_t)most));
-    e = (int)(bits >> 23) - 127;
-  }
-  factor[0] = __builtin_bit_cast(float, (uint32_t)(127 - e) << 23);
-  factor[1] = __builtin_bit_cast(float, (uint32_t)(127 + e) << 23);
+  if ((threadIdx.x & 63) == 0) lds[0][threadIdx.x >> 6] = h, lds[1][threadIdx.x >> 6] = w;
+  __syncthreads();
+  h = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
+  w = fmaxf(fmaxf(lds[1][0], lds[1][1]), fmaxf(lds[1][2], lds[1][3]));
+}
+// The exponent of the power of two that brings x > 0 to 2^14 to 2^15: half of fp16's range, so that rounding stays within it.
+__device__ __forceinline__ int gated_up(float x) { return 14 + 127 - (int)(__builtin_bit_cast(uint32_t, x) >> 23); }
+__device__ __forceinline__ float gated_power(int e) { return e < -126 ? 0.f : __builtin_bit_cast(float, (uint32_t)(127 + (e > 127 ? 127 : e)) << 23); }
+
+// factor[0]: the power of two that dg and du are held times; factor[1]: its reciprocal.
+__global__ __launch_bounds__(256) void gated_factor_kernel(const float* parts, int tokens, int weights, float* factor) {
+  float h, w;
+  gated_largest(parts, tokens, weights, h, w);
+  const float bound = kBoundSlope * h * sqrtf(w);
+  const int e = bound > 0.f ? gated_up(bound) : 0;
+  if (threadIdx.x == 0) factor[0] = gated_power(e), factor[1] = gated_power(-e);
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -472,7 +529,6 @@ struct GatedSpace {
   GemmSplit dx, dw;  // how the gradients' products go
   int terms;         // of dg and du, as that many times the tokens
 };
-constexpr int kMostParts = 256;
 
 static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool backward) {
   GatedSpace s = {};
@@ -487,7 +543,7 @@ static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool b
   }
   if (backward) {
     s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype) * s.terms);
-    s.parts = c.take(kMostParts * 4);
+    s.parts = c.take((kBoundTokens + kBoundWeights) * 4);
     s.factor = c.take(8);
     const int64_t half = up_to(F, 64);
     s.dx = gemm_split(dp, N * s.terms, 2 * half, planes(dtype));
@@ -646,11 +702,12 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
   float* factor = nullptr;
   if (DT == TMS_DTYPE_F16) {
     factor = (float*)(ws + s.factor);
-    const int64_t groups = (N * F / 8 + 255) / 256;
-    const int parts = (int)(groups < 1 ? 1 : groups > kMostParts ? kMostParts : groups);
-    hipLaunchKernelGGL(gated_most_kernel, dim3(parts), dim3(256), 0, st, (const uint16_t*)grad, N * F, (uint32_t*)(ws + s.parts));
-    if ((rc = check_launch("gated_most_kernel"))) return rc;
-    hipLaunchKernelGGL(gated_factor_kernel, dim3(1), dim3(64), 0, st, (const uint32_t*)(ws + s.parts), parts, factor);
+    const int tokens = (int)(N < kBoundTokens ? N : kBoundTokens), rows = (int)((2 * F + 3) / 4), weights = rows < kBoundWeights ? rows : kBoundWeights;
+    float* parts = (float*)(ws + s.parts);
+    hipLaunchKernelGGL(gated_bounds_kernel, dim3((unsigned)(tokens + weights)), dim3(256), 0, st, (const uint16_t*)grad, (const uint16_t*)x, (const uint16_t*)wg,
+                       (const uint16_t*)wu, (int32_t)N, (int32_t)d, (int32_t)F, tokens, parts);
+    if ((rc = check_launch("gated_bounds_kernel"))) return rc;
+    hipLaunchKernelGGL(gated_factor_kernel, dim3(1), dim3(256), 0, st, (const float*)parts, tokens, weights, factor);
     if ((rc = check_launch("gated_factor_kernel"))) return rc;
   }
   const float* back = factor ? factor + 1 : nullptr;
