@@ -1,7 +1,10 @@
-"""The gated projection's gradients in fp16 where dg and du leave its range.
+"""The gated projection's gradients in fp16 where dg and du leave its range, above or below.
 
-Tolerances as in test_gpu_gated.py but for what is below fp16's normal numbers: 2^-38 of a token's largest |dh| times the
-norm of its row of x and the largest of the weights' rows."""
+Tolerances as in test_gpu_gated.py but for what is below fp16's normal numbers. dg and du of a token are held times a
+power of two that brings a bound of them, 1.2 max |dh| |x| max |W| with the norms of the token's row and of the weights'
+rows, to 2^14 to 2^15: what is lost is half of fp16's smallest number over that power, 2^-25 2^-14 1.2 max |dh| |x| |W|, less
+than 2^-38 of the product. The weights' gradients take x over that power, times one that brings the largest bound times |x| to
+2^14 to 2^15: 2^-25 lost of it, over 2^14 2^14 and times up to 2^15 of a bound, 2^-38 1.2 of the largest max |dh| |x|^2 |W| for each token."""
 import math
 
 import pytest
@@ -72,6 +75,20 @@ def test_large_factors(cuda, N, d, F, act):
         wg[:, 0] = torch.linspace(-600, 600, F, device="cuda").to(F16)
         G.mul_(2.0 ** -14)
     check(ts, G, act, f"g of 120,000, {N} x {d} x {F} {act}")
+
+
+@pytest.mark.parametrize("N,d,F", [(3, 64, 96), (40, 64, 96), (64, 77, 50), (200, 64, 96), (200, 77, 50), (300, 264, 600)])
+@pytest.mark.parametrize("below", [2.0 ** -14, 2.0 ** -18, 2.0 ** -22])
+@pytest.mark.parametrize("size", [2.0 ** 5, 1.0, 2.0 ** -4])
+def test_rows_far_below_others(cuda, size, below, N, d, F):
+    """Tokens whose gradients are far below the largest: each row's own gradient keeps its digits."""
+    ts, G = make(N, d, F, F16, seed=5, size=size)
+    with torch.no_grad():
+        G[1::3] *= below
+        G[2::3] *= math.sqrt(below)
+        if N > 3:
+            G[5] = 0
+    check(ts, G, "silu", f"rows of {below} below {size}, {N} x {d} x {F}")
 
 
 @pytest.mark.parametrize("N", [40, 200])

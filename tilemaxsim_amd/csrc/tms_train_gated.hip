@@ -24,9 +24,12 @@
 // would take them. The gradients then have two roundings, and an error of 1.4 times that of one: on average, but
 // in few tokens, where few elements make up the norm, of up to twice. Up to 64 tokens dg and du are therefore
 // two 16-bit terms, which the products take as twice as many tokens (a pass of 2 x 384 x 411 in bf16: 19.4 us, 16.5
-// with one; 64 x 4096 x 8192: 163, 145). In fp16 they are held times a power of two that brings a bound of them,
-// from the largest |dh| and the norms of x and of the weights, to 2^14 to 2^15: gradients as small as a mean over many tokens
-// leaves them keep their digits, and a factor beyond fp16's range, as u may be where act(g) is small, does not overflow.
+// with one; 64 x 4096 x 8192: 163, 145). In fp16 a token's are held times a power of two that
+// brings a bound of them, from its largest |dh| and the norms of its x and of the weights, to 2^14 to 2^15: a factor beyond
+// fp16's range, as u may be where act(g) is small, does not overflow, and a token whose gradients are far below another's (a loss
+// that only some tokens reach leaves many such) keeps its digits. dx takes the power out of its rows; the weights'
+// gradients, whose sums go over the tokens, take x over it, in fp16 times one power for all: what that loses of a token is
+// 2^-38 of the largest bound there is.
 #include <math.h>
 
 #include "tms_train_terms.h"
@@ -152,7 +155,7 @@ struct GatedGradEpilogue {
   static constexpr int kRowBytes = NP * 32 + 16;
   const void* grad;     // (rows, F), of the inputs' type
   uint16_t* P;
-  const float* factor;  // fp16: what they are held times
+  const float* held;  // fp16: what a token's are held times
   int64_t plane;
   int32_t rows, F, half, act;
 
@@ -165,13 +168,12 @@ struct GatedGradEpilogue {
     static_assert(MI == MIV, "rows of the wave's LDS");
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, f0 = m / 2;
     typedef typename std::conditional<F32, float, uint16_t>::type T;
-    float held = 1.f;
-    if constexpr (DT == TMS_DTYPE_F16) held = *factor;
     // The dh of the next 16 tokens are on their way while these are used: one by one, their latencies would take
     // as long as a third of the product.
     const bool whole = n + 16 * NI <= rows && f0 + 16 * NP <= F;
-    auto load = [&](int j, GatedVec<T, 4>(&to)[NP]) {
+    auto load = [&](int j, GatedVec<T, 4>(&to)[NP], float& times) {
       const int row = n + 16 * j + c;
+      if constexpr (DT == TMS_DTYPE_F16) times = row < rows ? held[row] : 0.f;
       const T* from = (const T*)grad + (int64_t)row * F + f0 + 4 * g;
 #pragma unroll
       for (int p = 0; p < NP; p++) {
@@ -184,10 +186,11 @@ struct GatedGradEpilogue {
       }
     };
     GatedVec<T, 4> dhs[2][NP];
-    load(0, dhs[0]);
+    float times[2];
+    load(0, dhs[0], times[0]);
 #pragma unroll
     for (int j = 0; j < NI; j++) {
-      if (j + 1 < NI) load(j + 1, dhs[(j + 1) & 1]);
+      if (j + 1 < NI) load(j + 1, dhs[(j + 1) & 1], times[(j + 1) & 1]);
 #pragma unroll
       for (int p = 0; p < NP; p++) {
 #pragma unroll
@@ -195,7 +198,7 @@ struct GatedGradEpilogue {
           float d, slope;
           if constexpr (F32) d = dhs[j & 1][p].v[e];
           else d = from16<DT>(dhs[j & 1][p].v[e]);
-          if constexpr (DT == TMS_DTYPE_F16) d *= held;
+          if constexpr (DT == TMS_DTYPE_F16) d *= times[j & 1];
           const float y = gated_act<ACT, F32, true>(acc[2 * p][j][e], slope);
           acc[2 * p][j][e] = d * acc[2 * p + 1][j][e] * slope;
           acc[2 * p + 1][j][e] = d * y;
@@ -236,26 +239,26 @@ struct GatedGradEpilogue {
   }
 };
 
-// Rows of a gradient, finished: times *factor (NULL: 1), in the inputs' type; row n from `half` on
+// Rows of a gradient, finished: times *factor, or a factor for each row (NULL: 1), in the inputs' type; row n from `half` on
 // is row n - half of the second output.
 template <int OUT>
 struct GatedRowsEpilogue {
   static constexpr int kRowBytes = 0;
   void *out, *out2;
   const float* factor;
-  int32_t rows, half, d;  // rows: of each output
+  int32_t rows, half, d, each;  // rows: of each output; each: 1 where rows have factors of their own, or 0
 
   template <int MI, int NI>
   __device__ __forceinline__ void operator()(f32x4 (&acc)[MI][NI], int m, int n, int, uint8_t*) const {
     typedef typename std::conditional<OUT == TMS_DTYPE_F32, float, uint16_t>::type T;
     const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
-    const float k = factor ? *factor : 1.f;
 #pragma unroll
     for (int j = 0; j < NI; j++) {
       int row = n + 16 * j + c;
       T* to = (T*)out;
       if (row >= half) to = (T*)out2, row -= half;
       if (row >= rows || to == nullptr) continue;
+      const float k = factor ? factor[row * each] : 1.f;
       to += (int64_t)row * d;
 #pragma unroll
       for (int i = 0; i < MI; i++) {
@@ -303,11 +306,10 @@ struct GatedSumEpilogue {
 // splits of 8192 x 1024, 67 MB of fp32, to bf16: 14 us).
 template <int OUT>
 __global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int splits, int64_t split, int32_t all, int32_t half, int32_t rows, int32_t d,
-                                                         int32_t dp, const float* factor, void* out, void* out2) {
+                                                         int32_t dp, const float* factor, int32_t each, void* out, void* out2) {
   typedef typename std::conditional<OUT == TMS_DTYPE_F32, float, uint16_t>::type T;
   const int quads = (d + 3) / 4;
   const int64_t n = (int64_t)all * quads;
-  const float k = factor ? *factor : 1.f;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / quads;
     const int col = (int)(i - row * quads) * 4;
@@ -315,6 +317,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int 
     const int64_t r = second ? row - half : row;
     T* to = (T*)(second ? out2 : out);
     if (r >= rows || to == nullptr) continue;
+    const float k = factor ? factor[r * each] : 1.f;
     const float* from = sums + row * dp + col;
     f32x4 x = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < splits; s += 4) {
@@ -343,9 +346,9 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int 
 
 // What fp16's dg and du are bounded by: |dg| <= 1.13 |dh| |u|, |du| <= |dh| |g| (no activation is further from 0 than its
 // argument, or steeper than 1.13), and |g|, |u| <= |x| |w| for the norms of the token's row and the weight's. A workgroup has
-// tokens (their largest |dh| times |x|: `parts`), or four rows of weights at a time (squares of their norms: `parts` from
-// kBoundTokens on). What is not finite is passed over: it makes its own rows what it will. 1229 x 768 x 2043: 6.2 us, 2.7 for
-// the factor.
+// tokens (`rows`: their largest |dh| times |x|; `parts`: the largest of those times |x| once more), or four rows of weights at a
+// time (squares of their norms: `parts` from kBoundTokens on). Infinite and NaN elements of dh, and rows that have any
+// elsewhere, are passed over: they make their own rows what they will. 1229 x 768 x 2043: 6.3 us.
 constexpr int kBoundTokens = 2048, kBoundWeights = 1024;
 constexpr float kBoundSlope = 1.2f;
 
@@ -373,7 +376,7 @@ __device__ __forceinline__ float gated_square_of(const uint16_t* row, int n, int
   return s;
 }
 __global__ __launch_bounds__(256) void gated_bounds_kernel(const uint16_t* dh, const uint16_t* x, const uint16_t* wg, const uint16_t* wu, int32_t N, int32_t d,
-                                                           int32_t F, int32_t tokens, float* parts) {
+                                                           int32_t F, int32_t tokens, float* parts, float* rows) {
   __shared__ float lds[2][4];
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   float most = 0.f;
@@ -395,7 +398,9 @@ __global__ __launch_bounds__(256) void gated_bounds_kernel(const uint16_t* dh, c
       __syncthreads();
       h = fmaxf(fmaxf(lds[0][0], lds[0][1]), fmaxf(lds[0][2], lds[0][3]));
       s = (lds[1][0] + lds[1][1]) + (lds[1][2] + lds[1][3]);
-      most = fmaxf(most, gated_finite(h * sqrtf(s)));
+      const float norm = sqrtf(s);
+      if (t == 0) rows[n] = h * norm;
+      most = fmaxf(most, gated_finite(h * norm * norm));
     }
     if (t == 0) parts[blockIdx.x] = most;
     return;
@@ -438,13 +443,41 @@ __device__ __forceinline__ void gated_largest(const float* parts, int tokens, in
 __device__ __forceinline__ int gated_up(float x) { return 14 + 127 - (int)(__builtin_bit_cast(uint32_t, x) >> 23); }
 __device__ __forceinline__ float gated_power(int e) { return e < -126 ? 0.f : __builtin_bit_cast(float, (uint32_t)(127 + (e > 127 ? 127 : e)) << 23); }
 
-// factor[0]: the power of two that dg and du are held times; factor[1]: its reciprocal.
-__global__ __launch_bounds__(256) void gated_factor_kernel(const float* parts, int tokens, int weights, float* factor) {
+// What each token's dg and du are held times, its reciprocal, and x times that reciprocal and a power of two that brings the
+// largest bound of that to 2^14 to 2^15 (`xs`, `terms` times one behind the other; *back: what takes the power out again).
+// 1229 x 768: 5.1 us, most of them the way of the parts.
+__global__ __launch_bounds__(256) void gated_scale_kernel(const float* parts, int tokens, int weights, const float* rows, const uint16_t* x, int32_t N, int32_t d,
+                                                          int32_t dp, int32_t terms, uint16_t* xs, float* held, float* held_back, float* back) {
   float h, w;
   gated_largest(parts, tokens, weights, h, w);
-  const float bound = kBoundSlope * h * sqrtf(w);
-  const int e = bound > 0.f ? gated_up(bound) : 0;
-  if (threadIdx.x == 0) factor[0] = gated_power(e), factor[1] = gated_power(-e);
+  w = kBoundSlope * sqrtf(w);
+  const float all = h * w * 0x1p-14f;  // a token's power takes its bound's exponent from 14
+  const int up = all > 0.f ? gated_up(all) : 0;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *back = gated_power(-up);
+  const int eights = dp / 8;
+  const int64_t n = (int64_t)N * eights;
+  for (int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x; k < n; k += (int64_t)gridDim.x * 256) {
+    const int64_t row = k / eights;
+    const int c = (int)(k - row * eights) * 8;
+    const float bound = rows[row] * w;
+    const bool some = bound > 0.f && bound < __builtin_inff();  // dg and du of others are zeros, or not finite
+    const int e = some ? gated_up(bound) : 0;
+    const float f = some ? gated_power(up - e) : 1.f;
+    if (c == 0) held[row] = gated_power(e), held_back[row] = gated_power(-e);
+    const uint16_t* from = x + row * d + c;
+    GatedVec<uint16_t, 8> v;
+    if (c + 8 <= d) {
+      v = *(const GatedVec<uint16_t, 8>*)from;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) v.v[i] = c + i < d ? from[i] : (uint16_t)0;
+    }
+    u32x4 out;
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+      out[i] = (uint32_t)to16<TMS_DTYPE_F16>(from16<TMS_DTYPE_F16>(v.v[2 * i]) * f) | (uint32_t)to16<TMS_DTYPE_F16>(from16<TMS_DTYPE_F16>(v.v[2 * i + 1]) * f) << 16;
+    for (int t = 0; t < terms; t++) *(u32x4*)(xs + ((int64_t)t * N + row) * dp + c) = out;
+  }
 }
 
 // ---------------------------------------------------------------- few tokens
@@ -525,10 +558,14 @@ __global__ __launch_bounds__(kFewWaves * 64) void gated_few_kernel(const void* x
 // ---------------------------------------------------------------- host
 
 struct GatedSpace {
-  int64_t x, wg, wu, p, parts, factor, sums, bytes;
+  int64_t x, wg, wu, p, sums, bytes;
+  int64_t parts, rows, xs, held, held_back, back;  // fp16
   GemmSplit dx, dw;  // how the gradients' products go
   int terms;         // of dg and du, as that many times the tokens
 };
+
+// How often x is laid out one behind the other for the weights' product: fp16 has another x for that.
+static int gated_laid(const GatedSpace& s, int dtype) { return dtype == TMS_DTYPE_F16 ? 1 : s.terms; }
 
 static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool backward) {
   GatedSpace s = {};
@@ -536,15 +573,22 @@ static GatedSpace gated_space(int64_t N, int64_t d, int64_t F, int dtype, bool b
   if (!backward && gated_few(N, d, F, dtype == TMS_DTYPE_F32)) return s;
   const int64_t dp = up_to(d, 8);
   s.terms = backward && dtype != TMS_DTYPE_F32 && N <= kFewTokens ? 2 : 1;
-  if (dtype == TMS_DTYPE_F32 || d % 8 || s.terms > 1) s.x = c.take(N * dp * 2 * planes(dtype) * s.terms);
+  const int laid = gated_laid(s, dtype);
+  if (dtype == TMS_DTYPE_F32 || d % 8 || laid > 1) s.x = c.take(N * dp * 2 * planes(dtype) * laid);
   if (dtype == TMS_DTYPE_F32 || d % 8) {
     s.wg = c.take(F * dp * 2 * planes(dtype));
     s.wu = c.take(F * dp * 2 * planes(dtype));
   }
   if (backward) {
     s.p = c.take(N * 2 * up_to(F, 64) * 2 * planes(dtype) * s.terms);
-    s.parts = c.take((kBoundTokens + kBoundWeights) * 4);
-    s.factor = c.take(8);
+    if (dtype == TMS_DTYPE_F16) {
+      s.parts = c.take((kBoundTokens + kBoundWeights) * 4);
+      s.rows = c.take(N * 4);
+      s.xs = c.take(N * dp * 2 * s.terms);
+      s.held = c.take(N * 4);
+      s.held_back = c.take(N * 4);
+      s.back = c.take(4);
+    }
     const int64_t half = up_to(F, 64);
     s.dx = gemm_split(dp, N * s.terms, 2 * half, planes(dtype));
     s.dw = gemm_split(dp, 2 * half, N * s.terms, planes(dtype));
@@ -599,7 +643,8 @@ static int gated_operands(const void* x, int64_t N, int64_t d, const void* wg, c
                           GatedOperands& o, hipStream_t st) {
   o = {(const uint16_t*)x, (const uint16_t*)wg, (const uint16_t*)wu};
   const bool all = dtype == TMS_DTYPE_F32 || d % 8;
-  if (!all && s.terms <= 1) return TMS_OK;
+  const int laid = gated_laid(s, dtype);
+  if (!all && laid <= 1) return TMS_OK;
   const int64_t dp = up_to(d, 8);
   uint16_t *px = (uint16_t*)(ws + s.x), *pg = (uint16_t*)(ws + s.wg), *pu = (uint16_t*)(ws + s.wu);
   GatedTerms t = {};
@@ -609,7 +654,7 @@ static int gated_operands(const void* x, int64_t N, int64_t d, const void* wg, c
     n++;
   };
   lay(x, px, N);
-  if (s.terms > 1) lay(x, px + N * dp, N);
+  if (laid > 1) lay(x, px + N * dp, N);
   o.x = px;
   if (all) {
     lay(wg, pg, F);
@@ -676,18 +721,18 @@ static int gated_forward(const void* x, int64_t N, int64_t d, const void* wg, co
 
 // A product to rows of d elements, at once or in splits; with terms > 1, of so many times `all` rows, summed.
 template <int DT, int PL, int OUT, bool BO, int PAIR>
-static int gated_rows(GemmArgs b, GemmSplit plan, int terms, int64_t all, int64_t half, int64_t rows, int64_t d, int64_t dp, const float* factor, float* sums, void* out,
-                      void* out2, const char* what, hipStream_t st) {
+static int gated_rows(GemmArgs b, GemmSplit plan, int terms, int64_t all, int64_t half, int64_t rows, int64_t d, int64_t dp, const float* factor, int each, float* sums,
+                      void* out, void* out2, const char* what, hipStream_t st) {
   b.splits = plan.splits;
   if (plan.splits * terms == 1) {
-    const GatedRowsEpilogue<OUT> e = {out, out2, factor, (int32_t)rows, (int32_t)half, (int32_t)d};
+    const GatedRowsEpilogue<OUT> e = {out, out2, factor, (int32_t)rows, (int32_t)half, (int32_t)d, (int32_t)each};
     return gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   }
   const GatedSumEpilogue e = {sums, terms * all * dp, (int32_t)(terms * all), (int32_t)dp};
   const int rc = gated_product<DT, PL, true, BO, PAIR>(b, plan.size, [&](auto) { return e; }, what, st);
   if (rc) return rc;
   hipLaunchKernelGGL(gated_join_kernel<OUT>, dim3(blocks_for(all * ((d + 3) / 4))), dim3(256), 0, st, sums, plan.splits * terms, all * dp, (int32_t)all,
-                     (int32_t)half, (int32_t)rows, (int32_t)d, (int32_t)dp, factor, out, out2);
+                     (int32_t)half, (int32_t)rows, (int32_t)d, (int32_t)dp, factor, (int32_t)each, out, out2);
   return check_launch("gated_join_kernel");
 }
 
@@ -699,22 +744,26 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
   if (rc) return rc;
   const int64_t dp = up_to(d, 8), half = up_to(F, 64), plane = N * 2 * half;
   uint16_t* P = (uint16_t*)(ws + s.p);
-  float* factor = nullptr;
+  const float *held = nullptr, *held_back = nullptr, *back = nullptr;
+  const uint16_t* xs = o.x;
   if (DT == TMS_DTYPE_F16) {
-    factor = (float*)(ws + s.factor);
     const int tokens = (int)(N < kBoundTokens ? N : kBoundTokens), rows = (int)((2 * F + 3) / 4), weights = rows < kBoundWeights ? rows : kBoundWeights;
     float* parts = (float*)(ws + s.parts);
     hipLaunchKernelGGL(gated_bounds_kernel, dim3((unsigned)(tokens + weights)), dim3(256), 0, st, (const uint16_t*)grad, (const uint16_t*)x, (const uint16_t*)wg,
-                       (const uint16_t*)wu, (int32_t)N, (int32_t)d, (int32_t)F, tokens, parts);
+                       (const uint16_t*)wu, (int32_t)N, (int32_t)d, (int32_t)F, tokens, parts, (float*)(ws + s.rows));
     if ((rc = check_launch("gated_bounds_kernel"))) return rc;
-    hipLaunchKernelGGL(gated_factor_kernel, dim3(1), dim3(256), 0, st, (const float*)parts, tokens, weights, factor);
-    if ((rc = check_launch("gated_factor_kernel"))) return rc;
+    const int64_t groups = (N * dp / 8 + 255) / 256;
+    hipLaunchKernelGGL(gated_scale_kernel, dim3((unsigned)(groups < 2048 ? groups : 2048)), dim3(256), 0, st, (const float*)parts, tokens, weights,
+                       (const float*)(ws + s.rows), (const uint16_t*)x, (int32_t)N, (int32_t)d, (int32_t)dp, (int32_t)s.terms, (uint16_t*)(ws + s.xs),
+                       (float*)(ws + s.held), (float*)(ws + s.held_back), (float*)(ws + s.back));
+    if ((rc = check_launch("gated_scale_kernel"))) return rc;
+    held = (const float*)(ws + s.held), held_back = (const float*)(ws + s.held_back), back = (const float*)(ws + s.back);
+    xs = (const uint16_t*)(ws + s.xs);
   }
-  const float* back = factor ? factor + 1 : nullptr;
   const GemmArgs a = gated_args(o, N, F, dp);
   auto form = [&](auto terms) {
     auto epi = [&](auto z) {
-      return GatedGradEpilogue<DT, (PL > 1), decltype(terms)::value, decltype(z)::MI>{grad, P, factor, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
+      return GatedGradEpilogue<DT, (PL > 1), decltype(terms)::value, decltype(z)::MI>{grad, P, held, plane, (int32_t)N, (int32_t)F, (int32_t)half, (int32_t)act};
     };
     return gated_product<DT, PL, false, false, kPairRows>(a, product_size(2 * F, N, dp, PL), epi, "train_gemm_kernel (dg, du)", st);
   };
@@ -734,12 +783,13 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.N = (int32_t)(N * s.terms);
     b.half = (int32_t)half;
     b.real = (int32_t)F;
-    rc = gated_rows<DT, PL, OUT, false, kPairDepth>(b, s.dx, s.terms, N, 0x7fffffff, N, d, dp, back, (float*)(ws + s.sums), dx, nullptr, "train_gemm_kernel (dx)", st);
+    rc = gated_rows<DT, PL, OUT, false, kPairDepth>(b, s.dx, s.terms, N, 0x7fffffff, N, d, dp, held_back, 1, (float*)(ws + s.sums), dx, nullptr,
+                                               "train_gemm_kernel (dx)", st);
     if (rc) return rc;
   }
   if (dwg || dwu) {  // m over d, n over F columns of dg and du, k over tokens
     GemmArgs b = {};
-    b.A = o.x;
+    b.A = xs;
     b.B = P;
     b.aplane = N * dp;
     b.bplane = plane;
@@ -747,7 +797,8 @@ static int gated_backward(const void* x, int64_t N, int64_t d, const void* wg, c
     b.ldb = b.N = (int32_t)(2 * half);
     b.M = (int32_t)dp;
     b.K = (int32_t)(N * s.terms);
-    rc = gated_rows<DT, PL, OUT, true, kSingle>(b, s.dw, 1, 2 * half, half, F, d, dp, back, (float*)(ws + s.sums), dwg, dwu, "train_gemm_kernel (dWg, dWu)", st);
+    rc = gated_rows<DT, PL, OUT, true, kSingle>(b, s.dw, 1, 2 * half, half, F, d, dp, back, 0, (float*)(ws + s.sums), dwg, dwu,
+                                            "train_gemm_kernel (dWg, dWu)", st);
   }
   return rc;
 }
