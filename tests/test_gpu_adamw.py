@@ -278,6 +278,28 @@ def test_one_element_in_two_places(cuda):
     assert int(state.steps) == 1 and bool((q < 1).all())
 
 
+def test_views_of_one_buffer(cuda):
+    """Strided parameters and copies side by side are stepped as each by itself; where they overlap they are refused, and
+    nothing has changed."""
+    import tilemaxsim_amd as tms
+    g = torch.Generator(device="cuda").manual_seed(7)
+    w, grad, c = (torch.randn(30, 80, generator=g, device="cuda") for _ in range(3))
+    keep, ckeep = w.clone(), c.clone()
+    for params, grads, copies in (([w[:, :50], w[:, 40:]], [grad[:, :50], grad[:, 40:]], None), ([w.t()[:, :3], w[2]], [grad.t()[:, :3], grad[2]], None),
+                                  ([w[:, :40]], [grad[:, :40]], [w[:, 39:79]]), ([w[:, :40]], [w[:, 30:70]], None), ([w[5:7].view(160)], [w.view(-1)[300:620:2]], None)):
+        state = tms.AdamWState(params)
+        with pytest.raises(ValueError, match="overlap"):
+            tms.adamw_(params, grads, state, copies=copies)
+        assert not state.steps.any() and not state.m.any() and torch.equal(w, keep)
+    ps, gs, cs = [w[:, :40], w[:, 40:60:2], w[:, 41:60:2]], [grad[:, :40], grad[:, 40:60:2], grad[:, 41:60:2]], [c[:, 40:], c[:, :10], c[:, 10:20]]
+    alone = [p.clone() for p in ps]
+    for p, x in zip(alone, gs):
+        tms.adamw_(p, x.contiguous(), tms.AdamWState(p))
+    tms.adamw_(ps, gs, tms.AdamWState(ps), copies=cs)
+    assert all(torch.equal(p, a) and torch.equal(x, a) for p, x, a in zip(ps, cs, alone))
+    assert torch.equal(w[:, 60:], keep[:, 60:]) and torch.equal(c[:, 20:40], ckeep[:, 20:40])
+
+
 def test_some_copies(cuda):
     """Copies of some parameters, of several types, and parameters of inference mode: each as by itself, versions counted."""
     import tilemaxsim_amd as tms

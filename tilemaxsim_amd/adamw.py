@@ -12,7 +12,7 @@ from array import array
 
 import torch
 
-from . import _check, _lib
+from . import _check, _lib, _overlap
 
 BLOCK = _lib.TMS_ADAMW_BLOCK
 
@@ -210,12 +210,9 @@ def adamw_(params, grads, state: AdamWState, lr=1e-3, betas=(0.9, 0.999), eps: f
         return ts if all(map(_contiguous, ts)) else [t if t.is_contiguous() else t.contiguous() for t in ts]
 
     p_to, c_to, g_from = whole(ps), whole(cs), whole(gs)
-    back = []
-    if p_to is not ps or c_to is not cs:
-        back = [(t, d) for t, d in zip([*ps, *cs], [*p_to, *c_to]) if t is not d]
-        at = [t.data_ptr() for t in (*ps, *cs) if t.numel()]
-        if len(set(at)) != len(at) or any(s == 0 and n > 1 for t, _ in back for s, n in zip(t.stride(), t.shape)):
-            raise ValueError(f"{fn}: two of the tensors (or elements of one) overlap")
+    back = [] if p_to is ps and c_to is cs else [(t, d) for t, d in zip([*ps, *cs], [*p_to, *c_to]) if t is not d]
+    if back or g_from is not gs:
+        _overlap.apart(fn, [*ps, *cs], gs)  # the library sees the copies
     n = len(ps)
     copied, kinds = [0] * n, g_kinds
     if len(given) == n:
