@@ -98,6 +98,23 @@ def test_training_runs(cuda, example):
     assert history.shape == (3, 5) and bool(torch.isfinite(history).all())
 
 
+def test_weights_are_the_parameters_roundings(cuda, example, monkeypatch):
+    """Every step of the example moves its fp32 parameters, and leaves in each 16-bit weight what its parameter rounds to."""
+    import tilemaxsim_amd as tms
+    step, seen = tms.adamw_, []
+
+    def watched(params, grads, state, copies=None, **how):
+        weights = list(copies)
+        before = [p.clone() for p in params]
+        step(params, grads, state, copies=weights, **how)
+        assert all(torch.equal(w.detach(), p.to(w.dtype)) for p, w in zip(params, weights))
+        seen.append((sum(int((p != b).sum()) for p, b in zip(params, before)), sum(p.numel() for p in params)))
+
+    monkeypatch.setattr(example.tms, "adamw_", watched)
+    example.train(steps=3, texts=8, vocabulary=503, show=None, layers=2)
+    assert len(seen) == 3 and all(moved > n // 2 for moved, n in seen)
+
+
 def test_a_captured_step(cuda, example):
     """Forward, backward and the optimizer's step in one graph, replayed with new batches, against eager steps."""
     import tilemaxsim_amd as tms
