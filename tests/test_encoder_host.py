@@ -373,3 +373,31 @@ def test_splits(rules):
     assert out[1] > 1  # few tiles
     rules.gemm_split_of(1024, 1 << 20, 8192, 1, out)
     assert list(out) == [0, 1]
+
+
+# ---------------------------------------------------------------- one token, one head, tangents
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32], ids=str)
+def test_strides_of_one_token_or_head_do_not_matter(dtype):
+    """Whatever stride a dimension of one element has, the C entry gets one that it takes, without a copy."""
+    import struct
+    from tilemaxsim_amd import attention
+    step = 16 // torch.empty(0, dtype=dtype).element_size()
+
+    def strides(*ts):
+        given = attention._describe(*ts, torch.tensor([0, ts[0].shape[0]]), None, None, 1.0, 0.0)
+        return struct.unpack("@3P6q3P5q2dq", given)[3:9]
+
+    wide, tall = torch.zeros(1, 4 * 64 + 3, dtype=dtype), torch.zeros(5, 1, 64, dtype=dtype)
+    views = [wide[:, :256].unflatten(1, (4, 64)), torch.zeros(1, 1, 67, dtype=dtype)[..., :64],
+             torch.zeros(64, dtype=dtype).as_strided((1, 1, 64), ((1 << 22) + 8, 3, 1)), tall.as_strided((5, 1, 64), (64, 3, 1)),
+             tall.as_strided((5, 1, 64), (64, 1 << 40, 1)), tall]
+    for x in views:
+        y = attention._rows(x)
+        assert y.data_ptr() == x.data_ptr() and y.shape == x.shape
+        for s in strides(y, y, y):
+            assert s % step == 0
+        assert all(0 <= s <= attention.MOST_STRIDE for s in strides(y, y, y)[::2])
+    x = torch.zeros(2, 67, dtype=dtype)[:, None, :64]  # two tokens: an odd stride counts
+    y = attention._rows(x)
+    assert y.data_ptr() != x.data_ptr() and y.is_contiguous()

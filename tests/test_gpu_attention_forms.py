@@ -1,5 +1,5 @@
 """Forms of attention that its general tests would not tell from another: two terms in short texts, far keys left out
-under a bias, and memory beside the tensors.
+under a bias, memory beside the tensors, and strides that a single token or head leaves open.
 
 References and bounds are those of test_gpu_attention.py."""
 import math
@@ -89,3 +89,27 @@ def test_nothing_beside_the_tensors_is_written(cuda, dt):
                                    ptr["dq"], ptr["dk"], ptr["dv"]))
             torch.cuda.synchronize()
             assert all(kept(flat) for flat, _ in bufs.values()), [name for name, (flat, _) in bufs.items() if not kept(flat)]
+
+
+@pytest.mark.parametrize("dt", DT, ids=str)
+@pytest.mark.parametrize("H,KV", [(1, 1), (3, 1), (4, 2)])
+def test_one_token_of_any_stride(cuda, H, KV, dt):
+    """A single token, and a single head, as views whose other strides the kernels could not read in place: what a call on
+    contiguous tensors gives."""
+    import tilemaxsim_amd as tms
+    for T in (1, 5):
+        (q, k, v), offsets, G = make([T], H, KV, 64, dt, seed=T)
+        want = tms.packed_attention(q, k, v, offsets)
+        grads = torch.autograd.grad(want, (q, k, v), G)
+        views = {
+            "odd token": lambda t: torch.empty(T, t.shape[1] * 64 + 4, device="cuda", dtype=dt)[:, :t.shape[1] * 64].unflatten(1, (t.shape[1], 64)),
+            "odd head": lambda t: torch.empty(T, t.shape[1], 68, device="cuda", dtype=dt)[..., :64],
+            "far token": lambda t: torch.empty(1, 1, 64, device="cuda", dtype=dt).as_strided((1, 1, 64), ((1 << 22) + 8, 64, 1)) if T == t.shape[1] == 1 else torch.empty_like(t),
+            "far head": lambda t: torch.empty(64 * T, device="cuda", dtype=dt).as_strided((T, 1, 64), (64, (1 << 40) + 3, 1)) if t.shape[1] == 1 else torch.empty_like(t),
+        }
+        for name, view in views.items():
+            with torch.no_grad():
+                xs = [view(t).copy_(t).detach().requires_grad_(True) for t in (q, k, v)]
+            out = tms.packed_attention(*xs, offsets.cuda())
+            assert torch.equal(out, want), (name, T)
+            assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, xs, G), grads)), (name, T)

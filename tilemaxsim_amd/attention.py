@@ -21,11 +21,17 @@ MOST_STRIDE = 1 << 22  # elements between tokens that the kernels read in place
 _pack = struct.Struct("@3P6q3P5q2dq").pack  # tms_attention
 
 
+def _strides(t: torch.Tensor) -> tuple[int, int, int]:
+    """Elements between tokens, heads and elements; 0 for a single token or head, whose stride means nothing."""
+    (tokens, heads, _), (token, head, one) = t.shape, t.stride()
+    return token if tokens > 1 else 0, head if heads > 1 else 0, one
+
+
 def _describe(q, k, v, offsets, prefix, slopes, scale, cap) -> bytes:
     T, H, D = q.shape
-    qt, qh, _ = q.stride()
-    kt, kh, _ = k.stride()
-    vt, vh, _ = v.stride()
+    qt, qh, _ = _strides(q)
+    kt, kh, _ = _strides(k)
+    vt, vh, _ = _strides(v)
     return _pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), qt, qh, kt, kh, vt, vh, offsets.data_ptr(),
                  0 if prefix is None else prefix.data_ptr(), 0 if slopes is None else slopes.data_ptr(), offsets.shape[0] - 1, T, H,
                  k.shape[1], D, scale, cap, _lib.DTYPE_CODES[q.dtype])
@@ -74,7 +80,7 @@ class _PackedAttention(torch.autograd.Function):
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """As it is where the kernels read it so (whole rows of a head, at 16-byte steps), else a copy."""
     step = 16 // t.element_size()
-    token, head, one = t.stride()
+    token, head, one = _strides(t)
     if one == 1 and token % step == 0 and head % step == 0 and token <= MOST_STRIDE and t.data_ptr() % 16 == 0:
         return t
     return _check.aligned(t)
