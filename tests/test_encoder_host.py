@@ -401,3 +401,12 @@ def test_strides_of_one_token_or_head_do_not_matter(dtype):
     x = torch.zeros(2, 67, dtype=dtype)[:, None, :64]  # two tokens: an odd stride counts
     y = attention._rows(x)
     assert y.data_ptr() != x.data_ptr() and y.is_contiguous()
+
+
+def test_tangents_of_slopes_are_refused():
+    import tilemaxsim_amd as tms
+    from torch.autograd import forward_ad
+    with forward_ad.dual_level():
+        slopes = forward_ad.make_dual(torch.zeros(4), torch.ones(4))
+        with pytest.raises(NotImplementedError, match="forward mode"):
+            tms.packed_attention(Q, K, K, O, slopes=slopes)

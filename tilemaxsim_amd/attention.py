@@ -174,6 +174,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
             raise ValueError(f"{fn}: slopes must be ({H},) float32, got {tuple(slopes.shape)} {slopes.dtype}")
         if slopes.requires_grad:
             raise NotImplementedError(f"{fn}: a gradient of the slopes")
+        _check.no_tangents(fn, (slopes,))
     if not usual:
         for name, t in (("q", q), ("k", k), ("v", v)):
             _check.on_gpu(name, t)
