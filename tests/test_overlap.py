@@ -90,3 +90,28 @@ def test_adamw_refuses_strided_tensors_that_overlap(monkeypatch):
     for params, grads, copies in cases:
         with pytest.raises(ValueError, match="overlap"):
             step_of(params, grads, copies, monkeypatch)
+
+
+def test_clipping_refuses_strided_tensors_that_overlap(monkeypatch):
+    """Gradients scaled in place, and scaled into others: a gradient's own tensor may be the gradient itself, as a whole."""
+    import tilemaxsim_amd as tms
+    from tilemaxsim_amd import grad_clip as module
+    monkeypatch.setattr(module, "_on_one_gpu", lambda *a: None)
+
+    class Launched(Exception):
+        pass
+
+    def launch(*a):
+        raise Launched
+
+    monkeypatch.setattr(module._lib, "launch", launch)
+    w, x = torch.zeros(30, 80), torch.zeros(30, 80)
+    for grads, out in (([w[:, :50], w[:, 40:]], None), ([w.t()[:, :3], w[2]], None), ([w[:1].expand(30, 80)], None), ([x[:, :40]], [w.view(-1).as_strided((30, 40), (30, 1))]),
+                       ([w[:, :40]], [w[:, 1:41]]), ([w[5:7].view(160)], [w.view(-1)[300:620:2]]), ([w.view(-1)[300:620:2]], [w[5:7].view(160)]),
+                       ([w[:, :40], x[:, :40]], [w[:, 40:], w[:, :40]]), ([w[:30, :30]], [w[:30, :30].t()])):
+        with pytest.raises(ValueError, match="overlap"):
+            tms.clip_grad_norm_(grads, 1.0, out=out)
+    for grads, out in (([w[:, :50], w[:, 50:]], None), ([w[:, ::2], w[:, 1::2]], None), ([w[:, :40]], [w[:, :40]]), ([w[:, :40]], [w[:, 40:]]),
+                       ([w[:1].expand(30, 80)], [x]), ([w[3:4], w[5].view(40, 2)[:, 0]], [w[3].as_strided((1, 80), (7, 1)), x[:20, 0:4:2].reshape(40)]), ([w[:, :40], w[:, :40]], [x[:, :40], x[:, 40:]])):
+        with pytest.raises(Launched):
+            tms.clip_grad_norm_(grads, 1.0, out=out)

@@ -12,7 +12,7 @@ from array import array
 
 import torch
 
-from . import _check, _lib
+from . import _check, _lib, _overlap
 
 _requires_grad = operator.attrgetter("requires_grad")
 _NORMS = {2.0: _lib.TMS_NORM_2, math.inf: _lib.TMS_NORM_INF}
@@ -80,12 +80,10 @@ def _table(src: list, src_kinds: list, dst: list, dst_kinds: list) -> array:
     return words
 
 
-def _apart(fn: str, ts: list) -> None:
-    """Strided tensors are written through copies of their own, one after another: two of one
-    address would take each other's place."""
-    at = [t.data_ptr() for t in ts if t.numel()]
-    if len(set(at)) != len(at):
-        raise ValueError(f"{fn}: two of the tensors overlap")
+def _same(t: torch.Tensor, o: torch.Tensor) -> bool:
+    """Whether a gradient and its tensor in `out` are the same elements."""
+    return t is o or (t.data_ptr() == o.data_ptr() and t.dtype == o.dtype
+                      and all(n < 2 or a == b for n, a, b in zip(t.shape, t.stride(), o.stride())))
 
 
 def _workspace(lib, count: int, dev: torch.device) -> torch.Tensor:
@@ -178,8 +176,8 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, error_if_n
     src = [t if t.is_contiguous() else t.contiguous() for t in ts]
     dst = src if to is ts else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in to]
     copies = [(o, d) for o, d in zip(to, dst) if o is not d]  # strided tensors' own elements
-    if copies:
-        _apart(fn, to)  # contiguous ones the library looks over
+    if copies or any(t is not x for t, x in zip(ts, src)):  # contiguous ones the library looks over
+        _overlap.apart(fn, to, [t for t, o in zip(ts, to) if not _same(t, o)])
     table = _table(src, kinds, dst, into)
     limit = ctypes.c_double(max_norm)
     status = _lib.launch(dev, lib.tms_grad_clip, table.buffer_info()[0], len(src), code, ctypes.addressof(limit),
