@@ -475,7 +475,7 @@ __global__ __launch_bounds__(256) void lce_hidden_kernel(const float* sums, int 
 // ---------------------------------------------------------------- host
 
 static int logits_size(int64_t N, int64_t V, int64_t dp, int dtype) {
-  return gemm_size(V, N, gemm_steps(dp, planes(dtype)), gemm_largest(planes(dtype)));
+  return terms_size(V, N, dp, planes(dtype), gemm_largest(planes(dtype)));
 }
 // Vocabulary rows that one RowStat of the forward pass covers: a wave's share of a tile.
 static int64_t stat_rows(int size) { return gemm_side(size) / 2; }

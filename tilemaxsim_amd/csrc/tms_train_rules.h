@@ -39,6 +39,27 @@ inline int gemm_size(int64_t m, int64_t n, int64_t steps, int largest = kGemm256
   return best;
 }
 
+inline int64_t gemm_groups(int size, int64_t m, int64_t n, int64_t splits) {
+  const int64_t side = gemm_side(size);
+  return up_to(m, side) / side * (up_to(n, side) / side) * splits;
+}
+
+// Microseconds of a product of m x n over k. Of three planes, tiles of 64 x 64 wait once a 64-step, with one workgroup a CU:
+// rounds of up to 256 of them, 0.97 a step. (fp32 logits of 500 x 8000 x 64, 1000 tiles of one step: 11.7, in tiles of 128
+// 7.5; 1024 x 4000 x 128: 15.4 / 11.6; 600 x 4000 x 64: 8.7 / 7.1, x 1024: 50 / 54; 400 x 4000 x 64: 6.2 / 6.9, x 256: 12.1 /
+// 16.0. 176 tiles over 2048: 33.0.)
+inline double terms_us(int size, int64_t m, int64_t n, int64_t k, int planes, int64_t splits) {
+  if (planes != 3 || size != kGemm64) return gemm_us(size, m, n, gemm_steps(k, planes), splits);
+  const double each = (double)((up_to(k, 64) / 64 + splits - 1) / splits);
+  return (double)((gemm_groups(size, m, n, splits) + 255) / 256) * (each * 0.97 + 1.6) + 1.5;
+}
+inline int terms_size(int64_t m, int64_t n, int64_t k, int planes, int largest) {  // largest: the largest tile to take
+  int best = largest;
+  for (int s = best + 1; s < kGemmSizes; s++)
+    if (terms_us(s, m, n, k, planes, 1) < terms_us(best, m, n, k, planes, 1)) best = s;
+  return best;
+}
+
 // How linear cross entropy's backward pass goes over the vocabulary.
 struct LcePlan {
   int64_t dp;      // width of a row of terms
@@ -55,12 +76,11 @@ constexpr int64_t kFewRows = 64;
 // and read but for the first piece, at about 4 TB/s) cost less than idle CUs.
 inline double lce_split(LcePlan& p, int64_t N, int64_t piece, int planes) {
   static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 20, 24, 32, 48, 64};
-  const int64_t steps = gemm_steps(piece, planes);
   double least = 1e30;
   for (int s : kSplits) {
     if (s > 1 && s * 2 > piece / 64) break;
     for (int size = gemm_largest(planes); size < kGemmSizes; size++) {
-      const double us = gemm_us(size, p.dp, N, steps, s) + (double)s * (double)N * (double)p.dp * 8 / 4e6;
+      const double us = terms_us(size, p.dp, N, piece, planes, s) + (double)s * (double)N * (double)p.dp * 8 / 4e6;
       if (us < least) least = us, p.splits = s, p.size_h = size;
     }
   }
@@ -73,7 +93,7 @@ inline double lce_split(LcePlan& p, int64_t N, int64_t piece, int planes) {
 // round of workgroups is a smaller part of a larger piece.)
 inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
   LcePlan best = {};
-  const int64_t dp = up_to(d > 0 ? d : 8, 8), steps_d = gemm_steps(dp, planes), steps_n = gemm_steps(N, planes);
+  const int64_t dp = up_to(d > 0 ? d : 8, 8);
   const int largest = gemm_largest(planes);
   const int64_t rows_p = N <= kFewRows ? kFewRows : up_to(N, 256);
   const int64_t tiles = up_to(V, 256) / 256;
@@ -87,9 +107,9 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
     p.rows_p = rows_p;
     p.piece = (tiles + n - 1) / n * 256;
     // P's product stores whole tiles: none taller than P, whatever the times say.
-    p.size_p = gemm_size(p.piece, N, steps_d, rows_p % gemm_side(largest) == 0 ? largest : kGemm64);
-    p.size_w = gemm_size(dp, p.piece, steps_n, largest);
-    const double us = gemm_us(p.size_p, p.piece, N, steps_d, 1) + gemm_us(p.size_w, dp, p.piece, steps_n, 1) + lce_split(p, N, p.piece, planes);
+    p.size_p = terms_size(p.piece, N, dp, planes, rows_p % gemm_side(largest) == 0 ? largest : kGemm64);
+    p.size_w = terms_size(dp, p.piece, N, planes, largest);
+    const double us = terms_us(p.size_p, p.piece, N, dp, planes, 1) + terms_us(p.size_w, dp, p.piece, N, planes, 1) + lce_split(p, N, p.piece, planes);
     const double all = us * (double)((tiles * 256 + p.piece - 1) / p.piece);
     if (all < least) least = all, best = p;
   }
@@ -101,19 +121,14 @@ inline LcePlan lce_plan(int64_t N, int64_t V, int64_t d, int planes) {
 // 8.2; 512 of 64 over 4096, 41.8 / 31.0. With k outside, 256 of 128 over 1024: 20.8 / 17.6.
 inline bool product_deep(int size, int64_t m, int64_t n, int64_t splits) {
   if (size == kGemm256) return false;
-  const int64_t side = gemm_side(size);
-  return up_to(m, side) / side * (up_to(n, side) / side) * splits <= (size == kGemm128 ? 256 : 512);
+  return gemm_groups(size, m, n, splits) <= (size == kGemm128 ? 256 : 512);
 }
 
-// Microseconds of a product of m x n over k. Of three planes, tiles of 64 x 64 wait once a 64-step, one workgroup a CU: 0.91
-// each, and 3.8 around them (176 tiles over 256, 768 and 2048 of k: 7.4, 14.6, 33.0; 352 over 1024: 34.6. With a wait a
-// product, 176 over 256: 12.7. Tiles of 128, 176 over 1024: 56.6).
+// Microseconds of a product of m x n over k that may take two steps a wait.
 inline double product_us(int size, int64_t m, int64_t n, int64_t k, int planes, int64_t splits) {
-  const int64_t side = gemm_side(size), groups = up_to(m, side) / side * (up_to(n, side) / side) * splits;
+  if (planes != 1 || !product_deep(size, m, n, splits)) return terms_us(size, m, n, k, planes, splits);
   const double each = (double)((up_to(k, 64) / 64 + splits - 1) / splits);
-  if (planes == 3 && size == kGemm64) return (double)((groups + 255) / 256) * (each * 0.91 + 3.8);
-  if (planes == 1 && product_deep(size, m, n, splits)) return size == kGemm128 ? each * 0.7 + 5.0 : each * (groups <= 256 ? 0.42 : 0.57) + 3.5;
-  return gemm_us(size, m, n, gemm_steps(k, planes), splits);
+  return size == kGemm128 ? each * 0.7 + 5.0 : each * (gemm_groups(size, m, n, splits) <= 256 ? 0.42 : 0.57) + 3.5;
 }
 inline int product_size(int64_t m, int64_t n, int64_t k, int planes) {
   int best = gemm_largest(planes);
