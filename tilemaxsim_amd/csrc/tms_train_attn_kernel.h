@@ -516,11 +516,115 @@ __global__ __launch_bounds__(kAttnThreads) void attn_norms_kernel(AttnArgs a) {
   if (threadIdx.x == 0) a.norms[blockIdx.x] = attn_max(attn_max(lds[0], lds[1]), attn_max(lds[2], lds[3]));
 }
 
+// ---------------------------------------------------------------- rows by themselves
+
+// Under a prefix mask a row shares tiles with tokens that it does not see, and if one of those is NaN or infinite, the 0 that
+// stands for it in the matrix instructions makes the row NaN. Rows of sums that are not finite are therefore formed
+// once more by one wave, from what they see alone, in fp32: 64 of the others at a time, one a lane for the scores, then one
+// after the other with the row's elements on the lanes. A row that is not finite by what it does see stays so. That takes
+// 30 to 100 times as long as with the matrix instructions, so rows that need not are not formed again: those whose own
+// statistic, or whole own token (which they see), is not finite, and all of a wave where every token in reach that some
+// row does not see is finite. (Two causal texts of 8192, 12 heads of 64, both directions: 1.4 ms, with a NaN that is
+// seen 1.2, with one in every 64th token 49.)
+// What it needs is formed anew or read again, so that next to nothing stays in registers for it while the tiles are gone over; calls without
+// prefixes take kernels without it (MASK: 100 causal texts of 200, 12 heads of 64, forward 38.9 us and backward 122.9, without the check 38.4 and 117.8).
+__device__ __forceinline__ int attn_lane() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
+__device__ __forceinline__ bool attn_finite(float x) { return fabsf(x) < __builtin_inff(); }
+
+// Whether a lane's sums of column j are all finite: their sum is, then (and where they are near fp32's limit perhaps not,
+// which only costs time).
+template <int DB, int NB>
+__device__ __forceinline__ bool attn_all_finite(const f32x4 (&acc)[DB][NB], int j) {
+  f32x4 x = acc[0][j];
+#pragma unroll
+  for (int d = 1; d < DB; d++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) x[e] += acc[d][j][e];
+  return attn_finite((x[0] + x[1]) + (x[2] + x[3]));
+}
+// The 16 rows (columns of the products) that any of a wave's lanes reports.
+__device__ __forceinline__ uint32_t attn_odd(bool here) {
+  const uint64_t b = __ballot(here);
+  return (uint32_t)(b | b >> 16 | b >> 32 | b >> 48) & 0xffffu;
+}
+
+// Whether a lane's quarter (pieces g, g + 4 ..) of a row has a finite element.
+template <int DT, int D>
+__device__ __forceinline__ bool attn_some_finite(const typename AttnType<DT>::E* x, int g) {
+  bool some = false;
+  for (int d = g; d < D; d += 4) some |= attn_finite(attn_float<DT>(x[d]));
+  return some;
+}
+// Whether all elements of rows from `from` up to `to` are finite: one row a lane.
+template <int DT, int D>
+__device__ bool attn_rows_finite(const typename AttnType<DT>::E* x, int64_t stride, int from, int to) {
+  typedef typename AttnType<DT>::Frag Frag;
+  bool bad = false;
+  for (int r = from + attn_lane(); r < to; r += 64)
+    for (int k = 0; k < D; k += 8) {
+      const Frag f = *(const Frag*)(x + r * stride + k);
+#pragma unroll
+      for (int e = 0; e < 8; e++) bad |= !attn_finite(attn_elem<DT>(f, e));
+    }
+  return __ballot(bad) == 0ull;
+}
+
+template <int DT, int D>
+__device__ __forceinline__ float attn_dot(const typename AttnType<DT>::E* x, const typename AttnType<DT>::E* y) {
+  typedef typename AttnType<DT>::Frag Frag;
+  float s = 0.f;
+#pragma unroll 2
+  for (int k = 0; k < D; k += 8) {
+    const Frag f = *(const Frag*)(x + k), h = *(const Frag*)(y + k);
+#pragma unroll
+    for (int e = 0; e < 8; e++) s = __builtin_fmaf(attn_elem<DT>(f, e), attn_elem<DT>(h, e), s);
+  }
+  return s;
+}
+
+// One row against those from `from` up to `to`, which it sees (or which see it). `own` is the row, and `x` its partners, of the
+// scores; `own2` and `y` of dP. Added to sum, element 64 u + lane: forward, P y; dq, dS x; dk and dv, dS x and (sum2) P y.
+template <int DT, int D, int KIND, AttnPass PASS>
+__device__ void attn_alone(const AttnArgs& a, int head, int row, int from, int to, const typename AttnType<DT>::E* own, const typename AttnType<DT>::E* own2,
+                           const typename AttnType<DT>::E* x, int64_t xs, const typename AttnType<DT>::E* y, int64_t ys, float lse, float delta,
+                           float (&sum)[(D + 63) / 64], float (&sum2)[(D + 63) / 64]) {
+  const int lane = attn_lane();
+  AttnScore<DT, KIND, 64> score;
+  score.init(a, head);
+  for (int r0 = from; r0 < to; r0 += 64) {
+    const int r = r0 + lane, n = to - r0 < 64 ? to - r0 : 64;
+    float p = 0.f, ds = 0.f;
+    if (r < to) {
+      float s = attn_dot<DT, D>(own, x + r * xs), slope = 1.f;
+      if constexpr (KIND == kAttnCap) {
+        s = score.cap2 > kAttnCoarse * kAttnLog2e ? score.template capped<true>(s, slope) : score.template capped<false>(s, slope);
+        slope *= 1.f / score.kSlope;
+      }
+      if (score.lean != 0.f) s = score.biased(s, (float)(row - r));
+      if constexpr (PASS == kAttnDkv) lse = a.lse[(int64_t)head * a.T + r], delta = a.delta[(int64_t)head * a.T + r];
+      p = __builtin_amdgcn_exp2f(__builtin_fmaf(s, score.unit, -lse));
+      if constexpr (PASS != kAttnForward) ds = p * (attn_dot<DT, D>(own2, y + r * ys) - delta) * slope;
+    }
+    for (int i = 0; i < n; i++) {
+      const float pi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), i));
+      const float di = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, ds), i));
+#pragma unroll
+      for (int u = 0; u < (D + 63) / 64; u++) {
+        const int d = 64 * u + lane;
+        if (d >= D) continue;
+        if constexpr (PASS != kAttnForward) sum[u] = __builtin_fmaf(di, attn_float<DT>(x[(r0 + i) * xs + d]), sum[u]);
+        if constexpr (PASS == kAttnForward) sum[u] = __builtin_fmaf(pi, attn_float<DT>(y[(r0 + i) * ys + d]), sum[u]);
+        if constexpr (PASS == kAttnDkv) sum2[u] = __builtin_fmaf(pi, attn_float<DT>(y[(r0 + i) * ys + d]), sum2[u]);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- forward
 
 // A workgroup has a tile of queries and goes over their keys; the running maximum, sum and o are in registers, and
 // the next tile's keys and values on their way while one is used. NB: blocks of 16 queries a wave. Times: above.
-template <int DT, int D, int NB, int KIND>
+template <int DT, int D, int NB, int KIND, bool MASK>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs a) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnForward)> Rows;
   typedef typename AttnType<DT>::E E;
@@ -684,16 +788,29 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
     }
   }
 
+  uint32_t odd[NB];
 #pragma unroll
   for (int j = 0; j < NB; j++) {
     const int row = row0 + 16 * j + c;
-    if (row >= t.end) continue;
     const float all = t.real ? sum[j] : 0.f;
     float z = all;
     z += __shfl_xor(z, 16);
     z += __shfl_xor(z, 32);
     const float inv = t.real ? 1.f / z : 0.f;
-    if (a.lse && g == 0) a.lse[(int64_t)head * a.T + row] = t.real ? top[j] + (log2f(z) - (float)attn_up<DT>()) : __builtin_inff();
+    top[j] = t.real ? top[j] + (log2f(z) - (float)attn_up<DT>()) : __builtin_inff();
+    odd[j] = 0;
+    if constexpr (MASK) {
+      odd[j] = attn_odd(!attn_all_finite(acc, j) && row < t.end && attn_finite(top[j]));
+      if (odd[j] != 0) {
+        const E* v = (const E*)a.v + head / a.many * a.vh;
+        const int unseen = row0 + 1 > t.prefix_end ? row0 + 1 : t.prefix_end, past = row0 + 16 * NB, end = (past > t.prefix_end ? past : t.prefix_end) + R;
+        odd[j] &= attn_odd(row < t.end && attn_some_finite<DT, D>(v + row * a.vt, g));
+        if (attn_rows_finite<DT, D>(v, a.vt, unseen, end < t.end ? end : t.end)) odd[j] = 0;
+      }
+    }
+    if (row >= t.end) continue;
+    if (a.lse && g == 0) a.lse[(int64_t)head * a.T + row] = top[j];
+    if (odd[j] >> c & 1) continue;
     const int64_t at = ((int64_t)row * a.H + head) * D;
 #pragma unroll
     for (int d = 0; d < DB; d++) {
@@ -707,6 +824,25 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
       struct __attribute__((packed, aligned(4 * sizeof(E)))) Four { E x[4]; };
       *(Four*)((E*)a.out + at + 16 * d + 4 * g) = Four{{o[0], o[1], o[2], o[3]}};
       if (DT != TMS_DTYPE_F32 && a.low) *(Four*)((E*)a.low + at + 16 * d + 4 * g) = Four{{l[0], l[1], l[2], l[3]}};
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    for (uint32_t m = MASK ? odd[j] : 0; m != 0; m &= m - 1) {
+      const int i = __builtin_ctz(m), row = row0 + 16 * j + i, kvh = head / a.many;
+      const int ln = attn_lane();
+      const float lse = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, top[j]), i));
+      float x[(D + 63) / 64] = {};
+      attn_alone<DT, D, KIND, kAttnForward>(a, head, row, t.begin, row + 1 > t.prefix_end ? row + 1 : t.prefix_end, (const E*)a.q + head * a.qh + row * a.qt, nullptr,
+                                            (const E*)a.k + kvh * a.kh, a.kt, (const E*)a.v + kvh * a.vh, a.vt, lse, 0.f, x, x);
+#pragma unroll
+      for (int u = 0; u < (D + 63) / 64; u++) {
+        const int64_t at = ((int64_t)row * a.H + head) * D + 64 * u + ln;
+        if (64 * u + ln >= D) continue;
+        const E o = attn_round<DT>(x[u]);
+        ((E*)a.out)[at] = o;
+        if (DT != TMS_DTYPE_F32 && a.low) ((E*)a.low)[at] = attn_round<DT>(x[u] - attn_float<DT>(o));
+      }
     }
   }
 }
@@ -761,7 +897,7 @@ __device__ __forceinline__ void attn_store(void* out, int64_t at, const f32x4 (&
 // and not 62.) And dS goes into its products as two 16-bit terms, as do P and dS in the kernel for dk and dv: where
 // few elements make up a gradient's norm, one rounding more than its own can be twice the error (256 texts of 64, 12 heads of
 // 64: 48 and 61 us, 46 and 58 with one term; 1024 of 16: 74 and 93, 72 and 88).
-template <int DT, int D, int NB, int KIND, bool SHORT>
+template <int DT, int D, int NB, int KIND, bool SHORT, bool MASK>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDq)> Rows;
   typedef typename AttnType<DT>::E E;
@@ -946,19 +1082,47 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       }
     }
   }
+  if (!a.dq) return;
+  uint32_t odd[NB];
 #pragma unroll
   for (int j = 0; j < NB; j++) {
     const int row = row0 + 16 * j + c;
-    if (row >= t.end) continue;
+    odd[j] = 0;
+    if constexpr (MASK) {
+      odd[j] = attn_odd(!attn_all_finite(acc, j) && row < t.end);
+      if (odd[j] != 0) {
+        __threadfence_block();  // delta is another lane's
+        const int64_t at = (int64_t)head * a.T + row;
+        odd[j] &= attn_odd(row < t.end && attn_finite(a.lse[at]) && attn_finite(a.delta[at]));
+        const int unseen = row0 + 1 > t.prefix_end ? row0 + 1 : t.prefix_end, past = row0 + 16 * NB, end = (past > t.prefix_end ? past : t.prefix_end) + R;
+        if (attn_rows_finite<DT, D>((const E*)a.k + head / a.many * a.kh, a.kt, unseen, end < t.end ? end : t.end)) odd[j] = 0;
+      }
+    }
+    if (row >= t.end || odd[j] >> c & 1) continue;
     const float f = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
-    if (a.dq) attn_store<DT>(a.dq, ((int64_t)row * a.H + head) * D, acc, j, f, g);
+    attn_store<DT>(a.dq, ((int64_t)row * a.H + head) * D, acc, j, f, g);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    for (uint32_t m = MASK ? odd[j] : 0; m != 0; m &= m - 1) {
+      const int i = __builtin_ctz(m), row = row0 + 16 * j + i, kvh = head / a.many;
+      const int ln = attn_lane();
+      const float l = a.lse[(int64_t)head * a.T + row], dl = a.delta[(int64_t)head * a.T + row];
+      float x[(D + 63) / 64] = {};
+      attn_alone<DT, D, KIND, kAttnDq>(a, head, row, t.begin, row + 1 > t.prefix_end ? row + 1 : t.prefix_end, (const E*)a.q + head * a.qh + row * a.qt,
+                                       (const E*)a.grad + ((int64_t)row * a.H + head) * D, (const E*)a.k + kvh * a.kh, a.kt, (const E*)a.v + kvh * a.vh, a.vt, l, dl,
+                                       x, x);
+#pragma unroll
+      for (int u = 0; u < (D + 63) / 64; u++)
+        if (64 * u + ln < D) ((E*)a.dq)[((int64_t)row * a.H + head) * D + 64 * u + ln] = attn_round<DT>(x[u] * a.scale);
+    }
   }
 }
 
 // dk and dv: a workgroup has a tile of keys and goes over the queries that see them, head by head of
 // those that share the keys. Both gradients' sums are as many registers as the keys and values: more than two
 // workgroups a CU spill (heads of 128, a bound of three: 166 us, 118 with two).
-template <int DT, int D, int NB, int KIND, bool SHORT>
+template <int DT, int D, int NB, int KIND, bool SHORT, bool MASK>
 __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(kAttnDkv)> Rows;
   typedef typename AttnType<DT>::E E;
@@ -976,6 +1140,7 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
   if (t.text < 0) return;
   const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4, wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int key0 = t.first + wave * 16 * NB;
+  const int head0 = kvh * a.many + part_of * a.many / a.parts, heads = kvh * a.many + (part_of + 1) * a.many / a.parts - head0;
 
   f32x4 dk[DB][NB], dv[DB][NB];
 #pragma unroll
@@ -998,7 +1163,6 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     int rows = t.first < t.prefix_end ? t.begin : t.first, rows_end = t.end;
     const int mine = key0 >= t.end ? 0x7fffffff : key0 < t.prefix_end ? t.begin : key0;
     const int all = key0 + 16 * NB <= t.prefix_end || t.prefix_end == t.end ? t.begin : key0 + 16 * NB - 1;
-    const int head0 = kvh * a.many + part_of * a.many / a.parts, heads = kvh * a.many + (part_of + 1) * a.many / a.parts - head0;
     if constexpr (KIND == kAttnBias) {  // as far as the farthest of the heads reaches
       int reach = 0;
       for (int h = 0; h < heads; h++) {
@@ -1126,10 +1290,28 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
       }
     }
   }
+  uint32_t odd[NB];
 #pragma unroll
   for (int j = 0; j < NB; j++) {
     const int key = key0 + 16 * j + c;
-    if (key >= t.end) continue;
+    odd[j] = 0;
+    if constexpr (MASK) {
+      odd[j] = attn_odd(!(attn_all_finite(dk, j) && attn_all_finite(dv, j)) && key < t.end);
+      if (odd[j] != 0) {
+        const int from = key0 < t.prefix_end ? t.begin : key0 - R, last = key0 + 16 * NB - 1;
+        bool all = true;
+        for (int head = head0; head < head0 + heads; head++) {
+          const E *q = (const E*)a.q + head * a.qh, *grad = (const E*)a.grad + (int64_t)head * D;
+          const int64_t gt = (int64_t)a.H * D;
+          odd[j] &= attn_odd(key < t.end && attn_finite(a.lse[(int64_t)head * a.T + key]) && attn_some_finite<DT, D>(grad + key * gt, g));
+          if (odd[j] == 0) break;
+          const int begin = from > t.begin ? from : t.begin, end = last < t.end ? last : t.end;
+          all = all && attn_rows_finite<DT, D>(q, a.qt, begin, end) && attn_rows_finite<DT, D>(grad, gt, begin, end);
+        }
+        if (all) odd[j] = 0;
+      }
+    }
+    if (key >= t.end || odd[j] >> c & 1) continue;
     const int64_t at = ((int64_t)key * a.KV + kvh) * D;
     const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
     const float fv = !t.real ? 0.f : 1.f / (float)(1 << attn_up<DT>());
@@ -1141,6 +1323,29 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     }
     if (a.dk) attn_store<DT>(a.dk, at, dk, j, fk, g);
     if (a.dv) attn_store<DT>(a.dv, at, dv, j, fv, g);
+  }
+#pragma unroll
+  for (int j = 0; j < NB; j++) {
+    for (uint32_t m = MASK ? odd[j] : 0; m != 0; m &= m - 1) {
+      const int key = key0 + 16 * j + __builtin_ctz(m);
+      float x[(D + 63) / 64] = {}, y[(D + 63) / 64] = {};
+      for (int head = head0; head < head0 + heads; head++)
+        attn_alone<DT, D, KIND, kAttnDkv>(a, head, key, key < t.prefix_end ? t.begin : key, t.end, (const E*)a.k + kvh * a.kh + key * a.kt,
+                                          (const E*)a.v + kvh * a.vh + key * a.vt, (const E*)a.q + head * a.qh, a.qt, (const E*)a.grad + (int64_t)head * D,
+                                          (int64_t)a.H * D, 0.f, 0.f, x, y);
+#pragma unroll
+      for (int u = 0; u < (D + 63) / 64; u++) {
+        const int64_t at = ((int64_t)key * a.KV + kvh) * D + 64 * u + attn_lane(), one = a.T * a.KV * D;
+        if (64 * u + attn_lane() >= D) continue;
+        if (a.parts > 1) {
+          a.sums[2 * part_of * one + at] = x[u] * a.scale;
+          a.sums[(2 * part_of + 1) * one + at] = y[u];
+          continue;
+        }
+        if (a.dk) ((E*)a.dk)[at] = attn_round<DT>(x[u] * a.scale);
+        if (a.dv) ((E*)a.dv)[at] = attn_round<DT>(y[u]);
+      }
+    }
   }
 }
 
@@ -1170,32 +1375,32 @@ __global__ __launch_bounds__(kAttnThreads) void attn_join_kernel(const float* su
 
 // ---------------------------------------------------------------- launches
 
-template <int DT, int D, int NB, int KIND, AttnPass PASS>
+template <int DT, int D, int NB, int KIND, AttnPass PASS, bool MASK>
 static int attn_launch(AttnArgs a, hipStream_t st) {
   typedef AttnRows<DT, D, attn_rows<DT, D, NB>(PASS)> Rows;
   a.slots = (int32_t)attn_slots(a.T, a.B, 64 * NB);
   const dim3 grid((unsigned)attn_grid(a.slots, PASS == kAttnDkv ? a.KV * a.parts : a.H)), threads(kAttnThreads);  // below 2^23
   constexpr size_t lds = 4 * (size_t)Rows::kBytes;
   if constexpr (PASS == kAttnForward) {
-    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, KIND>), grid, threads, lds, st, a);
+    hipLaunchKernelGGL((attn_forward_kernel<DT, D, NB, KIND, MASK>), grid, threads, lds, st, a);
     return check_launch("attn_forward_kernel");
   } else if constexpr (PASS == kAttnDq) {
     if constexpr (NB == 1) {
       if (attn_short(a.T, a.B)) {
-        hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, true>), grid, threads, lds, st, a);
+        hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, true, MASK>), grid, threads, lds, st, a);
         return check_launch("attn_dq_kernel");
       }
     }
-    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, false>), grid, threads, lds, st, a);
+    hipLaunchKernelGGL((attn_dq_kernel<DT, D, NB, KIND, false, MASK>), grid, threads, lds, st, a);
     return check_launch("attn_dq_kernel");
   } else {
     constexpr size_t both = lds + 4 * Rows::R * sizeof(float);
     bool few = false;
     if constexpr (NB == 1 && DT != TMS_DTYPE_F32) {
       few = attn_short(a.T, a.B);
-      if (few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, true>), grid, threads, both, st, a);
+      if (few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, true, MASK>), grid, threads, both, st, a);
     }
-    if (!few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, false>), grid, threads, both, st, a);
+    if (!few) hipLaunchKernelGGL((attn_dkv_kernel<DT, D, NB, KIND, false, MASK>), grid, threads, both, st, a);
     const int rc = check_launch("attn_dkv_kernel");
     if (rc || a.parts == 1) return rc;
     const int64_t n = a.T * a.KV * D, groups = (n / 2 + kAttnThreads - 1) / kAttnThreads;
@@ -1217,12 +1422,16 @@ constexpr bool attn_two(AttnPass pass) {
   if (pass == kAttnDkv) return D <= 64 || (D == 96 && KIND == kAttnPlain);
   return pass == kAttnForward || D < 128 || KIND == kAttnPlain;
 }
+template <int DT, int D, int KIND, AttnPass PASS, bool MASK>
+static int attn_run_mask(const AttnArgs& a, hipStream_t st) {
+  if constexpr (attn_two<DT, D, KIND>(PASS)) {
+    if (attn_wide(a.T, a.B, PASS == kAttnDkv ? (int64_t)a.KV * a.parts : a.H)) return attn_launch<DT, D, 2, KIND, PASS, MASK>(a, st);
+  }
+  return attn_launch<DT, D, 1, KIND, PASS, MASK>(a, st);
+}
 template <int DT, int D, int KIND, AttnPass PASS>
 static int attn_run_pass(const AttnArgs& a, hipStream_t st) {
-  if constexpr (attn_two<DT, D, KIND>(PASS)) {
-    if (attn_wide(a.T, a.B, PASS == kAttnDkv ? (int64_t)a.KV * a.parts : a.H)) return attn_launch<DT, D, 2, KIND, PASS>(a, st);
-  }
-  return attn_launch<DT, D, 1, KIND, PASS>(a, st);
+  return a.prefix != nullptr ? attn_run_mask<DT, D, KIND, PASS, true>(a, st) : attn_run_mask<DT, D, KIND, PASS, false>(a, st);
 }
 template <int DT, int D, int KIND>
 static int attn_run_kind(const AttnArgs& a, AttnPass pass, hipStream_t st) {
