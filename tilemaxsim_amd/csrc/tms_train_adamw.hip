@@ -81,7 +81,8 @@ struct AdamList {
   int32_t count;
 };
 
-// 32 mixed bits of 32 (a xor-shift-multiply hash; every input bit reaches every output bit).
+// 32 mixed bits of 32: a xor-shift-multiply hash, with the shifts and constants that C. Wellons found for the least bias
+// ("Prospecting for Hash Functions", 2018); every input bit reaches every output bit.
 __device__ __forceinline__ uint32_t adam_mix(uint32_t x) {
   x = (x ^ (x >> 16)) * 0x7feb352du;
   x = (x ^ (x >> 15)) * 0x846ca68bu;
