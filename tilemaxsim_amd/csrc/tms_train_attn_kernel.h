@@ -1099,7 +1099,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       }
     }
     if (row >= t.end || odd[j] >> c & 1) continue;
-    const float f = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
+    const bool one = (row + 1 > t.prefix_end ? row + 1 : t.prefix_end) == t.begin + 1;  // the row sees one key: P = 1, dS = 0 (but for roundings)
+    const float f = !t.real || one ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
     attn_store<DT>(a.dq, ((int64_t)row * a.H + head) * D, acc, j, f, g);
   }
 #pragma unroll
@@ -1108,13 +1109,15 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
       const int i = __builtin_ctz(m), row = row0 + 16 * j + i, kvh = head / a.many;
       const int ln = attn_lane();
       const float l = a.lse[(int64_t)head * a.T + row], dl = a.delta[(int64_t)head * a.T + row];
+      const int sees = row + 1 > t.prefix_end ? row + 1 : t.prefix_end;
+      const float f = sees == t.begin + 1 ? 0.f : a.scale;
       float x[(D + 63) / 64] = {};
-      attn_alone<DT, D, KIND, kAttnDq>(a, head, row, t.begin, row + 1 > t.prefix_end ? row + 1 : t.prefix_end, (const E*)a.q + head * a.qh + row * a.qt,
+      attn_alone<DT, D, KIND, kAttnDq>(a, head, row, t.begin, sees, (const E*)a.q + head * a.qh + row * a.qt,
                                        (const E*)a.grad + ((int64_t)row * a.H + head) * D, (const E*)a.k + kvh * a.kh, a.kt, (const E*)a.v + kvh * a.vh, a.vt, l, dl,
                                        x, x);
 #pragma unroll
       for (int u = 0; u < (D + 63) / 64; u++)
-        if (64 * u + ln < D) ((E*)a.dq)[((int64_t)row * a.H + head) * D + 64 * u + ln] = attn_round<DT>(x[u] * a.scale);
+        if (64 * u + ln < D) ((E*)a.dq)[((int64_t)row * a.H + head) * D + 64 * u + ln] = attn_round<DT>(x[u] * f);
     }
   }
 }
@@ -1313,7 +1316,8 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
     }
     if (key >= t.end || odd[j] >> c & 1) continue;
     const int64_t at = ((int64_t)key * a.KV + kvh) * D;
-    const float fk = !t.real ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
+    // of a text of one token dS is 0, but for roundings
+    const float fk = !t.real || t.end - t.begin == 1 ? 0.f : (DT == TMS_DTYPE_F16 ? a.scale / range[j].held : a.scale) / AttnScore<DT, KIND, Rows::R>::kSlope;
     const float fv = !t.real ? 0.f : 1.f / (float)(1 << attn_up<DT>());
     if (a.parts > 1) {
       const int64_t one = a.T * a.KV * D;
