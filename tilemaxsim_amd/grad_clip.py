@@ -52,6 +52,9 @@ def _list(fn: str, tensors, of_a_graph=None) -> tuple[list, list]:
     return ts, kinds
 
 
+_contiguous = torch.Tensor.is_contiguous
+
+
 def _on_one_gpu(fn: str, ts: list) -> None:
     on = {t.get_device() for t in ts}  # -1: not on a GPU
     if len(on) > 1 or -1 in on:
@@ -173,10 +176,13 @@ def clip_grad_norm_(tensors, max_norm: float, norm_type: float = 2.0, error_if_n
     lib = _lib.load()
     norm = torch.empty((), dtype=torch.float32, device=dev)
     ws = _workspace(lib, len(ts), dev)
-    src = [t if t.is_contiguous() else t.contiguous() for t in ts]
-    dst = src if to is ts else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in to]
-    copies = [(o, d) for o, d in zip(to, dst) if o is not d]  # strided tensors' own elements
-    if copies or any(t is not x for t, x in zip(ts, src)):  # contiguous ones the library looks over
+    src = ts if all(map(_contiguous, ts)) else [t if t.is_contiguous() else t.contiguous() for t in ts]
+    if to is ts:
+        dst = src
+    else:
+        dst = to if all(map(_contiguous, to)) else [o if o.is_contiguous() else torch.empty_like(o, memory_format=torch.contiguous_format) for o in to]
+    copies = [] if dst is to else [(o, d) for o, d in zip(to, dst) if o is not d]  # strided tensors' own elements
+    if copies or src is not ts:  # contiguous ones the library looks over
         _overlap.apart(fn, to, [t for t, o in zip(ts, to) if not _same(t, o)])
     table = _table(src, kinds, dst, into)
     limit = ctypes.c_double(max_norm)
