@@ -146,7 +146,7 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, offsets:
 
     Returns:
         (T, H, D) of q's dtype. Rows of no text are zero (as their gradients are); what stands
-        there, and in other texts, is not seen, NaN included.
+        there, in other texts and behind a prefix mask is not seen, NaN included.
 
     Scores, softmax and sums are fp32; probabilities and their gradients are rounded to the
     inputs' type between two products (backward, where texts are short, to two terms of it). Every sum has one order.
