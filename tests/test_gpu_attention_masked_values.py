@@ -111,6 +111,40 @@ def test_one_token_anywhere(cuda, prefix, D, dt):
 
 
 @pytest.mark.parametrize("dt", DT, ids=str)
+@pytest.mark.parametrize("H,KV,D", [(1, 1, 64), (4, 2, 32), (2, 1, 128), (24, 24, 96)])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_seen_and_unseen(cuda, H, KV, D, value, dt):
+    """A bad value that a row sees, in one column, and another that it does not, in another column next to it."""
+    import tilemaxsim_amd as tms
+    n = 3001 if H == 24 else 300
+    ts, offsets, G = make([n], H, KV, D, dt, seed=H)
+    q, k, v = ts
+    want, off = reference(*ts, offsets, G, prefix=0)
+    with torch.no_grad():
+        v2 = v.clone()
+        v2[10, :, 3], v2[120, :, 5] = value, value
+    out = tms.packed_attention(q, k, v2, offsets, prefix=0)
+    fine = torch.ones_like(out, dtype=torch.bool)
+    fine[10:, :, 3] = fine[120:, :, 5] = False
+    agree((out.detach(),), want[:1], off[:1], dict(out=fine), f"values {D} {dt}")
+    assert not torch.isfinite(out[10:, :, 3]).any() and not torch.isfinite(out[120:, :, 5]).any()
+    with torch.no_grad():
+        g = G.clone()
+        g[120, :, 3], g[70, :, 5] = value, value
+    grads = torch.autograd.grad(tms.packed_attention(q, k, v, offsets, prefix=0), ts, g)
+    # rows 70 and 120 reach the keys up to them, in their own columns of dv, and in all of dk
+    fine = torch.ones_like(v, dtype=torch.bool)
+    fine[:121, :, 3] = fine[:71, :, 5] = False
+    g0 = G.clone()
+    g0[120], g0[70] = 0, 0
+    without, off0 = reference(*ts, offsets, g0, prefix=0)
+    behind = torch.arange(121, n, device="cuda")
+    agree((out.detach(), *grads), without, off0, dict(out=behind[:0], dq=behind, dk=behind, dv=behind), f"gradients {D} {dt}")
+    agree((grads[2],), [want[3]], [off[3]], dict(out=fine), f"gradients, dv {D} {dt}")
+    assert not torch.isfinite(grads[2][:121, :, 3]).any() and not torch.isfinite(grads[2][:71, :, 5]).any() and not torch.isfinite(grads[1][:121]).any()
+
+
+@pytest.mark.parametrize("dt", DT, ids=str)
 def test_seen_tokens_do(cuda, dt):
     """A value that a row sees reaches it where it stands: in its column of the output, infinite with its sign."""
     import tilemaxsim_amd as tms

@@ -522,10 +522,11 @@ __global__ __launch_bounds__(kAttnThreads) void attn_norms_kernel(AttnArgs a) {
 // stands for it in the matrix instructions makes the row NaN. Rows of sums that are not finite are therefore formed
 // once more by one wave, from what they see alone, in fp32: 64 of the others at a time, one a lane for the scores, then one
 // after the other with the row's elements on the lanes. A row that is not finite by what it does see stays so. That takes
-// 30 to 100 times as long as with the matrix instructions, so rows that need not are not formed again: those whose own
-// statistic, or whole own token (which they see), is not finite, and all of a wave where every token in reach that some
-// row does not see is finite. (Two causal texts of 8192, 12 heads of 64, both directions: 1.4 ms, with a NaN that is
-// seen 1.2, with one in every 64th token 49.)
+// 50 times as long as with the matrix instructions, so rows that need not are not formed again: those whose own
+// statistic is not finite; all of a wave where every token in reach that some row does not see is finite; and those that are finite but in
+// columns where their own token, or one that all of the wave's rows see, is not. What is left are rows close to the first bad token
+// of a column. (Two causal texts of 8192, 12 heads of 64, both directions: 1.4 ms; with NaN or infinities in one
+// token, one column, every 64th token or all of them 1.2 to 2.7.)
 // What it needs is formed anew or read again, so that next to nothing stays in registers for it while the tiles are gone over; calls without
 // prefixes take kernels without it (MASK: 100 causal texts of 200, 12 heads of 64, forward 38.9 us and backward 122.9, without the check 38.4 and 117.8).
 __device__ __forceinline__ int attn_lane() { return (int)__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)); }
@@ -548,13 +549,6 @@ __device__ __forceinline__ uint32_t attn_odd(bool here) {
   return (uint32_t)(b | b >> 16 | b >> 32 | b >> 48) & 0xffffu;
 }
 
-// Whether a lane's quarter (pieces g, g + 4 ..) of a row has a finite element.
-template <int DT, int D>
-__device__ __forceinline__ bool attn_some_finite(const typename AttnType<DT>::E* x, int g) {
-  bool some = false;
-  for (int d = g; d < D; d += 4) some |= attn_finite(attn_float<DT>(x[d]));
-  return some;
-}
 // Whether all elements of rows from `from` up to `to` are finite: one row a lane.
 template <int DT, int D>
 __device__ bool attn_rows_finite(const typename AttnType<DT>::E* x, int64_t stride, int from, int to) {
@@ -567,6 +561,39 @@ __device__ bool attn_rows_finite(const typename AttnType<DT>::E* x, int64_t stri
       for (int e = 0; e < 8; e++) bad |= !attn_finite(attn_elem<DT>(f, e));
     }
   return __ballot(bad) == 0ull;
+}
+
+// The columns in which any of those rows is not finite, as bits (of all lanes).
+template <int D>
+struct AttnColumns {
+  uint32_t bits[D / 32] = {};
+  template <int DT>
+  __device__ void add(const typename AttnType<DT>::E* x, int64_t stride, int from, int to) {
+    typedef typename AttnType<DT>::Frag Frag;
+    for (int r = from + attn_lane(); r < to; r += 64)
+#pragma unroll
+      for (int k = 0; k < D; k += 8) {
+        const Frag f = *(const Frag*)(x + r * stride + k);
+#pragma unroll
+        for (int e = 0; e < 8; e++) bits[k / 32] |= attn_finite(attn_elem<DT>(f, e)) ? 0u : 1u << ((k + e) % 32);
+      }
+#pragma unroll
+    for (int i = 0; i < D / 32; i++)
+#pragma unroll
+      for (int o = 32; o >= 1; o >>= 1) bits[i] |= __shfl_xor(bits[i], o);
+  }
+};
+// Whether a lane's sums of column j (elements 16 d + 4 g + e) are not finite where neither those columns nor its own token explain it.
+template <int DT, int D, int DB, int NB>
+__device__ __forceinline__ bool attn_unexplained(const f32x4 (&acc)[DB][NB], int j, const AttnColumns<D>& bad, const typename AttnType<DT>::E* own, int g) {
+  bool some = false;
+#pragma unroll
+  for (int d = 0; d < DB; d++) {
+    const uint32_t four = bad.bits[d / 2] >> (16 * (d & 1) + 4 * g) & 15u;
+#pragma unroll
+    for (int e = 0; e < 4; e++) some |= !attn_finite(acc[d][j][e]) && !(four >> e & 1) && attn_finite(attn_float<DT>(own[16 * d + 4 * g + e]));
+  }
+  return some;
 }
 
 template <int DT, int D>
@@ -804,8 +831,13 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_forward_kernel(AttnArgs 
       if (odd[j] != 0) {
         const E* v = (const E*)a.v + head / a.many * a.vh;
         const int unseen = row0 + 1 > t.prefix_end ? row0 + 1 : t.prefix_end, past = row0 + 16 * NB, end = (past > t.prefix_end ? past : t.prefix_end) + R;
-        odd[j] &= attn_odd(row < t.end && attn_some_finite<DT, D>(v + row * a.vt, g));
-        if (attn_rows_finite<DT, D>(v, a.vt, unseen, end < t.end ? end : t.end)) odd[j] = 0;
+        if (attn_rows_finite<DT, D>(v, a.vt, unseen, end < t.end ? end : t.end)) {
+          odd[j] = 0;
+        } else {
+          AttnColumns<D> bad;
+          bad.template add<DT>(v, a.vt, t.begin, unseen);
+          odd[j] &= attn_odd(row < t.end && attn_unexplained<DT, D>(acc, j, bad, v + row * a.vt, g));
+        }
       }
     }
     if (row >= t.end) continue;
@@ -1095,7 +1127,14 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dq_kernel(AttnArgs a) {
         const int64_t at = (int64_t)head * a.T + row;
         odd[j] &= attn_odd(row < t.end && attn_finite(a.lse[at]) && attn_finite(a.delta[at]));
         const int unseen = row0 + 1 > t.prefix_end ? row0 + 1 : t.prefix_end, past = row0 + 16 * NB, end = (past > t.prefix_end ? past : t.prefix_end) + R;
-        if (attn_rows_finite<DT, D>((const E*)a.k + head / a.many * a.kh, a.kt, unseen, end < t.end ? end : t.end)) odd[j] = 0;
+        const E* k = (const E*)a.k + head / a.many * a.kh;
+        if (odd[j] == 0 || attn_rows_finite<DT, D>(k, a.kt, unseen, end < t.end ? end : t.end)) {
+          odd[j] = 0;
+        } else {
+          AttnColumns<D> bad;
+          bad.template add<DT>(k, a.kt, t.begin, unseen);
+          odd[j] &= attn_odd(row < t.end && attn_unexplained<DT, D>(acc, j, bad, k + row * a.kt, g));
+        }
       }
     }
     if (row >= t.end || odd[j] >> c & 1) continue;
@@ -1302,16 +1341,31 @@ __global__ __launch_bounds__(kAttnThreads, 2) void attn_dkv_kernel(AttnArgs a) {
       odd[j] = attn_odd(!(attn_all_finite(dk, j) && attn_all_finite(dv, j)) && key < t.end);
       if (odd[j] != 0) {
         const int from = key0 < t.prefix_end ? t.begin : key0 - R, last = key0 + 16 * NB - 1;
-        bool all = true;
+        const int begin = from > t.begin ? from : t.begin, end = last < t.end ? last : t.end;  // of rows that some key is not seen by
+        const int64_t gt = (int64_t)a.H * D;
+        bool all = true, dead = false, some_v = key < t.end;  // dead: dk of all columns, or of this key's
+        AttnColumns<D> bad;
         for (int head = head0; head < head0 + heads; head++) {
           const E *q = (const E*)a.q + head * a.qh, *grad = (const E*)a.grad + (int64_t)head * D;
-          const int64_t gt = (int64_t)a.H * D;
-          odd[j] &= attn_odd(key < t.end && attn_finite(a.lse[(int64_t)head * a.T + key]) && attn_some_finite<DT, D>(grad + key * gt, g));
+          const int64_t at = (int64_t)head * a.T;
+          odd[j] &= attn_odd(key < t.end && attn_finite(a.lse[at + key]));
           if (odd[j] == 0) break;
-          const int begin = from > t.begin ? from : t.begin, end = last < t.end ? last : t.end;
           all = all && attn_rows_finite<DT, D>(q, a.qt, begin, end) && attn_rows_finite<DT, D>(grad, gt, begin, end);
+          bool lost = false, none = false;  // rows that all keys are seen by: of no delta, and of no P
+          for (int r = last + attn_lane(); r < t.end; r += 64) {
+            none |= !attn_finite(a.lse[at + r]);
+            lost |= !attn_finite(a.delta[at + r]);
+          }
+          if (__ballot(none) != 0ull) {
+            odd[j] = 0;
+            break;
+          }
+          dead |= __ballot(lost) != 0ull || (key < t.end && !attn_finite(a.delta[at + key]));
+          bad.template add<DT>(grad, gt, last, t.end);
+          some_v = some_v && attn_unexplained<DT, D>(dv, j, bad, grad + key * gt, g);
         }
         if (all) odd[j] = 0;
+        odd[j] &= attn_odd(some_v || (key < t.end && !dead && !attn_all_finite(dk, j)));
       }
     }
     if (key >= t.end || odd[j] >> c & 1) continue;
