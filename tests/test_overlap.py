@@ -28,11 +28,11 @@ def refused(written, read=()):
 def test_against_every_place():
     """Random strided views of one buffer, of several element sizes: refused where two places are one, and only there."""
     rng = random.Random(0)
-    flat = torch.zeros(4096, dtype=torch.uint8)
+    flat = torch.zeros(8192, dtype=torch.uint8)
     outcomes = []
     for _ in range(3000):
         views = []
-        for _ in range(rng.choice((1, 2, 2, 3))):
+        for _ in range(rng.choice((1, 2, 2, 3, 4))):
             dt = rng.choice((torch.float32, torch.bfloat16, torch.float32))
             dims = rng.randint(1, 3)
             shape = [rng.choice((1, 2, 3, 5, 8)) for _ in range(dims)]
@@ -57,6 +57,23 @@ def test_views_of_one_buffer():
     assert not refused([w[:0], w[:, :0], w]) and not refused([w[0, 0], w[0, 1:]]) and refused([w[0, 1], w[0, 1:]])
     wide = torch.empty(1 << 16, 64)  # no list of places: strides are compared
     assert not refused([wide[:, :32], wide[:, 32:]]) and refused([wide[:, :33], wide[:, 32:]])
+
+
+def test_many_columns_of_one_matrix():
+    """Hundreds of views side by side are told from each other in a moment; one that reaches into its neighbour is found."""
+    import time
+    w = torch.zeros(50, 4096)
+    columns = [w[:, 8 * i:8 * i + 8] for i in range(512)]
+    began = time.perf_counter()
+    assert not refused(columns) and not refused(columns[::2], columns[1::2])
+    assert time.perf_counter() - began < 1.0  # pair by pair: some 131,000 comparisons of 10 us
+    assert refused([*columns[:100], w[:, 799:808], *columns[101:]]) and refused(columns[:9], [w[3:4, 5:9], w[:, 4000]])
+    assert not refused([*columns[:100], *columns[101:]], [w[:, 800:804], w[2, 804:806]])
+    halves = [w[::2, :64], w[1::2, :64], w[::2, 64:], w[1::2, 64:]]  # rows in turn: another pitch than the matrix's
+    assert not refused(halves) and refused([*halves, w[3:4, 10:20]])
+    assert refused([w.as_strided((49, 10), (4096, 1), 4090), w[:, :8], w[:, 8:16]])  # behind a row's end, into the next one
+    flat = torch.zeros(100)
+    assert not refused([flat[::2], flat[1:50:2], flat[51:60:2], flat[61:62], flat[63:64]]) and refused([flat[::2], flat[1:50:2], flat[50:51]])
 
 
 def test_what_takes_too_long_to_tell_is_refused():

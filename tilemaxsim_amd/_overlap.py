@@ -75,24 +75,62 @@ def _meet(a: torch.Tensor, b: torch.Tensor) -> bool:
     return _solvable([*_dims(a), *theirs, *inner], target)
 
 
+def _apart(fn: str, order: list, begins: list, ends: list, pair) -> None:
+    """Goes over spans in order of their begins, and asks pair(i, j) of those that overlap."""
+    near: list = []  # those that reach the next one's begin
+    for i in order:
+        if near:
+            at = begins[i]
+            near = [j for j in near if ends[j] > at]
+            if any(pair(i, j) for j in near):
+                raise ValueError(f"{fn}: two of the tensors overlap")
+        near.append(i)
+
+
 def apart(fn: str, written: list, read: list) -> None:
     """Refuses tensors of which a written one shares memory with another one, or with itself."""
     ts, writes = [*written, *read], len(written)
     begins = list(map(torch.Tensor.data_ptr, ts))
     sizes = list(map(torch.Tensor.numel, ts))
     ends = [at + n * size for at, n, size in zip(begins, sizes, map(torch.Tensor.element_size, ts))]
-    strided = [i for i, whole in enumerate(map(torch.Tensor.is_contiguous, ts)) if not whole]
+    strided = {i for i, whole in enumerate(map(torch.Tensor.is_contiguous, ts)) if not whole and sizes[i]}
     for i in strided:
-        if i < writes and sizes[i] and _folds(ts[i]):
+        if i < writes and _folds(ts[i]):
             raise ValueError(f"{fn}: two elements of a tensor overlap")
         ends[i] = begins[i] + ts[i].element_size() + sum(s * most for s, most in _dims(ts[i]))
-    strided = set(strided)
-    near: list = []  # tensors that reach the next one's begin
-    for i in sorted((i for i, n in enumerate(sizes) if n), key=begins.__getitem__):
-        at = begins[i]
-        if near:
-            near = [j for j in near if ends[j] > at]
-            for j in near:
-                if (i < writes or j < writes) and (i not in strided and j not in strided or _meet(ts[i], ts[j])):
-                    raise ValueError(f"{fn}: two of the tensors overlap")
-        near.append(i)
+
+    def pair(i: int, j: int) -> bool:
+        if i >= writes and j >= writes:
+            return False
+        if i not in strided and j not in strided:
+            return begins[i] < ends[j] and begins[j] < ends[i]
+        return _meet(ts[i], ts[j])
+
+    order = sorted((i for i, n in enumerate(sizes) if n), key=begins.__getitem__)
+    first = 0
+    while first < len(order):  # tensors whose spans hang together
+        last, reach = first + 1, ends[order[first]]
+        while last < len(order) and begins[order[last]] < reach:
+            reach = max(reach, ends[order[last]])
+            last += 1
+        group, first = order[first:last], last
+        rows = _rows(group, ts, begins) if len(group) > 2 and not strided.isdisjoint(group) else None
+        _apart(fn, *(rows or (group, begins, ends)), pair)
+
+
+def _rows(group: list, ts: list, begins: list):
+    """Views of some columns of one matrix as spans within its rows (many of them would be compared pair by pair
+    otherwise): the order, begins and ends; None if they are no such views."""
+    pitch, at, to = None, {}, {}
+    for i in group:
+        dims = _dims(ts[i])
+        if not dims:
+            return None
+        s = max(s for s, _ in dims)
+        inner = ts[i].element_size() + sum(r * most for r, most in dims) - s * max(most for r, most in dims if r == s)
+        at[i] = (begins[i] - begins[group[0]]) % (pitch or s or 1)
+        to[i] = at[i] + inner
+        if s != (pitch or s) or not s or to[i] > s:
+            return None
+        pitch = s
+    return sorted(group, key=at.__getitem__), at, to

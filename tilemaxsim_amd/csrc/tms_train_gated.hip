@@ -13,7 +13,7 @@
 //
 // Bound by the matrix cores, the tiles' ends behind them. 16,384 tokens, 1024 x 4096, bf16: forward 267 us (1.03 PFLOP/s), dg
 // and du 317 (their ends form two functions and write 268 MB), dx 269, both weights' gradients 273 and 14 for
-// the join of two splits. 1229 x 768 x 2043: 16, 22, 18 + 5 and 17 us, where tiles of 128 fill the chip once
+// the join of two splits. 1229 x 768 x 2043, fp16: 19, 23, 17 + 5 and 17 us, where tiles of 128 fill the chip once
 // and a quarter, or less than once (two steps a wait).
 //
 // Few tokens take a kernel of their own: bound by reading the weights once, which needs every CU to have
@@ -348,7 +348,8 @@ __global__ __launch_bounds__(256) void gated_join_kernel(const float* sums, int 
 // argument, or steeper than 1.13), and |g|, |u| <= |x| |w| for the norms of the token's row and the weight's. A workgroup has
 // tokens (`rows`: their largest |dh| times |x|; `parts`: the largest of those times |x| once more), or four rows of weights at a
 // time (squares of their norms: `parts` from kBoundTokens on). Infinite and NaN elements of dh, and rows that have any
-// elsewhere, are passed over: they make their own rows what they will. 1229 x 768 x 2043: 6.3 us.
+// elsewhere, are passed over: they make their own rows what they will. 1229 x 768 x 2043: 6.3 us; 16,384 x
+// 1024 x 4096: 38, bound by reading them (5.0 TB/s).
 constexpr int kBoundTokens = 2048, kBoundWeights = 1024;
 constexpr float kBoundSlope = 1.2f;
 
@@ -445,7 +446,7 @@ __device__ __forceinline__ float gated_power(int e) { return e < -126 ? 0.f : __
 
 // What each token's dg and du are held times, its reciprocal, and x times that reciprocal and a power of two that brings the
 // largest bound of that to 2^14 to 2^15 (`xs`, `terms` times one behind the other; *back: what takes the power out again).
-// 1229 x 768: 5.1 us, most of them the way of the parts.
+// 1229 x 768: 5.1 us, most of them the way of the parts; 16,384 x 1024: 17.
 __global__ __launch_bounds__(256) void gated_scale_kernel(const float* parts, int tokens, int weights, const float* rows, const uint16_t* x, int32_t N, int32_t d,
                                                           int32_t dp, int32_t terms, uint16_t* xs, float* held, float* held_back, float* back) {
   float h, w;
